@@ -63,9 +63,9 @@ def stale(name: str) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> list:
     """Builds every target that is missing or older than its source; returns
-    the library paths.  Where /root/reference is absent it only reports what
-    is already built."""
-    if not REF_ROOT.exists():
+    the library paths.  Where the reference's sources are absent it only
+    reports what is already built."""
+    if not all((REF_ROOT / rel).exists() for rel, *_ in TARGETS.values()):
         return sorted(OUT.glob("*.so"))
     os.environ["TORCH_CUDA_ARCH_LIST"] = "10.0"
     from torch.utils.cpp_extension import load_inline
