@@ -49,9 +49,9 @@ int current_device_info(DeviceInfo* out) {
   return DSA_OK;
 }
 
-int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
-                   uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
-                   uint32_t box_outer) {
+namespace {
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   std::call_once(g_encode_once, []() {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -61,13 +61,37 @@ int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     cudaGetLastError();
   });
-  if (g_encode == nullptr) return DSA_ERR_TENSOR_MAP;
+  return g_encode;
+}
+
+}  // namespace
+
+int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                   uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner,
+                   uint32_t box_outer) {
+  if (encoder() == nullptr) return DSA_ERR_TENSOR_MAP;
   if (!aligned16(base) || (row_pitch_bytes & 15u) != 0) return DSA_ERR_MISALIGNED;
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_pitch_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DSA_OK : DSA_ERR_TENSOR_MAP;
+}
+
+int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                   uint64_t middle, uint64_t outer, uint64_t middle_pitch_bytes,
+                   uint64_t outer_pitch_bytes, uint32_t box_inner, uint32_t box_middle) {
+  if (encoder() == nullptr) return DSA_ERR_TENSOR_MAP;
+  if (!aligned16(base) || ((middle_pitch_bytes | outer_pitch_bytes) & 15u) != 0)
+    return DSA_ERR_MISALIGNED;
+  cuuint64_t dims[3] = {inner, middle, outer};
+  cuuint64_t strides[2] = {middle_pitch_bytes, outer_pitch_bytes};
+  cuuint32_t box[3] = {box_inner, box_middle, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? DSA_OK : DSA_ERR_TENSOR_MAP;

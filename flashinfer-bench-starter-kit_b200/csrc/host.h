@@ -31,6 +31,12 @@ int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
                    uint64_t inner, uint64_t outer, uint64_t row_pitch_bytes,
                    uint32_t box_inner, uint32_t box_outer);
 
+// Same for a 3-D tensor: inner x middle x outer elements, the box one outer
+// index deep.
+int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                   uint64_t middle, uint64_t outer, uint64_t middle_pitch_bytes,
+                   uint64_t outer_pitch_bytes, uint32_t box_inner, uint32_t box_middle);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launches the indexer's top-2048 select over `rows` score rows (one CTA

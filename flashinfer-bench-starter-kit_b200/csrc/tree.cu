@@ -1,0 +1,1194 @@
+// tree.cu -- attention for a tree of drafted tokens over the paged ckv / kpe
+// cache, and the accumulation of the attention weights its rows give to the
+// cached tokens (sm_100a).
+//
+// Request b has prefix_lens[b] cached tokens and n drafts (rows cu[b] ..
+// cu[b+1]-1 of the queries), whose own cache rows follow at positions
+// prefix .. prefix + n - 1.  With c_k, e_k the ckv / kpe rows of position k,
+// for draft i and head h
+//   s_k = scale * (q_nope . c_k + q_pe . e_k)
+//   visible: k < prefix, or k = prefix + j with bit j of draft i's mask set
+//   lse = log2 sum_k 2^(s_k log2 e),   out = sum_k 2^(s_k log2 e - lse) c_k
+// and the weights kernel adds sum_{i,h} 2^(s_k log2 e - lse_ih) to position
+// k's accumulator.
+//
+// All heads share one key, so the n * H (draft, head) pairs of a request are
+// one tall set of query rows.  They are taken kRows = 64 at a time (a group);
+// a work unit is one group against one 64-token page.  Per unit
+//   S^T[64 tokens, 64 rows] = K[64, 576] . Q[64, 576]^T   36 x (M64 N64 K16)
+//   O^T[512, 64] += V^T[512, 64 tokens] . P^T[64 tokens, 64] 16 x (M128 N64 K16)
+// with V the ckv part of the K tile in shared memory, read MN-major.  The
+// transposed form leaves O^T in 256 TMEM columns (64 rows in the plain form
+// would take half the lanes of 512) and makes P an operand that the softmax
+// warps write without a transpose (MN-major, one 128-byte row per token).
+// K tile 72 KB x 2 stages + Q 72 KB + P 8 KB fill the shared memory, which
+// is what limits a CTA to 64 rows: at 64 rows the tile's 72 KB come from L2
+// or HBM in about the time of its MMAs (1152 + 768 clocks, measured 32 and 48
+// a piece).
+//
+// Units are ordered (request, chunk of tiles, group, tile) and cut into equal
+// contiguous slices, one per CTA ("stream-K").  Chunks are at least a slice
+// long, so the groups of a request walk the same pages at the same time on
+// neighbouring CTAs and share them through L2.  A slice's pieces that do not
+// cover their group's whole context are written as fp32 records (slot 0: the
+// piece at the slice's start, slot 1: the one at its end; no other can be
+// partial) and joined by combine_kernel.
+#include <cuda_bf16.h>
+
+#include <mutex>
+
+#include "dsa_b200.h"
+#include "host.h"
+#include "ptx.cuh"
+
+namespace dsa {
+namespace tree {
+
+constexpr int kCkv = DSA_CKV_DIM;            // 512
+constexpr int kKpe = DSA_KPE_DIM;            // 64
+constexpr int kTok = DSA_PAGE_SIZE;          // 64 tokens per tile: one page
+constexpr int kRows = 64;                    // query rows per group
+constexpr int kChunks = 9;                   // 8 ckv + 1 kpe pieces of 64 columns
+constexpr int kChunkBytes = 64 * 128;        // 8192
+constexpr int kTileBytes = kChunks * kChunkBytes;  // 73728: a K tile, or a group's Q
+constexpr int kSoftWarps = 8;                // warps 0-7: two sets of four, 32 rows each
+constexpr int kLoadWarp = 8;                 // TMA
+constexpr int kLogitWarp = 9;                // S^T MMAs (owns TMEM)
+constexpr int kValueWarp = 10;               // O^T MMAs
+constexpr int kThreads = 352;
+constexpr int kTmemCols = 512;
+constexpr uint32_t kColS = 0;                // S^T buffers at [0,64) and [64,128)
+constexpr uint32_t kColO = 128;              // O^T: 4 blocks of 128 dims x 64 columns
+constexpr float kRescaleThreshold = 8.0f;    // log2 units, see the softmax warps
+constexpr int kPartFloats = kRows * kCkv;    // a partial record's O, [row][dim]
+constexpr int kSumTiles = 16;                // weights: tiles whose sums wait in shared memory
+constexpr int kSumTilesShared = 8;           // ... when several groups re-read them through L2
+
+constexpr uint32_t kIdescS = idesc_make(1, 1, false, false, 64, 64);
+constexpr uint32_t kIdescO = idesc_make(1, 1, true, true, 128, 64);
+
+constexpr int kOffQ = 2 * kTileBytes;          // 147456
+constexpr int kOffP = kOffQ + kTileBytes;      // 221184: P, or the weights' sums
+constexpr int kOffBar = kOffP + kTok * 128;    // 229376
+constexpr int kOffMisc = kOffBar + 128;
+constexpr int kOffRed = kOffMisc + 128;        // [4][64] floats
+constexpr int kOffAlpha = kOffRed + 1024;      // [64]
+constexpr int kOffSum = kOffAlpha + 256;       // [64]
+constexpr int kOffMax = kOffSum + 256;         // [64]
+constexpr int kSmemBytes = 1024 + kOffMax + 256;
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+static_assert(2 * kSumTiles * kTok * 4 <= kTok * 128, "the weights' sums take P's place");
+
+constexpr int kMaxRequests = 65536;
+constexpr int kPlanHead = 4;                   // plan words: total units, total groups
+
+struct Params {
+  const int32_t* prefix_lens;
+  const int32_t* block_table;
+  const int32_t* cu;
+  const long long* mask;
+  int num_requests, num_drafts, heads, max_pages, mask_words;
+  int num_pages;
+  float scale_log2;
+  unsigned int* status;
+  unsigned long long wait_limit_ns;
+  // attention
+  __nv_bfloat16* out;
+  float* lse_out;
+  float* part_o;    // [2 * grid][kPartFloats]
+  float* part_ml;   // [2 * grid][kRows][2]
+  int* plan;        // total units, total groups, -, -, first unit [B], first group [B], request of group
+  // weights
+  const float* lse_in;
+  const float* acc;
+  float* acc_out;
+  int64_t acc_stride, acc_out_stride;
+};
+
+struct Request {
+  int prefix, n, row0;  // cached tokens, drafts, first draft's row
+  int rows, groups, tiles;
+};
+
+// Request b as its inputs give it; what they give wrongly is clamped or, if
+// it cannot be, taken as a request without drafts.
+__device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
+  Request r;
+  const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
+  const int cap = p.max_pages * kTok;
+  r.prefix = __ldg(p.prefix_lens + b);
+  r.row0 = lo;
+  r.n = hi - lo;
+  bad = false;
+  if (lo < 0 || hi < lo || hi > p.num_drafts || r.n > cap) {
+    r.n = 0;
+    bad = true;
+  }
+  if (r.prefix < 0) {
+    r.prefix = 0;
+    bad = true;
+  }
+  if (r.prefix > cap - r.n) {
+    r.prefix = cap - r.n;
+    bad = true;
+  }
+  bad |= (r.n + 63) / 64 > p.mask_words;
+  r.rows = r.n * p.heads;
+  r.groups = (r.rows + kRows - 1) / kRows;
+  r.tiles = r.n == 0 ? 0 : (r.prefix + r.n + kTok - 1) / kTok;
+  return r;
+}
+
+// Slice boundaries: CTA c of `ctas` has units [start(c), start(c+1)).
+__device__ __forceinline__ int slice_start(int total, int c, int ctas) {
+  return static_cast<int>(static_cast<int64_t>(total) * c / ctas);
+}
+// The CTA whose slice holds unit u: the largest c with start(c) <= u.
+__device__ __forceinline__ int slice_of(int total, int u, int ctas) {
+  return static_cast<int>((static_cast<int64_t>(u + 1) * ctas - 1) / total);
+}
+__device__ __forceinline__ int slice_len(int total, int ctas) { return (total + ctas - 1) / ctas; }
+
+// Tiles are cut into `chunks_of` nearly equal chunks, each at least a slice
+// long (one chunk when a single group would walk them all anyway).
+__device__ __forceinline__ int chunks_of(const Request& r, int slice) {
+  if (r.groups <= 1) return 1;
+  const int c = r.tiles / slice;
+  return c < 1 ? 1 : c;
+}
+__device__ __forceinline__ int chunk_start(const Request& r, int chunks, int c) {
+  return static_cast<int>(static_cast<int64_t>(r.tiles) * c / chunks);
+}
+
+// The position of unit `rel` (counted from its request's first): chunk,
+// group and tile.
+struct Place {
+  int chunk, group, tile, t0, t1;  // t0, t1: the chunk's tiles
+};
+__device__ __forceinline__ Place place_of(const Request& r, int chunks, int rel) {
+  Place q;
+  const int t = rel / r.groups;  // rel = groups * t0 + ...: the chunk is the one holding tile t
+  q.chunk = static_cast<int>((static_cast<int64_t>(t + 1) * chunks - 1) / r.tiles);
+  q.t0 = chunk_start(r, chunks, q.chunk);
+  q.t1 = chunk_start(r, chunks, q.chunk + 1);
+  const int in = rel - r.groups * q.t0;
+  const int len = q.t1 - q.t0;
+  q.group = in / len;
+  q.tile = q.t0 + in - q.group * len;
+  return q;
+}
+
+// A run of tiles of one group.
+struct Segment {
+  int b, group, t0, t1;
+  Request r;
+  bool whole;             // attention: covers the group's whole context
+  int slot;               // attention: record slot if it does not
+  bool first_group, last_group;  // weights: of this run of tiles
+};
+
+// The segments of a CTA's slice, in order; every role walks its own copy.
+template <bool kWeights>
+struct Walker {
+  const Params& p;
+  int u, u0, u1, slice;
+  int b, first;           // request and its first unit
+  Request r;
+  int chunks;
+  Place at;               // attention: next unit's place
+  int run0, run1, end, g; // weights: current run of tiles, end of the slice's tiles, next group
+
+  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, int b0, int first_unit)
+      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(b0), first(first_unit) {
+    if (u0 < u1) enter();
+  }
+
+  __device__ void enter() {
+    bool bad;
+    r = load_request(p, b, bad);
+    if (r.tiles == 0) {
+      run0 = run1 = end = 0;
+      g = 0;
+      return;
+    }
+    if constexpr (kWeights) {
+      // A tile belongs to the slice that its first unit falls into.
+      const int lo = u0 - first, hi = u1 - first;
+      run0 = lo <= 0 ? 0 : (lo + r.groups - 1) / r.groups;
+      end = (hi + r.groups - 1) / r.groups;
+      if (end > r.tiles) end = r.tiles;
+      start_run();
+    } else {
+      chunks = chunks_of(r, slice);
+      at = place_of(r, chunks, u - first);
+    }
+  }
+  __device__ void start_run() {
+    const int most = r.groups > 1 ? kSumTilesShared : kSumTiles;
+    run1 = run0 + most < end ? run0 + most : end;
+    g = 0;
+  }
+  __device__ bool leave() {  // to the next request that has units in the slice
+    for (;;) {
+      first += r.groups * r.tiles;
+      ++b;
+      if (b >= p.num_requests || first >= u1) return false;
+      if constexpr (!kWeights) u = first;
+      enter();
+      if (r.tiles > 0) return true;
+    }
+  }
+
+  __device__ bool next(Segment& s) {
+    if constexpr (kWeights) {
+      if (u0 >= u1) return false;
+      while (run0 >= run1)
+        if (b >= p.num_requests || !leave()) return false;
+      s.b = b;
+      s.r = r;
+      s.group = g;
+      s.t0 = run0;
+      s.t1 = run1;
+      s.first_group = g == 0;
+      s.last_group = g == r.groups - 1;
+      if (++g == r.groups) {
+        run0 = run1;
+        start_run();
+      }
+      return true;
+    } else {
+      if (u >= u1) return false;
+      s.b = b;
+      s.r = r;
+      s.group = at.group;
+      s.t0 = at.tile;
+      int len = at.t1 - at.tile;
+      if (len > u1 - u) len = u1 - u;
+      s.t1 = s.t0 + len;
+      s.whole = s.t0 == 0 && s.t1 == r.tiles;
+      s.slot = u == u0 ? 0 : 1;
+      u += len;
+      if (u < u1) {
+        if (++at.group == r.groups) {
+          at.group = 0;
+          ++at.chunk;
+        }
+        if (at.chunk == chunks) {
+          if (!leave()) u = u1;
+        } else {
+          at.t0 = chunk_start(r, chunks, at.chunk);
+          at.t1 = chunk_start(r, chunks, at.chunk + 1);
+          at.tile = at.t0;
+        }
+      }
+      return true;
+    }
+  }
+};
+
+// Bits of one thread's 8 columns (rows of Q) that see position pos, which
+// lies at or behind the prefix.
+__device__ __forceinline__ uint32_t visible_columns(const Params& p, const Segment& s, int pos, const int (&draft)[8]) {
+  const int j = pos - s.r.prefix;
+  uint32_t m = 0;
+  if (j < s.r.n && j < 64 * p.mask_words) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const long long w = __ldg(p.mask + static_cast<int64_t>(s.r.row0 + draft[k]) * p.mask_words + (j >> 6));
+      m |= static_cast<uint32_t>((w >> (j & 63)) & 1) << k;
+    }
+  }
+  return m;
+}
+
+template <bool kWeights>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__ CUtensorMap kpe_map,
+            const __grid_constant__ CUtensorMap qn_map, const __grid_constant__ CUtensorMap qp_map, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_mem = smem + kOffQ;
+  uint8_t* p_mem = smem + kOffP;
+  float* sums = reinterpret_cast<float*>(p_mem);  // weights: [2 sets][kSumTiles][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint64_t* kv_full = bars;        // [2]
+  uint64_t* kv_empty = bars + 2;   // [2]
+  uint64_t* s_full = bars + 4;     // [2]
+  uint64_t* s_empty = bars + 6;    // [2]
+  uint64_t* q_full = bars + 8;
+  uint64_t* q_empty = bars + 9;
+  uint64_t* p_full = bars + 10;
+  uint64_t* pv_done = bars + 11;
+  uint64_t* o_empty = bars + 12;
+  uint64_t* drain = bars + 13;     // [2]
+  int* misc = reinterpret_cast<int*>(smem + kOffMisc);
+  uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
+  int* abort_flag = misc + 1;
+  int* found = misc + 2;           // first request of the slice, its first unit
+  int* warp_sums = misc + 4;       // [11] units, then [11] groups
+  float* red = reinterpret_cast<float*>(smem + kOffRed);
+  float* alpha_s = reinterpret_cast<float*>(smem + kOffAlpha);
+  float* sum_s = reinterpret_cast<float*>(smem + kOffSum);
+  float* max_s = reinterpret_cast<float*>(smem + kOffMax);
+
+  const int tid = threadIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], kSoftWarps);
+      mbar_init(&drain[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(p_full, kSoftWarps);
+    mbar_init(pv_done, 1);
+    mbar_init(o_empty, kSoftWarps);
+    *abort_flag = 0;
+    found[0] = p.num_requests;
+    found[1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == kLoadWarp && elect_one()) {
+    prefetch_tensor_map(&ckv_map);
+    prefetch_tensor_map(&kpe_map);
+    prefetch_tensor_map(&qn_map);
+    prefetch_tensor_map(&qp_map);
+  }
+  if (warp == kLogitWarp) tmem_alloc(tmem_base_smem, kTmemCols);
+  griddep_launch_dependents();
+  griddep_wait();
+
+  // ---- plan: total units, and the request that holds this slice's first one.
+  // Every CTA sums all requests (one or two loads a thread for ordinary
+  // batches) instead of waiting for a planning launch.
+  const int per = (p.num_requests + kThreads - 1) / kThreads;
+  const int b_lo = min(tid * per, p.num_requests), b_hi = min(b_lo + per, p.num_requests);
+  int units = 0, groups = 0;
+  bool any_bad = false, decreasing = false;
+  for (int b = b_lo; b < b_hi; ++b) {
+    bool bad;
+    const Request r = load_request(p, b, bad);
+    decreasing |= __ldg(p.cu + b + 1) < __ldg(p.cu + b);
+    units += r.groups * r.tiles;
+    groups += r.groups;
+    any_bad |= bad;
+  }
+  if (any_bad && blockIdx.x == 0) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
+  int iu = units, ig = groups;  // inclusive over the warp
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, iu, o), c = __shfl_up_sync(0xffffffffu, ig, o);
+    if (lane >= o) {
+      iu += a;
+      ig += c;
+    }
+  }
+  if (lane == 31) {
+    warp_sums[warp] = iu;
+    warp_sums[11 + warp] = ig;
+  }
+  tc_fence_before();
+  // Where cu_drafts decreases, requests could share rows, and the sums below
+  // exceed what the host checked: such a call does nothing.
+  const bool nothing = __syncthreads_or(decreasing);
+  tc_fence_after();
+  int total = 0, total_groups = 0, before = iu - units, gbefore = ig - groups;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) {
+      before += warp_sums[w];
+      gbefore += warp_sums[11 + w];
+    }
+    total += warp_sums[w];
+    total_groups += warp_sums[11 + w];
+  }
+  if (nothing) total = total_groups = units = 0;
+  const int ctas = gridDim.x;
+  const int u0 = slice_start(total, blockIdx.x, ctas), u1 = slice_start(total, blockIdx.x + 1, ctas);
+  const int slice = slice_len(total, ctas);
+  const bool keeper = !kWeights && blockIdx.x == 0;  // writes the plan that combine_kernel reads
+  if (keeper || (u0 >= before && u0 < before + units)) {
+    for (int b = b_lo; b < b_hi && !nothing; ++b) {
+      bool bad;
+      const Request r = load_request(p, b, bad);
+      const int un = r.groups * r.tiles;
+      if (u0 >= before && u0 < before + un) {
+        found[0] = b;
+        found[1] = before;
+      }
+      if (keeper) {
+        p.plan[kPlanHead + b] = before;
+        p.plan[kPlanHead + p.num_requests + b] = gbefore;
+        for (int g = 0; g < r.groups; ++g) p.plan[kPlanHead + 2 * p.num_requests + gbefore + g] = b;
+      }
+      before += un;
+      gbefore += r.groups;
+    }
+    if (keeper && tid == 0) {
+      p.plan[0] = total;
+      p.plan[1] = total_groups;
+    }
+  }
+  __syncthreads();
+
+  const uint32_t tmem_base = *tmem_base_smem;
+  const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
+  Walker<kWeights> walk(p, u0, u1, slice, found[0], found[1]);
+  Segment s;
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads
+    int i = 0, segs = 0;
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+      int pages = 0;
+      for (int t = s.t0; t < s.t1 && ok; ++t, ++i) {
+        const int k = (t - s.t0) & 31;
+        if (k == 0) pages = t + lane < s.t1 ? __ldg(row + t + lane) : 0;
+        int page = __shfl_sync(0xffffffffu, pages, k);
+        // A page outside the pool reads as zeros (a box outside the tensor
+        // is filled with them); its tokens are masked below.
+        if (page < 0 || page >= p.num_pages) page = p.num_pages;
+        const int st = i & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((i >> 1) & 1) ^ 1, wctx));
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* dst = smem + st * kTileBytes;
+          mbar_arrive_expect_tx(&kv_full[st], kTileBytes);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) tma_load_3d(dst + c * kChunkBytes, &ckv_map, &kv_full[st], c * 64, 0, page);
+          tma_load_3d(dst + 8 * kChunkBytes, &kpe_map, &kv_full[st], 0, 0, page);
+        }
+        if (t == s.t0) {
+          // The group's queries, behind its first tile.  Rows behind the
+          // request's own are another's or zeros; their columns are never
+          // written out.
+          ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (segs & 1) ^ 1, wctx));
+          if (!ok) {
+            ++i;
+            break;
+          }
+          const int row_q = s.r.row0 * p.heads + s.group * kRows;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(q_full, kTileBytes);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) tma_load_2d(q_mem + c * kChunkBytes, &qn_map, q_full, c * 64, row_q);
+            tma_load_2d(q_mem + 8 * kChunkBytes, &qp_map, q_full, 0, row_q);
+          }
+          ++segs;
+        }
+      }
+    }
+    // Copies still in flight (after an abort) land before the CTA exits: the
+    // last one of each stage and of Q, whose phases nothing refills.
+    if (lane == 0) {
+      if (i >= 1) mbar_drain(&kv_full[(i - 1) & 1], ((i - 1) >> 1) & 1, p.status);
+      if (i >= 2) mbar_drain(&kv_full[(i - 2) & 1], ((i - 2) >> 1) & 1, p.status);
+      if (segs >= 1) mbar_drain(q_full, (segs - 1) & 1, p.status);
+    }
+  } else if (warp == kLogitWarp) {
+    // ------------------------------------------------------------ S^T = K Q^T
+    const uint64_t k_desc = sdesc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t q_desc = sdesc_sw128(smem_u32(q_mem), 16, 1024);
+    int i = 0, segs = 0;
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      for (int t = s.t0; t < s.t1; ++t, ++i) {
+        const int st = i & 1;
+        if (t == s.t0) ok = mbar_wait(q_full, segs & 1, wctx);
+        ok = ok && mbar_wait(&kv_full[st], (i >> 1) & 1, wctx);
+        ok = ok && mbar_wait(&s_empty[st], ((i >> 1) & 1) ^ 1, wctx);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t a = k_desc + st * (kTileBytes >> 4);
+          const uint32_t d = tmem_base + kColS + 64u * st;
+#pragma unroll
+          for (int k = 0; k < 4 * kChunks; ++k)  // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
+            umma_bf16(d, a + (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2,
+                      q_desc + (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2, kIdescS, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[st]);
+          if (t == s.t1 - 1) umma_commit(q_empty);
+          if (kWeights) umma_commit(&kv_empty[st]);
+        }
+        __syncwarp();
+      }
+      ++segs;
+    }
+    if (elect_one()) {
+      umma_commit(&drain[0]);
+      mbar_drain(&drain[0], 0, p.status);
+    }
+    __syncwarp();
+  } else if (warp == kValueWarp) {
+    // ------------------------------------------------------------ O^T += V^T P^T
+    if constexpr (!kWeights) {
+      const uint64_t v_desc = sdesc_sw128(smem_u32(smem), kChunkBytes, 1024);
+      const uint64_t p_desc = sdesc_sw128(smem_u32(p_mem), kChunkBytes, 1024);
+      int i = 0, segs = 0;
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1;
+          ok = mbar_wait(p_full, i & 1, wctx);
+          if (t == s.t0) ok = ok && mbar_wait(o_empty, (segs & 1) ^ 1, wctx);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t more = t == s.t0 ? 0u : 1u;
+          if (elect_one()) {
+            const uint64_t a = v_desc + st * (kTileBytes >> 4);
+#pragma unroll
+            for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)  // 128 dims are two pieces; a K16 step is 16 token rows of 128 bytes
+                umma_bf16(tmem_base + kColO + 64u * mb, a + mb * (2 * kChunkBytes >> 4) + kk * (2048 >> 4),
+                          p_desc + kk * (2048 >> 4), kIdescO, kk > 0 ? 1u : more);
+            umma_commit(&kv_empty[st]);
+            umma_commit(pv_done);
+          }
+          __syncwarp();
+        }
+        ++segs;
+      }
+      if (elect_one()) {
+        umma_commit(&drain[1]);
+        mbar_drain(&drain[1], 0, p.status);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    // Set `set` of four warps has the columns (query rows) 32 set .. +31 of
+    // S^T; in it, warp sp reads tokens 16 sp .. +15 (the M = 64 accumulator
+    // has them in lanes 0-15 of its sub-partition), thread (lane) the tokens
+    // r0 and r0 + 8 and the columns col(k), k = 0..7.
+    const int set = warp >> 2, sp = warp & 3;
+    const int r0 = 16 * sp + (lane >> 2);
+    const int c0 = 32 * set + 2 * (lane & 3);
+    auto col = [&](int k) { return c0 + 8 * (k >> 1) + (k & 1); };
+    const uint32_t lane_base = static_cast<uint32_t>(32 * sp) << 16;
+    const int e = tid & 127;  // thread of the set
+    int i = 0;
+    bool ok = true;
+
+    if constexpr (kWeights) {
+      // What no unit writes: the tiles behind every request's tokens, spread
+      // over all CTAs.
+      if (p.acc_out != p.acc) {
+        const int64_t tiles = static_cast<int64_t>(p.num_requests) * p.max_pages;
+        for (int64_t q = static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6); q < tiles; q += 4 * ctas) {
+          const int b = static_cast<int>(q / p.max_pages), t = static_cast<int>(q % p.max_pages);
+          bool bad;
+          if (!nothing && t < load_request(p, b, bad).tiles) continue;
+          const int64_t at = static_cast<int64_t>(t) * kTok + (tid & 63);
+          p.acc_out[b * p.acc_out_stride + at] = p.acc[b * p.acc_stride + at];
+        }
+      }
+      while (walk.next(s)) {
+        float lse[8];
+        int draft[8];
+        uint32_t live = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = s.group * kRows + col(k);
+          const bool in = row < s.r.rows;
+          lse[k] = in ? __ldg(p.lse_in + static_cast<int64_t>(s.r.row0) * p.heads + row) : 0.f;
+          draft[k] = in ? row / p.heads : 0;
+          if (in && lse[k] != -INFINITY) live |= 1u << k;  // a row that saw nothing gives nothing
+        }
+        const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+        int next_page = __ldg(bt + s.t0);
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1;
+          const int page = next_page;
+          if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
+          uint32_t see0 = live, see1 = live;
+          if (page < 0 || page >= p.num_pages) {
+            see0 = see1 = 0;
+            if (e == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
+          } else if ((t + 1) * kTok > s.r.prefix) {
+            const int pos = t * kTok + r0;
+            if (pos >= s.r.prefix) see0 &= visible_columns(p, s, pos, draft);
+            if (pos + 8 >= s.r.prefix) see1 &= visible_columns(p, s, pos + 8, draft);
+          }
+          ok = ok && mbar_wait(&s_full[st], (i >> 1) & 1, wctx);
+          tc_fence_after();
+          float v[16];
+          tmem_ld_16x32_wait(tmem_base + lane_base + kColS + 64u * st + 32u * set, v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[st]);
+          float w0 = 0.f, w1 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int f = 4 * (k >> 1) + (k & 1);
+            const float a = ex2_approx(fmaf(v[f], p.scale_log2, -lse[k]));
+            const float c = ex2_approx(fmaf(v[f + 2], p.scale_log2, -lse[k]));
+            w0 += (see0 >> k) & 1 ? a : 0.f;
+            w1 += (see1 >> k) & 1 ? c : 0.f;
+          }
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+          w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
+          w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+          w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
+          if ((lane & 3) == 0) {
+            // The same thread adds a token's groups one after the other.
+            float* to = sums + (set * kSumTiles + (t - s.t0)) * kTok + r0;
+            to[0] = s.first_group ? w0 : to[0] + w0;
+            to[8] = s.first_group ? w1 : to[8] + w1;
+          }
+        }
+        if (s.last_group) {
+          named_barrier_sync(3, 32 * kSoftWarps);
+          for (int q = tid; q < (s.t1 - s.t0) * kTok; q += 32 * kSoftWarps) {
+            const int64_t at = static_cast<int64_t>(s.t0) * kTok + q;
+            p.acc_out[s.b * p.acc_out_stride + at] =
+                p.acc[s.b * p.acc_stride + at] + (sums[q] + sums[kSumTiles * kTok + q]);
+          }
+          named_barrier_sync(3, 32 * kSoftWarps);
+        }
+      }
+    } else {
+      // Online softmax in base 2.  The running max m[k] of a column is the
+      // same in every thread that has it.  It moves only when some token of
+      // the tile exceeds it by more than kRescaleThreshold (always at a
+      // segment's first tile), which one OR-barrier per tile tells the set;
+      // only then is the tile's max reduced over the tokens and O rescaled.
+      // P <= 2^8 then, and l adds P in fp32.  P is rounded to bf16 for the
+      // MMA (off by at most 2^-9 of itself, independently per token; l uses
+      // the unrounded values), as any bf16 tensor-core product needs.
+      while (walk.next(s)) {
+        float m[8], l[8];
+        int draft[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m[k] = -INFINITY;
+          l[k] = 0.f;
+          const int row = s.group * kRows + col(k);
+          draft[k] = row < s.r.rows ? row / p.heads : 0;
+        }
+        const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+        int next_page = __ldg(bt + s.t0);
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1;
+          const int page = next_page;
+          if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
+          uint32_t see0 = 0xffu, see1 = 0xffu;
+          const bool tail = (t + 1) * kTok > s.r.prefix;
+          if (page < 0 || page >= p.num_pages) {
+            see0 = see1 = 0;
+            if (e == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
+          } else if (tail) {
+            const int pos = t * kTok + r0;
+            if (pos >= s.r.prefix) see0 = visible_columns(p, s, pos, draft);
+            if (pos + 8 >= s.r.prefix) see1 = visible_columns(p, s, pos + 8, draft);
+          }
+          ok = ok && mbar_wait(&s_full[st], (i >> 1) & 1, wctx);
+          tc_fence_after();
+          float v[16];
+          tmem_ld_16x32_wait(tmem_base + lane_base + kColS + 64u * st + 32u * set, v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[st]);
+          float x0[8], x1[8];
+          bool need = false;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int f = 4 * (k >> 1) + (k & 1);
+            x0[k] = (see0 >> k) & 1 ? v[f] * p.scale_log2 : -INFINITY;
+            x1[k] = (see1 >> k) & 1 ? v[f + 2] * p.scale_log2 : -INFINITY;
+            const float over = m[k] + kRescaleThreshold;
+            need |= x0[k] > over || x1[k] > over;
+          }
+          if (named_barrier_or(1 + set, 128, need)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float mt = fmaxf(x0[k], x1[k]);
+              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
+              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+              if (lane < 4) red[kRows * sp + col(k)] = mt;
+            }
+            named_barrier_sync(1 + set, 128);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float* r = red + col(k);
+              const float mt = fmaxf(fmaxf(r[0], r[kRows]), fmaxf(r[2 * kRows], r[3 * kRows]));
+              float alpha = 1.f;
+              if (mt > m[k] + kRescaleThreshold) {
+                alpha = exp2f(m[k] - mt);  // 0 when m was -inf
+                m[k] = mt;
+              }
+              l[k] *= alpha;
+              if (sp == 0 && lane < 4) alpha_s[col(k)] = alpha;
+            }
+            named_barrier_sync(1 + set, 128);
+            if (t > s.t0) {
+              // O holds PV(i - 1) before it is rescaled.
+              ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+              tc_fence_after();
+#pragma unroll 1
+              for (int mb = 0; mb < 4; ++mb) {
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t at = tmem_base + lane_base + kColO + 64u * mb + 32u * set + 16u * h;
+                  float o[16];
+                  tmem_ld16(at, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int c = 0; c < 16; ++c) o[c] *= alpha_s[32 * set + 16 * h + c];
+                  tmem_st16(at, o);
+                }
+              }
+              tmem_wait_st();
+            }
+          }
+          if (tail) {
+            // Cache rows at and behind the prefix may be masked and hold
+            // anything; a zero weight would still turn an infinity or NaN
+            // among them into NaN.  The logits have been read (S^T is done),
+            // so such values are zeroed in the V tile; a row that does see
+            // one has its NaN from the logit.
+            ok = ok && mbar_wait(&kv_full[st], (i >> 1) & 1, wctx);
+            const int from = s.r.prefix > t * kTok ? s.r.prefix - t * kTok : 0;
+            for (int q = tid; q < (kTok - from) * 64; q += 32 * kSoftWarps) {
+              // 16-byte piece q & 7 of row from + (q >> 6) in piece (q >> 3) & 7
+              uint4* at = reinterpret_cast<uint4*>(smem + st * kTileBytes + ((q >> 3) & 7) * kChunkBytes +
+                                                   (from + (q >> 6)) * 128 + (q & 7) * 16);
+              uint4 w = *at;
+              uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+              bool changed = false;
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                if ((ww[z] & 0x7F80u) == 0x7F80u) {
+                  ww[z] &= 0xFFFF0000u;
+                  changed = true;
+                }
+                if ((ww[z] & 0x7F800000u) == 0x7F800000u) {
+                  ww[z] &= 0x0000FFFFu;
+                  changed = true;
+                }
+              }
+              if (changed) *at = w;
+            }
+          }
+          uint32_t p0[4], p1[4];
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            float a[2], c[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // m == -inf: the column has seen nothing yet and every x is
+              // -inf (weight 0) or NaN (kept).
+              const float mm = m[k + h] == -INFINITY ? 0.f : m[k + h];
+              a[h] = ex2_approx(x0[k + h] - mm);
+              c[h] = ex2_approx(x1[k + h] - mm);
+              l[k + h] += a[h] + c[h];
+            }
+            const __nv_bfloat162 pa = __floats2bfloat162_rn(a[0], a[1]), pc = __floats2bfloat162_rn(c[0], c[1]);
+            p0[k >> 1] = *reinterpret_cast<const uint32_t*>(&pa);
+            p1[k >> 1] = *reinterpret_cast<const uint32_t*>(&pc);
+          }
+          // P was last read by PV(i - 1).
+          if (i > 0) ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+          {
+            // One 128-byte row per token, 16-byte pieces swizzled by token & 7
+            // (the same for r0 and r0 + 8): a warp's stores meet no bank twice.
+            uint8_t* at = p_mem + r0 * 128 + 4 * (lane & 3);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int piece = ((4 * set + j) ^ (r0 & 7)) << 4;
+              *reinterpret_cast<uint32_t*>(at + piece) = p0[j];
+              *reinterpret_cast<uint32_t*>(at + 1024 + piece) = p1[j];
+            }
+          }
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full);
+        }
+
+        // ---- the segment's end: denominators over the tokens, then O.
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float v = l[k];
+          v += __shfl_xor_sync(0xffffffffu, v, 4);
+          v += __shfl_xor_sync(0xffffffffu, v, 8);
+          v += __shfl_xor_sync(0xffffffffu, v, 16);
+          if (lane < 4) {
+            red[kRows * sp + col(k)] = v;
+            if (sp == 0) max_s[col(k)] = m[k];
+          }
+        }
+        named_barrier_sync(1 + set, 128);
+        const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kRows;
+        const int rows = min(kRows, s.r.rows - s.group * kRows);  // of the group
+        const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + s.slot;
+        if (e < 32) {
+          const int c = 32 * set + e;
+          const float sum = (red[c] + red[kRows + c]) + (red[2 * kRows + c] + red[3 * kRows + c]);
+          if (s.whole) {
+            sum_s[c] = sum == 0.f ? 0.f : 1.f / sum;
+            if (c < rows) p.lse_out[row_q + c] = sum == 0.f ? -INFINITY : max_s[c] + log2f(sum);
+          } else {
+            *reinterpret_cast<float2*>(p.part_ml + (rec * kRows + c) * 2) = make_float2(max_s[c], sum);
+          }
+        }
+        ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+        named_barrier_sync(1 + set, 128);
+        tc_fence_after();
+#pragma unroll 1
+        for (int mb = 0; mb < 4; ++mb) {
+          const int dim = 128 * mb + 32 * sp + lane;
+          float o[32];
+          tmem_ld32_wait(tmem_base + lane_base + kColO + 64u * mb + 32u * set, o);
+          if (s.whole) {
+            // Neighbouring lanes swap halves, so that each stores two dims
+            // of one row.
+            const bool odd = lane & 1;
+            __nv_bfloat16* out = p.out + row_q * kCkv + (dim & ~1);
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const float a = o[c] * sum_s[32 * set + c], b = o[c + 1] * sum_s[32 * set + c + 1];
+              const float got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+              const int row = 32 * set + c + (odd ? 1 : 0);
+              if (row < rows)
+                *reinterpret_cast<__nv_bfloat162*>(out + static_cast<int64_t>(row) * kCkv) =
+                    odd ? __floats2bfloat162_rn(got, b) : __floats2bfloat162_rn(a, got);
+            }
+          } else {
+            float* to = p.part_o + rec * kPartFloats + 32 * set * kCkv + dim;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (32 * set + c < rows) to[c * kCkv] = o[c];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kLogitWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// Joins the records of a group that several slices share: per row
+//   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L,
+// in slice order.  Block (group, y) has rows 4y .. 4y + 3, a thread four dims
+// of each.
+constexpr int kJoinRows = 4;
+constexpr int kMaxCtas = 256;
+
+__global__ void __launch_bounds__(128) combine_kernel(const Params p, int ctas) {
+  griddep_wait();
+  __shared__ int recs[2 * kMaxCtas];
+  __shared__ float weight[kJoinRows][2 * kMaxCtas];
+  __shared__ int warp_count[4];
+  const int total = p.plan[0];
+  const int gi = blockIdx.x;
+  if (gi >= p.plan[1]) return;
+  const int b = p.plan[kPlanHead + 2 * p.num_requests + gi];
+  const int first = p.plan[kPlanHead + b];
+  const int group = gi - p.plan[kPlanHead + p.num_requests + b];
+  bool bad;
+  const Request r = load_request(p, b, bad);
+  const int rows = min(kRows, r.rows - group * kRows);
+  const int y0 = blockIdx.y * kJoinRows;
+  if (y0 >= rows) return;
+  const int chunks = chunks_of(r, slice_len(total, ctas));
+  if (chunks == 1) {
+    const int a = first + group * r.tiles;
+    if (slice_of(total, a, ctas) == slice_of(total, a + r.tiles - 1, ctas)) return;  // written whole
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // The records that belong to this group, in slice order.
+  const int c_lo = slice_of(total, first, ctas), c_hi = slice_of(total, first + r.groups * r.tiles - 1, ctas);
+  int count = 0;
+  for (int base = 2 * c_lo; base < 2 * (c_hi + 1); base += 128) {
+    const int cand = base + tid, c = cand >> 1;
+    bool mine = false;
+    if (c <= c_hi) {
+      const int u0 = slice_start(total, c, ctas), u1 = slice_start(total, c + 1, ctas);
+      const int u = (cand & 1) ? u1 - 1 : u0;
+      if (u0 < u1 && u >= first && u < first + r.groups * r.tiles) {
+        const Place q = place_of(r, chunks, u - first);
+        mine = q.group == group;
+        if (cand & 1)  // the last piece, unless it is the first one too
+          mine = mine && first + r.groups * q.t0 + q.group * (q.t1 - q.t0) > u0;
+      }
+    }
+    const unsigned int votes = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) warp_count[warp] = __popc(votes);
+    __syncthreads();
+    int at = count + __popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < 4; ++w) {
+      if (w < warp) at += warp_count[w];
+      count += warp_count[w];
+    }
+    if (mine) recs[at] = cand;
+    __syncthreads();
+  }
+  {
+    // Warp w: the weights of row y0 + w.
+    const int row = y0 + warp;
+    float M = -INFINITY, L = 0.f;
+    if (row < rows) {
+      for (int k = lane; k < count; k += 32)
+        M = fmaxf(M, __ldcg(p.part_ml + (static_cast<int64_t>(recs[k]) * kRows + row) * 2));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      for (int k = lane; k < count; k += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(
+            p.part_ml + (static_cast<int64_t>(recs[k]) * kRows + row) * 2));
+        const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        L = fmaf(ml.y, w, L);
+        weight[warp][k] = w;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      __syncwarp();
+      for (int k = lane; k < count; k += 32) weight[warp][k] *= inv;
+      if (lane == 0)
+        p.lse_out[static_cast<int64_t>(r.row0) * p.heads + group * kRows + row] =
+            L == 0.f ? -INFINITY : M + log2f(L);
+    }
+  }
+  __syncthreads();
+  float4 acc[kJoinRows];
+#pragma unroll
+  for (int y = 0; y < kJoinRows; ++y) acc[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int k = 0; k < count; ++k) {
+    const float4* src = reinterpret_cast<const float4*>(p.part_o + static_cast<int64_t>(recs[k]) * kPartFloats) + tid;
+#pragma unroll
+    for (int y = 0; y < kJoinRows; ++y) {
+      if (y0 + y < rows) {
+        const float4 v = __ldcg(src + (y0 + y) * (kCkv / 4));
+        const float w = weight[y][k];
+        acc[y].x = fmaf(v.x, w, acc[y].x);
+        acc[y].y = fmaf(v.y, w, acc[y].y);
+        acc[y].z = fmaf(v.z, w, acc[y].z);
+        acc[y].w = fmaf(v.w, w, acc[y].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int y = 0; y < kJoinRows; ++y) {
+    if (y0 + y < rows) {
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc[y].x, acc[y].y), __floats2bfloat162_rn(acc[y].z, acc[y].w)};
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(r.row0) * p.heads + group * kRows + y0 + y) * kCkv +
+                                4 * tid) = *reinterpret_cast<const uint2*>(h);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+std::once_flag g_once[64];
+int g_status[64];
+
+struct Layout {
+  size_t part_ml, part_o, plan, bytes;
+};
+
+// Upper bound of the groups of all requests: sum ceil(n_b H / 64).
+inline int64_t groups_bound(int64_t drafts, int64_t heads, int64_t requests) {
+  return drafts * heads / kRows + requests;
+}
+
+inline Layout layout(int64_t drafts, int64_t heads, int64_t requests, int sms) {
+  Layout a;
+  a.part_ml = kWorkspaceHeader;
+  a.part_o = a.part_ml + static_cast<size_t>(2 * sms) * kRows * 2 * sizeof(float);
+  a.plan = a.part_o + static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
+  // Rounded up generously, so that ordinary batches all need the same bytes
+  // and a workspace does not move between them.
+  size_t words = kPlanHead + 2 * static_cast<size_t>(requests) + static_cast<size_t>(groups_bound(drafts, heads, requests));
+  words = (words + 65535) / 65536 * 65536;
+  a.bytes = a.plan + words * sizeof(int);
+  return a;
+}
+
+inline bool sizes_ok(int64_t drafts, int64_t heads, int64_t requests) {
+  return drafts >= 0 && heads >= 1 && heads <= 128 && requests >= 0 && requests <= kMaxRequests &&
+         drafts * heads <= (1 << 28);
+}
+
+int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64_t ckv_page, int64_t ckv_row,
+                    const void* kpe, int64_t kpe_page, int64_t kpe_row, int64_t num_pages,
+                    const int32_t* prefix_lens, const int32_t* block_table, const int32_t* cu, const int64_t* mask,
+                    int32_t requests, int32_t drafts, int32_t heads, int32_t max_pages, int32_t mask_words,
+                    float sm_scale, void* workspace, size_t workspace_bytes, bool records, DeviceInfo* info,
+                    Params* prm, CUtensorMap (&maps)[4]) {
+  if (!q_nope || !q_pe || !ckv || !kpe || !prefix_lens || !block_table || !cu || !mask || !workspace)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (num_pages < 1 || num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || mask_words < 1 ||
+      mask_words > 64)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (groups_bound(drafts, heads, requests) * max_pages > 0x7FFFFFFF) return DSA_ERR_INVALID_ARGUMENT;
+  if (ckv_row < kCkv * 2 || kpe_row < kKpe * 2 || ckv_page < 0 || kpe_page < 0) return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(workspace) ||
+      ((ckv_page | ckv_row | kpe_page | kpe_row) & 15))
+    return DSA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(prefix_lens) | reinterpret_cast<uintptr_t>(block_table) |
+       reinterpret_cast<uintptr_t>(cu)) & 3u)
+    return DSA_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(mask) & 7u) return DSA_ERR_MISALIGNED;
+  int st = current_device_info(info);
+  if (st != DSA_OK) return st;
+  if (static_cast<size_t>(kSmemBytes) > info->max_smem_optin || info->num_sms > kMaxCtas)
+    return DSA_ERR_UNSUPPORTED_DEVICE;
+  const Layout a = layout(drafts, heads, requests, info->num_sms);
+  if (workspace_bytes < (records ? a.bytes : kWorkspaceHeader)) return DSA_ERR_WORKSPACE_TOO_SMALL;
+  std::call_once(g_once[info->device], [&]() {
+    g_status[info->device] =
+        cudaFuncSetAttribute(tree_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) ==
+                    cudaSuccess &&
+                cudaFuncSetAttribute(tree_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) ==
+                    cudaSuccess
+            ? DSA_OK
+            : DSA_ERR_CUDA;
+  });
+  if (g_status[info->device] != DSA_OK) return g_status[info->device];
+  const uint64_t rows = static_cast<uint64_t>(drafts) * heads;
+  if ((st = encode_tmap_3d(&maps[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ckv, kCkv, kTok, num_pages, ckv_row, ckv_page,
+                           64, kTok)) != DSA_OK)
+    return st;
+  if ((st = encode_tmap_3d(&maps[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kpe, kKpe, kTok, num_pages, kpe_row, kpe_page,
+                           64, kTok)) != DSA_OK)
+    return st;
+  if ((st = encode_tmap_2d(&maps[2], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, q_nope, kCkv, rows, kCkv * 2, 64, kRows)) !=
+      DSA_OK)
+    return st;
+  if ((st = encode_tmap_2d(&maps[3], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, q_pe, kKpe, rows, kKpe * 2, 64, kRows)) !=
+      DSA_OK)
+    return st;
+  *prm = Params{};
+  prm->prefix_lens = prefix_lens;
+  prm->block_table = block_table;
+  prm->cu = cu;
+  prm->mask = reinterpret_cast<const long long*>(mask);
+  prm->num_requests = requests;
+  prm->num_drafts = drafts;
+  prm->heads = heads;
+  prm->max_pages = max_pages;
+  prm->mask_words = mask_words;
+  prm->num_pages = static_cast<int>(num_pages);
+  prm->scale_log2 = sm_scale * 1.4426950408889634f;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  prm->status = reinterpret_cast<unsigned int*>(ws);
+  prm->wait_limit_ns = kWaitLimitNs;
+  if (records) {
+    prm->part_ml = reinterpret_cast<float*>(ws + a.part_ml);
+    prm->part_o = reinterpret_cast<float*>(ws + a.part_o);
+    prm->plan = reinterpret_cast<int*>(ws + a.plan);
+  }
+  return DSA_OK;
+}
+
+}  // namespace tree
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" size_t dsa_tree_attention_workspace_bytes(int32_t num_drafts, int32_t num_heads, int32_t num_requests) {
+  if (!tree::sizes_ok(num_drafts, num_heads, num_requests)) return 0;
+  DeviceInfo info;
+  // Without a usable device, size for the largest SM count of the family.
+  const int sms = current_device_info(&info) == DSA_OK ? info.num_sms : 160;
+  return tree::layout(num_drafts, num_heads, num_requests, sms).bytes;
+}
+
+extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const void* ckv_cache,
+                                      int64_t ckv_page_bytes, int64_t ckv_row_bytes, const void* kpe_cache,
+                                      int64_t kpe_page_bytes, int64_t kpe_row_bytes, int64_t num_pages,
+                                      const int32_t* prefix_lens, const int32_t* block_table,
+                                      const int32_t* cu_drafts, const int64_t* tree_mask, int32_t num_requests,
+                                      int32_t num_drafts, int32_t num_heads, int32_t max_pages, int32_t mask_words,
+                                      float sm_scale, void* output, float* lse, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  if (!tree::sizes_ok(num_drafts, num_heads, num_requests)) return DSA_ERR_INVALID_ARGUMENT;
+  if (num_drafts == 0 || num_requests == 0) return DSA_OK;
+  if (!output || !lse) return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(output) || (reinterpret_cast<uintptr_t>(lse) & 3u)) return DSA_ERR_MISALIGNED;
+  DeviceInfo info;
+  tree::Params prm;
+  CUtensorMap maps[4];
+  const int st = tree::check_and_setup(q_nope, q_pe, ckv_cache, ckv_page_bytes, ckv_row_bytes, kpe_cache,
+                                       kpe_page_bytes, kpe_row_bytes, num_pages, prefix_lens, block_table, cu_drafts,
+                                       tree_mask, num_requests, num_drafts, num_heads, max_pages, mask_words, sm_scale,
+                                       workspace, workspace_bytes, true, &info, &prm, maps);
+  if (st != DSA_OK) return st;
+  prm.out = static_cast<__nv_bfloat16*>(output);
+  prm.lse_out = lse;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (launch_programmatic(tree::tree_kernel<false>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
+                          maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  const unsigned int groups =
+      static_cast<unsigned int>(tree::groups_bound(num_drafts, num_heads, num_requests));
+  if (launch_programmatic(tree::combine_kernel, dim3(groups, tree::kRows / tree::kJoinRows), dim3(128), 0, s, prm,
+                          info.num_sms) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  return DSA_OK;
+}
+
+extern "C" int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const void* ckv_cache,
+                                    int64_t ckv_page_bytes, int64_t ckv_row_bytes, const void* kpe_cache,
+                                    int64_t kpe_page_bytes, int64_t kpe_row_bytes, int64_t num_pages,
+                                    const int32_t* prefix_lens, const int32_t* block_table, const int32_t* cu_drafts,
+                                    const int64_t* tree_mask, int32_t num_requests, int32_t num_drafts,
+                                    int32_t num_heads, int32_t max_pages, int32_t mask_words, float sm_scale,
+                                    const float* lse, const float* acc, int64_t acc_stride, float* acc_out,
+                                    int64_t acc_out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!tree::sizes_ok(num_drafts, num_heads, num_requests)) return DSA_ERR_INVALID_ARGUMENT;
+  if (num_requests == 0) return DSA_OK;
+  if (!lse || !acc || !acc_out) return DSA_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(acc) | reinterpret_cast<uintptr_t>(acc_out)) & 3u)
+    return DSA_ERR_MISALIGNED;
+  if (max_pages < 1 || acc_stride < static_cast<int64_t>(max_pages) * tree::kTok ||
+      acc_out_stride < static_cast<int64_t>(max_pages) * tree::kTok || (acc == acc_out && acc_stride != acc_out_stride))
+    return DSA_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (num_drafts == 0) {  // nothing to add
+    if (acc != acc_out &&
+        cudaMemcpy2DAsync(acc_out, acc_out_stride * 4, acc, acc_stride * 4, static_cast<size_t>(max_pages) * tree::kTok * 4,
+                          num_requests, cudaMemcpyDeviceToDevice, s) != cudaSuccess)
+      return DSA_ERR_CUDA;
+    return DSA_OK;
+  }
+  DeviceInfo info;
+  tree::Params prm;
+  CUtensorMap maps[4];
+  const int st = tree::check_and_setup(q_nope, q_pe, ckv_cache, ckv_page_bytes, ckv_row_bytes, kpe_cache,
+                                       kpe_page_bytes, kpe_row_bytes, num_pages, prefix_lens, block_table, cu_drafts,
+                                       tree_mask, num_requests, num_drafts, num_heads, max_pages, mask_words, sm_scale,
+                                       workspace, workspace_bytes, false, &info, &prm, maps);
+  if (st != DSA_OK) return st;
+  prm.lse_in = lse;
+  prm.acc = acc;
+  prm.acc_stride = acc_stride;
+  prm.acc_out = acc_out;
+  prm.acc_out_stride = acc_out_stride;
+  if (launch_programmatic(tree::tree_kernel<true>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
+                          maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  return DSA_OK;
+}

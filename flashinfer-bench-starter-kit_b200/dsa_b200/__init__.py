@@ -12,7 +12,7 @@ The kernels live in libdsa_b200.so (C ABI: include/dsa_b200.h); there is no
 CPU or library fallback.
 """
 
-from . import attention, indexer, workloads  # noqa: F401
+from . import attention, evict, indexer, tree, workloads  # noqa: F401
 from ._native import DsaError, LIB_PATH  # noqa: F401
 
-__all__ = ["attention", "indexer", "workloads", "DsaError", "LIB_PATH"]
+__all__ = ["attention", "evict", "indexer", "tree", "workloads", "DsaError", "LIB_PATH"]

@@ -14,6 +14,8 @@ import torch
 
 LIB_PATH = pathlib.Path(__file__).resolve().with_name("libdsa_b200.so")
 
+WORKSPACE_HEADER = 256  # bytes at the start of every workspace; the status word is the first of them
+
 DSA_OK = 0
 DEV_BAD_SEQ_LEN = 0x1
 DEV_BAD_PAGE = 0x2
@@ -23,6 +25,10 @@ DEV_STALE_WORKSPACE = 0x10
 
 # name -> (restype, argtypes); every symbol include/dsa_b200.h declares.
 _P = ctypes.c_void_p
+# q_nope, q_pe, ckv with its pitches, kpe with its, pages, prefix_lens, block_table, cu_drafts, tree_mask,
+# five sizes, sm_scale
+_TREE = [_P, _P, _P, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, _P, _P,
+         _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_float]
 SIGNATURES = {
     "dsa_b200_abi_version": (ctypes.c_int, []),
     "dsa_b200_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -43,6 +49,10 @@ SIGNATURES = {
     "dsa_indexer_prefill_run": (ctypes.c_int, [_P, _P, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_int32, _P, _P, ctypes.c_size_t,
                                                _P]),
+    "dsa_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "dsa_tree_attention_run": (ctypes.c_int, _TREE + [_P, _P, _P, ctypes.c_size_t, _P]),
+    "dsa_tree_weights_run": (ctypes.c_int, _TREE + [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_size_t,
+                                                    _P]),
     "dsa_b200_test_inject": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
 }
 

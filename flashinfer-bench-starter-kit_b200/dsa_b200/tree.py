@@ -1,0 +1,191 @@
+"""Attention for a tree of drafted tokens over the paged ckv / kpe cache
+(speculative decoding; destination-passing style).
+
+    run(q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts,
+        tree_mask, sm_scale, output, lse) -> None
+
+Request r has ``prefix_lens[r]`` cached tokens and the drafts
+``cu_drafts[r] .. cu_drafts[r+1]-1`` (rows of ``q_nope`` / ``q_pe``), whose own
+ckv / kpe rows are in the cache already, behind the prefix: the j-th draft at
+position ``prefix_lens[r] + j`` of the request's ``block_table`` row.  A draft
+sees the whole prefix and the drafts whose bits its row of ``tree_mask`` has
+(``masks_from_parents`` makes the rows of a tree).  One draft per request with
+its own bit set is plain dense decoding.
+
+Unlike ``dsa_b200.attention.run``, which reads 2048 selected slots, this reads
+every visible token.  ``lse`` is the base-2 log-sum-exp of the scaled logits;
+a row that sees nothing yields output 0 and lse -inf.
+
+* Any 1 to 128 heads; up to ``64 * tree_mask.shape[1]`` drafts per request.
+* ``ckv_cache`` ``[pages, 64, 512]`` and ``kpe_cache`` ``[pages, 64, 64]`` may be
+  strided (pages and rows at multiples of 16 bytes), such as two slices of one
+  ``[pages, 64, 576]`` cache; they are never copied.
+* Cache rows that a mask hides may hold anything, infinities and NaN included.
+* Query rows outside of ``[cu_drafts[0], cu_drafts[-1])`` are left as they are.
+* Lengths stay on the device; every launch goes to the current stream and can
+  be captured into a CUDA graph (make one call on the capturing stream first,
+  so that its workspace exists).  Calls that overlap need different streams,
+  and graphs captured on one stream must not be replayed at the same time.
+* Lengths that do not fit, page ids outside the pool and drafts that do not
+  fit the mask set a sticky status bit (``device_status``), as for the other
+  operators; with ``DSA_B200_CHECK=1`` each call synchronises and raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import os
+
+import torch
+
+from . import _native, workspace
+
+PAGE_SIZE = 64
+DIM_CKV = 512
+DIM_KPE = 64
+MAX_HEADS = 128
+MAX_MASK_WORDS = 64
+
+_CHECK = os.environ.get("DSA_B200_CHECK", "0") not in ("", "0")
+_ws_bytes: dict = {}  # (device index, drafts, heads, requests) -> workspace bytes
+
+
+def masks_from_parents(parents) -> list:
+    """``tree_mask`` rows (lists of signed 64-bit words) of one request's drafts:
+    ``parents[j]`` is the index of draft j's parent, below j, or -1 if it
+    follows the prefix directly.  Every draft sees its ancestors and itself."""
+    bits = []
+    for j, par in enumerate(parents):
+        if not -1 <= par < j:
+            raise ValueError(f"parents[{j}] is {par}: a parent comes before its children")
+        bits.append((1 << j) | (bits[par] if par >= 0 else 0))
+    words = max(1, (len(bits) + 63) // 64)
+    rows = [[(m >> (64 * w)) & ((1 << 64) - 1) for w in range(words)] for m in bits]
+    return [[w - (1 << 64) if w >> 63 else w for w in row] for row in rows]
+
+
+def _strides(name: str, t: torch.Tensor, width: int, fail) -> tuple:
+    """(page stride, row stride) in bytes of a [pages, 64, width] bf16 cache."""
+    if t.dim() != 3 or t.shape[1] != PAGE_SIZE or t.shape[2] != width:
+        fail(f"{name} must be [pages, {PAGE_SIZE}, {width}], got {tuple(t.shape)}")
+    if t.shape[0] < 1:
+        fail(f"{name} has no pages")
+    page, row, col = t.stride()
+    if t.shape[0] == 1:  # a stride that is never taken
+        page = PAGE_SIZE * row
+    if col != 1 or row < width or page < row or row % 8 or page % 8 or t.data_ptr() % 16:
+        fail(f"{name} must have contiguous rows, 16-byte aligned (strides {t.stride()})")
+    return 2 * page, 2 * row
+
+
+def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts, tree_mask,
+               more) -> tuple:
+    """The checks shared with ``dsa_b200.evict.accumulate``; returns the sizes and
+    the arguments of the C entry points up to ``mask_words``, and the tensors
+    that hold them."""
+    dev = q_nope.device
+    if dev.type != "cuda":
+        fail("tensors must be on a CUDA device")
+    for name, t in (("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache),
+                    ("prefix_lens", prefix_lens), ("block_table", block_table),
+                    ("cu_drafts", cu_drafts), ("tree_mask", tree_mask), *more):
+        if t.device != dev:
+            fail(f"{name} is on {t.device}, expected {dev}")
+    for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
+        if t.dtype != torch.bfloat16:
+            fail(f"{name} must be bfloat16, got {t.dtype}")
+    if q_nope.dim() != 3 or q_nope.shape[2] != DIM_CKV or not 1 <= q_nope.shape[1] <= MAX_HEADS:
+        fail(f"q_nope must be [T, heads <= {MAX_HEADS}, {DIM_CKV}], got {tuple(q_nope.shape)}")
+    T, H = q_nope.shape[:2]
+    if q_pe.shape != (T, H, DIM_KPE):
+        fail(f"q_pe must be [{T}, {H}, {DIM_KPE}]")
+    ckv_page, ckv_row = _strides("ckv_cache", ckv_cache, DIM_CKV, fail)
+    kpe_page, kpe_row = _strides("kpe_cache", kpe_cache, DIM_KPE, fail)
+    if kpe_cache.shape[0] != ckv_cache.shape[0]:
+        fail("ckv_cache and kpe_cache must hold the same number of pages")
+    if block_table.dim() != 2 or block_table.shape[1] < 1:
+        fail("block_table must be [B, max_pages]")
+    if block_table.dtype != torch.int32 and block_table.dtype != torch.int64:
+        fail("block_table must be int32 or int64")
+    B, max_pages = block_table.shape
+    if prefix_lens.dtype != torch.int32 or prefix_lens.shape != (B,):
+        fail(f"prefix_lens must be int32 [{B}]")
+    if (cu_drafts.dtype != torch.int32 and cu_drafts.dtype != torch.int64) or cu_drafts.shape != (B + 1,):
+        fail(f"cu_drafts must be int32 [{B + 1}] (one more than block_table rows)")
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or \
+            not 1 <= tree_mask.shape[1] <= MAX_MASK_WORDS:
+        fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
+    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * max_pages > 0x7FFFFFFF:
+        fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
+    hold = (q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), _int32(block_table),
+            _int32(cu_drafts), tree_mask.contiguous(), ckv_cache, kpe_cache)
+    qn, qp, pl, bt, cu, tm = (t.data_ptr() for t in hold[:6])
+    args = (qn, qp, ckv_cache.data_ptr(), ckv_page, ckv_row, kpe_cache.data_ptr(), kpe_page, kpe_row,
+            ckv_cache.shape[0], pl, bt, cu, tm, B, T, H, max_pages, tree_mask.shape[1])
+    return dev, T, H, B, max_pages, args, hold
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _fail(msg: str) -> None:
+    raise ValueError(f"dsa_tree.run: {msg}")
+
+
+def _workspace_bytes(dev: torch.device, T: int, H: int, B: int) -> int:
+    key = (dev.index, T, H, B)
+    n = _ws_bytes.get(key)
+    if n is None:
+        if len(_ws_bytes) > 4096:
+            _ws_bytes.clear()
+        n = _ws_bytes[key] = _native.call_on(dev, _native.lib().dsa_tree_attention_workspace_bytes, T, H, B)
+    return n
+
+
+def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor,
+        prefix_lens: torch.Tensor, block_table: torch.Tensor, cu_drafts: torch.Tensor, tree_mask: torch.Tensor,
+        sm_scale, output: torch.Tensor, lse: torch.Tensor) -> None:
+    # Every message is formatted only on failure: this runs once per step and layer.
+    dev, T, H, B, _, args, hold = check_rows(_fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table,
+                                             cu_drafts, tree_mask, (("output", output), ("lse", lse)))
+    if output.dtype != torch.bfloat16 or output.shape != q_nope.shape or not output.is_contiguous():
+        _fail(f"output must be contiguous bfloat16 [{T}, {H}, {DIM_CKV}]")
+    if lse.dtype != torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
+        _fail(f"lse must be contiguous float32 [{T}, {H}]")
+    if isinstance(sm_scale, torch.Tensor):
+        sm_scale = float(sm_scale.item())
+    if T == 0 or B == 0:
+        return
+    cur = _native.current_stream(dev)
+    ws = workspace.get(dev, "tree", _workspace_bytes(dev, T, H, B), cur)
+    st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, float(sm_scale), output.data_ptr(),
+                         lse.data_ptr(), ws.data_ptr(), ws.numel(), cur)
+    _native.check(st, "dsa_tree_attention_run")
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        raise_on_device_status(dev)
+
+
+def device_status(device: torch.device, clear: bool = True) -> int:
+    """OR of the sticky device status bits of every tree attention workspace on
+    `device` (synchronises)."""
+    return read_status(device, "tree", clear)
+
+
+def read_status(device: torch.device, name: str, clear: bool) -> int:
+    bits = 0
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    for ws in workspace.buffers_of(device, name):
+        out = ctypes.c_uint32(0)
+        with torch.cuda.device(device):
+            st = _native.lib().dsa_read_device_status(ctypes.c_void_p(ws.data_ptr()), ctypes.byref(out),
+                                                      int(clear), stream)
+        _native.check(st, "dsa_read_device_status")
+        bits |= int(out.value)
+    return bits
+
+
+def raise_on_device_status(device: torch.device) -> None:
+    bits = device_status(device, clear=True)
+    if bits:
+        raise _native.DsaError(f"dsa_tree: {_native.describe_device_status(bits)} (status bits {bits:#x})")

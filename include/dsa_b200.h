@@ -239,6 +239,79 @@ DSA_API int dsa_index_cache_write(const void* k, const int64_t* slot_mapping, in
                                   void* k_index_cache_fp8, int64_t num_pages, int32_t ue8m0,
                                   uint32_t* status, void* stream);
 
+/* Bytes of device workspace dsa_tree_attention_run needs: a 256-byte header,
+ * two fp32 records of 64 rows per SM (39 MB in all) for contexts that several
+ * SMs share, and the plan of the call.  The same for all ordinary batches
+ * (up to some 60000 rows groups and requests).  0 for sizes that
+ * dsa_tree_attention_run refuses.  Zero-fill it once (its status word);
+ * nothing else in it carries over from call to call. */
+DSA_API size_t dsa_tree_attention_workspace_bytes(int32_t num_drafts, int32_t num_heads,
+                                                  int32_t num_requests);
+
+/* Attention of a tree of drafted tokens over the paged ckv / kpe cache
+ * (speculative decoding; one draft per request is plain dense decoding).
+ * Request r has prefix_lens[r] cached tokens and the drafts
+ * cu_drafts[r] .. cu_drafts[r+1]-1, whose ckv / kpe rows lie in the cache
+ * behind the prefix (position prefix + j for its j-th draft).  A draft sees
+ * the whole prefix and those drafts of its request whose bits its mask has.
+ *
+ *   q_nope        [num_drafts, num_heads, 512] bf16, contiguous
+ *   q_pe          [num_drafts, num_heads, 64] bf16, contiguous
+ *   ckv_cache     num_pages pages of 64 rows of 512 bf16; pages lie
+ *                 ckv_page_bytes apart and a page's rows ckv_row_bytes
+ *                 (multiples of 16: ckv and kpe may be slices of one cache)
+ *   kpe_cache     the same with rows of 64 bf16
+ *   prefix_lens   [num_requests] int32
+ *   block_table   [num_requests, max_pages] int32
+ *   cu_drafts     [num_requests + 1] int32; rows outside of
+ *                 [cu_drafts[0], cu_drafts[num_requests]) are left as they are
+ *   tree_mask     [num_drafts, mask_words] int64: bit j & 63 of word j / 64
+ *                 is set if the draft sees its request's j-th draft (itself
+ *                 and its ancestors, as a rule); 64 * mask_words drafts a
+ *                 request at most
+ *   output        [num_drafts, num_heads, 512] bf16
+ *   lse           [num_drafts, num_heads] fp32, base-2 log-sum-exp of the
+ *                 scaled logits; a row that sees nothing has -inf, output 0
+ *
+ * 1 <= num_heads <= 128.  Masked cache rows may hold anything.  Data-dependent
+ * errors: lengths that do not fit the table (clamped), drafts that do not fit
+ * cu_drafts or the mask (left out): DSA_DEV_BAD_SEQ_LEN; page ids outside the
+ * pool (their tokens are masked): DSA_DEV_BAD_PAGE. */
+DSA_API int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const void* ckv_cache,
+                                   int64_t ckv_page_bytes, int64_t ckv_row_bytes,
+                                   const void* kpe_cache, int64_t kpe_page_bytes,
+                                   int64_t kpe_row_bytes, int64_t num_pages,
+                                   const int32_t* prefix_lens, const int32_t* block_table,
+                                   const int32_t* cu_drafts, const int64_t* tree_mask,
+                                   int32_t num_requests, int32_t num_drafts, int32_t num_heads,
+                                   int32_t max_pages, int32_t mask_words, float sm_scale,
+                                   void* output, float* lse, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* Accumulates the attention weight that each cached token got from the rows
+ * of a dsa_tree_attention_run with the same arguments:
+ *   acc_out[r, k] = acc[r, k] + sum over drafts i of r, heads h that see k of
+ *                   2^(scaled logit - lse[i, h])
+ * for every position k < max_pages * 64 (+ 0 behind a request's tokens).
+ *
+ *   lse           [num_drafts, num_heads] fp32, as the attention gave it
+ *   acc           [num_requests, max_pages * 64] fp32, rows acc_stride apart
+ *   acc_out       likewise; may be acc itself, else the two do not overlap
+ *
+ * The sums run in a fixed order (no atomics).  The workspace holds only the
+ * status word (256 bytes). */
+DSA_API int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const void* ckv_cache,
+                                 int64_t ckv_page_bytes, int64_t ckv_row_bytes,
+                                 const void* kpe_cache, int64_t kpe_page_bytes,
+                                 int64_t kpe_row_bytes, int64_t num_pages,
+                                 const int32_t* prefix_lens, const int32_t* block_table,
+                                 const int32_t* cu_drafts, const int64_t* tree_mask,
+                                 int32_t num_requests, int32_t num_drafts, int32_t num_heads,
+                                 int32_t max_pages, int32_t mask_words, float sm_scale,
+                                 const float* lse, const float* acc, int64_t acc_stride,
+                                 float* acc_out, int64_t acc_out_stride, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* Copies the sticky device status word of `workspace` to *status_out
  * (synchronising `stream`), and zeroes it when `clear` is non-zero.
  * No counterpart in the reference, which has no error channel

@@ -1,0 +1,72 @@
+"""CPU tests of tree attention and weight accumulation: the C ABI's and the
+Python entry points' refusals, and the mask helper."""
+
+import ctypes
+
+import pytest
+import torch
+
+from dsa_b200 import _native, evict, tree
+
+P = ctypes.c_void_p
+
+
+def call(lib, requests=1, drafts=2, heads=16, max_pages=4, words=1, pages=3, q=16, ckv=16, ckv_page=65536, ckv_row=1024,
+         kpe_page=8192, kpe_row=128, mask=16, ws=16, nbytes=1 << 30, out=16):
+    return lib.dsa_tree_attention_run(P(q), P(16), P(ckv), ckv_page, ckv_row, P(16), kpe_page, kpe_row, pages, P(16), P(16),
+                                      P(16), P(mask), requests, drafts, heads, max_pages, words, 0.1, P(out), P(16), P(ws),
+                                      nbytes, None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(requests=-1), 1), (dict(drafts=-1), 1), (dict(heads=0), 1), (dict(heads=129), 1), (dict(requests=65537), 1),
+    (dict(drafts=0), 0), (dict(requests=0), 0), (dict(q=None), 1), (dict(ws=None), 1), (dict(out=None), 1),
+    (dict(pages=0), 1), (dict(max_pages=0), 1), (dict(words=0), 1), (dict(words=65), 1), (dict(ckv_row=512), 1),
+    (dict(ckv=8), 2), (dict(ckv_page=65528), 2), (dict(kpe_row=136), 2), (dict(mask=20), 2), (dict(out=8), 2),
+    (dict(max_pages=1 << 24, drafts=1 << 16), 1),
+])
+def test_c_abi_refuses_bad_arguments(change, status):
+    assert call(_native.lib(), **change) == status
+
+
+def test_workspace_sizes():
+    lib = _native.lib()
+    small, big = (lib.dsa_tree_attention_workspace_bytes(t, 16, b) for t, b in ((1, 1), (4096, 1024)))
+    assert small == big > 0  # ordinary batches share one workspace
+    assert lib.dsa_tree_attention_workspace_bytes(1 << 20, 128, 65536) > big
+    assert lib.dsa_tree_attention_workspace_bytes(1, 200, 1) == 0
+
+
+def test_masks_from_parents():
+    rows = tree.masks_from_parents([-1, 0, 0, 2, -1])
+    assert rows == [[0b1], [0b11], [0b101], [0b1101], [0b10000]]
+    chain = tree.masks_from_parents(list(range(-1, 69)))
+    assert len(chain[0]) == 2 and chain[63] == [-1, 0] and chain[69] == [-1, 63]
+    with pytest.raises(ValueError):
+        tree.masks_from_parents([-1, 1])
+    assert tree.masks_from_parents([]) == []
+
+
+def test_entry_points_refuse_cpu_tensors():
+    a = dict(q_nope=torch.zeros(1, 16, 512), q_pe=torch.zeros(1, 16, 64), ckv_cache=torch.zeros(1, 64, 512),
+             kpe_cache=torch.zeros(1, 64, 64), prefix_lens=torch.zeros(1), block_table=torch.zeros(1, 1),
+             cu_drafts=torch.zeros(2), tree_mask=torch.zeros(1, 1), sm_scale=0.1)
+    with pytest.raises(ValueError, match="CUDA"):
+        tree.run(**a, output=torch.zeros(1), lse=torch.zeros(1))
+    with pytest.raises(ValueError, match="CUDA"):
+        evict.accumulate(**a, lse=torch.zeros(1), acc=torch.zeros(1), out=torch.zeros(1))
+
+
+def test_cache_strides():
+    def fail(msg):
+        raise ValueError(msg)
+
+    both = torch.zeros(3, 64, 576, dtype=torch.bfloat16)
+    assert tree._strides("ckv", both[:, :, :512], 512, fail) == (2 * 64 * 576, 2 * 576)
+    assert tree._strides("kpe", both[:, :, 512:], 64, fail) == (2 * 64 * 576, 2 * 576)
+    assert tree._strides("ckv", both[:1, :, :512], 512, fail) == (2 * 64 * 576, 2 * 576)
+    for bad in (both[:, :, 4:516], both[:, :, :511], torch.zeros(3, 64, 580, dtype=torch.bfloat16)[:, :, :512],
+                both[:, :, :512].transpose(0, 1), both[:0, :, :512], both[:1, :, :512].expand(3, 64, 512),
+                both.flatten(0, 1)[:, :512]):
+        with pytest.raises(ValueError):
+            tree._strides("ckv", bad, 512, fail)

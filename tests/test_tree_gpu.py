@@ -1,0 +1,299 @@
+"""GPU parity of tree attention (dsa_b200.tree.run) and of the accumulated
+attention weights (dsa_b200.evict.accumulate) with the 64-bit oracle, whose
+error bounds are the tolerances, at the sizes and masks where they can go
+wrong."""
+
+import math
+
+import pytest
+import torch
+
+from dsa_b200 import DsaError, evict, tree
+from oracle import tree as otree
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 1.0 / math.sqrt(192.0)
+
+
+class Case:
+    """Seeded inputs on the CPU (`host`) and the device; drafts form a random tree."""
+
+    def __init__(self, prefixes, drafts, heads, seed=0, device="cuda", extra_pages=2, words=None, scale=1.0, tail=0):
+        g = torch.Generator().manual_seed(seed)
+        normal = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)  # noqa: E731
+        B, T = len(prefixes), sum(drafts)
+        need = [(p + n + 63) // 64 for p, n in zip(prefixes, drafts)]
+        width = max(1, max(need))
+        pool = sum(need) + extra_pages
+        perm = torch.randperm(pool, generator=g)
+        table = torch.full((B, width), -1, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = perm[at:at + n].int()
+            at += n
+        words = words or max(1, (max(drafts) + 63) // 64)
+        rows = []
+        for n in drafts:
+            parents = [int(torch.randint(-1, j, (1,), generator=g)) if j and j % 3 == 0 else j - 1 for j in range(n)]
+            rows += [r + [0] * (words - len(r)) for r in (tree.masks_from_parents(parents) if n else [])]
+        total = T + tail
+        rows += [[-1] * words] * tail
+        self.q_nope = (normal(total, heads, 512).float() * scale).to(torch.bfloat16)
+        self.q_pe = normal(total, heads, 64)
+        self.ckv, self.kpe = normal(pool, 64, 512), normal(pool, 64, 64)
+        self.prefix = torch.tensor(prefixes, dtype=torch.int32)
+        self.table = table
+        self.cu = torch.tensor([0, *drafts]).cumsum(0).int()
+        self.mask = torch.tensor(rows, dtype=torch.int64).reshape(total, words)
+        self.device, self.T, self.H, self.B = device, total, heads, B
+
+    def args(self):
+        return [t.to(self.device) for t in (self.q_nope, self.q_pe, self.ckv, self.kpe, self.prefix, self.table, self.cu,
+                                            self.mask)]
+
+    def outs(self):
+        return (torch.full((self.T, self.H, 512), 7.0, dtype=torch.bfloat16, device=self.device),
+                torch.full((self.T, self.H), 7.0, device=self.device))
+
+    def reference(self):
+        return otree.tree_reference(self.q_nope, self.q_pe, self.ckv, self.kpe, self.prefix, self.table, self.cu,
+                                    self.mask, SCALE)
+
+    def check(self, out, lse):
+        ro, rl, bo, bl = self.reference()
+        mine = ~torch.isnan(rl)
+        out, lse = out.cpu().double(), lse.cpu().double()
+        assert torch.equal(lse[mine] == -math.inf, rl[mine] == -math.inf)
+        fin = mine & (rl != -math.inf)
+        assert ((lse - rl).abs() <= bl)[fin].all(), float((lse - rl).abs()[fin].max())
+        bad = ((out - ro).abs() > bo)[mine]
+        assert not bad.any(), (int(bad.sum()), float((out - ro).abs()[mine].max()))
+        assert (out[~mine] == 7).all() and (lse[~mine] == 7).all()
+
+
+def run(c, args=None):
+    out, lse = c.outs()
+    tree.run(*(args or c.args()), SCALE, out, lse)
+    torch.cuda.synchronize()
+    return out, lse
+
+
+@pytest.mark.parametrize("prefixes,drafts,heads", [
+    ([0], [1], 16),                        # the draft alone
+    ([1], [1], 1),                         # one head
+    ([63], [1], 16), ([64], [1], 16), ([65], [2], 16),   # the page's border
+    ([300], [4], 16),                      # one full group
+    ([300], [5], 16),                      # a partial second group
+    ([100, 5, 700], [3, 0, 4], 16),        # a request without drafts
+    ([130], [7], 5),                       # rows that split a draft's heads between groups
+    ([70, 200], [2, 1], 128),              # all heads
+    ([190], [70], 3),                      # two mask words, drafts across pages
+    ([10, 2000, 900, 64, 0], [1, 2, 9, 3, 6], 8),
+    ([9000], [9], 16),                     # several groups over several slices
+    ([20000], [1], 16),                    # one group over all slices
+])
+def test_matches_the_oracle(cuda_device, prefixes, drafts, heads):
+    c = Case(prefixes, drafts, heads, seed=len(prefixes) + sum(prefixes), device=cuda_device)
+    c.check(*run(c))
+
+
+def test_many_requests(cuda_device):
+    g = torch.Generator().manual_seed(3)
+    prefixes = torch.randint(0, 200, (401,), generator=g).tolist()
+    drafts = torch.randint(0, 6, (401,), generator=g).tolist()
+    c = Case(prefixes, drafts, 4, seed=5, device=cuda_device)
+    c.check(*run(c))
+
+
+def test_rows_that_see_nothing(cuda_device):
+    c = Case([0, 40], [6, 3], 16, seed=9, device=cuda_device)
+    c.mask[1] = 0       # nothing at all: output 0, lse -inf
+    c.mask[2, 0] = 1    # the first draft only, not itself
+    c.mask[7] = 0       # the prefix only
+    out, lse = run(c)
+    c.check(out, lse)
+    assert (lse[1] == -math.inf).all() and (out[1] == 0).all()
+
+
+def test_masked_places_may_hold_anything(cuda_device):
+    c = Case([70, 0], [9, 5], 16, seed=11, device=cuda_device)
+    c.mask[:, 0] &= ~0b100  # nobody sees the third draft of either request
+    for b, p in ((0, 70), (1, 0)):
+        s = int(otree.slots(c.table[b], p + 3)[-1])
+        c.ckv.view(-1, 512)[s, ::3] = math.nan
+        c.ckv.view(-1, 512)[s, 1::3] = math.inf
+        c.kpe.view(-1, 64)[s] = -math.inf
+    used = torch.zeros(c.ckv.shape[0] * 64, dtype=torch.bool)
+    for b, n in ((0, 79), (1, 5)):
+        used[otree.slots(c.table[b], n)] = True
+    c.ckv.view(-1, 512)[~used] = math.nan   # behind the last token, and pages of nobody
+    c.kpe.view(-1, 64)[~used] = math.inf
+    out, lse = run(c)
+    assert torch.isfinite(out.float()).all() and torch.isfinite(lse).all()
+    # A masked row gives nothing to any logit it is not in: the oracle masks it too.
+    c.ckv, c.kpe = c.ckv.nan_to_num(0, 0, 0), c.kpe.nan_to_num(0, 0, 0)
+    c.check(out, lse)
+
+
+def test_a_draft_that_only_some_rows_see_is_nan_to_those_alone(cuda_device):
+    c = Case([100], [4], 16, seed=12, device=cuda_device)
+    c.mask[:, 0] = torch.tensor([1, 3, 5, 9])  # all follow draft 0; drafts 1, 2, 3 see themselves
+    s = int(otree.slots(c.table[0], 102)[-1])  # draft 1
+    c.ckv.view(-1, 512)[s, 5] = math.nan
+    out, lse = run(c)
+    assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
+    for i in (0, 2, 3):
+        assert torch.isfinite(out[i].float()).all() and torch.isfinite(lse[i]).all()
+
+
+def test_rising_logits_move_the_maximum(cuda_device):
+    """Logits that grow along the context by far more than the rescaling
+    threshold, so that O is rescaled again and again."""
+    c = Case([1500], [3], 16, seed=13, device=cuda_device, scale=0.05)
+    s = otree.slots(c.table[0], 1500)
+    ramp = torch.linspace(-3, 3, 1500)[:, None]
+    c.q_pe[:] = 1.0
+    c.kpe.view(-1, 64)[s] = (ramp * torch.ones(1, 64)).to(torch.bfloat16)
+    c.check(*run(c))
+    c.kpe.view(-1, 64)[s] = (-ramp * torch.ones(1, 64)).to(torch.bfloat16)
+    c.check(*run(c))
+
+
+def test_strided_caches_and_wide_tables(cuda_device):
+    c = Case([200, 77], [3, 5], 16, seed=14, device=cuda_device)
+    args = c.args()
+    both = torch.full((c.ckv.shape[0], 67, 584), math.nan, dtype=torch.bfloat16, device=cuda_device)
+    both[:, :64, :512], both[:, :64, 512:576] = args[2], args[3]
+    args[2], args[3] = both[:, :64, :512], both[:, :64, 512:576]
+    wide = torch.full((c.B, 40), -1, dtype=torch.int64, device=cuda_device)
+    wide[:, :c.table.shape[1]] = args[5]
+    args[5], args[6] = wide, args[6].long()
+    qs = torch.empty(c.T, 2 * c.H, 512, dtype=torch.bfloat16, device=cuda_device)[:, ::2]
+    qs.copy_(args[0])
+    args[0] = qs
+    c.check(*run(c, args))
+
+
+def test_rows_behind_the_last_request_are_left(cuda_device):
+    c = Case([64, 3], [2, 2], 16, seed=15, device=cuda_device, tail=3)
+    out, lse = run(c)
+    assert (out[4:] == 7).all() and (lse[4:] == 7).all()
+    c.check(out, lse)
+
+
+def test_pages_outside_the_pool_are_masked_and_reported(cuda_device):
+    c = Case([200], [2], 16, seed=16, device=cuda_device)
+    args = c.args()
+    args[5][0, 1] = c.ckv.shape[0] + 5
+    out, lse = c.outs()
+    with pytest.raises(DsaError, match="page pool"):
+        tree.run(*args, SCALE, out, lse)
+    assert torch.isfinite(out.float()).all() and torch.isfinite(lse).all()
+    assert tree.device_status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("prefix,cu", [([-3], [0, 2]), ([100000], [0, 2]), ([10], [0, 3]), ([10], [2, 0]), ([10], [-1, 2])])
+def test_lengths_that_do_not_fit_are_reported(cuda_device, prefix, cu):
+    c = Case([10], [2], 16, seed=17, device=cuda_device)
+    args = c.args()
+    args[4] = torch.tensor(prefix, dtype=torch.int32, device=cuda_device)
+    args[6] = torch.tensor(cu, dtype=torch.int32, device=cuda_device)
+    out, lse = c.outs()
+    with pytest.raises(DsaError, match="seq_len"):
+        tree.run(*args, SCALE, out, lse)
+    c.check(*run(c))  # the workspace is as good as before
+
+
+def test_graphs_streams_and_repeats_give_the_same_bits(cuda_device):
+    c = Case([3000, 500, 0], [9, 2, 3], 16, seed=18, device=cuda_device)
+    args = c.args()
+    out, lse = run(c, args)
+    for _ in range(3):
+        o2, l2 = run(c, args)
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+    side = torch.cuda.Stream(cuda_device)
+    o3, l3 = c.outs()
+    with torch.cuda.stream(side):
+        tree.run(*args, SCALE, o3, l3)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        o4, l4 = c.outs()
+        with torch.cuda.graph(graph, stream=side):
+            tree.run(*args, SCALE, o4, l4)
+    assert torch.equal(out, o3) and torch.equal(lse, l3)
+    args[4][0] = 10  # the lengths of the replay are the device's
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    c.prefix[0] = 10
+    c.check(o4, l4)
+
+
+def weigh(c, args=None, acc=None, lse=None, out=None):
+    args = args or c.args()
+    if lse is None:
+        lse = run(c, args)[1]
+    if acc is None:
+        acc = torch.rand(c.B, args[5].shape[1] * 64, generator=torch.Generator().manual_seed(1)).to(c.device)
+    if out is None:
+        out = torch.full_like(acc, 7.0)
+    evict.accumulate(*args, SCALE, lse, acc, out)
+    torch.cuda.synchronize()
+    return lse, acc, out
+
+
+@pytest.mark.parametrize("prefixes,drafts,heads", [
+    ([0], [1], 16), ([63], [1], 16), ([64], [1], 1), ([300], [5], 16), ([100, 5, 700], [3, 0, 4], 16),
+    ([130], [7], 5), ([190], [70], 3), ([70, 200], [2, 1], 128), ([9000], [9], 16), ([20000], [1], 16),
+    ([10, 2000, 900, 64, 0], [1, 2, 9, 3, 6], 8),
+])
+def test_weights_match_the_oracle(cuda_device, prefixes, drafts, heads):
+    c = Case(prefixes, drafts, heads, seed=len(prefixes) + sum(prefixes), device=cuda_device)
+    lse, acc, out = weigh(c)
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    err = (out.cpu().double() - want).abs()
+    assert (err <= off).all(), (float(err.max()), float(off.max()))
+    # every row's weights sum to one, up to the errors of its weights
+    given = (out - acc).cpu().double().sum(1)
+    rows = torch.tensor([n * heads for n in drafts], dtype=torch.float64)
+    assert ((given - rows).abs() <= off.sum(1) + acc.cpu().double().sum(1) * 2.0 ** -23 + rows * 2.0 ** -10).all()
+
+
+def test_weights_in_place_repeat_and_skip_what_saw_nothing(cuda_device):
+    c = Case([0, 2500], [3, 9], 16, seed=21, device=cuda_device)
+    c.mask[1] = 0
+    args = c.args()
+    used = torch.zeros(c.ckv.shape[0] * 64, dtype=torch.bool)
+    used[otree.slots(c.table[0], 3)] = True
+    used[otree.slots(c.table[1], 2509)] = True
+    args[2].view(-1, 512)[~used.to(cuda_device)] = math.nan
+    lse, acc, out = weigh(c, args)
+    assert torch.isfinite(out).all()
+    twice = acc.clone()
+    weigh(c, args, acc=twice, lse=lse, out=twice)
+    assert torch.equal(twice, out)
+    again = weigh(c, args, acc=acc, lse=lse)[2]
+    assert torch.equal(again, out)
+    strided = torch.full((c.B, acc.shape[1] + 5), 3.0, device=cuda_device)
+    view = strided[:, :acc.shape[1]]
+    weigh(c, args, acc=acc, lse=lse, out=view)
+    assert torch.equal(view, out) and (strided[:, acc.shape[1]:] == 3).all()
+
+
+def test_no_drafts_at_all(cuda_device):
+    c = Case([5, 70], [1, 1], 16, seed=22, device=cuda_device)
+    args = c.args()
+    acc = torch.rand(2, args[5].shape[1] * 64, device=cuda_device)
+    out = torch.zeros_like(acc)
+    args[6].zero_()
+    o, l = c.outs()
+    tree.run(*args, SCALE, o, l)
+    evict.accumulate(*args, SCALE, l, acc, out)
+    assert (o == 7).all() and (l == 7).all() and torch.equal(out, acc)
+    args[0], args[1], args[7] = args[0][:0], args[1][:0], args[7][:0]
+    out.zero_()
+    tree.run(*args, SCALE, o[:0], l[:0])
+    evict.accumulate(*args, SCALE, l[:0], acc, out)
+    assert torch.equal(out, acc)
