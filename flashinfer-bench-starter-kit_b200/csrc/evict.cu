@@ -1,0 +1,473 @@
+// evict.cu -- eviction from the paged caches by accumulated attention weight.
+//
+// Request r has L = seq_lens[r] tokens and keeps at most `budget` of them:
+// the first num_sink, the last num_recent, and of the tokens between those
+// with the largest accumulated weight (equal ones: the earlier; NaN counts as
+// largest).  Their order stays.  Two kernels:
+//
+// select_kernel: one thread-block cluster per request.  Each CTA holds its
+//   slice of the request's weights in shared memory, read from HBM once (4 B
+//   per token).  The boundary weight is found by radix: a histogram of the
+//   order key's top 11 bits, then of the next 11 and the last 10 among the
+//   keys that share the boundary's bits, each summed over the cluster through
+//   distributed shared memory.  The kept positions then come out in order: a
+//   token's place is the number kept before it, from ballots, a scan over
+//   the CTA's warps and the counts of the lower CTAs.
+// move_kernel: copies the kept tokens' rows of every cache to their new
+//   pages, 1288 B per token in and out; HBM-bound.
+#include <mutex>
+
+#include "dsa_b200.h"
+#include "host.h"
+#include "ptx.cuh"
+
+namespace dsa {
+namespace evict {
+
+constexpr int kPage = DSA_PAGE_SIZE;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxCluster = 8;             // the portable limit
+constexpr int kMaxResident = 49152;        // weights a CTA can hold (192 KB)
+constexpr int kSteps = 8;                  // emission: tokens per thread and round
+
+struct Params {
+  const float* acc;
+  int64_t acc_stride;
+  const int32_t* seq_lens;
+  const int32_t* block_table;
+  const int32_t* new_block_table;
+  int requests, max_pages, new_max_pages;
+  int budget, num_sink, num_recent;
+  int resident;                            // weights that fit the CTA's shared memory
+  uint8_t* ckv;
+  uint8_t* kpe;
+  uint8_t* index;                          // may be null
+  int64_t ckv_page, ckv_row, kpe_page, kpe_row;
+  int num_pages;
+  int32_t* keep;
+  int32_t* new_seq_lens;
+  float* new_acc;
+  int64_t new_acc_stride;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ int length_of(const Params& p, int b, bool& bad) {
+  const int L = __ldg(p.seq_lens + b);
+  const int cap = p.max_pages * kPage;
+  bad = L < 0 || L > cap;
+  return L < 0 ? 0 : (L > cap ? cap : L);
+}
+
+// Exclusive sum of v over the block's threads, and the total.
+__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += a;
+  }
+  if (lane == 31) scratch[warp] = inc;
+  __syncthreads();
+  int before = inc - v;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
+  }
+  __syncthreads();
+  return before;
+}
+
+__global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
+  extern __shared__ float held[];          // this CTA's weights, if they fit
+  __shared__ int hist[3][kBins];
+  __shared__ int counts[2];                // tokens above the boundary key, and at it
+  __shared__ int scratch[2 * kWarps];
+  __shared__ int found[3];                 // boundary bin, kept ones needed from it, its size
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int b = blockIdx.x / ctas;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  bool bad;
+  const int L = length_of(p, b, bad);
+  if (bad && rank == 0 && tid == 0) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
+  const float* acc = p.acc + b * p.acc_stride;
+  int32_t* keep = p.keep + static_cast<int64_t>(b) * p.budget;
+  float* new_acc = p.new_acc + b * p.new_acc_stride;
+  const int kept = L < p.budget ? L : p.budget;
+  const int t0 = rank * kThreads + tid, step = ctas * kThreads;
+  if (t0 == 0) p.new_seq_lens[b] = kept;
+  // Behind what is kept.
+  for (int i = kept + t0; i < p.budget; i += step) keep[i] = -1;
+  for (int i = kept + t0; i < p.new_max_pages * kPage; i += step) new_acc[i] = 0.f;
+  if (L <= p.budget) {
+    for (int i = t0; i < L; i += step) {
+      keep[i] = i;
+      new_acc[i] = acc[i];
+    }
+    return;  // the whole cluster leaves here
+  }
+  for (int i = t0; i < p.num_sink + p.num_recent; i += step) {
+    const bool first = i < p.num_sink;
+    const int pos = first ? i : L - p.num_recent + (i - p.num_sink);
+    const int to = first ? i : p.budget - p.num_recent + (i - p.num_sink);
+    keep[to] = pos;
+    new_acc[to] = acc[pos];
+  }
+  int need = p.budget - p.num_sink - p.num_recent;  // from the middle; fewer than it has
+  if (need == 0) return;
+
+  const int middle = L - p.num_sink - p.num_recent;
+  const int slice = (middle + ctas - 1) / ctas;
+  const int lo = min(rank * slice, middle), n = min(slice, middle - lo);
+  const float* mine = acc + p.num_sink + lo;
+  const bool fits = slice <= p.resident;
+  for (int i = tid; i < 3 * kBins; i += kThreads) hist[0][i] = 0;
+  __syncthreads();
+
+  // ---- boundary key: 11 + 11 + 10 bits.
+  uint32_t prefix = 0;                     // the boundary key's bits so far
+  uint32_t above = 0xffffffffu;            // kept for sure: keys > above
+  int ties = 0;                            // kept ones among keys == above
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const int bins = pass == 2 ? 1024 : kBins;
+    const int upper = shift + (pass == 2 ? 10 : 11);
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const int i = i0 + tid;
+      const bool in = i < n;
+      float v = 0.f;
+      if (in) {
+        if (pass == 0 || !fits) {
+          v = mine[i];
+          if (fits) held[i] = v;
+        } else {
+          v = held[i];
+        }
+      }
+      const uint32_t key = score_key(v);
+      bool count = in && (pass == 0 || (key >> upper) == prefix);
+      const int bin = static_cast<int>((key >> shift) & (bins - 1));
+      // Weights repeat (tokens that were never read have exactly 0): the
+      // lanes that share the first counting lane's bin add theirs at once.
+      const unsigned int act = __ballot_sync(0xffffffffu, count);
+      if (act != 0) {
+        const int lead = __ffs(act) - 1;
+        const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);
+        const unsigned int same = __ballot_sync(0xffffffffu, count && bin == lead_bin);
+        if (lane == lead) atomicAdd(&hist[pass][lead_bin], __popc(same));
+        if (count && bin != lead_bin) atomicAdd(&hist[pass][bin], 1);
+      }
+    }
+    cluster_sync();
+    // Thread t has four bins, in descending order over the threads.
+    constexpr int kPer = kBins / kThreads;
+    int c[kPer], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int bin = bins - 1 - (kPer * tid + j);
+      c[j] = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (bin >= 0 && r < ctas) c[j] += ld_cluster(&hist[pass][bin], r);
+      sum += c[j];
+    }
+    int total;
+    int before = block_scan(sum, scratch, total);
+    if (before < need && need <= before + sum) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (before < need && need <= before + c[j]) {
+          found[0] = bins - 1 - (kPer * tid + j);
+          found[1] = need - before;
+          found[2] = c[j];
+        }
+        before += c[j];
+      }
+    }
+    __syncthreads();
+    prefix = (prefix << (pass == 2 ? 10 : 11)) | static_cast<uint32_t>(found[0]);
+    need = found[1];
+    const bool all = found[2] == need;     // the whole bin is kept: no key bits below matter
+    __syncthreads();
+    if (all || pass == 2) {
+      above = all ? (prefix << shift) - 1u : prefix;  // not below 0: some key of the middle is not kept
+      ties = all ? 0 : need;
+      break;
+    }
+  }
+
+  // ---- counts of every CTA, then the positions in order.
+  int gt = 0, eq = 0;
+  for (int i = tid; i < n; i += kThreads) {
+    const uint32_t key = score_key(fits ? held[i] : mine[i]);
+    gt += key > above;
+    eq += key == above;
+  }
+  int total_gt, total_eq;
+  block_scan(gt, scratch, total_gt);
+  block_scan(eq, scratch, total_eq);
+  if (tid == 0) {
+    counts[0] = total_gt;
+    counts[1] = total_eq;
+  }
+  cluster_sync();
+  int gt_before = 0, eq_before = 0;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) {
+    if (r >= rank) break;
+    gt_before += ld_cluster(&counts[0], r);
+    eq_before += ld_cluster(&counts[1], r);
+  }
+  // The last remote read of this kernel: a CTA leaves once all have made theirs.
+  cluster_arrive();
+  // eq_before ties of lower CTAs come first; `ties` are kept in all.
+  for (int i0 = 0; i0 < n; i0 += kThreads * kSteps) {
+    unsigned int above_mask[kSteps], tie_mask[kSteps];
+    int g = 0, q = 0;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int i = i0 + (warp * kSteps + j) * 32 + lane;
+      uint32_t key = 0;
+      const bool in = i < n;
+      if (in) key = score_key(fits ? held[i] : mine[i]);
+      above_mask[j] = __ballot_sync(0xffffffffu, in && key > above);
+      tie_mask[j] = __ballot_sync(0xffffffffu, in && key == above);
+      g += __popc(above_mask[j]);
+      q += __popc(tie_mask[j]);
+    }
+    if (lane == 0) {
+      scratch[warp] = g;
+      scratch[kWarps + warp] = q;
+    }
+    __syncthreads();
+    int wg = gt_before, wq = eq_before;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) {
+        wg += scratch[w];
+        wq += scratch[kWarps + w];
+      }
+      gt_before += scratch[w];
+      eq_before += scratch[kWarps + w];
+    }
+    __syncthreads();
+    const unsigned int lt = (1u << lane) - 1u;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const bool up = (above_mask[j] >> lane) & 1, tie = (tie_mask[j] >> lane) & 1;
+      const int g_at = wg + __popc(above_mask[j] & lt), q_at = wq + __popc(tie_mask[j] & lt);
+      if (up || (tie && q_at < ties)) {
+        const int to = p.num_sink + g_at + min(q_at, ties);
+        const int i = i0 + (warp * kSteps + j) * 32 + lane;
+        keep[to] = p.num_sink + lo + i;
+        new_acc[to] = fits ? held[i] : mine[i];
+      }
+      wg += __popc(above_mask[j]);
+      wq += __popc(tie_mask[j]);
+    }
+  }
+  cluster_wait();
+}
+
+// A warp moves kMoveTokens tokens at a time: all their loads (5 KB) are in
+// flight before the first store.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveWarps = kMoveThreads / 32;
+constexpr int kMoveTokens = 4;
+constexpr int kIndexRow = DSA_INDEX_DIM;               // 128 bytes, then the page's 64 scales
+constexpr int kIndexScales = kPage * kIndexRow;
+
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int per_row = (p.budget + kMoveTokens - 1) / kMoveTokens;
+  const int64_t all = static_cast<int64_t>(p.requests) * per_row;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kMoveWarps;
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * kMoveWarps + (threadIdx.x >> 5); w < all; w += step) {
+    const int b = static_cast<int>(w / per_row), i0 = static_cast<int>(w % per_row) * kMoveTokens;
+    // Lane l looks up token l & 3 of the four.
+    const int i = i0 + (lane & (kMoveTokens - 1));
+    const int pos = i < p.budget ? __ldcg(p.keep + static_cast<int64_t>(b) * p.budget + i) : -1;
+    int from = -1, to = -1;                            // pages; from < 0: nothing to move
+    if (pos >= 0) {
+      from = __ldg(p.block_table + static_cast<int64_t>(b) * p.max_pages + pos / kPage);
+      to = __ldg(p.new_block_table + static_cast<int64_t>(b) * p.new_max_pages + i / kPage);
+      if (from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages) {
+        if (lane < kMoveTokens) atomicOr(p.status, DSA_DEV_BAD_PAGE);
+        from = -1;
+      }
+    }
+    const int row = pos & (kPage - 1);
+    if (__all_sync(0xffffffffu, from < 0)) continue;
+    // ckv: 64 pieces of 16 bytes a token, two a lane.
+    int f[kMoveTokens], t[kMoveTokens];
+    uint4 c[2 * kMoveTokens];
+#pragma unroll
+    for (int k = 0; k < kMoveTokens; ++k) {
+      f[k] = __shfl_sync(0xffffffffu, from, k);
+      t[k] = __shfl_sync(0xffffffffu, to, k);
+      const int r = __shfl_sync(0xffffffffu, row, k);
+      if (f[k] >= 0) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.ckv + f[k] * p.ckv_page + r * p.ckv_row) + lane;
+        c[2 * k] = __ldcs(src);
+        c[2 * k + 1] = __ldcs(src + 32);
+      }
+    }
+    // kpe and index keys: 8 pieces a token, lane l has piece l & 7 of token l >> 3.
+    const int k = lane >> 3, piece = 16 * (lane & 7);
+    const int fk = __shfl_sync(0xffffffffu, from, k), tk = __shfl_sync(0xffffffffu, to, k);
+    const int rk = __shfl_sync(0xffffffffu, row, k), dk = (i0 + k) & (kPage - 1);
+    uint4 e = make_uint4(0u, 0u, 0u, 0u), x = e;
+    uint32_t scale = 0;
+    if (fk >= 0) {
+      e = __ldcs(reinterpret_cast<const uint4*>(p.kpe + fk * p.kpe_page + rk * p.kpe_row + piece));
+      if (p.index != nullptr) {
+        const uint8_t* page = p.index + static_cast<int64_t>(fk) * DSA_INDEX_PAGE_BYTES;
+        x = __ldcs(reinterpret_cast<const uint4*>(page + rk * kIndexRow + piece));
+        if (piece == 0) scale = __ldcs(reinterpret_cast<const uint32_t*>(page + kIndexScales + 4 * rk));
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kMoveTokens; ++q) {
+      if (f[q] >= 0) {
+        uint4* dst =
+            reinterpret_cast<uint4*>(p.ckv + t[q] * p.ckv_page + ((i0 + q) & (kPage - 1)) * p.ckv_row) + lane;
+        dst[0] = c[2 * q];
+        dst[32] = c[2 * q + 1];
+      }
+    }
+    if (fk >= 0) {
+      *reinterpret_cast<uint4*>(p.kpe + tk * p.kpe_page + dk * p.kpe_row + piece) = e;
+      if (p.index != nullptr) {
+        uint8_t* page = p.index + static_cast<int64_t>(tk) * DSA_INDEX_PAGE_BYTES;
+        *reinterpret_cast<uint4*>(page + dk * kIndexRow + piece) = x;
+        if (piece == 0) *reinterpret_cast<uint32_t*>(page + kIndexScales + 4 * dk) = scale;
+      }
+    }
+  }
+}
+
+// CTAs per request: as many as the portable cluster limit, the SMs (two
+// 512-thread CTAs each) and the table's width can use.
+int cluster_for(int requests, int max_pages, int sms) {
+  int c = kMaxCluster;
+  while (c > 1 && (static_cast<int64_t>(requests) * c > 2 * sms || static_cast<int64_t>(max_pages) * kPage <= 2048 * (c / 2)))
+    c /= 2;
+  return c;
+}
+
+std::once_flag g_once[64];
+int g_status[64];
+
+}  // namespace evict
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const int32_t* seq_lens,
+                                   const int32_t* block_table, const int32_t* new_block_table, int32_t num_requests,
+                                   int32_t max_pages, int32_t new_max_pages, void* ckv_cache, int64_t ckv_page_bytes,
+                                   int64_t ckv_row_bytes, void* kpe_cache, int64_t kpe_page_bytes,
+                                   int64_t kpe_row_bytes, void* k_index_cache_fp8, int64_t num_pages, int32_t budget,
+                                   int32_t num_sink, int32_t num_recent, int32_t* keep, int32_t* new_seq_lens,
+                                   float* new_acc, int64_t new_acc_stride, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (num_requests < 0 || num_requests > 65536) return DSA_ERR_INVALID_ARGUMENT;
+  if (num_requests == 0) return DSA_OK;
+  if (!acc || !seq_lens || !block_table || !new_block_table || !ckv_cache || !kpe_cache || !keep || !new_seq_lens ||
+      !new_acc || !workspace)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (num_pages < 1 || num_pages > 0x7FFFFFFF || max_pages < 1 || max_pages > (1 << 24) || new_max_pages < 1 ||
+      new_max_pages > (1 << 24))
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (budget < 1 || budget > new_max_pages * evict::kPage || num_sink < 0 || num_recent < 0 ||
+      static_cast<int64_t>(num_sink) + num_recent > budget)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (acc_stride < static_cast<int64_t>(max_pages) * evict::kPage ||
+      new_acc_stride < static_cast<int64_t>(new_max_pages) * evict::kPage)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (ckv_row_bytes < DSA_CKV_DIM * 2 || kpe_row_bytes < DSA_KPE_DIM * 2 || ckv_page_bytes < 0 || kpe_page_bytes < 0)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(ckv_cache) || !aligned16(kpe_cache) || !aligned16(k_index_cache_fp8) || !aligned16(workspace) ||
+      ((ckv_page_bytes | ckv_row_bytes | kpe_page_bytes | kpe_row_bytes) & 15))
+    return DSA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(acc) | reinterpret_cast<uintptr_t>(seq_lens) |
+       reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(new_block_table) |
+       reinterpret_cast<uintptr_t>(keep) | reinterpret_cast<uintptr_t>(new_seq_lens) |
+       reinterpret_cast<uintptr_t>(new_acc)) & 3u)
+    return DSA_ERR_MISALIGNED;
+  if (workspace_bytes < kWorkspaceHeader) return DSA_ERR_WORKSPACE_TOO_SMALL;
+  DeviceInfo info;
+  int st = current_device_info(&info);
+  if (st != DSA_OK) return st;
+  std::call_once(evict::g_once[info.device], [&]() {
+    evict::g_status[info.device] =
+        cudaFuncSetAttribute(evict::select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             evict::kMaxResident * 4) == cudaSuccess
+            ? DSA_OK
+            : DSA_ERR_CUDA;
+  });
+  if (evict::g_status[info.device] != DSA_OK) return evict::g_status[info.device];
+
+  evict::Params p{};
+  p.acc = acc;
+  p.acc_stride = acc_stride;
+  p.seq_lens = seq_lens;
+  p.block_table = block_table;
+  p.new_block_table = new_block_table;
+  p.requests = num_requests;
+  p.max_pages = max_pages;
+  p.new_max_pages = new_max_pages;
+  p.budget = budget;
+  p.num_sink = num_sink;
+  p.num_recent = num_recent;
+  p.ckv = static_cast<uint8_t*>(ckv_cache);
+  p.kpe = static_cast<uint8_t*>(kpe_cache);
+  p.index = static_cast<uint8_t*>(k_index_cache_fp8);
+  p.ckv_page = ckv_page_bytes;
+  p.ckv_row = ckv_row_bytes;
+  p.kpe_page = kpe_page_bytes;
+  p.kpe_row = kpe_row_bytes;
+  p.num_pages = static_cast<int>(num_pages);
+  p.keep = keep;
+  p.new_seq_lens = new_seq_lens;
+  p.new_acc = new_acc;
+  p.new_acc_stride = new_acc_stride;
+  p.status = static_cast<unsigned int*>(workspace);
+
+  const int ctas = evict::cluster_for(num_requests, max_pages, info.num_sms);
+  const int64_t slice = (static_cast<int64_t>(max_pages) * evict::kPage + ctas - 1) / ctas;
+  p.resident = static_cast<int>(slice < evict::kMaxResident ? slice : evict::kMaxResident);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned int>(num_requests) * ctas);
+  cfg.blockDim = dim3(evict::kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.resident) * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned int>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, evict::select_kernel, p) != cudaSuccess) return DSA_ERR_CUDA;
+  const int64_t warps = static_cast<int64_t>(num_requests) * ((budget + evict::kMoveTokens - 1) / evict::kMoveTokens);
+  const int64_t blocks = (warps + evict::kMoveWarps - 1) / evict::kMoveWarps;
+  const int64_t most = static_cast<int64_t>(info.num_sms) * 8;
+  if (launch_programmatic(evict::move_kernel, dim3(static_cast<unsigned int>(blocks < most ? blocks : most)),
+                          dim3(evict::kMoveThreads), 0, s, p) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  return DSA_OK;
+}

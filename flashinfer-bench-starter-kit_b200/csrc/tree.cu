@@ -899,12 +899,12 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p, int ctas) 
   __shared__ int recs[2 * kMaxCtas];
   __shared__ float weight[kJoinRows][2 * kMaxCtas];
   __shared__ int warp_count[4];
-  const int total = p.plan[0];
+  const int total = __ldcg(p.plan);
   const int gi = blockIdx.x;
-  if (gi >= p.plan[1]) return;
-  const int b = p.plan[kPlanHead + 2 * p.num_requests + gi];
-  const int first = p.plan[kPlanHead + b];
-  const int group = gi - p.plan[kPlanHead + p.num_requests + b];
+  if (gi >= __ldcg(p.plan + 1)) return;
+  const int b = __ldcg(p.plan + kPlanHead + 2 * p.num_requests + gi);
+  const int first = __ldcg(p.plan + kPlanHead + b);
+  const int group = gi - __ldcg(p.plan + kPlanHead + p.num_requests + b);
   bool bad;
   const Request r = load_request(p, b, bad);
   const int rows = min(kRows, r.rows - group * kRows);

@@ -53,6 +53,10 @@ SIGNATURES = {
     "dsa_tree_attention_run": (ctypes.c_int, _TREE + [_P, _P, _P, ctypes.c_size_t, _P]),
     "dsa_tree_weights_run": (ctypes.c_int, _TREE + [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_size_t,
                                                     _P]),
+    "dsa_cache_evict_run": (ctypes.c_int, [_P, ctypes.c_int64, _P, _P, _P, ctypes.c_int32, ctypes.c_int32,
+                                           ctypes.c_int32, _P, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
+                                           ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                           ctypes.c_int32, _P, _P, _P, ctypes.c_int64, _P, ctypes.c_size_t, _P]),
     "dsa_b200_test_inject": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
 }
 

@@ -3,8 +3,10 @@
 
     accumulate(q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table,
                cu_drafts, tree_mask, sm_scale, lse, acc, out) -> None
+    run(acc, seq_lens, block_table, new_block_table, ckv_cache, kpe_cache,
+        k_index_cache_fp8, num_sink, num_recent, keep, new_seq_lens, new_acc) -> None
 
-The attention weight that every cached token got from the rows of a
+``accumulate``: the attention weight that every cached token got from the rows of a
 ``dsa_b200.tree.run`` with the same arguments (``lse`` is what that call gave),
 summed over its rows and heads and added to the token's accumulator:
 
@@ -16,6 +18,21 @@ request (not by cache slot, so requests that share pages keep sums of their
 own); ``out`` may be ``acc``.  Every element of ``out`` is written.  To count
 accepted drafts only, pass their rows alone, with a ``cu_drafts`` and masks to
 match.  The sums run in a fixed order, so that results repeat.
+
+``run``: a request with more than ``budget = keep.shape[1]`` tokens keeps its
+first ``num_sink``, its last ``num_recent`` and, of the tokens between them, those
+of largest ``acc`` (equal: the earlier; NaN is largest), ``budget`` in all; the
+others keep everything.  What is kept stays in order: position ``keep[r, i]``
+(ascending, then -1) becomes position i of ``new_block_table``'s row, in the ckv
+and kpe caches and, unless it is None, in the indexer's FP8 key cache.
+``new_seq_lens`` and ``new_acc`` (float32 ``[B, new_max_pages * 64]``, 0 behind the
+kept tokens) go with the new table.
+
+The new pages are pages of the same pool that no row of ``block_table`` uses; the
+old ones are not changed, so requests may share them, and the caller frees
+them.  With ``DSA_B200_CHECK=1`` a call whose new pages are also old ones, or
+given twice, raises.  Streams, graphs and device status bits are as for
+``dsa_b200.tree``.
 """
 
 from __future__ import annotations
@@ -25,6 +42,7 @@ import torch
 from . import _native, tree, workspace
 
 PAGE_SIZE = 64
+INDEX_PAGE_BYTES = PAGE_SIZE * 128 + PAGE_SIZE * 4
 
 
 def _fail_acc(msg: str) -> None:
@@ -71,6 +89,91 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
     _native.check(st, "dsa_tree_weights_run")
     if tree._CHECK and not torch.cuda.is_current_stream_capturing():
         raise_on_device_status(dev)
+
+
+def _fail_run(msg: str) -> None:
+    raise ValueError(f"dsa_evict.run: {msg}")
+
+
+def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, new_block_table: torch.Tensor,
+        ckv_cache: torch.Tensor, kpe_cache: torch.Tensor, k_index_cache_fp8, num_sink: int, num_recent: int,
+        keep: torch.Tensor, new_seq_lens: torch.Tensor, new_acc: torch.Tensor) -> None:
+    dev = acc.device
+    if dev.type != "cuda":
+        _fail_run("tensors must be on a CUDA device")
+    for name, t in (("seq_lens", seq_lens), ("block_table", block_table), ("new_block_table", new_block_table),
+                    ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache), ("k_index_cache_fp8", k_index_cache_fp8),
+                    ("keep", keep), ("new_seq_lens", new_seq_lens), ("new_acc", new_acc)):
+        if t is not None and t.device != dev:
+            _fail_run(f"{name} is on {t.device}, expected {dev}")
+    for name, t in (("block_table", block_table), ("new_block_table", new_block_table)):
+        if t.dim() != 2 or t.shape[1] < 1 or t.shape[0] != block_table.shape[0]:
+            _fail_run(f"{name} must be [B, pages]")
+        if t.dtype != torch.int32 and t.dtype != torch.int64:
+            _fail_run(f"{name} must be int32 or int64")
+    B, max_pages = block_table.shape
+    new_pages = new_block_table.shape[1]
+    for name, t in (("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
+        if t.dtype != torch.bfloat16:
+            _fail_run(f"{name} must be bfloat16, got {t.dtype}")
+    ckv_page, ckv_row = tree._strides("ckv_cache", ckv_cache, tree.DIM_CKV, _fail_run)
+    kpe_page, kpe_row = tree._strides("kpe_cache", kpe_cache, tree.DIM_KPE, _fail_run)
+    pages = ckv_cache.shape[0]
+    if kpe_cache.shape[0] != pages:
+        _fail_run("ckv_cache and kpe_cache must hold the same number of pages")
+    if k_index_cache_fp8 is not None:
+        if k_index_cache_fp8.element_size() != 1 or not k_index_cache_fp8.is_contiguous():
+            _fail_run("k_index_cache_fp8 must be a contiguous 1-byte tensor (written in place)")
+        if k_index_cache_fp8.numel() != pages * INDEX_PAGE_BYTES:
+            _fail_run(f"k_index_cache_fp8 holds {k_index_cache_fp8.numel()} bytes, not {pages} pages of {INDEX_PAGE_BYTES}")
+        if k_index_cache_fp8.data_ptr() % 16:
+            _fail_run("k_index_cache_fp8 must be 16-byte aligned")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,):
+        _fail_run(f"seq_lens must be int32 [{B}]")
+    if new_seq_lens.dtype != torch.int32 or new_seq_lens.shape != (B,) or not new_seq_lens.is_contiguous():
+        _fail_run(f"new_seq_lens must be contiguous int32 [{B}]")
+    if keep.dtype != torch.int32 or keep.dim() != 2 or keep.shape[0] != B or not keep.is_contiguous():
+        _fail_run(f"keep must be contiguous int32 [{B}, budget]")
+    budget = keep.shape[1]
+    if not 1 <= budget <= new_pages * PAGE_SIZE:
+        _fail_run(f"a budget of {budget} tokens (keep.shape[1]) does not fit new_block_table's {new_pages} pages")
+    if num_sink < 0 or num_recent < 0 or num_sink + num_recent > budget:
+        _fail_run(f"num_sink {num_sink} and num_recent {num_recent} must fit the budget of {budget}")
+    _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_run)
+    _rows_of("new_acc", new_acc, (B, new_pages * PAGE_SIZE), _fail_run)
+    if acc.data_ptr() == new_acc.data_ptr() and B > 0:
+        _fail_run("new_acc must not be acc")
+    if B == 0:
+        return
+    if B > 65536 or max_pages > 1 << 24 or new_pages > 1 << 24:
+        _fail_run(f"{B} requests of {max_pages} pages are more than one call takes")
+    sl, bt, nbt = seq_lens.contiguous(), tree._int32(block_table), tree._int32(new_block_table)
+    check = tree._CHECK and not torch.cuda.is_current_stream_capturing()
+    if check:
+        _check_new_pages(sl, bt, nbt, budget, pages)
+    cur = _native.current_stream(dev)
+    ws = workspace.get(dev, "evict", _native.WORKSPACE_HEADER, cur)
+    st = _native.call_on(dev, _native.lib().dsa_cache_evict_run, acc.data_ptr(), _pitch(acc), sl.data_ptr(),
+                         bt.data_ptr(), nbt.data_ptr(), B, max_pages, new_pages, ckv_cache.data_ptr(), ckv_page, ckv_row,
+                         kpe_cache.data_ptr(), kpe_page, kpe_row,
+                         None if k_index_cache_fp8 is None else k_index_cache_fp8.data_ptr(), pages, budget, num_sink,
+                         num_recent, keep.data_ptr(), new_seq_lens.data_ptr(), new_acc.data_ptr(), _pitch(new_acc),
+                         ws.data_ptr(), ws.numel(), cur)
+    _native.check(st, "dsa_cache_evict_run")
+    if check:
+        raise_on_device_status(dev)
+
+
+def _check_new_pages(seq_lens, block_table, new_block_table, budget: int, pages: int) -> None:
+    """Raises if a page to be written is one that is read, or is given twice (synchronises)."""
+    def used(lens, table):
+        need = (lens.long().clamp(0, table.shape[1] * PAGE_SIZE) + PAGE_SIZE - 1) // PAGE_SIZE
+        ids = table[torch.arange(table.shape[1], device=table.device) < need[:, None]].long()
+        return torch.bincount(ids[(ids >= 0) & (ids < pages)], minlength=pages)
+
+    old, new = used(seq_lens, block_table), used(seq_lens.clamp(max=budget), new_block_table)
+    if bool(((new > 1) | ((new > 0) & (old > 0))).any()):
+        raise ValueError("dsa_evict.run: a page of new_block_table is given twice or still in use by block_table")
 
 
 def device_status(device: torch.device, clear: bool = True) -> int:

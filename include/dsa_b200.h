@@ -312,6 +312,41 @@ DSA_API int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const voi
                                  float* acc_out, int64_t acc_out_stride, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/* Evicts tokens by accumulated attention weight and moves what is kept to new
+ * pages.  Request r has seq_lens[r] tokens.  If they are more than `budget`,
+ * its first num_sink and last num_recent tokens are kept, and of those between
+ * them the ones of largest acc (equal: the earlier; NaN is largest), `budget`
+ * in all; else all are kept.  The order of the kept tokens stays.
+ *
+ *   acc               [num_requests, max_pages * 64] fp32, rows acc_stride apart
+ *   seq_lens          [num_requests] int32
+ *   block_table       [num_requests, max_pages] int32
+ *   new_block_table   [num_requests, new_max_pages] int32, budget <=
+ *                     64 * new_max_pages: pages of the same pool that no
+ *                     request's block_table row uses (several requests may
+ *                     share pages to move from: nothing there is changed)
+ *   ckv_cache, kpe_cache  as for dsa_tree_attention_run, written in place
+ *   k_index_cache_fp8 num_pages pages of 8448 bytes, or NULL
+ *   keep              [num_requests, budget] int32: the kept positions,
+ *                     ascending, then -1
+ *   new_seq_lens      [num_requests] int32
+ *   new_acc           [num_requests, new_max_pages * 64] fp32, rows
+ *                     new_acc_stride apart: acc of the kept tokens, then 0
+ *
+ * Token keep[r, i] becomes token i of the new table's row.  Data-dependent
+ * errors: a seq_len outside [0, max_pages * 64] (clamped):
+ * DSA_DEV_BAD_SEQ_LEN; a page outside the pool (its tokens are not moved):
+ * DSA_DEV_BAD_PAGE.  The workspace holds only the status word (256 bytes). */
+DSA_API int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const int32_t* seq_lens,
+                                const int32_t* block_table, const int32_t* new_block_table,
+                                int32_t num_requests, int32_t max_pages, int32_t new_max_pages,
+                                void* ckv_cache, int64_t ckv_page_bytes, int64_t ckv_row_bytes,
+                                void* kpe_cache, int64_t kpe_page_bytes, int64_t kpe_row_bytes,
+                                void* k_index_cache_fp8, int64_t num_pages, int32_t budget,
+                                int32_t num_sink, int32_t num_recent, int32_t* keep,
+                                int32_t* new_seq_lens, float* new_acc, int64_t new_acc_stride,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 /* Copies the sticky device status word of `workspace` to *status_out
  * (synchronising `stream`), and zeroes it when `clear` is non-zero.
  * No counterpart in the reference, which has no error channel

@@ -70,3 +70,37 @@ def test_cache_strides():
                 both.flatten(0, 1)[:, :512]):
         with pytest.raises(ValueError):
             tree._strides("ckv", bad, 512, fail)
+
+
+def evict_call(lib, requests=1, max_pages=4, new_pages=2, pages=9, budget=100, sink=4, recent=8, acc=16, acc_stride=256,
+               new_stride=128, ckv=16, ckv_row=1024, index=16, keep=16, nbytes=256):
+    return lib.dsa_cache_evict_run(P(acc), acc_stride, P(16), P(16), P(16), requests, max_pages, new_pages, P(ckv), 65536,
+                                   ckv_row, P(16), 8192, 128, P(index), pages, budget, sink, recent, P(keep), P(16), P(16),
+                                   new_stride, P(16), nbytes, None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(requests=-1), 1), (dict(requests=0), 0), (dict(requests=65537), 1), (dict(acc=None), 1), (dict(keep=None), 1),
+    (dict(budget=0), 1), (dict(budget=129), 1), (dict(sink=-1), 1), (dict(sink=60, recent=41), 1), (dict(pages=0), 1),
+    (dict(max_pages=0), 1), (dict(acc_stride=255), 1), (dict(new_stride=127), 1), (dict(ckv_row=1000), 1),
+    (dict(ckv_row=1032), 2), (dict(ckv=8), 2), (dict(index=8), 2), (dict(acc=18), 2), (dict(nbytes=255), 3),
+])
+def test_evict_c_abi_refuses_bad_arguments(change, status):
+    assert evict_call(_native.lib(), **change) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(lse=None), 1), (dict(acc=18), 2), (dict(stride=100), 1), (dict(out=16, out_stride=300), 1), (dict(requests=0), 0),
+])
+def test_weights_c_abi_refuses_bad_arguments(change, status):
+    a = dict(lse=16, acc=16, stride=256, out=32, out_stride=256, requests=1) | change
+    assert _native.lib().dsa_tree_weights_run(
+        P(16), P(16), P(16), 65536, 1024, P(16), 8192, 128, 3, P(16), P(16), P(16), P(16), a["requests"], 2, 16, 4, 1, 0.1,
+        P(a["lse"]), P(a["acc"]), a["stride"], P(a["out"]), a["out_stride"], P(16), 256, None) == status
+
+
+def test_evict_oracle():
+    from oracle import tree as otree
+    acc = torch.tensor([[3.0, 1.0, 2.0, 2.0, 0.0, 9.0], [float("nan"), 1, 5, 5, 5, 0]])
+    assert otree.evict_reference(acc, torch.tensor([6, 5]), 3, 1, 1) == [[0, 2, 5], [0, 2, 4]]
+    assert otree.evict_reference(acc, torch.tensor([6, 3]), 3, 0, 0) == [[0, 2, 5], [0, 1, 2]]
