@@ -67,20 +67,26 @@ constexpr int kSumTilesShared = 8;           // ... when several groups re-read 
 constexpr uint32_t kIdescS = idesc_make(1, 1, false, false, 64, 64);
 constexpr uint32_t kIdescO = idesc_make(1, 1, true, true, 128, 64);
 
+// A tile moves in two halves with barriers of their own: ckv pieces 0-3, which
+// O^T's blocks 0 and 1 need, and pieces 4-7 with kpe.
+constexpr int kHalfBytes = 4 * kChunkBytes;  // and kChunkBytes more in the second
+
 constexpr int kOffQ = 2 * kTileBytes;          // 147456
 constexpr int kOffP = kOffQ + kTileBytes;      // 221184: P, or the weights' sums
 constexpr int kOffBar = kOffP + kTok * 128;    // 229376
-constexpr int kOffMisc = kOffBar + 128;
-constexpr int kOffRed = kOffMisc + 128;        // [4][64] floats
-constexpr int kOffAlpha = kOffRed + 1024;      // [64]
-constexpr int kOffSum = kOffAlpha + 256;       // [64]
-constexpr int kOffMax = kOffSum + 256;         // [64]
+constexpr int kOffMisc = kOffBar + 192;
+constexpr int kOffRed = kOffMisc + 32;         // [4][64] floats
+constexpr int kOffFactor = kOffRed + 1024;     // [64]
+constexpr int kOffMax = kOffFactor + 256;      // [64]
 constexpr int kSmemBytes = 1024 + kOffMax + 256;
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 static_assert(2 * kSumTiles * kTok * 4 <= kTok * 128, "the weights' sums take P's place");
 
 constexpr int kMaxRequests = 65536;
-constexpr int kPlanHead = 4;                   // plan words: total units, total groups
+constexpr int kMaxCtas = 256;
+// Plan, in ints: the group of each record (-1: none), then first row and rows
+// of each group.
+constexpr int kPlanGroups = 2 * kMaxCtas;
 
 struct Params {
   const int32_t* prefix_lens;
@@ -97,7 +103,7 @@ struct Params {
   float* lse_out;
   float* part_o;    // [2 * grid][kPartFloats]
   float* part_ml;   // [2 * grid][kRows][2]
-  int* plan;        // total units, total groups, -, -, first unit [B], first group [B], request of group
+  int* plan;        // see kPlanGroups
   // weights
   const float* lse_in;
   const float* acc;
@@ -181,6 +187,7 @@ __device__ __forceinline__ Place place_of(const Request& r, int chunks, int rel)
 // A run of tiles of one group.
 struct Segment {
   int b, group, t0, t1;
+  int group_index;        // attention: over all requests
   Request r;
   bool whole;             // attention: covers the group's whole context
   int slot;               // attention: record slot if it does not
@@ -193,13 +200,14 @@ struct Walker {
   const Params& p;
   int u, u0, u1, slice;
   int b, first;           // request and its first unit
+  int first_group;        // its first group, over all requests
   Request r;
   int chunks;
   Place at;               // attention: next unit's place
   int run0, run1, end, g; // weights: current run of tiles, end of the slice's tiles, next group
 
-  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, int b0, int first_unit)
-      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(b0), first(first_unit) {
+  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, const int* found)
+      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(found[0]), first(found[1]), first_group(found[2]) {
     if (u0 < u1) enter();
   }
 
@@ -231,6 +239,7 @@ struct Walker {
   __device__ bool leave() {  // to the next request that has units in the slice
     for (;;) {
       first += r.groups * r.tiles;
+      first_group += r.groups;
       ++b;
       if (b >= p.num_requests || first >= u1) return false;
       if constexpr (!kWeights) u = first;
@@ -261,6 +270,7 @@ struct Walker {
       s.b = b;
       s.r = r;
       s.group = at.group;
+      s.group_index = first_group + at.group;
       s.t0 = at.tile;
       int len = at.t1 - at.tile;
       if (len > u1 - u) len = u1 - u;
@@ -312,24 +322,23 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   uint8_t* p_mem = smem + kOffP;
   float* sums = reinterpret_cast<float*>(p_mem);  // weights: [2 sets][kSumTiles][64]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint64_t* kv_full = bars;        // [2]
-  uint64_t* kv_empty = bars + 2;   // [2]
-  uint64_t* s_full = bars + 4;     // [2]
-  uint64_t* s_empty = bars + 6;    // [2]
-  uint64_t* q_full = bars + 8;
-  uint64_t* q_empty = bars + 9;
-  uint64_t* p_full = bars + 10;
-  uint64_t* pv_done = bars + 11;
-  uint64_t* o_empty = bars + 12;
-  uint64_t* drain = bars + 13;     // [2]
+  uint64_t* kv_full = bars;        // [2 stages][2 halves]
+  uint64_t* q_full = bars + 4;     // [2 halves]
+  uint64_t* q_empty = bars + 6;
+  uint64_t* s_full = bars + 7;     // [2]
+  uint64_t* s_empty = bars + 9;    // [2]
+  uint64_t* p_full = bars + 11;
+  uint64_t* half_done = bars + 12; // [2]: O^T blocks 0 and 1 done, the stage's first half is free
+  uint64_t* pv_done = bars + 14;   // [2]: all blocks done, the stage is free
+  uint64_t* o_empty = bars + 16;
+  uint64_t* drain = bars + 17;     // [2]
   int* misc = reinterpret_cast<int*>(smem + kOffMisc);
   uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
   int* abort_flag = misc + 1;
-  int* found = misc + 2;           // first request of the slice, its first unit
-  int* warp_sums = misc + 4;       // [11] units, then [11] groups
+  int* found = misc + 2;                     // the slice's first request, its first unit and group
   float* red = reinterpret_cast<float*>(smem + kOffRed);
-  float* alpha_s = reinterpret_cast<float*>(smem + kOffAlpha);
-  float* sum_s = reinterpret_cast<float*>(smem + kOffSum);
+  int* warp_sums = reinterpret_cast<int*>(red);  // planning: [11] units, [11] groups
+  float* factor_s = reinterpret_cast<float*>(smem + kOffFactor);  // O's rescaling; at the end 1 / l
   float* max_s = reinterpret_cast<float*>(smem + kOffMax);
 
   const int tid = threadIdx.x;
@@ -337,21 +346,13 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   const int lane = tid & 31;
 
   if (tid == 0) {
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
-      mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], kSoftWarps);
-      mbar_init(&drain[s], 1);
-    }
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    for (int x = 0; x < 19; ++x) mbar_init(&bars[x], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&s_empty[s], kSoftWarps);
     mbar_init(p_full, kSoftWarps);
-    mbar_init(pv_done, 1);
     mbar_init(o_empty, kSoftWarps);
     *abort_flag = 0;
     found[0] = p.num_requests;
-    found[1] = 0;
+    found[1] = found[2] = 0;
     fence_mbar_init();
   }
   if (warp == kLoadWarp && elect_one()) {
@@ -398,7 +399,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   // exceed what the host checked: such a call does nothing.
   const bool nothing = __syncthreads_or(decreasing);
   tc_fence_after();
-  int total = 0, total_groups = 0, before = iu - units, gbefore = ig - groups;
+  int total = 0, before = iu - units, gbefore = ig - groups;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) {
@@ -406,131 +407,144 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       gbefore += warp_sums[11 + w];
     }
     total += warp_sums[w];
-    total_groups += warp_sums[11 + w];
   }
-  if (nothing) total = total_groups = units = 0;
+  if (nothing) total = units = 0;
   const int ctas = gridDim.x;
   const int u0 = slice_start(total, blockIdx.x, ctas), u1 = slice_start(total, blockIdx.x + 1, ctas);
   const int slice = slice_len(total, ctas);
-  const bool keeper = !kWeights && blockIdx.x == 0;  // writes the plan that combine_kernel reads
-  if (keeper || (u0 >= before && u0 < before + units)) {
-    for (int b = b_lo; b < b_hi && !nothing; ++b) {
+  const bool keeper = !kWeights && blockIdx.x == 0;  // writes the groups for combine_kernel
+  if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
+    for (int b = b_lo; b < b_hi; ++b) {
       bool bad;
       const Request r = load_request(p, b, bad);
       const int un = r.groups * r.tiles;
       if (u0 >= before && u0 < before + un) {
         found[0] = b;
         found[1] = before;
+        found[2] = gbefore;
       }
       if (keeper) {
-        p.plan[kPlanHead + b] = before;
-        p.plan[kPlanHead + p.num_requests + b] = gbefore;
-        for (int g = 0; g < r.groups; ++g) p.plan[kPlanHead + 2 * p.num_requests + gbefore + g] = b;
+        int2* to = reinterpret_cast<int2*>(p.plan + kPlanGroups) + gbefore;
+        for (int g = 0; g < r.groups; ++g)
+          to[g] = make_int2(r.row0 * p.heads + g * kRows, min(kRows, r.rows - g * kRows));
       }
       before += un;
       gbefore += r.groups;
-    }
-    if (keeper && tid == 0) {
-      p.plan[0] = total;
-      p.plan[1] = total_groups;
     }
   }
   __syncthreads();
 
   const uint32_t tmem_base = *tmem_base_smem;
   const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
-  Walker<kWeights> walk(p, u0, u1, slice, found[0], found[1]);
+  Walker<kWeights> walk(p, u0, u1, slice, found);
   Segment s;
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------ loads
-    int i = 0, segs = 0;
-    bool ok = true;
-    while (ok && walk.next(s)) {
-      const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
-      int pages = 0;
-      for (int t = s.t0; t < s.t1 && ok; ++t, ++i) {
-        const int k = (t - s.t0) & 31;
-        if (k == 0) pages = t + lane < s.t1 ? __ldg(row + t + lane) : 0;
-        int page = __shfl_sync(0xffffffffu, pages, k);
-        // A page outside the pool reads as zeros (a box outside the tensor
-        // is filled with them); its tokens are masked below.
-        if (page < 0 || page >= p.num_pages) page = p.num_pages;
-        const int st = i & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((i >> 1) & 1) ^ 1, wctx));
-        if (!ok) break;
-        if (elect_one()) {
+    // This role and the next two are one thread each: a warp-wide wait before
+    // every issue (vote, re-election) costs some 250 clocks, a thread's own
+    // about 60, and the tensor pipe idles meanwhile.
+    if (elect_one()) {
+      int i = 0, segs = 0;
+      int halves = 0, q_halves = 0;  // issued
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+        int next_page = __ldg(row + s.t0);
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          // A page outside the pool reads as zeros (a box outside the tensor
+          // is filled with them); its tokens are masked below.
+          const int page = next_page < 0 || next_page >= p.num_pages ? p.num_pages : next_page;
+          if (t + 1 < s.t1) next_page = __ldg(row + t + 1);
+          const int st = i & 1;
+          const uint32_t parity = ((i >> 1) & 1) ^ 1;
           uint8_t* dst = smem + st * kTileBytes;
-          mbar_arrive_expect_tx(&kv_full[st], kTileBytes);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) tma_load_3d(dst + c * kChunkBytes, &ckv_map, &kv_full[st], c * 64, 0, page);
-          tma_load_3d(dst + 8 * kChunkBytes, &kpe_map, &kv_full[st], 0, 0, page);
-        }
-        if (t == s.t0) {
-          // The group's queries, behind its first tile.  Rows behind the
-          // request's own are another's or zeros; their columns are never
-          // written out.
-          ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (segs & 1) ^ 1, wctx));
-          if (!ok) {
-            ++i;
-            break;
-          }
-          const int row_q = s.r.row0 * p.heads + s.group * kRows;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(q_full, kTileBytes);
+          for (int h = 0; h < 2; ++h) {
+            // The weights' S^T alone reads a stage.
+            uint64_t* free_bar = kWeights ? &s_full[st] : (h == 0 ? &half_done[st] : &pv_done[st]);
+            ok = ok && mbar_wait(free_bar, parity, wctx);
+            if (!ok) break;
+            uint64_t* bar = &kv_full[2 * st + h];
+            mbar_arrive_expect_tx(bar, kHalfBytes + h * kChunkBytes);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) tma_load_2d(q_mem + c * kChunkBytes, &qn_map, q_full, c * 64, row_q);
-            tma_load_2d(q_mem + 8 * kChunkBytes, &qp_map, q_full, 0, row_q);
+            for (int c = 4 * h; c < 4 * h + 4; ++c)
+              tma_load_3d(dst + c * kChunkBytes, &ckv_map, bar, c * 64, 0, page);
+            if (h == 1) tma_load_3d(dst + 8 * kChunkBytes, &kpe_map, bar, 0, 0, page);
+            ++halves;
           }
-          ++segs;
+          if (t == s.t0 && ok) {
+            // The group's queries, behind its first tile.  Rows behind the
+            // request's own are another's or zeros; their columns are never
+            // written out.
+            const int row_q = s.r.row0 * p.heads + s.group * kRows;
+            ok = mbar_wait(q_empty, (segs & 1) ^ 1, wctx);
+            if (ok) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                mbar_arrive_expect_tx(&q_full[h], kHalfBytes + h * kChunkBytes);
+#pragma unroll
+                for (int c = 4 * h; c < 4 * h + 4; ++c)
+                  tma_load_2d(q_mem + c * kChunkBytes, &qn_map, &q_full[h], c * 64, row_q);
+                if (h == 1) tma_load_2d(q_mem + 8 * kChunkBytes, &qp_map, &q_full[h], 0, row_q);
+                ++q_halves;
+              }
+              ++segs;
+            }
+          }
+          if (!ok) break;
         }
       }
+      // Copies still in flight (after an abort) land before the CTA exits: of
+      // each half the last two, whose phases nothing refills.
+      for (int h = 0; h < 2; ++h) {
+        const int tiles = (halves + 1 - h) / 2;
+        for (int k = tiles - 1; k >= 0 && k >= tiles - 2; --k)
+          mbar_drain(&kv_full[2 * (k & 1) + h], (k >> 1) & 1, p.status);
+        const int qs = (q_halves + 1 - h) / 2;
+        if (qs >= 1) mbar_drain(&q_full[h], (qs - 1) & 1, p.status);
+      }
     }
-    // Copies still in flight (after an abort) land before the CTA exits: the
-    // last one of each stage and of Q, whose phases nothing refills.
-    if (lane == 0) {
-      if (i >= 1) mbar_drain(&kv_full[(i - 1) & 1], ((i - 1) >> 1) & 1, p.status);
-      if (i >= 2) mbar_drain(&kv_full[(i - 2) & 1], ((i - 2) >> 1) & 1, p.status);
-      if (segs >= 1) mbar_drain(q_full, (segs - 1) & 1, p.status);
-    }
+    __syncwarp();
   } else if (warp == kLogitWarp) {
     // ------------------------------------------------------------ S^T = K Q^T
-    const uint64_t k_desc = sdesc_sw128(smem_u32(smem), 16, 1024);
-    const uint64_t q_desc = sdesc_sw128(smem_u32(q_mem), 16, 1024);
-    int i = 0, segs = 0;
-    bool ok = true;
-    while (ok && walk.next(s)) {
-      for (int t = s.t0; t < s.t1; ++t, ++i) {
-        const int st = i & 1;
-        if (t == s.t0) ok = mbar_wait(q_full, segs & 1, wctx);
-        ok = ok && mbar_wait(&kv_full[st], (i >> 1) & 1, wctx);
-        ok = ok && mbar_wait(&s_empty[st], ((i >> 1) & 1) ^ 1, wctx);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
+    if (elect_one()) {
+      const uint64_t k_desc = sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t q_desc = sdesc_sw128(smem_u32(q_mem), 16, 1024);
+      int i = 0, segs = 0;
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1;
           const uint64_t a = k_desc + st * (kTileBytes >> 4);
           const uint32_t d = tmem_base + kColS + 64u * st;
+          ok = mbar_wait(&s_empty[st], ((i >> 1) & 1) ^ 1, wctx);
 #pragma unroll
-          for (int k = 0; k < 4 * kChunks; ++k)  // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
-            umma_bf16(d, a + (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2,
-                      q_desc + (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2, kIdescS, k > 0 ? 1u : 0u);
+          for (int h = 0; h < 2; ++h) {
+            if (t == s.t0) ok = ok && mbar_wait(&q_full[h], segs & 1, wctx);
+            ok = ok && mbar_wait(&kv_full[2 * st + h], (i >> 1) & 1, wctx);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 16 * h; k < 16 + 20 * h; ++k) {
+              // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
+              const uint32_t at = (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2;
+              umma_bf16(d, a + at, q_desc + at, kIdescS, k > 0 ? 1u : 0u);
+            }
+          }
+          if (!ok) break;
           umma_commit(&s_full[st]);
           if (t == s.t1 - 1) umma_commit(q_empty);
-          if (kWeights) umma_commit(&kv_empty[st]);
         }
-        __syncwarp();
+        ++segs;
       }
-      ++segs;
-    }
-    if (elect_one()) {
       umma_commit(&drain[0]);
       mbar_drain(&drain[0], 0, p.status);
     }
     __syncwarp();
   } else if (warp == kValueWarp) {
     // ------------------------------------------------------------ O^T += V^T P^T
-    if constexpr (!kWeights) {
+    if (!kWeights && elect_one()) {
       const uint64_t v_desc = sdesc_sw128(smem_u32(smem), kChunkBytes, 1024);
       const uint64_t p_desc = sdesc_sw128(smem_u32(p_mem), kChunkBytes, 1024);
       int i = 0, segs = 0;
@@ -538,33 +552,28 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       while (ok && walk.next(s)) {
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           const int st = i & 1;
-          ok = mbar_wait(p_full, i & 1, wctx);
-          if (t == s.t0) ok = ok && mbar_wait(o_empty, (segs & 1) ^ 1, wctx);
-          ok = __all_sync(0xffffffffu, ok);
+          if (t == s.t0) ok = mbar_wait(o_empty, (segs & 1) ^ 1, wctx);
+          ok = ok && mbar_wait(p_full, i & 1, wctx);
           if (!ok) break;
           tc_fence_after();
           const uint32_t more = t == s.t0 ? 0u : 1u;
-          if (elect_one()) {
-            const uint64_t a = v_desc + st * (kTileBytes >> 4);
+          const uint64_t a = v_desc + st * (kTileBytes >> 4);
 #pragma unroll
-            for (int mb = 0; mb < 4; ++mb)
+          for (int mb = 0; mb < 4; ++mb) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)  // 128 dims are two pieces; a K16 step is 16 token rows of 128 bytes
-                umma_bf16(tmem_base + kColO + 64u * mb, a + mb * (2 * kChunkBytes >> 4) + kk * (2048 >> 4),
-                          p_desc + kk * (2048 >> 4), kIdescO, kk > 0 ? 1u : more);
-            umma_commit(&kv_empty[st]);
-            umma_commit(pv_done);
+            for (int kk = 0; kk < 4; ++kk)  // 128 dims are two pieces; a K16 step is 16 token rows of 128 bytes
+              umma_bf16(tmem_base + kColO + 64u * mb, a + mb * (2 * kChunkBytes >> 4) + kk * (2048 >> 4),
+                        p_desc + kk * (2048 >> 4), kIdescO, kk > 0 ? 1u : more);
+            if (mb == 1) umma_commit(&half_done[st]);
           }
-          __syncwarp();
+          umma_commit(&pv_done[st]);
         }
         ++segs;
       }
-      if (elect_one()) {
-        umma_commit(&drain[1]);
-        mbar_drain(&drain[1], 0, p.status);
-      }
-      __syncwarp();
+      umma_commit(&drain[1]);
+      mbar_drain(&drain[1], 0, p.status);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
     // Set `set` of four warps has the columns (query rows) 32 set .. +31 of
@@ -666,6 +675,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       // P <= 2^8 then, and l adds P in fp32.  P is rounded to bf16 for the
       // MMA (off by at most 2^-9 of itself, independently per token; l uses
       // the unrounded values), as any bf16 tensor-core product needs.
+      int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
+      if (tid == 0) group_of[0] = group_of[1] = -1;
       while (walk.next(s)) {
         float m[8], l[8];
         int draft[8];
@@ -729,12 +740,12 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
                 m[k] = mt;
               }
               l[k] *= alpha;
-              if (sp == 0 && lane < 4) alpha_s[col(k)] = alpha;
+              if (sp == 0 && lane < 4) factor_s[col(k)] = alpha;
             }
             named_barrier_sync(1 + set, 128);
             if (t > s.t0) {
               // O holds PV(i - 1) before it is rescaled.
-              ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+              ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
               tc_fence_after();
 #pragma unroll 1
               for (int mb = 0; mb < 4; ++mb) {
@@ -745,7 +756,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
                   tmem_ld16(at, o);
                   tmem_wait_ld();
 #pragma unroll
-                  for (int c = 0; c < 16; ++c) o[c] *= alpha_s[32 * set + 16 * h + c];
+                  for (int c = 0; c < 16; ++c) o[c] *= factor_s[32 * set + 16 * h + c];
                   tmem_st16(at, o);
                 }
               }
@@ -758,7 +769,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             // among them into NaN.  The logits have been read (S^T is done),
             // so such values are zeroed in the V tile; a row that does see
             // one has its NaN from the logit.
-            ok = ok && mbar_wait(&kv_full[st], (i >> 1) & 1, wctx);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ok = ok && mbar_wait(&kv_full[2 * st + h], (i >> 1) & 1, wctx);
             const int from = s.r.prefix > t * kTok ? s.r.prefix - t * kTok : 0;
             for (int q = tid; q < (kTok - from) * 64; q += 32 * kSoftWarps) {
               // 16-byte piece q & 7 of row from + (q >> 6) in piece (q >> 3) & 7
@@ -799,7 +811,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             p1[k >> 1] = *reinterpret_cast<const uint32_t*>(&pc);
           }
           // P was last read by PV(i - 1).
-          if (i > 0) ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+          if (i > 0) ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
           {
             // One 128-byte row per token, 16-byte pieces swizzled by token & 7
             // (the same for r0 and r0 + 8): a warp's stores meet no bank twice.
@@ -833,17 +845,18 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
         const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kRows;
         const int rows = min(kRows, s.r.rows - s.group * kRows);  // of the group
         const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + s.slot;
+        if (tid == 0 && !s.whole) group_of[s.slot] = s.group_index;
         if (e < 32) {
           const int c = 32 * set + e;
           const float sum = (red[c] + red[kRows + c]) + (red[2 * kRows + c] + red[3 * kRows + c]);
           if (s.whole) {
-            sum_s[c] = sum == 0.f ? 0.f : 1.f / sum;
+            factor_s[c] = sum == 0.f ? 0.f : 1.f / sum;
             if (c < rows) p.lse_out[row_q + c] = sum == 0.f ? -INFINITY : max_s[c] + log2f(sum);
           } else {
             *reinterpret_cast<float2*>(p.part_ml + (rec * kRows + c) * 2) = make_float2(max_s[c], sum);
           }
         }
-        ok = ok && mbar_wait(pv_done, (i - 1) & 1, wctx);
+        ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
         named_barrier_sync(1 + set, 128);
         tc_fence_after();
 #pragma unroll 1
@@ -858,7 +871,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             __nv_bfloat16* out = p.out + row_q * kCkv + (dim & ~1);
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              const float a = o[c] * sum_s[32 * set + c], b = o[c + 1] * sum_s[32 * set + c + 1];
+              const float a = o[c] * factor_s[32 * set + c], b = o[c + 1] * factor_s[32 * set + c + 1];
               const float got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
               const int row = 32 * set + c + (odd ? 1 : 0);
               if (row < rows)
@@ -889,112 +902,109 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 
 // Joins the records of a group that several slices share: per row
 //   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L,
-// in slice order.  Block (group, y) has rows 4y .. 4y + 3, a thread four dims
-// of each.
-constexpr int kJoinRows = 4;
-constexpr int kMaxCtas = 256;
+// in an order that the slices alone give.  Block x has the group x, or where
+// groups outnumber records the group of record x if x is its first one;
+// block y its rows y * rows_per_block ...  Two half blocks take every other
+// record of a row, a thread four dims: the loads are latency-bound, so many
+// are in flight at once.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 8;       // most rows per block: one warp finds a row's weights
+constexpr int kJoinDepth = 8;      // records whose loads a thread has in flight
 
-__global__ void __launch_bounds__(128) combine_kernel(const Params p, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads)
+combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   griddep_wait();
   __shared__ int recs[2 * kMaxCtas];
   __shared__ float weight[kJoinRows][2 * kMaxCtas];
-  __shared__ int warp_count[4];
-  const int total = __ldcg(p.plan);
-  const int gi = blockIdx.x;
-  if (gi >= __ldcg(p.plan + 1)) return;
-  const int b = __ldcg(p.plan + kPlanHead + 2 * p.num_requests + gi);
-  const int first = __ldcg(p.plan + kPlanHead + b);
-  const int group = gi - __ldcg(p.plan + kPlanHead + p.num_requests + b);
-  bool bad;
-  const Request r = load_request(p, b, bad);
-  const int rows = min(kRows, r.rows - group * kRows);
-  const int y0 = blockIdx.y * kJoinRows;
-  if (y0 >= rows) return;
-  const int chunks = chunks_of(r, slice_len(total, ctas));
-  if (chunks == 1) {
-    const int a = first + group * r.tiles;
-    if (slice_of(total, a, ctas) == slice_of(total, a + r.tiles - 1, ctas)) return;  // written whole
-  }
+  __shared__ int warp_count[2][kJoinThreads / 32];
+  __shared__ float4 other[kCkv / 4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // The records that belong to this group, in slice order.
-  const int c_lo = slice_of(total, first, ctas), c_hi = slice_of(total, first + r.groups * r.tiles - 1, ctas);
-  int count = 0;
-  for (int base = 2 * c_lo; base < 2 * (c_hi + 1); base += 128) {
-    const int cand = base + tid, c = cand >> 1;
-    bool mine = false;
-    if (c <= c_hi) {
-      const int u0 = slice_start(total, c, ctas), u1 = slice_start(total, c + 1, ctas);
-      const int u = (cand & 1) ? u1 - 1 : u0;
-      if (u0 < u1 && u >= first && u < first + r.groups * r.tiles) {
-        const Place q = place_of(r, chunks, u - first);
-        mine = q.group == group;
-        if (cand & 1)  // the last piece, unless it is the first one too
-          mine = mine && first + r.groups * q.t0 + q.group * (q.t1 - q.t0) > u0;
-      }
-    }
-    const unsigned int votes = __ballot_sync(0xffffffffu, mine);
-    if (lane == 0) warp_count[warp] = __popc(votes);
-    __syncthreads();
-    int at = count + __popc(votes & ((1u << lane) - 1u));
-    for (int w = 0; w < 4; ++w) {
-      if (w < warp) at += warp_count[w];
-      count += warp_count[w];
-    }
-    if (mine) recs[at] = cand;
-    __syncthreads();
+  const int x = blockIdx.x;
+  const int group = by_record ? __ldcg(p.plan + x) : x;
+  int mine[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = tid + k * kJoinThreads;
+    mine[k] = r < 2 * ctas ? __ldcg(p.plan + r) : -1;
   }
-  {
-    // Warp w: the weights of row y0 + w.
-    const int row = y0 + warp;
-    float M = -INFINITY, L = 0.f;
-    if (row < rows) {
-      for (int k = lane; k < count; k += 32)
-        M = fmaxf(M, __ldcg(p.part_ml + (static_cast<int64_t>(recs[k]) * kRows + row) * 2));
+  if (group < 0) return;
+  const int2 info = __ldcg(reinterpret_cast<const int2*>(p.plan + kPlanGroups) + group);
+  unsigned int votes[2];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      for (int k = lane; k < count; k += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(
-            p.part_ml + (static_cast<int64_t>(recs[k]) * kRows + row) * 2));
-        const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-        L = fmaf(ml.y, w, L);
-        weight[warp][k] = w;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      __syncwarp();
-      for (int k = lane; k < count; k += 32) weight[warp][k] *= inv;
-      if (lane == 0)
-        p.lse_out[static_cast<int64_t>(r.row0) * p.heads + group * kRows + row] =
-            L == 0.f ? -INFINITY : M + log2f(L);
-    }
+  for (int k = 0; k < 2; ++k) {
+    votes[k] = __ballot_sync(0xffffffffu, mine[k] == group);
+    if (lane == 0) warp_count[k][warp] = __popc(votes[k]);
   }
   __syncthreads();
-  float4 acc[kJoinRows];
+  int count = 0;
 #pragma unroll
-  for (int y = 0; y < kJoinRows; ++y) acc[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int k = 0; k < count; ++k) {
-    const float4* src = reinterpret_cast<const float4*>(p.part_o + static_cast<int64_t>(recs[k]) * kPartFloats) + tid;
+  for (int k = 0; k < 2; ++k) {
+    int at = count;
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+      if (w < warp) at += warp_count[k][w];
+      count += warp_count[k][w];
+    }
+    if (mine[k] == group) recs[at + __popc(votes[k] & ((1u << lane) - 1u))] = tid + k * kJoinThreads;
+  }
+  __syncthreads();
+  if (count == 0 || (by_record && recs[0] != x)) return;  // written whole; or another block's
+  const int y0 = blockIdx.y * rows_per_block;
+  const int rows = min(rows_per_block, info.y - y0);
+  if (rows <= 0) return;
+  if (warp < rows) {
+    float M = -INFINITY, L = 0.f;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + y0 + warp;
+    for (int k = lane; k < count; k += 32) {
+      const float2 v = __ldcg(ml + static_cast<int64_t>(recs[k]) * kRows);
+      M = fmaxf(M, v.x);
+      weight[warp][k] = v.x;
+    }
 #pragma unroll
-    for (int y = 0; y < kJoinRows; ++y) {
-      if (y0 + y < rows) {
-        const float4 v = __ldcg(src + (y0 + y) * (kCkv / 4));
-        const float w = weight[y][k];
-        acc[y].x = fmaf(v.x, w, acc[y].x);
-        acc[y].y = fmaf(v.y, w, acc[y].y);
-        acc[y].z = fmaf(v.z, w, acc[y].z);
-        acc[y].w = fmaf(v.w, w, acc[y].w);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int k = lane; k < count; k += 32) {
+      const float m = weight[warp][k], l = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kRows].y);
+      const float w = m == -INFINITY ? 0.f : exp2f(m - M);
+      L = fmaf(l, w, L);
+      weight[warp][k] = w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    __syncwarp();
+    for (int k = lane; k < count; k += 32) weight[warp][k] *= inv;
+    if (lane == 0) p.lse_out[info.x + y0 + warp] = L == 0.f ? -INFINITY : M + log2f(L);
+  }
+  __syncthreads();
+  const int half = tid >> 7, d4 = tid & 127;
+  for (int y = 0; y < rows; ++y) {
+    const float4* src = reinterpret_cast<const float4*>(p.part_o) + (y0 + y) * (kCkv / 4) + d4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = half; k0 < count; k0 += 2 * kJoinDepth) {
+      float4 v[kJoinDepth];
+#pragma unroll
+      for (int j = 0; j < kJoinDepth; ++j)
+        if (k0 + 2 * j < count) v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + 2 * j]) * (kPartFloats / 4));
+#pragma unroll
+      for (int j = 0; j < kJoinDepth; ++j) {
+        if (k0 + 2 * j < count) {
+          const float w = weight[y][k0 + 2 * j];
+          acc.x = fmaf(v[j].x, w, acc.x);
+          acc.y = fmaf(v[j].y, w, acc.y);
+          acc.z = fmaf(v[j].z, w, acc.z);
+          acc.w = fmaf(v[j].w, w, acc.w);
+        }
       }
     }
-  }
-#pragma unroll
-  for (int y = 0; y < kJoinRows; ++y) {
-    if (y0 + y < rows) {
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc[y].x, acc[y].y), __floats2bfloat162_rn(acc[y].z, acc[y].w)};
-      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(r.row0) * p.heads + group * kRows + y0 + y) * kCkv +
-                                4 * tid) = *reinterpret_cast<const uint2*>(h);
+    if (half == 1) other[d4] = acc;
+    __syncthreads();
+    if (half == 0) {
+      const float4 o = other[d4];
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x + o.x, acc.y + o.y),
+                             __floats2bfloat162_rn(acc.z + o.z, acc.w + o.w)};
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(info.x) + y0 + y) * kCkv + 4 * d4) =
+          *reinterpret_cast<const uint2*>(h);
     }
+    __syncthreads();
   }
 }
 
@@ -1018,7 +1028,7 @@ inline Layout layout(int64_t drafts, int64_t heads, int64_t requests, int sms) {
   a.plan = a.part_o + static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
   // Rounded up generously, so that ordinary batches all need the same bytes
   // and a workspace does not move between them.
-  size_t words = kPlanHead + 2 * static_cast<size_t>(requests) + static_cast<size_t>(groups_bound(drafts, heads, requests));
+  size_t words = kPlanGroups + 2 * static_cast<size_t>(groups_bound(drafts, heads, requests));
   words = (words + 65535) / 65536 * 65536;
   a.bytes = a.plan + words * sizeof(int);
   return a;
@@ -1140,10 +1150,14 @@ extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, cons
   if (launch_programmatic(tree::tree_kernel<false>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
                           maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
     return DSA_ERR_CUDA;
-  const unsigned int groups =
-      static_cast<unsigned int>(tree::groups_bound(num_drafts, num_heads, num_requests));
-  if (launch_programmatic(tree::combine_kernel, dim3(groups, tree::kRows / tree::kJoinRows), dim3(128), 0, s, prm,
-                          info.num_sms) != cudaSuccess)
+  // Few groups: a block per row, so that a long context's many records are
+  // read by many SMs; many groups: few records each, and fewer blocks.
+  const int64_t groups = tree::groups_bound(num_drafts, num_heads, num_requests);
+  const bool by_record = groups > 2 * info.num_sms;
+  const unsigned int across = static_cast<unsigned int>(by_record ? 2 * info.num_sms : groups);
+  const int rows = across <= 32 ? 1 : (across <= 64 ? 2 : (across <= 128 ? 4 : tree::kJoinRows));
+  if (launch_programmatic(tree::combine_kernel, dim3(across, tree::kRows / rows), dim3(tree::kJoinThreads), 0, s, prm,
+                          info.num_sms, rows, by_record) != cudaSuccess)
     return DSA_ERR_CUDA;
   if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   return DSA_OK;
