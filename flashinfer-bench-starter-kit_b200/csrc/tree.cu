@@ -614,6 +614,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           draft[k] = in ? row / p.heads : 0;
           if (in && lse[k] != -INFINITY) live |= 1u << k;  // a row that saw nothing gives nothing
         }
+        const bool all_live = __all_sync(0xffffffffu, live == 0xffu);
         const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
         int next_page = __ldg(bt + s.t0);
         for (int t = s.t0; t < s.t1; ++t, ++i) {
@@ -621,10 +622,12 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           const int page = next_page;
           if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
           uint32_t see0 = live, see1 = live;
-          if (page < 0 || page >= p.num_pages) {
+          const bool lost = page < 0 || page >= p.num_pages;
+          const bool tail = (t + 1) * kTok > s.r.prefix;
+          if (lost) {
             see0 = see1 = 0;
             if (e == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
-          } else if ((t + 1) * kTok > s.r.prefix) {
+          } else if (tail) {
             const int pos = t * kTok + r0;
             if (pos >= s.r.prefix) see0 &= visible_columns(p, s, pos, draft);
             if (pos + 8 >= s.r.prefix) see1 &= visible_columns(p, s, pos + 8, draft);
@@ -640,10 +643,21 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int f = 4 * (k >> 1) + (k & 1);
-            const float a = ex2_approx(fmaf(v[f], p.scale_log2, -lse[k]));
-            const float c = ex2_approx(fmaf(v[f + 2], p.scale_log2, -lse[k]));
-            w0 += (see0 >> k) & 1 ? a : 0.f;
-            w1 += (see1 >> k) & 1 ? c : 0.f;
+            v[f] = ex2_approx(fmaf(v[f], p.scale_log2, -lse[k]));
+            v[f + 2] = ex2_approx(fmaf(v[f + 2], p.scale_log2, -lse[k]));
+          }
+          if (all_live && !tail && !lost) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              w0 += v[4 * (k >> 1) + (k & 1)];
+              w1 += v[4 * (k >> 1) + (k & 1) + 2];
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              w0 += (see0 >> k) & 1 ? v[4 * (k >> 1) + (k & 1)] : 0.f;
+              w1 += (see1 >> k) & 1 ? v[4 * (k >> 1) + (k & 1) + 2] : 0.f;
+            }
           }
           w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
           w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
@@ -673,19 +687,26 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       // segment's first tile), which one OR-barrier per tile tells the set;
       // only then is the tile's max reduced over the tokens and O rescaled.
       // P <= 2^8 then, and l adds P in fp32.  P is rounded to bf16 for the
-      // MMA (off by at most 2^-9 of itself, independently per token; l uses
+      // MMA (off by at most 2^-8 of itself, independently per token; l uses
       // the unrounded values), as any bf16 tensor-core product needs.
+      // A tile's path from S^T to P is what its K stage waits for, so the
+      // ordinary tile takes one FMA, one max and one exponential a value:
+      // d = s * scale - m, masked in the tiles that need it only.
       int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
       if (tid == 0) group_of[0] = group_of[1] = -1;
       while (walk.next(s)) {
-        float m[8], l[8];
+        float m[8], minus[8], l[8];  // minus: -m, or 0 while the column has seen nothing
         int draft[8];
+        bool unset = false;          // some column of this thread has seen nothing yet
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          m[k] = -INFINITY;
-          l[k] = 0.f;
           const int row = s.group * kRows + col(k);
-          draft[k] = row < s.r.rows ? row / p.heads : 0;
+          const bool in = row < s.r.rows;
+          m[k] = in ? -INFINITY : 0.f;
+          minus[k] = in ? 0.f : -INFINITY;  // no row of the group: all weights 0
+          l[k] = 0.f;
+          draft[k] = in ? row / p.heads : 0;
+          unset |= in;
         }
         const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
         int next_page = __ldg(bt + s.t0);
@@ -695,7 +716,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
           uint32_t see0 = 0xffu, see1 = 0xffu;
           const bool tail = (t + 1) * kTok > s.r.prefix;
-          if (page < 0 || page >= p.num_pages) {
+          const bool lost = page < 0 || page >= p.num_pages;
+          if (lost) {
             see0 = see1 = 0;
             if (e == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
           } else if (tail) {
@@ -710,26 +732,37 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[st]);
-          float x0[8], x1[8];
-          bool need = false;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int f = 4 * (k >> 1) + (k & 1);
-            x0[k] = (see0 >> k) & 1 ? v[f] * p.scale_log2 : -INFINITY;
-            x1[k] = (see1 >> k) & 1 ? v[f + 2] * p.scale_log2 : -INFINITY;
-            const float over = m[k] + kRescaleThreshold;
-            need |= x0[k] > over || x1[k] > over;
-          }
-          if (named_barrier_or(1 + set, 128, need)) {
+          float d0[8], d1[8];  // tokens r0 and r0 + 8
+          auto differences = [&]() {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              float mt = fmaxf(x0[k], x1[k]);
+              const int f = 4 * (k >> 1) + (k & 1);
+              d0[k] = fmaf(v[f], p.scale_log2, minus[k]);
+              d1[k] = fmaf(v[f + 2], p.scale_log2, minus[k]);
+            }
+            if (tail || lost) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                if (!((see0 >> k) & 1)) d0[k] = -INFINITY;
+                if (!((see1 >> k) & 1)) d1[k] = -INFINITY;
+              }
+            }
+          };
+          differences();
+          float most = d0[0];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) most = fmaxf(most, fmaxf(d0[k], d1[k]));
+          if (named_barrier_or(1 + set, 128, unset || most > kRescaleThreshold)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float mt = fmaxf(d0[k], d1[k]) - minus[k];
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
               if (lane < 4) red[kRows * sp + col(k)] = mt;
             }
             named_barrier_sync(1 + set, 128);
+            unset = false;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float* r = red + col(k);
@@ -738,10 +771,13 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
               if (mt > m[k] + kRescaleThreshold) {
                 alpha = exp2f(m[k] - mt);  // 0 when m was -inf
                 m[k] = mt;
+                minus[k] = -mt;
               }
               l[k] *= alpha;
+              unset |= m[k] == -INFINITY;
               if (sp == 0 && lane < 4) factor_s[col(k)] = alpha;
             }
+            differences();
             named_barrier_sync(1 + set, 128);
             if (t > s.t0) {
               // O holds PV(i - 1) before it is rescaled.
@@ -799,11 +835,10 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             float a[2], c[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              // m == -inf: the column has seen nothing yet and every x is
-              // -inf (weight 0) or NaN (kept).
-              const float mm = m[k + h] == -INFINITY ? 0.f : m[k + h];
-              a[h] = ex2_approx(x0[k + h] - mm);
-              c[h] = ex2_approx(x1[k + h] - mm);
+              // A column that has seen nothing has only -inf (weight 0) and
+              // NaN (kept) here.
+              a[h] = ex2_approx(d0[k + h]);
+              c[h] = ex2_approx(d1[k + h]);
               l[k + h] += a[h] + c[h];
             }
             const __nv_bfloat162 pa = __floats2bfloat162_rn(a[0], a[1]), pc = __floats2bfloat162_rn(c[0], c[1]);
