@@ -75,7 +75,7 @@ constexpr int kOffQ = 2 * kTileBytes;          // 147456
 constexpr int kOffP = kOffQ + kTileBytes;      // 221184: P, or the weights' sums
 constexpr int kOffBar = kOffP + kTok * 128;    // 229376
 constexpr int kOffMisc = kOffBar + 192;
-constexpr int kOffRed = kOffMisc + 32;         // [4][64] floats
+constexpr int kOffRed = kOffMisc + 96;         // [4][64] floats
 constexpr int kOffFactor = kOffRed + 1024;     // [64]
 constexpr int kOffMax = kOffFactor + 256;      // [64]
 constexpr int kSmemBytes = 1024 + kOffMax + 256;
@@ -114,10 +114,18 @@ struct Params {
 struct Request {
   int prefix, n, row0;  // cached tokens, drafts, first draft's row
   int rows, groups, tiles;
+  int span;             // units per group: its tiles and, for the attention, kLead more
 };
+
+// Starting a group (its queries, the pipeline's first tile, O's way out) takes
+// about as long as two more tiles.  So a group counts kLead units more than
+// its tiles, at its start, when slices are cut: short contexts then share
+// SMs evenly (64 x 65536 tokens: no change).
+constexpr int kLead = 2;
 
 // Request b as its inputs give it; what they give wrongly is clamped or, if
 // it cannot be, taken as a request without drafts.
+template <bool kWeights>
 __device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
   Request r;
   const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
@@ -142,47 +150,52 @@ __device__ __forceinline__ Request load_request(const Params& p, int b, bool& ba
   r.rows = r.n * p.heads;
   r.groups = (r.rows + kRows - 1) / kRows;
   r.tiles = r.n == 0 ? 0 : (r.prefix + r.n + kTok - 1) / kTok;
+  r.span = r.n == 0 || kWeights ? r.tiles : r.tiles + kLead;
   return r;
 }
 
-// Slice boundaries: CTA c of `ctas` has units [start(c), start(c+1)).
+// Slice boundaries: CTA c of `ctas` has units [start(c), start(c+1)), with
+// start(c) = floor(total * c / ctas) in 32-bit steps.
 __device__ __forceinline__ int slice_start(int total, int c, int ctas) {
-  return static_cast<int>(static_cast<int64_t>(total) * c / ctas);
+  const int q = total / ctas;
+  return q * c + (total - q * ctas) * c / ctas;
 }
-// The CTA whose slice holds unit u: the largest c with start(c) <= u.
-__device__ __forceinline__ int slice_of(int total, int u, int ctas) {
-  return static_cast<int>((static_cast<int64_t>(u + 1) * ctas - 1) / total);
-}
-__device__ __forceinline__ int slice_len(int total, int ctas) { return (total + ctas - 1) / ctas; }
+__device__ __forceinline__ int slice_len(int total, int ctas) { return total / ctas + (total % ctas != 0); }
 
-// Tiles are cut into `chunks_of` nearly equal chunks, each at least a slice
-// long (one chunk when a single group would walk them all anyway).
+// A group's units are cut into `chunks_of` nearly equal chunks, each at least
+// a slice long (one chunk when a single group would walk them all anyway).
+// There are at most half as many as CTAs, so the products below fit 32 bits.
 __device__ __forceinline__ int chunks_of(const Request& r, int slice) {
   if (r.groups <= 1) return 1;
-  const int c = r.tiles / slice;
+  const int c = r.span / slice;
   return c < 1 ? 1 : c;
 }
-__device__ __forceinline__ int chunk_start(const Request& r, int chunks, int c) {
-  return static_cast<int>(static_cast<int64_t>(r.tiles) * c / chunks);
-}
+__device__ __forceinline__ int chunk_start(const Request& r, int chunks, int c) { return r.span * c / chunks; }
 
-// The position of unit `rel` (counted from its request's first): chunk,
-// group and tile.
+// The place of unit `rel`, counted from its request's first.
 struct Place {
-  int chunk, group, tile, t0, t1;  // t0, t1: the chunk's tiles
+  int chunk, group, unit, u0, u1;  // unit of the group; u0, u1: the chunk's units
 };
 __device__ __forceinline__ Place place_of(const Request& r, int chunks, int rel) {
   Place q;
-  const int t = rel / r.groups;  // rel = groups * t0 + ...: the chunk is the one holding tile t
-  q.chunk = static_cast<int>((static_cast<int64_t>(t + 1) * chunks - 1) / r.tiles);
-  q.t0 = chunk_start(r, chunks, q.chunk);
-  q.t1 = chunk_start(r, chunks, q.chunk + 1);
-  const int in = rel - r.groups * q.t0;
-  const int len = q.t1 - q.t0;
+  const int t = rel / r.groups;  // rel = groups * u0 + ...: the chunk is the one holding unit t
+  q.chunk = ((t + 1) * chunks - 1) / r.span;
+  q.u0 = chunk_start(r, chunks, q.chunk);
+  q.u1 = chunk_start(r, chunks, q.chunk + 1);
+  const int in = rel - r.groups * q.u0;
+  const int len = q.u1 - q.u0;
   q.group = in / len;
-  q.tile = q.t0 + in - q.group * len;
+  q.unit = q.u0 + in - q.group * len;
   return q;
 }
+
+// Where a slice starts, as the plan found it.
+struct Start {
+  int b, first, first_group;  // request, its first unit and group over all requests
+  int chunks;
+  Request r;
+  Place at;
+};
 
 // A run of tiles of one group.
 struct Segment {
@@ -206,30 +219,22 @@ struct Walker {
   Place at;               // attention: next unit's place
   int run0, run1, end, g; // weights: current run of tiles, end of the slice's tiles, next group
 
-  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, const int* found)
-      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(found[0]), first(found[1]), first_group(found[2]) {
-    if (u0 < u1) enter();
+  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, const Start& st)
+      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(st.b), first(st.first), first_group(st.first_group) {
+    if (u0 >= u1) return;
+    r = st.r;
+    chunks = st.chunks;
+    at = st.at;
+    if constexpr (kWeights) start_tiles();
   }
 
-  __device__ void enter() {
-    bool bad;
-    r = load_request(p, b, bad);
-    if (r.tiles == 0) {
-      run0 = run1 = end = 0;
-      g = 0;
-      return;
-    }
-    if constexpr (kWeights) {
-      // A tile belongs to the slice that its first unit falls into.
-      const int lo = u0 - first, hi = u1 - first;
-      run0 = lo <= 0 ? 0 : (lo + r.groups - 1) / r.groups;
-      end = (hi + r.groups - 1) / r.groups;
-      if (end > r.tiles) end = r.tiles;
-      start_run();
-    } else {
-      chunks = chunks_of(r, slice);
-      at = place_of(r, chunks, u - first);
-    }
+  __device__ void start_tiles() {
+    // A tile belongs to the slice that its first unit falls into.
+    const int lo = u0 - first, hi = u1 - first;
+    run0 = lo <= 0 ? 0 : (lo + r.groups - 1) / r.groups;
+    end = (hi + r.groups - 1) / r.groups;
+    if (end > r.tiles) end = r.tiles;
+    start_run();
   }
   __device__ void start_run() {
     const int most = r.groups > 1 ? kSumTilesShared : kSumTiles;
@@ -238,13 +243,20 @@ struct Walker {
   }
   __device__ bool leave() {  // to the next request that has units in the slice
     for (;;) {
-      first += r.groups * r.tiles;
+      first += r.groups * r.span;
       first_group += r.groups;
       ++b;
       if (b >= p.num_requests || first >= u1) return false;
-      if constexpr (!kWeights) u = first;
-      enter();
-      if (r.tiles > 0) return true;
+      bool bad;
+      r = load_request<kWeights>(p, b, bad);
+      if (r.tiles == 0) continue;
+      if constexpr (kWeights) {
+        start_tiles();
+      } else {
+        chunks = chunks_of(r, slice);
+        at = place_of(r, chunks, 0);
+      }
+      return true;
     }
   }
 
@@ -266,32 +278,34 @@ struct Walker {
       }
       return true;
     } else {
-      if (u >= u1) return false;
-      s.b = b;
-      s.r = r;
-      s.group = at.group;
-      s.group_index = first_group + at.group;
-      s.t0 = at.tile;
-      int len = at.t1 - at.tile;
-      if (len > u1 - u) len = u1 - u;
-      s.t1 = s.t0 + len;
-      s.whole = s.t0 == 0 && s.t1 == r.tiles;
-      s.slot = u == u0 ? 0 : 1;
-      u += len;
-      if (u < u1) {
-        if (++at.group == r.groups) {
-          at.group = 0;
-          ++at.chunk;
+      while (u < u1) {
+        s.b = b;
+        s.r = r;
+        s.group = at.group;
+        s.group_index = first_group + at.group;
+        int len = at.u1 - at.unit;
+        if (len > u1 - u) len = u1 - u;
+        s.t0 = at.unit < kLead ? 0 : at.unit - kLead;
+        s.t1 = at.unit + len - kLead;
+        s.whole = s.t0 == 0 && s.t1 == r.tiles;
+        s.slot = u == u0 ? 0 : 1;
+        u += len;
+        if (u < u1) {
+          if (++at.group == r.groups) {
+            at.group = 0;
+            ++at.chunk;
+          }
+          if (at.chunk == chunks) {
+            if (!leave()) u = u1;
+          } else {
+            at.u0 = chunk_start(r, chunks, at.chunk);
+            at.u1 = chunk_start(r, chunks, at.chunk + 1);
+            at.unit = at.u0;
+          }
         }
-        if (at.chunk == chunks) {
-          if (!leave()) u = u1;
-        } else {
-          at.t0 = chunk_start(r, chunks, at.chunk);
-          at.t1 = chunk_start(r, chunks, at.chunk + 1);
-          at.tile = at.t0;
-        }
+        if (s.t1 > s.t0) return true;  // else a slice's end within the lead
       }
-      return true;
+      return false;
     }
   }
 };
@@ -335,7 +349,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   int* misc = reinterpret_cast<int*>(smem + kOffMisc);
   uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
   int* abort_flag = misc + 1;
-  int* found = misc + 2;                     // the slice's first request, its first unit and group
+  Start* found = reinterpret_cast<Start*>(misc + 2);
+  static_assert(8 + sizeof(Start) <= kOffRed - kOffMisc, "misc");
   float* red = reinterpret_cast<float*>(smem + kOffRed);
   int* warp_sums = reinterpret_cast<int*>(red);  // planning: [11] units, [11] groups
   float* factor_s = reinterpret_cast<float*>(smem + kOffFactor);  // O's rescaling; at the end 1 / l
@@ -351,8 +366,6 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     mbar_init(p_full, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
     *abort_flag = 0;
-    found[0] = p.num_requests;
-    found[1] = found[2] = 0;
     fence_mbar_init();
   }
   if (warp == kLoadWarp && elect_one()) {
@@ -372,11 +385,13 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   const int b_lo = min(tid * per, p.num_requests), b_hi = min(b_lo + per, p.num_requests);
   int units = 0, groups = 0;
   bool any_bad = false, decreasing = false;
+  Request mine;  // the thread's first (for ordinary batches its only) request
   for (int b = b_lo; b < b_hi; ++b) {
     bool bad;
-    const Request r = load_request(p, b, bad);
+    const Request r = load_request<kWeights>(p, b, bad);
+    if (b == b_lo) mine = r;
     decreasing |= __ldg(p.cu + b + 1) < __ldg(p.cu + b);
-    units += r.groups * r.tiles;
+    units += r.groups * r.span;
     groups += r.groups;
     any_bad |= bad;
   }
@@ -416,12 +431,11 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
     for (int b = b_lo; b < b_hi; ++b) {
       bool bad;
-      const Request r = load_request(p, b, bad);
-      const int un = r.groups * r.tiles;
+      const Request r = b == b_lo ? mine : load_request<kWeights>(p, b, bad);
+      const int un = r.groups * r.span;
       if (u0 >= before && u0 < before + un) {
-        found[0] = b;
-        found[1] = before;
-        found[2] = gbefore;
+        const int chunks = kWeights ? 1 : chunks_of(r, slice);
+        *found = Start{b, before, gbefore, chunks, r, place_of(r, chunks, u0 - before)};
       }
       if (keeper) {
         int2* to = reinterpret_cast<int2*>(p.plan + kPlanGroups) + gbefore;
@@ -436,7 +450,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 
   const uint32_t tmem_base = *tmem_base_smem;
   const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
-  Walker<kWeights> walk(p, u0, u1, slice, found);
+  Walker<kWeights> walk(p, u0, u1, slice, *found);
   Segment s;
 
   if (warp == kLoadWarp) {
@@ -597,7 +611,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
         for (int64_t q = static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6); q < tiles; q += 4 * ctas) {
           const int b = static_cast<int>(q / p.max_pages), t = static_cast<int>(q % p.max_pages);
           bool bad;
-          if (!nothing && t < load_request(p, b, bad).tiles) continue;
+          if (!nothing && t < load_request<kWeights>(p, b, bad).tiles) continue;
           const int64_t at = static_cast<int64_t>(t) * kTok + (tid & 63);
           p.acc_out[b * p.acc_out_stride + at] = p.acc[b * p.acc_stride + at];
         }
@@ -753,13 +767,24 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < 8; ++k) most = fmaxf(most, fmaxf(d0[k], d1[k]));
           if (named_barrier_or(1 + set, 128, unset || most > kRescaleThreshold)) {
+            {
+              // Over the warp's 8 token pairs (lane bits 2-4): at each step a
+              // lane keeps half of its columns and sends the others.
+              float mt[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              float mt = fmaxf(d0[k], d1[k]) - minus[k];
-              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
-              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
-              mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
-              if (lane < 4) red[kRows * sp + col(k)] = mt;
+              for (int k = 0; k < 8; ++k) mt[k] = fmaxf(d0[k], d1[k]) - minus[k];
+              int k0 = 0;  // the column that is left
+#pragma unroll
+              for (int half = 4; half >= 1; half /= 2) {
+                const bool up = lane & (4 * half);
+#pragma unroll
+                for (int k = 0; k < half; ++k) {
+                  const float send = up ? mt[k] : mt[k + half];
+                  mt[k] = fmaxf(up ? mt[k + half] : mt[k], __shfl_xor_sync(0xffffffffu, send, 4 * half));
+                }
+                if (up) k0 += half;
+              }
+              red[kRows * sp + col(k0)] = mt[0];
             }
             named_barrier_sync(1 + set, 128);
             unset = false;
@@ -986,6 +1011,16 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   const int y0 = blockIdx.y * rows_per_block;
   const int rows = min(rows_per_block, info.y - y0);
   if (rows <= 0) return;
+  // The first records' loads of the first row need no weights: they go first.
+  const int half = tid >> 7, d4 = tid & 127;
+  const float4* src = reinterpret_cast<const float4*>(p.part_o) + y0 * (kCkv / 4) + d4;
+  float4 v[kJoinDepth];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < kJoinDepth; ++j)
+      if (k0 + 2 * j < count) v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + 2 * j]) * (kPartFloats / 4));
+  };
+  load(half);
   if (warp < rows) {
     float M = -INFINITY, L = 0.f;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + y0 + warp;
@@ -1010,15 +1045,10 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
     if (lane == 0) p.lse_out[info.x + y0 + warp] = L == 0.f ? -INFINITY : M + log2f(L);
   }
   __syncthreads();
-  const int half = tid >> 7, d4 = tid & 127;
   for (int y = 0; y < rows; ++y) {
-    const float4* src = reinterpret_cast<const float4*>(p.part_o) + (y0 + y) * (kCkv / 4) + d4;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = half; k0 < count; k0 += 2 * kJoinDepth) {
-      float4 v[kJoinDepth];
-#pragma unroll
-      for (int j = 0; j < kJoinDepth; ++j)
-        if (k0 + 2 * j < count) v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + 2 * j]) * (kPartFloats / 4));
+      if (y > 0 || k0 > half) load(k0);
 #pragma unroll
       for (int j = 0; j < kJoinDepth; ++j) {
         if (k0 + 2 * j < count) {
@@ -1030,6 +1060,7 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
         }
       }
     }
+    src += kCkv / 4;
     if (half == 1) other[d4] = acc;
     __syncthreads();
     if (half == 0) {
@@ -1085,7 +1116,7 @@ int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64
   if (num_pages < 1 || num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || mask_words < 1 ||
       mask_words > 64)
     return DSA_ERR_INVALID_ARGUMENT;
-  if (groups_bound(drafts, heads, requests) * max_pages > 0x7FFFFFFF) return DSA_ERR_INVALID_ARGUMENT;
+  if (groups_bound(drafts, heads, requests) * (max_pages + kLead) > 0x7FFFFFFF) return DSA_ERR_INVALID_ARGUMENT;
   if (ckv_row < kCkv * 2 || kpe_row < kKpe * 2 || ckv_page < 0 || kpe_page < 0) return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(workspace) ||
       ((ckv_page | ckv_row | kpe_page | kpe_row) & 15))

@@ -115,7 +115,7 @@ def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_tabl
     if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or \
             not 1 <= tree_mask.shape[1] <= MAX_MASK_WORDS:
         fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
-    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * max_pages > 0x7FFFFFFF:
+    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * (max_pages + 2) > 0x7FFFFFFF:
         fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
     hold = (q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), _int32(block_table),
             _int32(cu_drafts), tree_mask.contiguous(), ckv_cache, kpe_cache)
