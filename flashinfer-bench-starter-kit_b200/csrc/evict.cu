@@ -9,8 +9,8 @@
 //   slice of the request's weights in shared memory, read from HBM once (4 B
 //   per token).  The boundary weight is found by radix: a histogram of the
 //   order key's top 11 bits, then of the next 11 and the last 10 among the
-//   keys that share the boundary's bits, each summed over the cluster through
-//   distributed shared memory.  The kept positions then come out in order: a
+//   keys that share the boundary's bits, each added up in the first CTA's
+//   shared memory and read from there by all.  The kept positions then come out in order: a
 //   token's place is the number kept before it, from ballots, a scan over
 //   the CTA's warps and the counts of the lower CTAs.
 // move_kernel: copies the kept tokens' rows of every cache to their new
@@ -30,6 +30,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;             // the portable limit
 constexpr int kMaxResident = 49152;        // weights a CTA can hold (192 KB)
+constexpr int kBatch = 8;                  // tokens a thread has in flight
 constexpr int kSteps = 8;                  // emission: tokens per thread and round
 
 struct Params {
@@ -84,9 +85,10 @@ __device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
 
 __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   extern __shared__ float held[];          // this CTA's weights, if they fit
-  __shared__ int hist[3][kBins];
+  __shared__ __align__(16) int hist[3][kBins];  // the first CTA's ends as the cluster's
   __shared__ int counts[2];                // tokens above the boundary key, and at it
   __shared__ int scratch[2 * kWarps];
+  __shared__ int lower[2];                 // counts of the lower CTAs
   __shared__ int found[3];                 // boundary bin, kept ones needed from it, its size
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   const float* mine = acc + p.num_sink + lo;
   const bool fits = slice <= p.resident;
   for (int i = tid; i < 3 * kBins; i += kThreads) hist[0][i] = 0;
+  cluster_arrive();                        // waited for before the first remote access
   __syncthreads();
 
   // ---- boundary key: 11 + 11 + 10 bits.
@@ -140,52 +143,71 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bins = pass == 2 ? 1024 : kBins;
     const int upper = shift + (pass == 2 ? 10 : 11);
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
-      const int i = i0 + tid;
-      const bool in = i < n;
-      float v = 0.f;
-      if (in) {
-        if (pass == 0 || !fits) {
-          v = mine[i];
-          if (fits) held[i] = v;
-        } else {
-          v = held[i];
+    for (int i0 = 0; i0 < n; i0 += kThreads * kBatch) {
+      float v[kBatch];
+      if (pass == 0 || !fits) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + j * kThreads + tid;
+          v[j] = i < n ? __ldg(mine + i) : 0.f;
+        }
+        if (fits) {
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j)
+            if (i0 + j * kThreads + tid < n) held[i0 + j * kThreads + tid] = v[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + j * kThreads + tid;
+          v[j] = i < n ? held[i] : 0.f;
         }
       }
-      const uint32_t key = score_key(v);
-      bool count = in && (pass == 0 || (key >> upper) == prefix);
-      const int bin = static_cast<int>((key >> shift) & (bins - 1));
-      // Weights repeat (tokens that were never read have exactly 0): the
-      // lanes that share the first counting lane's bin add theirs at once.
-      const unsigned int act = __ballot_sync(0xffffffffu, count);
-      if (act != 0) {
-        const int lead = __ffs(act) - 1;
-        const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);
-        const unsigned int same = __ballot_sync(0xffffffffu, count && bin == lead_bin);
-        if (lane == lead) atomicAdd(&hist[pass][lead_bin], __popc(same));
-        if (count && bin != lead_bin) atomicAdd(&hist[pass][bin], 1);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t key = score_key(v[j]);
+        const bool count = i0 + j * kThreads + tid < n && (pass == 0 || (key >> upper) == prefix);
+        const int bin = static_cast<int>((key >> shift) & (bins - 1));
+        // Weights repeat (tokens that were never read have exactly 0): the
+        // lanes that share the first counting lane's bin add theirs at once.
+        const unsigned int act = __ballot_sync(0xffffffffu, count);
+        if (act != 0) {
+          const int lead = __ffs(act) - 1;
+          const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);
+          const unsigned int same = __ballot_sync(0xffffffffu, count && bin == lead_bin);
+          if (lane == lead) atomicAdd(&hist[pass][lead_bin], __popc(same));
+          if (count && bin != lead_bin) atomicAdd(&hist[pass][bin], 1);
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) cluster_wait();
+    if (rank != 0) {
+      for (int bin = tid; bin < bins; bin += kThreads) {
+        const int c = hist[pass][bin];
+        if (c != 0) add_cluster(&hist[pass][bin], 0, c);
       }
     }
     cluster_sync();
     // Thread t has four bins, in descending order over the threads.
-    constexpr int kPer = kBins / kThreads;
-    int c[kPer], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int bin = bins - 1 - (kPer * tid + j);
-      c[j] = 0;
-#pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r)
-        if (bin >= 0 && r < ctas) c[j] += ld_cluster(&hist[pass][bin], r);
-      sum += c[j];
+    static_assert(kBins == 4 * kThreads, "four bins a thread");
+    const int top = bins - 4 - 4 * tid;
+    int c[4] = {0, 0, 0, 0};
+    if (top >= 0) {
+      const int4 q = ld_cluster4(reinterpret_cast<const int4*>(&hist[pass][top]), 0);
+      c[0] = q.w;
+      c[1] = q.z;
+      c[2] = q.y;
+      c[3] = q.x;
     }
+    const int sum = c[0] + c[1] + c[2] + c[3];
     int total;
     int before = block_scan(sum, scratch, total);
     if (before < need && need <= before + sum) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
+      for (int j = 0; j < 4; ++j) {
         if (before < need && need <= before + c[j]) {
-          found[0] = bins - 1 - (kPer * tid + j);
+          found[0] = top + 3 - j;
           found[1] = need - before;
           found[2] = c[j];
         }
@@ -206,6 +228,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
 
   // ---- counts of every CTA, then the positions in order.
   int gt = 0, eq = 0;
+#pragma unroll 4
   for (int i = tid; i < n; i += kThreads) {
     const uint32_t key = score_key(fits ? held[i] : mine[i]);
     gt += key > above;
@@ -219,15 +242,22 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     counts[1] = total_eq;
   }
   cluster_sync();
-  int gt_before = 0, eq_before = 0;
+  if (warp == 0) {
+    int g = lane < rank ? ld_cluster(&counts[0], lane) : 0, q = lane < rank ? ld_cluster(&counts[1], lane) : 0;
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r) {
-    if (r >= rank) break;
-    gt_before += ld_cluster(&counts[0], r);
-    eq_before += ld_cluster(&counts[1], r);
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+      g += __shfl_xor_sync(0xffffffffu, g, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (lane == 0) {
+      lower[0] = g;
+      lower[1] = q;
+    }
   }
-  // The last remote read of this kernel: a CTA leaves once all have made theirs.
+  __syncthreads();
+  // That was the last remote access: a CTA leaves once all have made theirs.
   cluster_arrive();
+  int gt_before = lower[0], eq_before = lower[1];
   // eq_before ties of lower CTAs come first; `ties` are kept in all.
   for (int i0 = 0; i0 < n; i0 += kThreads * kSteps) {
     unsigned int above_mask[kSteps], tie_mask[kSteps];

@@ -50,7 +50,7 @@ def _fail_acc(msg: str) -> None:
 
 
 def _rows_of(name: str, t: torch.Tensor, shape: tuple, fail) -> None:
-    if t.dtype != torch.float32 or tuple(t.shape) != shape:
+    if t.dtype is not torch.float32 or t.shape != shape:
         fail(f"{name} must be float32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
     if t.stride(1) != 1 or (shape[0] > 1 and t.stride(0) < shape[1]):
         fail(f"{name} must have contiguous rows that do not overlap (strides {t.stride()})")
@@ -63,10 +63,11 @@ def _pitch(t: torch.Tensor) -> int:
 def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor,
                prefix_lens: torch.Tensor, block_table: torch.Tensor, cu_drafts: torch.Tensor,
                tree_mask: torch.Tensor, sm_scale, lse: torch.Tensor, acc: torch.Tensor, out: torch.Tensor) -> None:
-    dev, T, H, B, max_pages, args, hold = tree.check_rows(
-        _fail_acc, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts, tree_mask,
-        (("lse", lse), ("acc", acc), ("out", out)))
-    if lse.dtype != torch.float32 or lse.shape != (T, H):
+    at, T, H, B, max_pages, args, hold = tree.check_rows(
+        _fail_acc, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts, tree_mask)
+    if lse.get_device() != at or acc.get_device() != at or out.get_device() != at:
+        tree.check_device(_fail_acc, q_nope=q_nope, lse=lse, acc=acc, out=out)
+    if lse.dtype is not torch.float32 or lse.shape != (T, H):
         _fail_acc(f"lse must be float32 [{T}, {H}]")
     _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_acc)
     _rows_of("out", out, (B, max_pages * PAGE_SIZE), _fail_acc)
@@ -82,6 +83,7 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
             out.copy_(acc)
         return
     lse = lse.contiguous()
+    dev = q_nope.device
     cur = _native.current_stream(dev)
     ws = workspace.get(dev, "evict", _native.WORKSPACE_HEADER, cur)
     st = _native.call_on(dev, _native.lib().dsa_tree_weights_run, *args, float(sm_scale), lse.data_ptr(),
@@ -98,28 +100,26 @@ def _fail_run(msg: str) -> None:
 def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, new_block_table: torch.Tensor,
         ckv_cache: torch.Tensor, kpe_cache: torch.Tensor, k_index_cache_fp8, num_sink: int, num_recent: int,
         keep: torch.Tensor, new_seq_lens: torch.Tensor, new_acc: torch.Tensor) -> None:
-    dev = acc.device
-    if dev.type != "cuda":
-        _fail_run("tensors must be on a CUDA device")
-    for name, t in (("seq_lens", seq_lens), ("block_table", block_table), ("new_block_table", new_block_table),
-                    ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache), ("k_index_cache_fp8", k_index_cache_fp8),
-                    ("keep", keep), ("new_seq_lens", new_seq_lens), ("new_acc", new_acc)):
-        if t is not None and t.device != dev:
-            _fail_run(f"{name} is on {t.device}, expected {dev}")
-    for name, t in (("block_table", block_table), ("new_block_table", new_block_table)):
-        if t.dim() != 2 or t.shape[1] < 1 or t.shape[0] != block_table.shape[0]:
-            _fail_run(f"{name} must be [B, pages]")
-        if t.dtype != torch.int32 and t.dtype != torch.int64:
-            _fail_run(f"{name} must be int32 or int64")
+    # Every message is formatted only on failure: small batches wait for the host.
+    at = acc.get_device()
+    if at < 0 or seq_lens.get_device() != at or block_table.get_device() != at or new_block_table.get_device() != at or \
+            ckv_cache.get_device() != at or kpe_cache.get_device() != at or keep.get_device() != at or \
+            new_seq_lens.get_device() != at or new_acc.get_device() != at or \
+            (k_index_cache_fp8 is not None and k_index_cache_fp8.get_device() != at):
+        tree.check_device(_fail_run, acc=acc, seq_lens=seq_lens, block_table=block_table, new_block_table=new_block_table,
+                          ckv_cache=ckv_cache, kpe_cache=kpe_cache, k_index_cache_fp8=k_index_cache_fp8, keep=keep,
+                          new_seq_lens=new_seq_lens, new_acc=new_acc)
+    if len(block_table.shape) != 2 or block_table.shape[1] < 1:
+        _fail_run("block_table must be [B, max_pages]")
     B, max_pages = block_table.shape
+    if len(new_block_table.shape) != 2 or new_block_table.shape[0] != B or new_block_table.shape[1] < 1:
+        _fail_run(f"new_block_table must be [{B}, new_max_pages]")
     new_pages = new_block_table.shape[1]
-    for name, t in (("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
-        if t.dtype != torch.bfloat16:
-            _fail_run(f"{name} must be bfloat16, got {t.dtype}")
-    ckv_page, ckv_row = tree._strides("ckv_cache", ckv_cache, tree.DIM_CKV, _fail_run)
-    kpe_page, kpe_row = tree._strides("kpe_cache", kpe_cache, tree.DIM_KPE, _fail_run)
-    pages = ckv_cache.shape[0]
-    if kpe_cache.shape[0] != pages:
+    if ckv_cache.dtype is not torch.bfloat16 or kpe_cache.dtype is not torch.bfloat16:
+        _fail_run(f"ckv_cache and kpe_cache must be bfloat16, got {ckv_cache.dtype} and {kpe_cache.dtype}")
+    pages, ckv_page, ckv_row = tree._strides("ckv_cache", ckv_cache, tree.DIM_CKV, _fail_run)
+    kpe_pages, kpe_page, kpe_row = tree._strides("kpe_cache", kpe_cache, tree.DIM_KPE, _fail_run)
+    if kpe_pages != pages:
         _fail_run("ckv_cache and kpe_cache must hold the same number of pages")
     if k_index_cache_fp8 is not None:
         if k_index_cache_fp8.element_size() != 1 or not k_index_cache_fp8.is_contiguous():
@@ -147,7 +147,10 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
         return
     if B > 65536 or max_pages > 1 << 24 or new_pages > 1 << 24:
         _fail_run(f"{B} requests of {max_pages} pages are more than one call takes")
-    sl, bt, nbt = seq_lens.contiguous(), tree._int32(block_table), tree._int32(new_block_table)
+    sl = seq_lens.contiguous()
+    bt = tree._int32("block_table", block_table, _fail_run)
+    nbt = tree._int32("new_block_table", new_block_table, _fail_run)
+    dev = acc.device
     check = tree._CHECK and not torch.cuda.is_current_stream_capturing()
     if check:
         _check_new_pages(sl, bt, nbt, budget, pages)

@@ -65,68 +65,83 @@ def masks_from_parents(parents) -> list:
 
 
 def _strides(name: str, t: torch.Tensor, width: int, fail) -> tuple:
-    """(page stride, row stride) in bytes of a [pages, 64, width] bf16 cache."""
-    if t.dim() != 3 or t.shape[1] != PAGE_SIZE or t.shape[2] != width:
-        fail(f"{name} must be [pages, {PAGE_SIZE}, {width}], got {tuple(t.shape)}")
-    if t.shape[0] < 1:
+    """(pages, page stride, row stride) of a [pages, 64, width] bf16 cache, strides in bytes."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != PAGE_SIZE or shape[2] != width:
+        fail(f"{name} must be [pages, {PAGE_SIZE}, {width}], got {tuple(shape)}")
+    pages = shape[0]
+    if pages < 1:
         fail(f"{name} has no pages")
     page, row, col = t.stride()
-    if t.shape[0] == 1:  # a stride that is never taken
+    if pages == 1:  # a stride that is never taken
         page = PAGE_SIZE * row
     if col != 1 or row < width or page < row or row % 8 or page % 8 or t.data_ptr() % 16:
         fail(f"{name} must have contiguous rows, 16-byte aligned (strides {t.stride()})")
-    return 2 * page, 2 * row
+    return pages, 2 * page, 2 * row
 
 
-def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts, tree_mask,
-               more) -> tuple:
+def check_device(fail, **tensors) -> None:
+    """Names the tensor that is not where the first one is (called once that is known)."""
+    first = next(iter(tensors.values()))
+    if not first.is_cuda:
+        fail("tensors must be on a CUDA device")
+    for name, t in tensors.items():
+        if t is not None and t.device != first.device:
+            fail(f"{name} is on {t.device}, expected {first.device}")
+
+
+def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table, cu_drafts, tree_mask) -> tuple:
     """The checks shared with ``dsa_b200.evict.accumulate``; returns the sizes and
     the arguments of the C entry points up to ``mask_words``, and the tensors
-    that hold them."""
-    dev = q_nope.device
-    if dev.type != "cuda":
-        fail("tensors must be on a CUDA device")
-    for name, t in (("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache),
-                    ("prefix_lens", prefix_lens), ("block_table", block_table),
-                    ("cu_drafts", cu_drafts), ("tree_mask", tree_mask), *more):
-        if t.device != dev:
-            fail(f"{name} is on {t.device}, expected {dev}")
-    for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
-        if t.dtype != torch.bfloat16:
-            fail(f"{name} must be bfloat16, got {t.dtype}")
-    if q_nope.dim() != 3 or q_nope.shape[2] != DIM_CKV or not 1 <= q_nope.shape[1] <= MAX_HEADS:
-        fail(f"q_nope must be [T, heads <= {MAX_HEADS}, {DIM_CKV}], got {tuple(q_nope.shape)}")
-    T, H = q_nope.shape[:2]
+    that hold them.  Every message is formatted only on failure: this runs once
+    per step and layer, and short contexts wait for the host."""
+    at = q_nope.get_device()
+    if at < 0 or q_pe.get_device() != at or ckv_cache.get_device() != at or kpe_cache.get_device() != at or \
+            prefix_lens.get_device() != at or block_table.get_device() != at or cu_drafts.get_device() != at or \
+            tree_mask.get_device() != at:
+        check_device(fail, q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache, prefix_lens=prefix_lens,
+                     block_table=block_table, cu_drafts=cu_drafts, tree_mask=tree_mask)
+    bf16 = torch.bfloat16
+    if q_nope.dtype is not bf16 or q_pe.dtype is not bf16 or ckv_cache.dtype is not bf16 or kpe_cache.dtype is not bf16:
+        for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
+            if t.dtype is not bf16:
+                fail(f"{name} must be bfloat16, got {t.dtype}")
+    shape = q_nope.shape
+    if len(shape) != 3 or shape[2] != DIM_CKV or not 1 <= shape[1] <= MAX_HEADS:
+        fail(f"q_nope must be [T, heads <= {MAX_HEADS}, {DIM_CKV}], got {tuple(shape)}")
+    T, H, _ = shape
     if q_pe.shape != (T, H, DIM_KPE):
         fail(f"q_pe must be [{T}, {H}, {DIM_KPE}]")
-    ckv_page, ckv_row = _strides("ckv_cache", ckv_cache, DIM_CKV, fail)
-    kpe_page, kpe_row = _strides("kpe_cache", kpe_cache, DIM_KPE, fail)
-    if kpe_cache.shape[0] != ckv_cache.shape[0]:
+    pages, ckv_page, ckv_row = _strides("ckv_cache", ckv_cache, DIM_CKV, fail)
+    kpe_pages, kpe_page, kpe_row = _strides("kpe_cache", kpe_cache, DIM_KPE, fail)
+    if kpe_pages != pages:
         fail("ckv_cache and kpe_cache must hold the same number of pages")
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
         fail("block_table must be [B, max_pages]")
-    if block_table.dtype != torch.int32 and block_table.dtype != torch.int64:
-        fail("block_table must be int32 or int64")
-    B, max_pages = block_table.shape
-    if prefix_lens.dtype != torch.int32 or prefix_lens.shape != (B,):
+    B, max_pages = shape
+    if prefix_lens.dtype is not torch.int32 or prefix_lens.shape != (B,):
         fail(f"prefix_lens must be int32 [{B}]")
-    if (cu_drafts.dtype != torch.int32 and cu_drafts.dtype != torch.int64) or cu_drafts.shape != (B + 1,):
+    if cu_drafts.shape != (B + 1,):
         fail(f"cu_drafts must be int32 [{B + 1}] (one more than block_table rows)")
-    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or \
-            not 1 <= tree_mask.shape[1] <= MAX_MASK_WORDS:
+    shape = tree_mask.shape
+    if tree_mask.dtype is not torch.int64 or len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= MAX_MASK_WORDS:
         fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
     if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * (max_pages + 2) > 0x7FFFFFFF:
         fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
-    hold = (q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), _int32(block_table),
-            _int32(cu_drafts), tree_mask.contiguous(), ckv_cache, kpe_cache)
-    qn, qp, pl, bt, cu, tm = (t.data_ptr() for t in hold[:6])
-    args = (qn, qp, ckv_cache.data_ptr(), ckv_page, ckv_row, kpe_cache.data_ptr(), kpe_page, kpe_row,
-            ckv_cache.shape[0], pl, bt, cu, tm, B, T, H, max_pages, tree_mask.shape[1])
-    return dev, T, H, B, max_pages, args, hold
+    qn, qp, pl, tm = q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), tree_mask.contiguous()
+    bt, cu = _int32("block_table", block_table, fail), _int32("cu_drafts", cu_drafts, fail)
+    args = (qn.data_ptr(), qp.data_ptr(), ckv_cache.data_ptr(), ckv_page, ckv_row, kpe_cache.data_ptr(), kpe_page, kpe_row,
+            pages, pl.data_ptr(), bt.data_ptr(), cu.data_ptr(), tm.data_ptr(), B, T, H, max_pages, shape[1])
+    return at, T, H, B, max_pages, args, (qn, qp, pl, bt, cu, tm)
 
 
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+def _int32(name: str, t: torch.Tensor, fail) -> torch.Tensor:
+    if t.dtype is not torch.int32:
+        if t.dtype is not torch.int64:
+            fail(f"{name} must be int32 or int64")
+        t = t.to(torch.int32)
+    return t.contiguous()
 
 
 def _fail(msg: str) -> None:
@@ -146,17 +161,19 @@ def _workspace_bytes(dev: torch.device, T: int, H: int, B: int) -> int:
 def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor,
         prefix_lens: torch.Tensor, block_table: torch.Tensor, cu_drafts: torch.Tensor, tree_mask: torch.Tensor,
         sm_scale, output: torch.Tensor, lse: torch.Tensor) -> None:
-    # Every message is formatted only on failure: this runs once per step and layer.
-    dev, T, H, B, _, args, hold = check_rows(_fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table,
-                                             cu_drafts, tree_mask, (("output", output), ("lse", lse)))
-    if output.dtype != torch.bfloat16 or output.shape != q_nope.shape or not output.is_contiguous():
+    at, T, H, B, _, args, hold = check_rows(_fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_table,
+                                            cu_drafts, tree_mask)
+    if output.get_device() != at or lse.get_device() != at:
+        check_device(_fail, q_nope=q_nope, output=output, lse=lse)
+    if output.dtype is not torch.bfloat16 or output.shape != q_nope.shape or not output.is_contiguous():
         _fail(f"output must be contiguous bfloat16 [{T}, {H}, {DIM_CKV}]")
-    if lse.dtype != torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
+    if lse.dtype is not torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
         _fail(f"lse must be contiguous float32 [{T}, {H}]")
     if isinstance(sm_scale, torch.Tensor):
-        sm_scale = float(sm_scale.item())
+        sm_scale = sm_scale.item()
     if T == 0 or B == 0:
         return
+    dev = q_nope.device
     cur = _native.current_stream(dev)
     ws = workspace.get(dev, "tree", _workspace_bytes(dev, T, H, B), cur)
     st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, float(sm_scale), output.data_ptr(),

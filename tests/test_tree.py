@@ -62,9 +62,9 @@ def test_cache_strides():
         raise ValueError(msg)
 
     both = torch.zeros(3, 64, 576, dtype=torch.bfloat16)
-    assert tree._strides("ckv", both[:, :, :512], 512, fail) == (2 * 64 * 576, 2 * 576)
-    assert tree._strides("kpe", both[:, :, 512:], 64, fail) == (2 * 64 * 576, 2 * 576)
-    assert tree._strides("ckv", both[:1, :, :512], 512, fail) == (2 * 64 * 576, 2 * 576)
+    assert tree._strides("ckv", both[:, :, :512], 512, fail) == (3, 2 * 64 * 576, 2 * 576)
+    assert tree._strides("kpe", both[:, :, 512:], 64, fail) == (3, 2 * 64 * 576, 2 * 576)
+    assert tree._strides("ckv", both[:1, :, :512], 512, fail) == (1, 2 * 64 * 576, 2 * 576)
     for bad in (both[:, :, 4:516], both[:, :, :511], torch.zeros(3, 64, 580, dtype=torch.bfloat16)[:, :, :512],
                 both[:, :, :512].transpose(0, 1), both[:0, :, :512], both[:1, :, :512].expand(3, 64, 512),
                 both.flatten(0, 1)[:, :512]):
