@@ -10,7 +10,9 @@
 //   per token).  The boundary weight is found by radix: a histogram of the
 //   order key's top 11 bits, then of the next 11 and the last 10 among the
 //   keys that share the boundary's bits, each added up in the first CTA's
-//   shared memory and read from there by all.  The kept positions then come out in order: a
+//   shared memory with the sums of every 32 bins: a warp of each CTA finds the
+//   boundary bin from those 64 sums and 32 bins, 384 bytes of remote reads
+//   (all 2048 bins from one SM took 4400 clocks a pass).  The kept positions then come out in order: a
 //   token's place is the number kept before it, from ballots, a scan over
 //   the CTA's warps and the counts of the lower CTAs.
 // move_kernel: copies the kept tokens' rows of every cache to their new
@@ -30,8 +32,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;             // the portable limit
 constexpr int kMaxResident = 49152;        // weights a CTA can hold (192 KB)
-constexpr int kBatch = 8;                  // tokens a thread has in flight
-constexpr int kSteps = 8;                  // emission: tokens per thread and round
+constexpr int kCoarse = kBins / 32;         // sums of 32 bins each
+constexpr uint32_t kZeroKey = 0x80000000u;  // score_key of 0
 
 struct Params {
   const float* acc;
@@ -61,40 +63,31 @@ __device__ __forceinline__ int length_of(const Params& p, int b, bool& bad) {
   return L < 0 ? 0 : (L > cap ? cap : L);
 }
 
-// Exclusive sum of v over the block's threads, and the total.
-__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = v;
+// Inclusive sum over the warp's lanes.
+__device__ __forceinline__ int warp_scan(int v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += a;
+    const int a = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += a;
   }
-  if (lane == 31) scratch[warp] = inc;
-  __syncthreads();
-  int before = inc - v;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scratch[w];
-    total += scratch[w];
-  }
-  __syncthreads();
-  return before;
+  return v;
 }
 
 __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
-  extern __shared__ float held[];          // this CTA's weights, if they fit
-  __shared__ __align__(16) int hist[3][kBins];  // the first CTA's ends as the cluster's
+  extern __shared__ uint32_t keys[];       // of this CTA's tokens, if they fit
+  __shared__ __align__(16) int hist[kBins];          // this CTA's, of one pass
+  __shared__ int sums[3][kBins], coarse[3][kCoarse];  // the cluster's, in its first CTA
   __shared__ int counts[2];                // tokens above the boundary key, and at it
-  __shared__ int scratch[2 * kWarps];
-  __shared__ int lower[2];                 // counts of the lower CTAs
+  __shared__ int lower[2];                 // those of the lower CTAs
+  __shared__ int scratch[2][kWarps];
   __shared__ int found[3];                 // boundary bin, kept ones needed from it, its size
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
   const int b = blockIdx.x / ctas;
   griddep_wait();
-  griddep_launch_dependents();
+  // The move kernel is not let in early: its blocks, waiting on the SMs, would
+  // keep clusters out (158 against 137 us at 32 x 65536 tokens to 8192).
 
   bool bad;
   const int L = length_of(p, b, bad);
@@ -115,6 +108,14 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     }
     return;  // the whole cluster leaves here
   }
+  int need = p.budget - p.num_sink - p.num_recent;  // from the middle; fewer than it has
+  const int middle = L - p.num_sink - p.num_recent;
+  const int slice = (middle + ctas - 1) / ctas;
+  const int lo = min(rank * slice, middle), n = min(slice, middle - lo);
+  const float* mine = acc + p.num_sink + lo;
+  const bool fits = slice <= p.resident;
+  if (fits && need > 0)
+    for (int i = tid; i < n; i += kThreads) cp_async4(smem_u32(keys + i), mine + i);
   for (int i = t0; i < p.num_sink + p.num_recent; i += step) {
     const bool first = i < p.num_sink;
     const int pos = first ? i : L - p.num_recent + (i - p.num_sink);
@@ -122,17 +123,16 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     keep[to] = pos;
     new_acc[to] = acc[pos];
   }
-  int need = p.budget - p.num_sink - p.num_recent;  // from the middle; fewer than it has
   if (need == 0) return;
-
-  const int middle = L - p.num_sink - p.num_recent;
-  const int slice = (middle + ctas - 1) / ctas;
-  const int lo = min(rank * slice, middle), n = min(slice, middle - lo);
-  const float* mine = acc + p.num_sink + lo;
-  const bool fits = slice <= p.resident;
-  for (int i = tid; i < 3 * kBins; i += kThreads) hist[0][i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+  if (rank == 0) {
+    for (int i = tid; i < 3 * kBins; i += kThreads) sums[0][i] = 0;
+    if (tid < 3 * kCoarse) coarse[0][tid] = 0;
+  }
   cluster_arrive();                        // waited for before the first remote access
+  cp_async_wait_all();                     // each thread turns its own copies into keys below
   __syncthreads();
+  auto key_of = [&](int i) { return fits ? keys[i] : score_key(mine[i]); };
 
   // ---- boundary key: 11 + 11 + 10 bits.
   uint32_t prefix = 0;                     // the boundary key's bits so far
@@ -143,75 +143,63 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bins = pass == 2 ? 1024 : kBins;
     const int upper = shift + (pass == 2 ? 10 : 11);
-    for (int i0 = 0; i0 < n; i0 += kThreads * kBatch) {
-      float v[kBatch];
-      if (pass == 0 || !fits) {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + j * kThreads + tid;
-          v[j] = i < n ? __ldg(mine + i) : 0.f;
-        }
-        if (fits) {
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j)
-            if (i0 + j * kThreads + tid < n) held[i0 + j * kThreads + tid] = v[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + j * kThreads + tid;
-          v[j] = i < n ? held[i] : 0.f;
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const int i = i0 + tid;
+      bool count = i < n;
+      uint32_t key = 0;
+      if (count) {
+        if (pass == 0 && fits) {
+          key = score_key(__uint_as_float(keys[i]));
+          keys[i] = key;
+        } else {
+          key = key_of(i);
         }
       }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const uint32_t key = score_key(v[j]);
-        const bool count = i0 + j * kThreads + tid < n && (pass == 0 || (key >> upper) == prefix);
-        const int bin = static_cast<int>((key >> shift) & (bins - 1));
-        // Weights repeat (tokens that were never read have exactly 0): the
-        // lanes that share the first counting lane's bin add theirs at once.
-        const unsigned int act = __ballot_sync(0xffffffffu, count);
-        if (act != 0) {
-          const int lead = __ffs(act) - 1;
-          const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);
-          const unsigned int same = __ballot_sync(0xffffffffu, count && bin == lead_bin);
-          if (lane == lead) atomicAdd(&hist[pass][lead_bin], __popc(same));
-          if (count && bin != lead_bin) atomicAdd(&hist[pass][bin], 1);
-        }
-      }
+      count = count && (pass == 0 || (key >> upper) == prefix);
+      // Tokens that were never read have exactly 0: a warp adds all of its at
+      // once.
+      const unsigned int zeros = __ballot_sync(0xffffffffu, count && key == kZeroKey);
+      if (zeros != 0 && lane == 0) atomicAdd(&hist[(kZeroKey >> shift) & (bins - 1)], __popc(zeros));
+      if (count && key != kZeroKey) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
     if (pass == 0) cluster_wait();
-    if (rank != 0) {
-      for (int bin = tid; bin < bins; bin += kThreads) {
-        const int c = hist[pass][bin];
-        if (c != 0) add_cluster(&hist[pass][bin], 0, c);
-      }
+    {
+      // Thread t adds its bins 4t .. 4t + 3 to the first CTA's, eight threads
+      // the sum of their 32, and clears them for the next pass.
+      static_assert(kBins == 4 * kThreads, "four bins a thread");
+      int4* own = reinterpret_cast<int4*>(hist) + tid;
+      const int4 q = *own;
+      *own = make_int4(0, 0, 0, 0);
+      int* to = &sums[pass][4 * tid];
+      if (q.x != 0) add_cluster(to, 0, q.x);
+      if (q.y != 0) add_cluster(to + 1, 0, q.y);
+      if (q.z != 0) add_cluster(to + 2, 0, q.z);
+      if (q.w != 0) add_cluster(to + 3, 0, q.w);
+      int sum = (q.x + q.y) + (q.z + q.w);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((tid & 7) == 0 && sum != 0) add_cluster(&coarse[pass][tid >> 3], 0, sum);
     }
     cluster_sync();
-    // Thread t has four bins, in descending order over the threads.
-    static_assert(kBins == 4 * kThreads, "four bins a thread");
-    const int top = bins - 4 - 4 * tid;
-    int c[4] = {0, 0, 0, 0};
-    if (top >= 0) {
-      const int4 q = ld_cluster4(reinterpret_cast<const int4*>(&hist[pass][top]), 0);
-      c[0] = q.w;
-      c[1] = q.z;
-      c[2] = q.y;
-      c[3] = q.x;
-    }
-    const int sum = c[0] + c[1] + c[2] + c[3];
-    int total;
-    int before = block_scan(sum, scratch, total);
-    if (before < need && need <= before + sum) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (before < need && need <= before + c[j]) {
-          found[0] = top + 3 - j;
-          found[1] = need - before;
-          found[2] = c[j];
-        }
-        before += c[j];
+    if (warp == 0) {
+      // From the largest bins down: lane l has two coarse sums, then one bin.
+      const int at = bins / 32 - 1 - 2 * lane;
+      const int c0 = at >= 0 ? ld_cluster(&coarse[pass][at], 0) : 0;
+      const int c1 = at >= 1 ? ld_cluster(&coarse[pass][at - 1], 0) : 0;
+      int before = warp_scan(c0 + c1) - (c0 + c1);
+      const bool here = before < need && need <= before + c0 + c1;
+      const int lead = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+      const bool second = need > before + c0;
+      const int block = __shfl_sync(0xffffffffu, second ? at - 1 : at, lead);
+      const int above_block = __shfl_sync(0xffffffffu, second ? before + c0 : before, lead);
+      const int bin = 32 * block + 31 - lane;
+      const int c = ld_cluster(&sums[pass][bin], 0);
+      before = above_block + warp_scan(c) - c;
+      if (before < need && need <= before + c) {
+        found[0] = bin;
+        found[1] = need - before;
+        found[2] = c;
       }
     }
     __syncthreads();
@@ -226,30 +214,41 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     }
   }
 
-  // ---- counts of every CTA, then the positions in order.
-  int gt = 0, eq = 0;
+  // ---- counts, then the positions in order.  A warp has a run of tokens, so
+  // that its first kept token's place needs one sum over the lower warps.
+  const int run = (n + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  const int w_lo = min(warp * run, n), w_hi = min(w_lo + run, n);
+  int g_at = 0, q_at = 0;                  // tokens above the boundary key, and at it, before the warp's next
 #pragma unroll 4
-  for (int i = tid; i < n; i += kThreads) {
-    const uint32_t key = score_key(fits ? held[i] : mine[i]);
-    gt += key > above;
-    eq += key == above;
+  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < w_hi ? key_of(i) : 0u;
+    g_at += __popc(__ballot_sync(0xffffffffu, i < w_hi && key > above));
+    q_at += __popc(__ballot_sync(0xffffffffu, i < w_hi && key == above));
   }
-  int total_gt, total_eq;
-  block_scan(gt, scratch, total_gt);
-  block_scan(eq, scratch, total_eq);
-  if (tid == 0) {
-    counts[0] = total_gt;
-    counts[1] = total_eq;
+  if (lane == 0) {
+    scratch[0][warp] = g_at;
+    scratch[1][warp] = q_at;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int g = lane < kWarps ? scratch[0][lane] : 0, q = lane < kWarps ? scratch[1][lane] : 0;
+    const int g_sum = warp_scan(g), q_sum = warp_scan(q);
+    if (lane < kWarps) {
+      scratch[0][lane] = g_sum - g;
+      scratch[1][lane] = q_sum - q;
+    }
+    if (lane == kWarps - 1) {
+      counts[0] = g_sum;
+      counts[1] = q_sum;
+    }
   }
   cluster_sync();
   if (warp == 0) {
     int g = lane < rank ? ld_cluster(&counts[0], lane) : 0, q = lane < rank ? ld_cluster(&counts[1], lane) : 0;
-#pragma unroll
-    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
-      g += __shfl_xor_sync(0xffffffffu, g, o);
-      q += __shfl_xor_sync(0xffffffffu, q, o);
-    }
-    if (lane == 0) {
+    g = warp_scan(g);
+    q = warp_scan(q);
+    if (lane == 31) {
       lower[0] = g;
       lower[1] = q;
     }
@@ -257,52 +256,23 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   __syncthreads();
   // That was the last remote access: a CTA leaves once all have made theirs.
   cluster_arrive();
-  int gt_before = lower[0], eq_before = lower[1];
-  // eq_before ties of lower CTAs come first; `ties` are kept in all.
-  for (int i0 = 0; i0 < n; i0 += kThreads * kSteps) {
-    unsigned int above_mask[kSteps], tie_mask[kSteps];
-    int g = 0, q = 0;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const int i = i0 + (warp * kSteps + j) * 32 + lane;
-      uint32_t key = 0;
-      const bool in = i < n;
-      if (in) key = score_key(fits ? held[i] : mine[i]);
-      above_mask[j] = __ballot_sync(0xffffffffu, in && key > above);
-      tie_mask[j] = __ballot_sync(0xffffffffu, in && key == above);
-      g += __popc(above_mask[j]);
-      q += __popc(tie_mask[j]);
+  g_at = lower[0] + scratch[0][warp];
+  q_at = lower[1] + scratch[1][warp];
+  const unsigned int lt = (1u << lane) - 1u;
+#pragma unroll 4
+  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < w_hi ? key_of(i) : 0u;
+    const bool up = i < w_hi && key > above, tie = i < w_hi && key == above;
+    const unsigned int up_mask = __ballot_sync(0xffffffffu, up), tie_mask = __ballot_sync(0xffffffffu, tie);
+    const int q = q_at + __popc(tie_mask & lt);  // ties before this token; the first `ties` are kept
+    if (up || (tie && q < ties)) {
+      const int to = p.num_sink + g_at + __popc(up_mask & lt) + min(q, ties);
+      keep[to] = p.num_sink + lo + i;
+      new_acc[to] = mine[i];
     }
-    if (lane == 0) {
-      scratch[warp] = g;
-      scratch[kWarps + warp] = q;
-    }
-    __syncthreads();
-    int wg = gt_before, wq = eq_before;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) {
-        wg += scratch[w];
-        wq += scratch[kWarps + w];
-      }
-      gt_before += scratch[w];
-      eq_before += scratch[kWarps + w];
-    }
-    __syncthreads();
-    const unsigned int lt = (1u << lane) - 1u;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const bool up = (above_mask[j] >> lane) & 1, tie = (tie_mask[j] >> lane) & 1;
-      const int g_at = wg + __popc(above_mask[j] & lt), q_at = wq + __popc(tie_mask[j] & lt);
-      if (up || (tie && q_at < ties)) {
-        const int to = p.num_sink + g_at + min(q_at, ties);
-        const int i = i0 + (warp * kSteps + j) * 32 + lane;
-        keep[to] = p.num_sink + lo + i;
-        new_acc[to] = fits ? held[i] : mine[i];
-      }
-      wg += __popc(above_mask[j]);
-      wq += __popc(tie_mask[j]);
-    }
+    g_at += __popc(up_mask);
+    q_at += __popc(tie_mask);
   }
   cluster_wait();
 }
@@ -347,8 +317,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
       const int r = __shfl_sync(0xffffffffu, row, k);
       if (f[k] >= 0) {
         const uint4* src = reinterpret_cast<const uint4*>(p.ckv + f[k] * p.ckv_page + r * p.ckv_row) + lane;
-        c[2 * k] = __ldcs(src);
-        c[2 * k + 1] = __ldcs(src + 32);
+        c[2 * k] = __ldcg(src);
+        c[2 * k + 1] = __ldcg(src + 32);
       }
     }
     // kpe and index keys: 8 pieces a token, lane l has piece l & 7 of token l >> 3.
@@ -358,11 +328,11 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
     uint4 e = make_uint4(0u, 0u, 0u, 0u), x = e;
     uint32_t scale = 0;
     if (fk >= 0) {
-      e = __ldcs(reinterpret_cast<const uint4*>(p.kpe + fk * p.kpe_page + rk * p.kpe_row + piece));
+      e = __ldcg(reinterpret_cast<const uint4*>(p.kpe + fk * p.kpe_page + rk * p.kpe_row + piece));
       if (p.index != nullptr) {
         const uint8_t* page = p.index + static_cast<int64_t>(fk) * DSA_INDEX_PAGE_BYTES;
-        x = __ldcs(reinterpret_cast<const uint4*>(page + rk * kIndexRow + piece));
-        if (piece == 0) scale = __ldcs(reinterpret_cast<const uint32_t*>(page + kIndexScales + 4 * rk));
+        x = __ldcg(reinterpret_cast<const uint4*>(page + rk * kIndexRow + piece));
+        if (piece == 0) scale = __ldcg(reinterpret_cast<const uint32_t*>(page + kIndexScales + 4 * rk));
       }
     }
 #pragma unroll
@@ -494,7 +464,7 @@ extern "C" int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const i
   if (cudaLaunchKernelEx(&cfg, evict::select_kernel, p) != cudaSuccess) return DSA_ERR_CUDA;
   const int64_t warps = static_cast<int64_t>(num_requests) * ((budget + evict::kMoveTokens - 1) / evict::kMoveTokens);
   const int64_t blocks = (warps + evict::kMoveWarps - 1) / evict::kMoveWarps;
-  const int64_t most = static_cast<int64_t>(info.num_sms) * 8;
+  const int64_t most = 0x7FFFFFFF;  // beyond, warps take several turns
   if (launch_programmatic(evict::move_kernel, dim3(static_cast<unsigned int>(blocks < most ? blocks : most)),
                           dim3(evict::kMoveThreads), 0, s, p) != cudaSuccess)
     return DSA_ERR_CUDA;
