@@ -64,8 +64,14 @@ constexpr int kPartFloats = kRows * kCkv;    // a partial record's O, [row][dim]
 constexpr int kSumTiles = 16;                // weights: tiles whose sums wait in shared memory
 constexpr int kSumTilesShared = 8;           // ... when several groups re-read them through L2
 
-constexpr uint32_t kIdescS = idesc_make(1, 1, false, false, 64, 64);
-constexpr uint32_t kIdescO = idesc_make(1, 1, true, true, 128, 64);
+// N is the group's rows, rounded up to what the instruction takes: a group of
+// 16 rows (one draft of 16 heads) costs the tensor core and shared memory
+// less than one of 64.  Columns behind it are neither computed nor read.
+constexpr uint32_t kIdescS = idesc_make(1, 1, false, false, 64, 0);
+constexpr uint32_t kIdescO = idesc_make(1, 1, true, true, 128, 0);
+__device__ __forceinline__ uint32_t with_rows(uint32_t idesc, int rows) {
+  return idesc | static_cast<uint32_t>((rows + 15) / 16 * 2) << 17;
+}
 
 // A tile moves in two halves with barriers of their own: ckv pieces 0-3, which
 // O^T's blocks 0 and 1 need, and pieces 4-7 with kpe.
@@ -102,7 +108,7 @@ struct Params {
   __nv_bfloat16* out;
   float* lse_out;
   float* part_o;    // [2 * grid][kPartFloats]
-  float* part_ml;   // [2 * grid][kRows][2]
+  float* part_ml;   // [2 * grid][kRows][4]: m, l, lr
   int* plan;        // see kPlanGroups
   // weights
   const float* lse_in;
@@ -200,6 +206,7 @@ struct Start {
 // A run of tiles of one group.
 struct Segment {
   int b, group, t0, t1;
+  __device__ int rows() const { return min(kRows, r.rows - group * kRows); }
   int group_index;        // attention: over all requests
   Request r;
   bool whole;             // attention: covers the group's whole context
@@ -528,6 +535,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       int i = 0, segs = 0;
       bool ok = true;
       while (ok && walk.next(s)) {
+        const uint32_t idesc = with_rows(kIdescS, s.rows());
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           const int st = i & 1;
           const uint64_t a = k_desc + st * (kTileBytes >> 4);
@@ -543,7 +551,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             for (int k = 16 * h; k < 16 + 20 * h; ++k) {
               // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
               const uint32_t at = (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2;
-              umma_bf16(d, a + at, q_desc + at, kIdescS, k > 0 ? 1u : 0u);
+              umma_bf16(d, a + at, q_desc + at, idesc, k > 0 ? 1u : 0u);
             }
           }
           if (!ok) break;
@@ -564,6 +572,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       int i = 0, segs = 0;
       bool ok = true;
       while (ok && walk.next(s)) {
+        const uint32_t idesc = with_rows(kIdescO, s.rows());
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           const int st = i & 1;
           if (t == s.t0) ok = mbar_wait(o_empty, (segs & 1) ^ 1, wctx);
@@ -577,7 +586,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)  // 128 dims are two pieces; a K16 step is 16 token rows of 128 bytes
               umma_bf16(tmem_base + kColO + 64u * mb, a + mb * (2 * kChunkBytes >> 4) + kk * (2048 >> 4),
-                        p_desc + kk * (2048 >> 4), kIdescO, kk > 0 ? 1u : more);
+                        p_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : more);
             if (mb == 1) umma_commit(&half_done[st]);
           }
           umma_commit(&pv_done[st]);
@@ -700,16 +709,18 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       // the tile exceeds it by more than kRescaleThreshold (always at a
       // segment's first tile), which one OR-barrier per tile tells the set;
       // only then is the tile's max reduced over the tokens and O rescaled.
-      // P <= 2^8 then, and l adds P in fp32.  P is rounded to bf16 for the
-      // MMA (off by at most 2^-8 of itself, independently per token; l uses
-      // the unrounded values), as any bf16 tensor-core product needs.
+      // P <= 2^8 then.  P is rounded to bf16 for the MMA (off by at most 2^-8
+      // of itself), as any bf16 tensor-core product needs.  O is divided by
+      // lr, the fp32 sum of the rounded weights, so that a row that hangs on a
+      // few tokens does not inherit their rounding; lse comes from l, the sum
+      // of the unrounded ones (both sums: under 1 % of the time).
       // A tile's path from S^T to P is what its K stage waits for, so the
       // ordinary tile takes one FMA, one max and one exponential a value:
       // d = s * scale - m, masked in the tiles that need it only.
       int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
       if (tid == 0) group_of[0] = group_of[1] = -1;
       while (walk.next(s)) {
-        float m[8], minus[8], l[8];  // minus: -m, or 0 while the column has seen nothing
+        float m[8], minus[8], l[8], lr[8];  // minus: -m, or 0 while the column has seen nothing
         int draft[8];
         bool unset = false;          // some column of this thread has seen nothing yet
 #pragma unroll
@@ -718,7 +729,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           const bool in = row < s.r.rows;
           m[k] = in ? -INFINITY : 0.f;
           minus[k] = in ? 0.f : -INFINITY;  // no row of the group: all weights 0
-          l[k] = 0.f;
+          l[k] = lr[k] = 0.f;
           draft[k] = in ? row / p.heads : 0;
           unset |= in;
         }
@@ -799,6 +810,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
                 minus[k] = -mt;
               }
               l[k] *= alpha;
+              lr[k] *= alpha;
               unset |= m[k] == -INFINITY;
               if (sp == 0 && lane < 4) factor_s[col(k)] = alpha;
             }
@@ -869,6 +881,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             const __nv_bfloat162 pa = __floats2bfloat162_rn(a[0], a[1]), pc = __floats2bfloat162_rn(c[0], c[1]);
             p0[k >> 1] = *reinterpret_cast<const uint32_t*>(&pa);
             p1[k >> 1] = *reinterpret_cast<const uint32_t*>(&pc);
+            lr[k] += __uint_as_float(p0[k >> 1] << 16) + __uint_as_float(p1[k >> 1] << 16);
+            lr[k + 1] += __uint_as_float(p0[k >> 1] & 0xFFFF0000u) + __uint_as_float(p1[k >> 1] & 0xFFFF0000u);
           }
           // P was last read by PV(i - 1).
           if (i > 0) ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
@@ -889,31 +903,39 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           if (lane == 0) mbar_arrive(p_full);
         }
 
-        // ---- the segment's end: denominators over the tokens, then O.
+        // ---- the segment's end: denominators over the tokens (while the last
+        // PV runs), then O.
+        auto over_tokens = [&](const float (&sum)[8]) {  // of column 32 set + e, for e < 32
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float v = l[k];
-          v += __shfl_xor_sync(0xffffffffu, v, 4);
-          v += __shfl_xor_sync(0xffffffffu, v, 8);
-          v += __shfl_xor_sync(0xffffffffu, v, 16);
-          if (lane < 4) {
-            red[kRows * sp + col(k)] = v;
-            if (sp == 0) max_s[col(k)] = m[k];
+          for (int k = 0; k < 8; ++k) {
+            float v = sum[k];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            if (lane < 4) red[kRows * sp + col(k)] = v;
           }
+          named_barrier_sync(1 + set, 128);
+          const float* r = red + 32 * set + (e & 31);
+          const float v = (r[0] + r[kRows]) + (r[2 * kRows] + r[3 * kRows]);
+          named_barrier_sync(1 + set, 128);
+          return v;
+        };
+        if (sp == 0 && lane < 4) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) max_s[col(k)] = m[k];
         }
-        named_barrier_sync(1 + set, 128);
+        const float sum = over_tokens(l), sum_r = over_tokens(lr);
         const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kRows;
-        const int rows = min(kRows, s.r.rows - s.group * kRows);  // of the group
+        const int rows = s.rows();
         const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + s.slot;
         if (tid == 0 && !s.whole) group_of[s.slot] = s.group_index;
         if (e < 32) {
           const int c = 32 * set + e;
-          const float sum = (red[c] + red[kRows + c]) + (red[2 * kRows + c] + red[3 * kRows + c]);
           if (s.whole) {
-            factor_s[c] = sum == 0.f ? 0.f : 1.f / sum;
+            factor_s[c] = sum_r == 0.f ? 0.f : 1.f / sum_r;
             if (c < rows) p.lse_out[row_q + c] = sum == 0.f ? -INFINITY : max_s[c] + log2f(sum);
           } else {
-            *reinterpret_cast<float2*>(p.part_ml + (rec * kRows + c) * 2) = make_float2(max_s[c], sum);
+            *reinterpret_cast<float4*>(p.part_ml + (rec * kRows + c) * 4) = make_float4(max_s[c], sum, sum_r, 0.f);
           }
         }
         ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
@@ -961,7 +983,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 }
 
 // Joins the records of a group that several slices share: per row
-//   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L,
+//   M = max m_i, L = sum l_i 2^(m_i - M), lse = M + log2 L,
+//   out = sum O_i 2^(m_i - M) / sum lr_i 2^(m_i - M),
 // in an order that the slices alone give.  Block x has the group x, or where
 // groups outnumber records the group of record x if x is its first one;
 // block y its rows y * rows_per_block ...  Two half blocks take every other
@@ -1022,24 +1045,28 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   };
   load(half);
   if (warp < rows) {
-    float M = -INFINITY, L = 0.f;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + y0 + warp;
+    float M = -INFINITY, L = 0.f, R = 0.f;
+    const float4* ml = reinterpret_cast<const float4*>(p.part_ml) + y0 + warp;
     for (int k = lane; k < count; k += 32) {
-      const float2 v = __ldcg(ml + static_cast<int64_t>(recs[k]) * kRows);
-      M = fmaxf(M, v.x);
-      weight[warp][k] = v.x;
+      const float m = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kRows].x);
+      M = fmaxf(M, m);
+      weight[warp][k] = m;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     for (int k = lane; k < count; k += 32) {
-      const float m = weight[warp][k], l = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kRows].y);
-      const float w = m == -INFINITY ? 0.f : exp2f(m - M);
-      L = fmaf(l, w, L);
+      const float4 q = __ldcg(ml + static_cast<int64_t>(recs[k]) * kRows);
+      const float w = q.x == -INFINITY ? 0.f : exp2f(q.x - M);
+      L = fmaf(q.y, w, L);
+      R = fmaf(q.z, w, R);
       weight[warp][k] = w;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    for (int o = 16; o > 0; o >>= 1) {
+      L += __shfl_xor_sync(0xffffffffu, L, o);
+      R += __shfl_xor_sync(0xffffffffu, R, o);
+    }
+    const float inv = R == 0.f ? 0.f : 1.f / R;
     __syncwarp();
     for (int k = lane; k < count; k += 32) weight[warp][k] *= inv;
     if (lane == 0) p.lse_out[info.x + y0 + warp] = L == 0.f ? -INFINITY : M + log2f(L);
@@ -1090,7 +1117,7 @@ inline int64_t groups_bound(int64_t drafts, int64_t heads, int64_t requests) {
 inline Layout layout(int64_t drafts, int64_t heads, int64_t requests, int sms) {
   Layout a;
   a.part_ml = kWorkspaceHeader;
-  a.part_o = a.part_ml + static_cast<size_t>(2 * sms) * kRows * 2 * sizeof(float);
+  a.part_o = a.part_ml + static_cast<size_t>(2 * sms) * kRows * 4 * sizeof(float);
   a.plan = a.part_o + static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
   // Rounded up generously, so that ordinary batches all need the same bytes
   // and a workspace does not move between them.

@@ -11,8 +11,10 @@ draft i sees position k if k < p, or k = p + j with bit j of its mask set.
 * the base-2 lse moves by at most the largest of its logits' errors, plus the
   exponential's and the sum's (2^-18 is far above both) and one rounding;
 * a weight moves relatively by ln 2 times its logit's and the lse's error;
-* P is rounded to bf16 before the second product: half a step, 2^-8 of each
-  weight at most, and the output once more, 2^-8 of its value.
+* P is rounded to bf16 before the second product, half a step, 2^-8 of each
+  weight at most, and divided by the rounded weights' sum: that moves the
+  output by at most 2^-8 of sum w |c| and 2^-8 of itself; its own rounding by
+  2^-8 of itself once more.
 """
 
 from __future__ import annotations
@@ -73,7 +75,7 @@ def tree_reference(q_nope, q_pe, ckv, kpe, prefix, table, cu, mask, scale):
         seen = torch.where(torch.isfinite(lse[lo:hi]), lse[lo:hi].abs(), 0.0)
         lse_off[lo:hi] = worst + 2.0 ** -18 + seen * 2.0 ** -23
         spread = w @ c.abs()
-        out_off[lo:hi] = spread * (2.0 ** -8 + 2 * math.log(2) * worst + 2.0 ** -17)[..., None] + out[lo:hi].abs() * 2.0 ** -8
+        out_off[lo:hi] = spread * (2.0 ** -8 + 2 * math.log(2) * worst + 2.0 ** -17)[..., None] + out[lo:hi].abs() * 2.0 ** -7
     return out, lse, out_off, lse_off
 
 
