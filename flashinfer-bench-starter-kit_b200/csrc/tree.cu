@@ -26,13 +26,14 @@
 // or HBM in about the time of its MMAs (1152 + 768 clocks, measured 32 and 48
 // a piece).
 //
-// Units are ordered (request, chunk of tiles, group, tile) and cut into equal
-// contiguous slices, one per CTA ("stream-K").  Chunks are at least a slice
-// long, so the groups of a request walk the same pages at the same time on
-// neighbouring CTAs and share them through L2.  A slice's pieces that do not
-// cover their group's whole context are written as fp32 records (slot 0: the
-// piece at the slice's start, slot 1: the one at its end; no other can be
-// partial) and joined by combine_kernel.
+// Units are ordered (request, group, tile) and cut into equal contiguous
+// slices, one per CTA ("stream-K").  (Ordering the groups of a request by
+// chunks of tiles, so that they walk the same pages at the same time, was
+// measured and is slower everywhere, 64 x 65536 tokens included: twice the
+// pieces, and L2 serves the second group well enough as it is.)  A slice's
+// pieces that do not cover their group's whole context are written as fp32
+// records (slot 0: the piece at the slice's start, slot 1: the one at its end;
+// no other can be partial) and joined by combine_kernel.
 #include <cuda_bf16.h>
 
 #include <mutex>
@@ -124,10 +125,11 @@ struct Request {
 };
 
 // Starting a group (its queries, the pipeline's first tile, O's way out) takes
-// about as long as two more tiles.  So a group counts kLead units more than
-// its tiles, at its start, when slices are cut: short contexts then share
-// SMs evenly (64 x 65536 tokens: no change).
-constexpr int kLead = 2;
+// about as long as three more tiles.  So a group counts kLead units more than
+// its tiles, at its start, when slices are cut (200 requests of 50-700 tokens:
+// 48.5 us at 0, 43.2 at 1, 39.4 at 2, 38.0 at 3, 38.5 at 4; long contexts: no
+// change).
+constexpr int kLead = 3;
 
 // Request b as its inputs give it; what they give wrongly is clamped or, if
 // it cannot be, taken as a request without drafts.
@@ -166,41 +168,11 @@ __device__ __forceinline__ int slice_start(int total, int c, int ctas) {
   const int q = total / ctas;
   return q * c + (total - q * ctas) * c / ctas;
 }
-__device__ __forceinline__ int slice_len(int total, int ctas) { return total / ctas + (total % ctas != 0); }
-
-// A group's units are cut into `chunks_of` nearly equal chunks, each at least
-// a slice long (one chunk when a single group would walk them all anyway).
-// There are at most half as many as CTAs, so the products below fit 32 bits.
-__device__ __forceinline__ int chunks_of(const Request& r, int slice) {
-  if (r.groups <= 1) return 1;
-  const int c = r.span / slice;
-  return c < 1 ? 1 : c;
-}
-__device__ __forceinline__ int chunk_start(const Request& r, int chunks, int c) { return r.span * c / chunks; }
-
-// The place of unit `rel`, counted from its request's first.
-struct Place {
-  int chunk, group, unit, u0, u1;  // unit of the group; u0, u1: the chunk's units
-};
-__device__ __forceinline__ Place place_of(const Request& r, int chunks, int rel) {
-  Place q;
-  const int t = rel / r.groups;  // rel = groups * u0 + ...: the chunk is the one holding unit t
-  q.chunk = ((t + 1) * chunks - 1) / r.span;
-  q.u0 = chunk_start(r, chunks, q.chunk);
-  q.u1 = chunk_start(r, chunks, q.chunk + 1);
-  const int in = rel - r.groups * q.u0;
-  const int len = q.u1 - q.u0;
-  q.group = in / len;
-  q.unit = q.u0 + in - q.group * len;
-  return q;
-}
-
 // Where a slice starts, as the plan found it.
 struct Start {
   int b, first, first_group;  // request, its first unit and group over all requests
-  int chunks;
   Request r;
-  Place at;
+  int group, unit;            // attention: of the request; of the group
 };
 
 // A run of tiles of one group.
@@ -218,20 +190,19 @@ struct Segment {
 template <bool kWeights>
 struct Walker {
   const Params& p;
-  int u, u0, u1, slice;
+  int u, u0, u1;
   int b, first;           // request and its first unit
   int first_group;        // its first group, over all requests
   Request r;
-  int chunks;
-  Place at;               // attention: next unit's place
+  int group, unit;        // attention: of the next unit
   int run0, run1, end, g; // weights: current run of tiles, end of the slice's tiles, next group
 
-  __device__ Walker(const Params& prm, int u0_, int u1_, int slice_, const Start& st)
-      : p(prm), u(u0_), u0(u0_), u1(u1_), slice(slice_), b(st.b), first(st.first), first_group(st.first_group) {
+  __device__ Walker(const Params& prm, int u0_, int u1_, const Start& st)
+      : p(prm), u(u0_), u0(u0_), u1(u1_), b(st.b), first(st.first), first_group(st.first_group) {
     if (u0 >= u1) return;
     r = st.r;
-    chunks = st.chunks;
-    at = st.at;
+    group = st.group;
+    unit = st.unit;
     if constexpr (kWeights) start_tiles();
   }
 
@@ -260,8 +231,7 @@ struct Walker {
       if constexpr (kWeights) {
         start_tiles();
       } else {
-        chunks = chunks_of(r, slice);
-        at = place_of(r, chunks, 0);
+        group = unit = 0;
       }
       return true;
     }
@@ -288,28 +258,16 @@ struct Walker {
       while (u < u1) {
         s.b = b;
         s.r = r;
-        s.group = at.group;
-        s.group_index = first_group + at.group;
-        int len = at.u1 - at.unit;
-        if (len > u1 - u) len = u1 - u;
-        s.t0 = at.unit < kLead ? 0 : at.unit - kLead;
-        s.t1 = at.unit + len - kLead;
+        s.group = group;
+        s.group_index = first_group + group;
+        const int len = min(r.span - unit, u1 - u);
+        s.t0 = unit < kLead ? 0 : unit - kLead;
+        s.t1 = unit + len - kLead;
         s.whole = s.t0 == 0 && s.t1 == r.tiles;
         s.slot = u == u0 ? 0 : 1;
         u += len;
-        if (u < u1) {
-          if (++at.group == r.groups) {
-            at.group = 0;
-            ++at.chunk;
-          }
-          if (at.chunk == chunks) {
-            if (!leave()) u = u1;
-          } else {
-            at.u0 = chunk_start(r, chunks, at.chunk);
-            at.u1 = chunk_start(r, chunks, at.chunk + 1);
-            at.unit = at.u0;
-          }
-        }
+        unit = 0;
+        if (u < u1 && ++group == r.groups && !leave()) u = u1;
         if (s.t1 > s.t0) return true;  // else a slice's end within the lead
       }
       return false;
@@ -433,7 +391,6 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   if (nothing) total = units = 0;
   const int ctas = gridDim.x;
   const int u0 = slice_start(total, blockIdx.x, ctas), u1 = slice_start(total, blockIdx.x + 1, ctas);
-  const int slice = slice_len(total, ctas);
   const bool keeper = !kWeights && blockIdx.x == 0;  // writes the groups for combine_kernel
   if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
     for (int b = b_lo; b < b_hi; ++b) {
@@ -441,8 +398,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       const Request r = b == b_lo ? mine : load_request<kWeights>(p, b, bad);
       const int un = r.groups * r.span;
       if (u0 >= before && u0 < before + un) {
-        const int chunks = kWeights ? 1 : chunks_of(r, slice);
-        *found = Start{b, before, gbefore, chunks, r, place_of(r, chunks, u0 - before)};
+        const int group = (u0 - before) / r.span;
+        *found = Start{b, before, gbefore, r, group, u0 - before - group * r.span};
       }
       if (keeper) {
         int2* to = reinterpret_cast<int2*>(p.plan + kPlanGroups) + gbefore;
@@ -457,7 +414,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 
   const uint32_t tmem_base = *tmem_base_smem;
   const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
-  Walker<kWeights> walk(p, u0, u1, slice, *found);
+  Walker<kWeights> walk(p, u0, u1, *found);
   Segment s;
 
   if (warp == kLoadWarp) {
@@ -987,47 +944,50 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 //   out = sum O_i 2^(m_i - M) / sum lr_i 2^(m_i - M),
 // in an order that the slices alone give.  Block x has the group x, or where
 // groups outnumber records the group of record x if x is its first one;
-// block y its rows y * rows_per_block ...  Two half blocks take every other
-// record of a row, a thread four dims: the loads are latency-bound, so many
-// are in flight at once.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 8;       // most rows per block: one warp finds a row's weights
+// block y its rows y * rows_per_block ...  Each kParts-th of the block takes every
+// kParts-th record of a row, a thread four dims: the loads are latency-bound,
+// so many are in flight at once.
+constexpr int kJoinRows = 8;       // most rows per block
 constexpr int kJoinDepth = 8;      // records whose loads a thread has in flight
 
-__global__ void __launch_bounds__(kJoinThreads)
+template <int kParts>
+__global__ void __launch_bounds__(128 * kParts)
 combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   griddep_wait();
+  constexpr int kJoinThreads = 128 * kParts;
+  constexpr int kLooks = 2 * kMaxCtas / kJoinThreads;  // records a thread looks at
   __shared__ int recs[2 * kMaxCtas];
   __shared__ float weight[kJoinRows][2 * kMaxCtas];
-  __shared__ int warp_count[2][kJoinThreads / 32];
-  __shared__ float4 other[kCkv / 4];
+  __shared__ int warp_count[kLooks][kJoinThreads / 32];
+  __shared__ float4 other[kParts > 1 ? kParts - 1 : 1][kCkv / 4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int x = blockIdx.x;
   const int group = by_record ? __ldcg(p.plan + x) : x;
-  int mine[2];
+  int mine[kLooks];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < kLooks; ++k) {
     const int r = tid + k * kJoinThreads;
     mine[k] = r < 2 * ctas ? __ldcg(p.plan + r) : -1;
   }
   if (group < 0) return;
   const int2 info = __ldcg(reinterpret_cast<const int2*>(p.plan + kPlanGroups) + group);
-  unsigned int votes[2];
+  unsigned int votes[kLooks];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < kLooks; ++k) {
     votes[k] = __ballot_sync(0xffffffffu, mine[k] == group);
     if (lane == 0) warp_count[k][warp] = __popc(votes[k]);
   }
   __syncthreads();
   int count = 0;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    int at = count;
+  for (int k = 0; k < kLooks; ++k) {
+    int at = count + __popc(votes[k] & ((1u << lane) - 1u));
+#pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) {
       if (w < warp) at += warp_count[k][w];
       count += warp_count[k][w];
     }
-    if (mine[k] == group) recs[at + __popc(votes[k] & ((1u << lane) - 1u))] = tid + k * kJoinThreads;
+    if (mine[k] == group) recs[at] = tid + k * kJoinThreads;
   }
   __syncthreads();
   if (count == 0 || (by_record && recs[0] != x)) return;  // written whole; or another block's
@@ -1035,22 +995,23 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   const int rows = min(rows_per_block, info.y - y0);
   if (rows <= 0) return;
   // The first records' loads of the first row need no weights: they go first.
-  const int half = tid >> 7, d4 = tid & 127;
+  const int part = tid >> 7, d4 = tid & 127;
   const float4* src = reinterpret_cast<const float4*>(p.part_o) + y0 * (kCkv / 4) + d4;
   float4 v[kJoinDepth];
   auto load = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < kJoinDepth; ++j)
-      if (k0 + 2 * j < count) v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + 2 * j]) * (kPartFloats / 4));
+      if (k0 + kParts * j < count)
+        v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + kParts * j]) * (kPartFloats / 4));
   };
-  load(half);
-  if (warp < rows) {
+  load(part);
+  for (int y = warp; y < rows; y += kJoinThreads / 32) {
     float M = -INFINITY, L = 0.f, R = 0.f;
-    const float4* ml = reinterpret_cast<const float4*>(p.part_ml) + y0 + warp;
+    const float4* ml = reinterpret_cast<const float4*>(p.part_ml) + y0 + y;
     for (int k = lane; k < count; k += 32) {
       const float m = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kRows].x);
       M = fmaxf(M, m);
-      weight[warp][k] = m;
+      weight[y][k] = m;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -1059,7 +1020,7 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
       const float w = q.x == -INFINITY ? 0.f : exp2f(q.x - M);
       L = fmaf(q.y, w, L);
       R = fmaf(q.z, w, R);
-      weight[warp][k] = w;
+      weight[y][k] = w;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -1068,18 +1029,18 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
     }
     const float inv = R == 0.f ? 0.f : 1.f / R;
     __syncwarp();
-    for (int k = lane; k < count; k += 32) weight[warp][k] *= inv;
-    if (lane == 0) p.lse_out[info.x + y0 + warp] = L == 0.f ? -INFINITY : M + log2f(L);
+    for (int k = lane; k < count; k += 32) weight[y][k] *= inv;
+    if (lane == 0) p.lse_out[info.x + y0 + y] = L == 0.f ? -INFINITY : M + log2f(L);
   }
   __syncthreads();
   for (int y = 0; y < rows; ++y) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = half; k0 < count; k0 += 2 * kJoinDepth) {
-      if (y > 0 || k0 > half) load(k0);
+    for (int k0 = part; k0 < count; k0 += kParts * kJoinDepth) {
+      if (y > 0 || k0 > part) load(k0);
 #pragma unroll
       for (int j = 0; j < kJoinDepth; ++j) {
-        if (k0 + 2 * j < count) {
-          const float w = weight[y][k0 + 2 * j];
+        if (k0 + kParts * j < count) {
+          const float w = weight[y][k0 + kParts * j];
           acc.x = fmaf(v[j].x, w, acc.x);
           acc.y = fmaf(v[j].y, w, acc.y);
           acc.z = fmaf(v[j].z, w, acc.z);
@@ -1088,12 +1049,18 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
       }
     }
     src += kCkv / 4;
-    if (half == 1) other[d4] = acc;
+    if (part > 0) other[part - 1][d4] = acc;
     __syncthreads();
-    if (half == 0) {
-      const float4 o = other[d4];
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x + o.x, acc.y + o.y),
-                             __floats2bfloat162_rn(acc.z + o.z, acc.w + o.w)};
+    if (part == 0) {
+#pragma unroll
+      for (int k = 0; k < kParts - 1; ++k) {
+        const float4 o = other[k][d4];
+        acc.x += o.x;
+        acc.y += o.y;
+        acc.z += o.z;
+        acc.w += o.w;
+      }
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x, acc.y), __floats2bfloat162_rn(acc.z, acc.w)};
       *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(info.x) + y0 + y) * kCkv + 4 * d4) =
           *reinterpret_cast<const uint2*>(h);
     }
@@ -1243,14 +1210,18 @@ extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, cons
   if (launch_programmatic(tree::tree_kernel<false>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
                           maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
     return DSA_ERR_CUDA;
-  // Few groups: a block per row, so that a long context's many records are
-  // read by many SMs; many groups: few records each, and fewer blocks.
+  // Up to 16 groups: a row a block of 512 threads, so that a long context's
+  // many records are read by many SMs with many loads in flight (1 request of
+  // 30000 tokens: 26.0 against 31.2 us with 256 threads).  More: a group has few
+  // records, and blocks of 128 threads and several rows cost less (40 requests
+  // of 1000-6000 tokens: 46.1 us; 48.7 with 256 threads, 56.1 with 512).
   const int64_t groups = tree::groups_bound(num_drafts, num_heads, num_requests);
   const bool by_record = groups > 2 * info.num_sms;
   const unsigned int across = static_cast<unsigned int>(by_record ? 2 * info.num_sms : groups);
   const int rows = across <= 32 ? 1 : (across <= 64 ? 2 : (across <= 128 ? 4 : tree::kJoinRows));
-  if (launch_programmatic(tree::combine_kernel, dim3(across, tree::kRows / rows), dim3(tree::kJoinThreads), 0, s, prm,
-                          info.num_sms, rows, by_record) != cudaSuccess)
+  const bool deep = across <= 16;
+  if (launch_programmatic(deep ? tree::combine_kernel<4> : tree::combine_kernel<1>, dim3(across, tree::kRows / rows),
+                          dim3(deep ? 512 : 128), 0, s, prm, info.num_sms, rows, by_record) != cudaSuccess)
     return DSA_ERR_CUDA;
   if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
   return DSA_OK;

@@ -127,7 +127,7 @@ def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_tabl
     shape = tree_mask.shape
     if tree_mask.dtype is not torch.int64 or len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= MAX_MASK_WORDS:
         fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
-    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * (max_pages + 2) > 0x7FFFFFFF:
+    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * (max_pages + 3) > 0x7FFFFFFF:
         fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
     qn, qp, pl, tm = q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), tree_mask.contiguous()
     bt, cu = _int32("block_table", block_table, fail), _int32("cu_drafts", cu_drafts, fail)
