@@ -275,6 +275,57 @@ struct Walker {
   }
 };
 
+// Weights: what no unit writes, the tiles behind each request's tokens.  The
+// (request, tile) places are spread over the CTAs; a CTA's warps take 32 of
+// its places at a time from a counter in shared memory: the value warp, which
+// the weights leave idle, from the start, the others when their tiles are done.
+__device__ __forceinline__ void copy_behind(const Params& p, bool nothing, int* counter) {
+  const int lane = threadIdx.x & 31;
+  const int places = p.num_requests * p.max_pages;
+  const int lo = slice_start(places, blockIdx.x, gridDim.x), hi = slice_start(places, blockIdx.x + 1, gridDim.x);
+  for (;;) {
+    int q0 = 0;
+    if (lane == 0) q0 = lo + 32 * atomicAdd(counter, 1);
+    q0 = __shfl_sync(0xffffffffu, q0, 0);
+    if (q0 >= hi) break;
+    const int q = q0 + lane;
+    const int b = q / p.max_pages, t = q - b * p.max_pages;
+    bool copy = q < hi;
+    if (copy && !nothing) {
+      bool bad;
+      copy = t >= load_request<true>(p, b, bad).tiles;
+    }
+    const int64_t from = b * p.acc_stride + static_cast<int64_t>(t) * kTok;
+    const int64_t to = b * p.acc_out_stride + static_cast<int64_t>(t) * kTok;
+    unsigned int todo = __ballot_sync(0xffffffffu, copy);
+    while (todo != 0) {
+      constexpr int kAtOnce = 8;
+      float v[kAtOnce][2];
+      unsigned int bits = todo;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int l = bits != 0 ? __ffs(bits) - 1 : 0;
+        const float* src = p.acc + __shfl_sync(0xffffffffu, from, l);
+        if (bits != 0) {
+          v[j][0] = src[lane];
+          v[j][1] = src[lane + 32];
+        }
+        bits &= bits - 1;
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int l = todo != 0 ? __ffs(todo) - 1 : 0;
+        float* dst = p.acc_out + __shfl_sync(0xffffffffu, to, l);
+        if (todo != 0) {
+          dst[lane] = v[j][0];
+          dst[lane + 32] = v[j][1];
+        }
+        todo &= todo - 1;
+      }
+    }
+  }
+}
+
 // Bits of one thread's 8 columns (rows of Q) that see position pos, which
 // lies at or behind the prefix.
 __device__ __forceinline__ uint32_t visible_columns(const Params& p, const Segment& s, int pos, const int (&draft)[8]) {
@@ -314,8 +365,9 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   int* misc = reinterpret_cast<int*>(smem + kOffMisc);
   uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
   int* abort_flag = misc + 1;
-  Start* found = reinterpret_cast<Start*>(misc + 2);
-  static_assert(8 + sizeof(Start) <= kOffRed - kOffMisc, "misc");
+  int* copied = misc + 2;                    // weights: see copy_behind
+  Start* found = reinterpret_cast<Start*>(misc + 3);
+  static_assert(12 + sizeof(Start) <= kOffRed - kOffMisc, "misc");
   float* red = reinterpret_cast<float*>(smem + kOffRed);
   int* warp_sums = reinterpret_cast<int*>(red);  // planning: [11] units, [11] groups
   float* factor_s = reinterpret_cast<float*>(smem + kOffFactor);  // O's rescaling; at the end 1 / l
@@ -331,6 +383,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     mbar_init(p_full, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
     *abort_flag = 0;
+    *copied = 0;
     fence_mbar_init();
   }
   if (warp == kLoadWarp && elect_one()) {
@@ -523,6 +576,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     __syncwarp();
   } else if (warp == kValueWarp) {
     // ------------------------------------------------------------ O^T += V^T P^T
+    if (kWeights && p.acc_out != p.acc) copy_behind(p, nothing, copied);
     if (!kWeights && elect_one()) {
       const uint64_t v_desc = sdesc_sw128(smem_u32(smem), kChunkBytes, 1024);
       const uint64_t p_desc = sdesc_sw128(smem_u32(p_mem), kChunkBytes, 1024);
@@ -570,19 +624,18 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     bool ok = true;
 
     if constexpr (kWeights) {
-      // What no unit writes: the tiles behind every request's tokens, spread
-      // over all CTAs.
-      if (p.acc_out != p.acc) {
-        const int64_t tiles = static_cast<int64_t>(p.num_requests) * p.max_pages;
-        for (int64_t q = static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6); q < tiles; q += 4 * ctas) {
-          const int b = static_cast<int>(q / p.max_pages), t = static_cast<int>(q % p.max_pages);
-          bool bad;
-          if (!nothing && t < load_request<kWeights>(p, b, bad).tiles) continue;
-          const int64_t at = static_cast<int64_t>(t) * kTok + (tid & 63);
-          p.acc_out[b * p.acc_out_stride + at] = p.acc[b * p.acc_stride + at];
-        }
-      }
+      // The accumulators that a run of tiles will be added to, read at its start.
+      constexpr int kOld = kSumTiles * kTok / (32 * kSoftWarps);
+      float old[kOld];
       while (walk.next(s)) {
+        if (s.first_group) {
+          const float* acc = p.acc + s.b * p.acc_stride + static_cast<int64_t>(s.t0) * kTok;
+#pragma unroll
+          for (int k = 0; k < kOld; ++k) {
+            const int q = tid + k * 32 * kSoftWarps;
+            old[k] = q < (s.t1 - s.t0) * kTok ? acc[q] : 0.f;
+          }
+        }
         float lse[8];
         int draft[8];
         uint32_t live = 0;
@@ -652,14 +705,16 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
         }
         if (s.last_group) {
           named_barrier_sync(3, 32 * kSoftWarps);
-          for (int q = tid; q < (s.t1 - s.t0) * kTok; q += 32 * kSoftWarps) {
-            const int64_t at = static_cast<int64_t>(s.t0) * kTok + q;
-            p.acc_out[s.b * p.acc_out_stride + at] =
-                p.acc[s.b * p.acc_stride + at] + (sums[q] + sums[kSumTiles * kTok + q]);
+          float* out = p.acc_out + s.b * p.acc_out_stride + static_cast<int64_t>(s.t0) * kTok;
+#pragma unroll
+          for (int k = 0; k < kOld; ++k) {
+            const int q = tid + k * 32 * kSoftWarps;
+            if (q < (s.t1 - s.t0) * kTok) out[q] = old[k] + (sums[q] + sums[kSumTiles * kTok + q]);
           }
           named_barrier_sync(3, 32 * kSoftWarps);
         }
       }
+      if (p.acc_out != p.acc) copy_behind(p, nothing, copied);
     } else {
       // Online softmax in base 2.  The running max m[k] of a column is the
       // same in every thread that has it.  It moves only when some token of
