@@ -57,7 +57,7 @@ struct Params {
 };
 
 __device__ __forceinline__ int length_of(const Params& p, int b, bool& bad) {
-  const int L = __ldg(p.seq_lens + b);
+  const int L = p.seq_lens[b];
   const int cap = p.max_pages * kPage;
   bad = L < 0 || L > cap;
   return L < 0 ? 0 : (L > cap ? cap : L);
@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
     const int pos = i < p.budget ? __ldcg(p.keep + static_cast<int64_t>(b) * p.budget + i) : -1;
     int from = -1, to = -1;                            // pages; from < 0: nothing to move
     if (pos >= 0) {
-      from = __ldg(p.block_table + static_cast<int64_t>(b) * p.max_pages + pos / kPage);
-      to = __ldg(p.new_block_table + static_cast<int64_t>(b) * p.new_max_pages + i / kPage);
+      from = p.block_table[static_cast<int64_t>(b) * p.max_pages + pos / kPage];
+      to = p.new_block_table[static_cast<int64_t>(b) * p.new_max_pages + i / kPage];
       if (from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages) {
         if (lane < kMoveTokens) atomicOr(p.status, DSA_DEV_BAD_PAGE);
         from = -1;

@@ -90,6 +90,8 @@ static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 static_assert(2 * kSumTiles * kTok * 4 <= kTok * 128, "the weights' sums take P's place");
 
 constexpr int kMaxRequests = 65536;
+constexpr int64_t kMaxRows = 1 << 24;          // drafts x heads
+constexpr int64_t kMaxUnits = 1 << 30;         // units and (request, page) places are counted in 32 bits
 constexpr int kMaxCtas = 256;
 // Plan, in ints: the group of each record (-1: none), then first row and rows
 // of each group.
@@ -131,14 +133,18 @@ struct Request {
 // change).
 constexpr int kLead = 3;
 
+// Inputs are read with plain loads, not through the non-coherent path: a
+// kernel launched programmatically may lie on an SM while the one before it
+// still writes them.
+//
 // Request b as its inputs give it; what they give wrongly is clamped or, if
 // it cannot be, taken as a request without drafts.
 template <bool kWeights>
 __device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
   Request r;
-  const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
+  const int lo = p.cu[b], hi = p.cu[b + 1];
   const int cap = p.max_pages * kTok;
-  r.prefix = __ldg(p.prefix_lens + b);
+  r.prefix = p.prefix_lens[b];
   r.row0 = lo;
   r.n = hi - lo;
   bad = false;
@@ -334,7 +340,7 @@ __device__ __forceinline__ uint32_t visible_columns(const Params& p, const Segme
   if (j < s.r.n && j < 64 * p.mask_words) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const long long w = __ldg(p.mask + static_cast<int64_t>(s.r.row0 + draft[k]) * p.mask_words + (j >> 6));
+      const long long w = p.mask[static_cast<int64_t>(s.r.row0 + draft[k]) * p.mask_words + (j >> 6)];
       m |= static_cast<uint32_t>((w >> (j & 63)) & 1) << k;
     }
   }
@@ -408,7 +414,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     bool bad;
     const Request r = load_request<kWeights>(p, b, bad);
     if (b == b_lo) mine = r;
-    decreasing |= __ldg(p.cu + b + 1) < __ldg(p.cu + b);
+    decreasing |= p.cu[b + 1] < p.cu[b];
     units += r.groups * r.span;
     groups += r.groups;
     any_bad |= bad;
@@ -481,12 +487,12 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
       bool ok = true;
       while (ok && walk.next(s)) {
         const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
-        int next_page = __ldg(row + s.t0);
+        int next_page = row[s.t0];
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           // A page outside the pool reads as zeros (a box outside the tensor
           // is filled with them); its tokens are masked below.
           const int page = next_page < 0 || next_page >= p.num_pages ? p.num_pages : next_page;
-          if (t + 1 < s.t1) next_page = __ldg(row + t + 1);
+          if (t + 1 < s.t1) next_page = row[t + 1];
           const int st = i & 1;
           const uint32_t parity = ((i >> 1) & 1) ^ 1;
           uint8_t* dst = smem + st * kTileBytes;
@@ -643,17 +649,17 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
         for (int k = 0; k < 8; ++k) {
           const int row = s.group * kRows + col(k);
           const bool in = row < s.r.rows;
-          lse[k] = in ? __ldg(p.lse_in + static_cast<int64_t>(s.r.row0) * p.heads + row) : 0.f;
+          lse[k] = in ? p.lse_in[static_cast<int64_t>(s.r.row0) * p.heads + row] : 0.f;
           draft[k] = in ? row / p.heads : 0;
           if (in && lse[k] != -INFINITY) live |= 1u << k;  // a row that saw nothing gives nothing
         }
         const bool all_live = __all_sync(0xffffffffu, live == 0xffu);
         const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
-        int next_page = __ldg(bt + s.t0);
+        int next_page = bt[s.t0];
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           const int st = i & 1;
           const int page = next_page;
-          if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
+          if (t + 1 < s.t1) next_page = bt[t + 1];
           uint32_t see0 = live, see1 = live;
           const bool lost = page < 0 || page >= p.num_pages;
           const bool tail = (t + 1) * kTok > s.r.prefix;
@@ -746,11 +752,11 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           unset |= in;
         }
         const int32_t* bt = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
-        int next_page = __ldg(bt + s.t0);
+        int next_page = bt[s.t0];
         for (int t = s.t0; t < s.t1; ++t, ++i) {
           const int st = i & 1;
           const int page = next_page;
-          if (t + 1 < s.t1) next_page = __ldg(bt + t + 1);
+          if (t + 1 < s.t1) next_page = bt[t + 1];
           uint32_t see0 = 0xffu, see1 = 0xffu;
           const bool tail = (t + 1) * kTok > s.r.prefix;
           const bool lost = page < 0 || page >= p.num_pages;
@@ -1136,22 +1142,20 @@ inline int64_t groups_bound(int64_t drafts, int64_t heads, int64_t requests) {
   return drafts * heads / kRows + requests;
 }
 
-inline Layout layout(int64_t drafts, int64_t heads, int64_t requests, int sms) {
+// The same for every call that is accepted, so that a workspace never has to
+// move (a captured graph would go on using the old one).
+inline Layout layout(int sms) {
   Layout a;
   a.part_ml = kWorkspaceHeader;
   a.part_o = a.part_ml + static_cast<size_t>(2 * sms) * kRows * 4 * sizeof(float);
   a.plan = a.part_o + static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
-  // Rounded up generously, so that ordinary batches all need the same bytes
-  // and a workspace does not move between them.
-  size_t words = kPlanGroups + 2 * static_cast<size_t>(groups_bound(drafts, heads, requests));
-  words = (words + 65535) / 65536 * 65536;
-  a.bytes = a.plan + words * sizeof(int);
+  a.bytes = a.plan + (kPlanGroups + 2 * static_cast<size_t>(groups_bound(kMaxRows, 1, kMaxRequests))) * sizeof(int);
   return a;
 }
 
 inline bool sizes_ok(int64_t drafts, int64_t heads, int64_t requests) {
   return drafts >= 0 && heads >= 1 && heads <= 128 && requests >= 0 && requests <= kMaxRequests &&
-         drafts * heads <= (1 << 28);
+         drafts * heads <= kMaxRows;
 }
 
 int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64_t ckv_page, int64_t ckv_row,
@@ -1165,7 +1169,7 @@ int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64
   if (num_pages < 1 || num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || mask_words < 1 ||
       mask_words > 64)
     return DSA_ERR_INVALID_ARGUMENT;
-  if (groups_bound(drafts, heads, requests) * (max_pages + kLead) > 0x7FFFFFFF) return DSA_ERR_INVALID_ARGUMENT;
+  if (groups_bound(drafts, heads, requests) * (max_pages + kLead) > kMaxUnits) return DSA_ERR_INVALID_ARGUMENT;
   if (ckv_row < kCkv * 2 || kpe_row < kKpe * 2 || ckv_page < 0 || kpe_page < 0) return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(ckv) || !aligned16(kpe) || !aligned16(workspace) ||
       ((ckv_page | ckv_row | kpe_page | kpe_row) & 15))
@@ -1178,7 +1182,7 @@ int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64
   if (st != DSA_OK) return st;
   if (static_cast<size_t>(kSmemBytes) > info->max_smem_optin || info->num_sms > kMaxCtas)
     return DSA_ERR_UNSUPPORTED_DEVICE;
-  const Layout a = layout(drafts, heads, requests, info->num_sms);
+  const Layout a = layout(info->num_sms);
   if (workspace_bytes < (records ? a.bytes : kWorkspaceHeader)) return DSA_ERR_WORKSPACE_TOO_SMALL;
   std::call_once(g_once[info->device], [&]() {
     g_status[info->device] =
@@ -1231,12 +1235,11 @@ int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64
 
 using namespace dsa;
 
-extern "C" size_t dsa_tree_attention_workspace_bytes(int32_t num_drafts, int32_t num_heads, int32_t num_requests) {
-  if (!tree::sizes_ok(num_drafts, num_heads, num_requests)) return 0;
+extern "C" size_t dsa_tree_attention_workspace_bytes(void) {
   DeviceInfo info;
   // Without a usable device, size for the largest SM count of the family.
   const int sms = current_device_info(&info) == DSA_OK ? info.num_sms : 160;
-  return tree::layout(num_drafts, num_heads, num_requests, sms).bytes;
+  return tree::layout(sms).bytes;
 }
 
 extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const void* ckv_cache,

@@ -49,7 +49,7 @@ SIGNATURES = {
     "dsa_indexer_prefill_run": (ctypes.c_int, [_P, _P, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_int32, _P, _P, ctypes.c_size_t,
                                                _P]),
-    "dsa_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "dsa_tree_attention_workspace_bytes": (ctypes.c_size_t, []),
     "dsa_tree_attention_run": (ctypes.c_int, _TREE + [_P, _P, _P, ctypes.c_size_t, _P]),
     "dsa_tree_weights_run": (ctypes.c_int, _TREE + [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_size_t,
                                                     _P]),

@@ -60,6 +60,18 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [B, width] float32 tensors with contiguous rows share memory."""
+    lo, hi = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
+    apart = (hi.data_ptr() - lo.data_ptr()) // 4
+    pitch, width = _pitch(lo), lo.shape[1]
+    if apart >= (lo.shape[0] - 1) * pitch + width:
+        return False
+    # Interleaved rows of one buffer, such as its left and right columns.
+    at = apart % pitch
+    return _pitch(hi) != pitch or at < width or at + hi.shape[1] > pitch
+
+
 def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor,
                prefix_lens: torch.Tensor, block_table: torch.Tensor, cu_drafts: torch.Tensor,
                tree_mask: torch.Tensor, sm_scale, lse: torch.Tensor, acc: torch.Tensor, out: torch.Tensor) -> None:
@@ -71,9 +83,9 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
         _fail_acc(f"lse must be float32 [{T}, {H}]")
     _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_acc)
     _rows_of("out", out, (B, max_pages * PAGE_SIZE), _fail_acc)
-    same = acc.data_ptr() == out.data_ptr()
-    if same and _pitch(acc) != _pitch(out):
-        _fail_acc("acc and out overlap")
+    same = acc.data_ptr() == out.data_ptr() and _pitch(acc) == _pitch(out)
+    if not same and B > 0 and _overlap(acc, out):
+        _fail_acc("out must be acc itself or not overlap it")
     if isinstance(sm_scale, torch.Tensor):
         sm_scale = float(sm_scale.item())
     if B == 0:
@@ -141,8 +153,8 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
         _fail_run(f"num_sink {num_sink} and num_recent {num_recent} must fit the budget of {budget}")
     _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_run)
     _rows_of("new_acc", new_acc, (B, new_pages * PAGE_SIZE), _fail_run)
-    if acc.data_ptr() == new_acc.data_ptr() and B > 0:
-        _fail_run("new_acc must not be acc")
+    if B > 0 and _overlap(acc, new_acc):
+        _fail_run("new_acc must not overlap acc")
     if B == 0:
         return
     if B > 65536 or max_pages > 1 << 24 or new_pages > 1 << 24:

@@ -47,7 +47,7 @@ MAX_HEADS = 128
 MAX_MASK_WORDS = 64
 
 _CHECK = os.environ.get("DSA_B200_CHECK", "0") not in ("", "0")
-_ws_bytes: dict = {}  # (device index, drafts, heads, requests) -> workspace bytes
+_ws_bytes: dict = {}  # device index -> dsa_tree_attention_workspace_bytes
 
 
 def masks_from_parents(parents) -> list:
@@ -127,7 +127,7 @@ def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_tabl
     shape = tree_mask.shape
     if tree_mask.dtype is not torch.int64 or len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= MAX_MASK_WORDS:
         fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
-    if T * H > 1 << 28 or B > 65536 or (T * H // 64 + B) * (max_pages + 3) > 0x7FFFFFFF:
+    if T * H > 1 << 24 or B > 65536 or (T * H // 64 + B) * (max_pages + 3) > 1 << 30:
         fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
     qn, qp, pl, tm = q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), tree_mask.contiguous()
     bt, cu = _int32("block_table", block_table, fail), _int32("cu_drafts", cu_drafts, fail)
@@ -148,13 +148,10 @@ def _fail(msg: str) -> None:
     raise ValueError(f"dsa_tree.run: {msg}")
 
 
-def _workspace_bytes(dev: torch.device, T: int, H: int, B: int) -> int:
-    key = (dev.index, T, H, B)
-    n = _ws_bytes.get(key)
+def _workspace_bytes(dev: torch.device) -> int:
+    n = _ws_bytes.get(dev.index)
     if n is None:
-        if len(_ws_bytes) > 4096:
-            _ws_bytes.clear()
-        n = _ws_bytes[key] = _native.call_on(dev, _native.lib().dsa_tree_attention_workspace_bytes, T, H, B)
+        n = _ws_bytes[dev.index] = _native.call_on(dev, _native.lib().dsa_tree_attention_workspace_bytes)
     return n
 
 
@@ -175,7 +172,7 @@ def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_c
         return
     dev = q_nope.device
     cur = _native.current_stream(dev)
-    ws = workspace.get(dev, "tree", _workspace_bytes(dev, T, H, B), cur)
+    ws = workspace.get(dev, "tree", _workspace_bytes(dev), cur)
     st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, float(sm_scale), output.data_ptr(),
                          lse.data_ptr(), ws.data_ptr(), ws.numel(), cur)
     _native.check(st, "dsa_tree_attention_run")

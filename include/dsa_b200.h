@@ -239,14 +239,12 @@ DSA_API int dsa_index_cache_write(const void* k, const int64_t* slot_mapping, in
                                   void* k_index_cache_fp8, int64_t num_pages, int32_t ue8m0,
                                   uint32_t* status, void* stream);
 
-/* Bytes of device workspace dsa_tree_attention_run needs: a 256-byte header,
- * two fp32 records of 64 rows per SM (39 MB in all) for contexts that several
- * SMs share, and the plan of the call.  The same for all ordinary batches
- * (up to some 60000 rows groups and requests).  0 for sizes that
- * dsa_tree_attention_run refuses.  Zero-fill it once (its status word);
- * nothing else in it carries over from call to call. */
-DSA_API size_t dsa_tree_attention_workspace_bytes(int32_t num_drafts, int32_t num_heads,
-                                                  int32_t num_requests);
+/* Bytes of device workspace dsa_tree_attention_run needs on this device, the
+ * same for every call: a 256-byte header, two fp32 records of 64 rows per SM
+ * (39 MB in all) for contexts that several SMs share, and the call's list of
+ * row groups (2.6 MB).  Zero-fill it once (its status word); nothing else in
+ * it carries over from call to call. */
+DSA_API size_t dsa_tree_attention_workspace_bytes(void);
 
 /* Attention of a tree of drafted tokens over the paged ckv / kpe cache
  * (speculative decoding; one draft per request is plain dense decoding).
@@ -273,7 +271,9 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(int32_t num_drafts, int32_t nu
  *   lse           [num_drafts, num_heads] fp32, base-2 log-sum-exp of the
  *                 scaled logits; a row that sees nothing has -inf, output 0
  *
- * 1 <= num_heads <= 128.  Masked cache rows may hold anything.  Data-dependent
+ * 1 <= num_heads <= 128; num_drafts * num_heads <= 2^24, num_requests <= 65536
+ * and (num_drafts * num_heads / 64 + num_requests) * (max_pages + 3) <= 2^30.
+ * Masked cache rows may hold anything.  Data-dependent
  * errors: lengths that do not fit the table (clamped), drafts that do not fit
  * cu_drafts or the mask (left out): DSA_DEV_BAD_SEQ_LEN; page ids outside the
  * pool (their tokens are masked): DSA_DEV_BAD_PAGE. */

@@ -193,7 +193,7 @@ def test_refusals(cuda_device):
     for change in (dict(num_sink=-1), dict(num_sink=200, num_recent=101), dict(keep=good["keep"][:, :0]),
                    dict(keep=torch.empty(2, 321, dtype=torch.int32, device=d)), dict(keep=good["keep"].long()),
                    dict(acc=good["acc"][:, 1:]), dict(acc=good["acc"].double()), dict(new_acc=good["new_acc"][:, :-1]),
-                   dict(new_acc=good["acc"][:, :320], acc=good["acc"]), dict(seq_lens=good["seq_lens"].long()),
+                   dict(new_acc=good["acc"][:, :320], acc=good["acc"]), dict(new_acc=good["acc"][:, 64:384]), dict(seq_lens=good["seq_lens"].long()),
                    dict(new_seq_lens=good["new_seq_lens"][:1]), dict(block_table=good["block_table"].float()),
                    dict(kpe_cache=good["kpe_cache"][1:]), dict(ckv_cache=good["ckv_cache"].half()),
                    dict(k_index_cache_fp8=good["k_index_cache_fp8"][1:]), dict(acc=good["acc"].cpu()),
@@ -303,3 +303,67 @@ def test_a_decode_loop_with_eviction(cuda_device):
     attention.run(dec.q_nope, dec.q_pe, dec.ckv_cache, dec.kpe_cache, topk, scale, so, sl)
     ro, rl = oatt.attention_reference(dec.q_nope, dec.q_pe, dec.ckv_cache, dec.kpe_cache, topk, scale)
     assert compare.harness_close(so.cpu(), ro, 1e-2, 1e-2).ok and compare.harness_close(sl.cpu(), rl, 1e-3, 1e-3).ok
+
+
+def test_pages_behind_four_gigabytes(cuda_device):
+    c = Case([900, 400], 300, cuda_device, seed=13)
+    ckv = torch.zeros(70000, 64, 512, dtype=torch.bfloat16, device=cuda_device)
+    kpe = torch.zeros(70000, 64, 64, dtype=torch.bfloat16, device=cuda_device)
+    index = torch.zeros(70000, 64, 1, 132, dtype=torch.uint8, device=cuda_device)
+    pages = c.ckv.shape[0]
+    to = 69999 - 500 * torch.arange(pages)
+    ckv[to.to(cuda_device)], kpe[to.to(cuda_device)] = c.ckv.to(cuda_device), c.kpe.to(cuda_device)
+    index[to.to(cuda_device)] = c.index.to(cuda_device)
+    far = lambda t: torch.where(t >= 0, to[t.clamp(min=0).long()], -1).to(cuda_device)  # noqa: E731
+    keep = torch.empty(2, 300, dtype=torch.int32, device=cuda_device)
+    seq, acc = torch.empty(2, dtype=torch.int32, device=cuda_device), torch.empty(2, 320, device=cuda_device)
+    evict.run(c.acc.to(cuda_device), c.seq.to(cuda_device), far(c.table), far(c.new_table), ckv, kpe, index, 4, 4, keep, seq, acc)
+    back = to.to(cuda_device)
+    c.check({"ckv": ckv[back].cpu(), "kpe": kpe[back].cpu(), "index": index[back].cpu(), "keep": keep.cpu(),
+             "seq": seq.cpu(), "acc": acc.cpu()}, 4, 4)
+
+
+def test_a_whole_step_in_one_graph(cuda_device):
+    """Attention, accumulation and eviction captured together and replayed for new lengths."""
+    d, scale = cuda_device, 1 / math.sqrt(192)
+    g = torch.Generator().manual_seed(14)
+    dec = workloads.make_decode_inputs([3000, 1200], seed=14, device=d, pool_pages=120)
+    used = {int(x) for x in dec.indexer.block_table.flatten() if x >= 0}
+    free = torch.tensor([x for x in range(120) if x not in used][:20], dtype=torch.int32)
+    new_bt = free.reshape(2, 10).to(d)
+    cu = torch.tensor([0, 2, 5], dtype=torch.int32, device=d)
+    mask = torch.tensor(tree.masks_from_parents([-1, 0]) + tree.masks_from_parents([-1, 0, 0]), device=d)
+    qn, qp = (torch.randn(5, 16, w, generator=g).to(torch.bfloat16).to(d) for w in (512, 64))
+    prefix = torch.tensor([2900, 1100], dtype=torch.int32, device=d)
+    seq = torch.empty_like(prefix)
+    bt = dec.indexer.block_table
+    acc, new_acc = torch.zeros(2, bt.shape[1] * 64, device=d), torch.zeros(2, 640, device=d)
+    out, lse = torch.zeros(5, 16, 512, dtype=torch.bfloat16, device=d), torch.zeros(5, 16, device=d)
+    keep, new_seq = torch.zeros(2, 600, dtype=torch.int32, device=d), torch.zeros_like(seq)
+
+    def step():
+        rows = (qn, qp, dec.ckv_cache, dec.kpe_cache, prefix, bt, cu, mask, scale)
+        tree.run(*rows, out, lse)
+        evict.accumulate(*rows, lse, acc, acc)
+        torch.add(prefix, cu[1:] - cu[:-1], out=seq)
+        evict.run(acc, seq, bt, new_bt, dec.ckv_cache, dec.kpe_cache, dec.indexer.k_index_cache_fp8, 4, 32, keep, new_seq, new_acc)
+
+    side = torch.cuda.Stream(d)
+    side.wait_stream(torch.cuda.current_stream(d))
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    for lengths in ([2900, 1100], [700, 400]):
+        prefix.copy_(torch.tensor(lengths, dtype=torch.int32))
+        acc.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        a, got = acc.cpu(), (keep.cpu(), new_seq.cpu(), new_acc.cpu())
+        kept = otree.evict_reference(a, seq.cpu(), 600, 4, 32)
+        for b, k in enumerate(kept):
+            assert int(got[1][b]) == len(k) and got[0][b, :len(k)].tolist() == k
+            assert torch.equal(got[2][b, :len(k)], a[b, k])
+        assert torch.allclose(a.sum(1), torch.tensor([32.0, 48.0]), rtol=1e-3)

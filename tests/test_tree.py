@@ -23,18 +23,16 @@ def call(lib, requests=1, drafts=2, heads=16, max_pages=4, words=1, pages=3, q=1
     (dict(drafts=0), 0), (dict(requests=0), 0), (dict(q=None), 1), (dict(ws=None), 1), (dict(out=None), 1),
     (dict(pages=0), 1), (dict(max_pages=0), 1), (dict(words=0), 1), (dict(words=65), 1), (dict(ckv_row=512), 1),
     (dict(ckv=8), 2), (dict(ckv_page=65528), 2), (dict(kpe_row=136), 2), (dict(mask=20), 2), (dict(out=8), 2),
-    (dict(max_pages=1 << 24, drafts=1 << 16), 1),
+    (dict(max_pages=1 << 24, drafts=1 << 16), 1), (dict(drafts=(1 << 20) + 1), 1), (dict(max_pages=(1 << 24) + 1), 1),
 ])
 def test_c_abi_refuses_bad_arguments(change, status):
     assert call(_native.lib(), **change) == status
 
 
-def test_workspace_sizes():
-    lib = _native.lib()
-    small, big = (lib.dsa_tree_attention_workspace_bytes(t, 16, b) for t, b in ((1, 1), (4096, 1024)))
-    assert small == big > 0  # ordinary batches share one workspace
-    assert lib.dsa_tree_attention_workspace_bytes(1 << 20, 128, 65536) > big
-    assert lib.dsa_tree_attention_workspace_bytes(1, 200, 1) == 0
+def test_workspace_is_the_same_for_every_call():
+    # without a GPU: two records of 64 rows for each of 160 SMs, and the groups of the largest call
+    records, groups = 2 * 160 * 64 * (512 + 4) * 4, 2 * (2 ** 24 // 64 + 65536) * 4
+    assert _native.lib().dsa_tree_attention_workspace_bytes() >= 256 + records * 148 // 160 + groups
 
 
 def test_masks_from_parents():
@@ -97,6 +95,19 @@ def test_weights_c_abi_refuses_bad_arguments(change, status):
     assert _native.lib().dsa_tree_weights_run(
         P(16), P(16), P(16), 65536, 1024, P(16), 8192, 128, 3, P(16), P(16), P(16), P(16), a["requests"], 2, 16, 4, 1, 0.1,
         P(a["lse"]), P(a["acc"]), a["stride"], P(a["out"]), a["out_stride"], P(16), 256, None) == status
+
+
+def test_overlapping_accumulators():
+    buf = torch.zeros(1000)
+    rows = lambda at, n, width, pitch: buf[at:].as_strided((n, width), (pitch, 1))  # noqa: E731
+    a = rows(0, 4, 64, 150)
+    assert not evict._overlap(a, rows(64, 4, 64, 150)) and not evict._overlap(rows(64, 4, 64, 150), a)
+    assert not evict._overlap(a, rows(514, 2, 64, 64))       # behind the last row
+    assert evict._overlap(a, rows(1, 4, 64, 150))
+    assert evict._overlap(a, rows(100, 4, 64, 150))          # wraps into the next row
+    assert evict._overlap(a, rows(64, 4, 64, 151))
+    assert evict._overlap(a, rows(513, 2, 64, 64))
+    assert not evict._overlap(rows(0, 1, 64, 7), rows(64, 1, 64, 7))
 
 
 def test_evict_oracle():

@@ -297,3 +297,110 @@ def test_no_drafts_at_all(cuda_device):
     tree.run(*args, SCALE, o[:0], l[:0])
     evict.accumulate(*args, SCALE, l[:0], acc, out)
     assert torch.equal(out, acc)
+
+
+def test_pages_behind_four_gigabytes(cuda_device):
+    """Page offsets that pass 32 bits, in a pool of 70000 pages (4.6 GB of ckv)."""
+    c = Case([300, 90], [4, 2], 16, seed=23, device=cuda_device)
+    args = c.args()
+    need = [int((t >= 0).sum()) for t in c.table]
+    ckv = torch.zeros(70000, 64, 512, dtype=torch.bfloat16, device=cuda_device)
+    kpe = torch.zeros(70000, 64, 64, dtype=torch.bfloat16, device=cuda_device)
+    far = torch.full_like(args[5], -1)
+    at = 69999
+    for b, n in enumerate(need):
+        for k in range(n):
+            far[b, k] = at
+            ckv[at], kpe[at] = args[2][args[5][b, k]], args[3][args[5][b, k]]
+            at -= 700
+    near = run(c, args)
+    args[2], args[3], args[5] = ckv, kpe, far
+    out, lse = run(c, args)
+    c.check(out, lse)
+    assert torch.equal(out, near[0]) and torch.equal(lse, near[1])
+    acc = torch.rand(2, far.shape[1] * 64, device=cuda_device)
+    got = weigh(c, args, acc=acc, lse=lse)[2]
+    assert torch.equal(got, weigh(c, c.args(), acc=acc, lse=lse)[2])
+
+
+def test_two_streams_and_two_graphs_at_once(cuda_device):
+    cases = [Case([4000, 900, 2500], [9, 2, 5], 16, seed=24, device=cuda_device),
+             Case([700, 6000], [20, 3], 8, seed=25, device=cuda_device)]
+    args = [c.args() for c in cases]
+    want = [run(c, a) for c, a in zip(cases, args)]
+    accs = [weigh(c, a, lse=w[1]) for c, a, w in zip(cases, args, want)]
+    streams = [torch.cuda.Stream(cuda_device) for _ in cases]
+    outs = [c.outs() for c in cases]
+    news = [torch.zeros_like(a[1]) for a in accs]
+    graphs = []
+    for c, a, o, w, n, s in zip(cases, args, outs, accs, news, streams):
+        s.wait_stream(torch.cuda.current_stream(cuda_device))
+        with torch.cuda.stream(s):
+            tree.run(*a, SCALE, *o)
+            evict.accumulate(*a, SCALE, o[1], w[1], n)
+            s.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                tree.run(*a, SCALE, *o)
+                evict.accumulate(*a, SCALE, o[1], w[1], n)
+    for together in (False, True):
+        for t in [*outs[0], *outs[1], *news]:
+            t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for c, a, o, w, n, s, g in zip(cases, args, outs, accs, news, streams, graphs):
+                with torch.cuda.stream(s):
+                    if together:
+                        g.replay()
+                    else:
+                        tree.run(*a, SCALE, *o)
+                        evict.accumulate(*a, SCALE, o[1], w[1], n)
+        torch.cuda.synchronize()
+        for o, w, n, a in zip(outs, want, news, accs):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]) and torch.equal(n, a[2])
+
+
+def test_other_requests_non_finite_queries_do_not_leak(cuda_device):
+    """A group's columns behind its rows hold the next request's queries."""
+    c = Case([500, 300], [1, 2], 16, seed=26, device=cuda_device)
+    args = c.args()
+    good = run(c, args)
+    args[0] = args[0].clone()
+    args[0][1:] = math.nan
+    out, lse = run(c, args)
+    assert torch.equal(out[0], good[0][0]) and torch.equal(lse[0], good[1][0])
+    assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
+    acc = torch.zeros(2, args[5].shape[1] * 64, device=cuda_device)
+    got = weigh(c, args, acc=acc, lse=lse)[2]
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1, :300]).all() and (got[1, 302:] == 0).all()
+
+
+def test_refusals(cuda_device):
+    c = Case([100, 20], [3, 2], 16, seed=27, device=cuda_device)
+    q, pe, ckv, kpe, prefix, table, cu, mask = c.args()
+    out, lse = c.outs()
+    good = dict(q_nope=q, q_pe=pe, ckv_cache=ckv, kpe_cache=kpe, prefix_lens=prefix, block_table=table, cu_drafts=cu,
+                tree_mask=mask, sm_scale=SCALE)
+    tree.run(**good, output=out, lse=lse)
+    acc = torch.zeros(2, table.shape[1] * 64, device=cuda_device)
+    evict.accumulate(**good, lse=lse, acc=acc, out=acc)
+    wrong = [dict(q_nope=q.float()), dict(q_nope=q[:, :, :511]), dict(q_nope=q.cpu()), dict(q_pe=pe[1:]), dict(q_pe=pe.half()),
+             dict(q_nope=q.repeat(1, 9, 1), q_pe=pe.repeat(1, 9, 1)), dict(ckv_cache=ckv.flatten(0, 1)), dict(ckv_cache=ckv[1:]),
+             dict(kpe_cache=kpe[:, :, :32]), dict(prefix_lens=prefix.long()), dict(prefix_lens=prefix[:1]),
+             dict(block_table=table.float()), dict(block_table=table[0]), dict(block_table=table[:1]), dict(cu_drafts=cu[:-1]),
+             dict(cu_drafts=cu.float()), dict(tree_mask=mask.int()), dict(tree_mask=mask[:, 0]), dict(tree_mask=mask[1:]),
+             dict(tree_mask=mask[:, :0]), dict(block_table=table.cpu())]
+    for change in wrong:
+        with pytest.raises(ValueError):
+            tree.run(**{**good, **change}, output=out, lse=lse)
+        with pytest.raises(ValueError):
+            evict.accumulate(**{**good, **change}, lse=lse, acc=acc, out=acc)
+    for o, l in ((out.float(), lse), (out[1:], lse), (out.transpose(0, 1), lse), (out, lse.double()), (out, lse[:, :8]),
+                 (out.cpu(), lse), (out, lse.t().contiguous().t())):
+        with pytest.raises(ValueError):
+            tree.run(**good, output=o, lse=l)
+    for l, a, o in ((lse.double(), acc, acc), (lse[1:], acc, acc), (lse, acc.double(), acc), (lse, acc[:, :-1], acc),
+                    (lse, acc, acc[:1]), (lse, acc.t().contiguous().t(), acc), (lse, acc, acc.cpu()),
+                    (lse, acc[:1].expand(2, -1), acc)):
+        with pytest.raises(ValueError):
+            evict.accumulate(**good, lse=l, acc=a, out=o)
