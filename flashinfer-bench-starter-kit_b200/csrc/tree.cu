@@ -74,14 +74,19 @@ __device__ __forceinline__ uint32_t with_rows(uint32_t idesc, int rows) {
   return idesc | static_cast<uint32_t>((rows + 15) / 16 * 2) << 17;
 }
 
-// A tile moves in two halves with barriers of their own: ckv pieces 0-3, which
-// O^T's blocks 0 and 1 need, and pieces 4-7 with kpe.
-constexpr int kHalfBytes = 4 * kChunkBytes;  // and kChunkBytes more in the second
+// A tile moves in four parts with barriers of their own: part x is the ckv
+// pieces 2x and 2x + 1, which O^T's block x needs, and the last has kpe too.
+// S^T starts with the first part that lands, and each block of O^T frees its
+// part for the tile after next.
+constexpr int kParts = 4;
+__device__ __forceinline__ constexpr uint32_t part_bytes(int x) {
+  return (x == kParts - 1 ? 3 : 2) * kChunkBytes;
+}
 
 constexpr int kOffQ = 2 * kTileBytes;          // 147456
 constexpr int kOffP = kOffQ + kTileBytes;      // 221184: P, or the weights' sums
 constexpr int kOffBar = kOffP + kTok * 128;    // 229376
-constexpr int kOffMisc = kOffBar + 192;
+constexpr int kOffMisc = kOffBar + 256;
 constexpr int kOffRed = kOffMisc + 96;         // [4][64] floats
 constexpr int kOffFactor = kOffRed + 1024;     // [64]
 constexpr int kOffMax = kOffFactor + 256;      // [64]
@@ -358,16 +363,19 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   uint8_t* p_mem = smem + kOffP;
   float* sums = reinterpret_cast<float*>(p_mem);  // weights: [2 sets][kSumTiles][64]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint64_t* kv_full = bars;        // [2 stages][2 halves]
-  uint64_t* q_full = bars + 4;     // [2 halves]
-  uint64_t* q_empty = bars + 6;
-  uint64_t* s_full = bars + 7;     // [2]
-  uint64_t* s_empty = bars + 9;    // [2]
-  uint64_t* p_full = bars + 11;
-  uint64_t* half_done = bars + 12; // [2]: O^T blocks 0 and 1 done, the stage's first half is free
-  uint64_t* pv_done = bars + 14;   // [2]: all blocks done, the stage is free
-  uint64_t* o_empty = bars + 16;
-  uint64_t* drain = bars + 17;     // [2]
+  uint64_t* kv_full = bars;                  // [2 stages][kParts]
+  uint64_t* kv_free = bars + 2 * kParts;     // [2][kParts]: the part's block of O^T is done
+  uint64_t* q_full = bars + 4 * kParts;      // [kParts]
+  uint64_t* q_empty = bars + 5 * kParts;
+  uint64_t* s_full = q_empty + 1;            // [2]
+  uint64_t* s_empty = q_empty + 3;           // [2]
+  uint64_t* p_full = q_empty + 5;
+  uint64_t* o_empty = q_empty + 6;
+  uint64_t* drain = q_empty + 7;             // [2]
+  constexpr int kBars = 5 * kParts + 9;
+  static_assert(kBars * 8 <= kOffMisc - kOffBar, "barriers");
+  // O^T's last block frees the stage's last part: all of PV(i) is done.
+  auto pv_done = [&](int i) { return &kv_free[(i & 1) * kParts + kParts - 1]; };
   int* misc = reinterpret_cast<int*>(smem + kOffMisc);
   uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
   int* abort_flag = misc + 1;
@@ -384,7 +392,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
   const int lane = tid & 31;
 
   if (tid == 0) {
-    for (int x = 0; x < 19; ++x) mbar_init(&bars[x], 1);
+    for (int x = 0; x < kBars; ++x) mbar_init(&bars[x], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&s_empty[s], kSoftWarps);
     mbar_init(p_full, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
@@ -483,7 +491,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
     // about 60, and the tensor pipe idles meanwhile.
     if (elect_one()) {
       int i = 0, segs = 0;
-      int halves = 0, q_halves = 0;  // issued
+      int parts = 0;  // issued
       bool ok = true;
       while (ok && walk.next(s)) {
         const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
@@ -497,18 +505,16 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           const uint32_t parity = ((i >> 1) & 1) ^ 1;
           uint8_t* dst = smem + st * kTileBytes;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int x = 0; x < kParts; ++x) {
             // The weights' S^T alone reads a stage.
-            uint64_t* free_bar = kWeights ? &s_full[st] : (h == 0 ? &half_done[st] : &pv_done[st]);
-            ok = ok && mbar_wait(free_bar, parity, wctx);
+            ok = ok && mbar_wait(kWeights ? &s_full[st] : &kv_free[st * kParts + x], parity, wctx);
             if (!ok) break;
-            uint64_t* bar = &kv_full[2 * st + h];
-            mbar_arrive_expect_tx(bar, kHalfBytes + h * kChunkBytes);
-#pragma unroll
-            for (int c = 4 * h; c < 4 * h + 4; ++c)
-              tma_load_3d(dst + c * kChunkBytes, &ckv_map, bar, c * 64, 0, page);
-            if (h == 1) tma_load_3d(dst + 8 * kChunkBytes, &kpe_map, bar, 0, 0, page);
-            ++halves;
+            uint64_t* bar = &kv_full[st * kParts + x];
+            mbar_arrive_expect_tx(bar, part_bytes(x));
+            tma_load_3d(dst + 2 * x * kChunkBytes, &ckv_map, bar, 128 * x, 0, page);
+            tma_load_3d(dst + (2 * x + 1) * kChunkBytes, &ckv_map, bar, 128 * x + 64, 0, page);
+            if (x == kParts - 1) tma_load_3d(dst + 8 * kChunkBytes, &kpe_map, bar, 0, 0, page);
+            ++parts;
           }
           if (t == s.t0 && ok) {
             // The group's queries, behind its first tile.  Rows behind the
@@ -518,13 +524,11 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             ok = mbar_wait(q_empty, (segs & 1) ^ 1, wctx);
             if (ok) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                mbar_arrive_expect_tx(&q_full[h], kHalfBytes + h * kChunkBytes);
-#pragma unroll
-                for (int c = 4 * h; c < 4 * h + 4; ++c)
-                  tma_load_2d(q_mem + c * kChunkBytes, &qn_map, &q_full[h], c * 64, row_q);
-                if (h == 1) tma_load_2d(q_mem + 8 * kChunkBytes, &qp_map, &q_full[h], 0, row_q);
-                ++q_halves;
+              for (int x = 0; x < kParts; ++x) {
+                mbar_arrive_expect_tx(&q_full[x], part_bytes(x));
+                tma_load_2d(q_mem + 2 * x * kChunkBytes, &qn_map, &q_full[x], 128 * x, row_q);
+                tma_load_2d(q_mem + (2 * x + 1) * kChunkBytes, &qn_map, &q_full[x], 128 * x + 64, row_q);
+                if (x == kParts - 1) tma_load_2d(q_mem + 8 * kChunkBytes, &qp_map, &q_full[x], 0, row_q);
               }
               ++segs;
             }
@@ -533,13 +537,12 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
         }
       }
       // Copies still in flight (after an abort) land before the CTA exits: of
-      // each half the last two, whose phases nothing refills.
-      for (int h = 0; h < 2; ++h) {
-        const int tiles = (halves + 1 - h) / 2;
+      // each part the last two, whose phases nothing refills.
+      for (int x = 0; x < kParts; ++x) {
+        const int tiles = (parts + kParts - 1 - x) / kParts;
         for (int k = tiles - 1; k >= 0 && k >= tiles - 2; --k)
-          mbar_drain(&kv_full[2 * (k & 1) + h], (k >> 1) & 1, p.status);
-        const int qs = (q_halves + 1 - h) / 2;
-        if (qs >= 1) mbar_drain(&q_full[h], (qs - 1) & 1, p.status);
+          mbar_drain(&kv_full[(k & 1) * kParts + x], (k >> 1) & 1, p.status);
+        if (segs >= 1) mbar_drain(&q_full[x], (segs - 1) & 1, p.status);
       }
     }
     __syncwarp();
@@ -558,13 +561,13 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           const uint32_t d = tmem_base + kColS + 64u * st;
           ok = mbar_wait(&s_empty[st], ((i >> 1) & 1) ^ 1, wctx);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (t == s.t0) ok = ok && mbar_wait(&q_full[h], segs & 1, wctx);
-            ok = ok && mbar_wait(&kv_full[2 * st + h], (i >> 1) & 1, wctx);
+          for (int x = 0; x < kParts; ++x) {
+            if (t == s.t0) ok = ok && mbar_wait(&q_full[x], segs & 1, wctx);
+            ok = ok && mbar_wait(&kv_full[st * kParts + x], (i >> 1) & 1, wctx);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int k = 16 * h; k < 16 + 20 * h; ++k) {
+            for (int k = 8 * x; k < 8 * x + (x == kParts - 1 ? 12 : 8); ++k) {
               // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
               const uint32_t at = (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2;
               umma_bf16(d, a + at, q_desc + at, idesc, k > 0 ? 1u : 0u);
@@ -604,9 +607,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             for (int kk = 0; kk < 4; ++kk)  // 128 dims are two pieces; a K16 step is 16 token rows of 128 bytes
               umma_bf16(tmem_base + kColO + 64u * mb, a + mb * (2 * kChunkBytes >> 4) + kk * (2048 >> 4),
                         p_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : more);
-            if (mb == 1) umma_commit(&half_done[st]);
+            umma_commit(&kv_free[st * kParts + mb]);
           }
-          umma_commit(&pv_done[st]);
         }
         ++segs;
       }
@@ -836,7 +838,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             named_barrier_sync(1 + set, 128);
             if (t > s.t0) {
               // O holds PV(i - 1) before it is rescaled.
-              ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
+              ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
               tc_fence_after();
 #pragma unroll 1
               for (int mb = 0; mb < 4; ++mb) {
@@ -861,7 +863,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             // so such values are zeroed in the V tile; a row that does see
             // one has its NaN from the logit.
 #pragma unroll
-            for (int h = 0; h < 2; ++h) ok = ok && mbar_wait(&kv_full[2 * st + h], (i >> 1) & 1, wctx);
+            for (int x = 0; x < kParts; ++x) ok = ok && mbar_wait(&kv_full[st * kParts + x], (i >> 1) & 1, wctx);
             const int from = s.r.prefix > t * kTok ? s.r.prefix - t * kTok : 0;
             for (int q = tid; q < (kTok - from) * 64; q += 32 * kSoftWarps) {
               // 16-byte piece q & 7 of row from + (q >> 6) in piece (q >> 3) & 7
@@ -903,7 +905,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             lr[k + 1] += __uint_as_float(p0[k >> 1] & 0xFFFF0000u) + __uint_as_float(p1[k >> 1] & 0xFFFF0000u);
           }
           // P was last read by PV(i - 1).
-          if (i > 0) ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
+          if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
           {
             // One 128-byte row per token, 16-byte pieces swizzled by token & 7
             // (the same for r0 and r0 + 8): a warp's stores meet no bank twice.
@@ -956,7 +958,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             *reinterpret_cast<float4*>(p.part_ml + (rec * kRows + c) * 4) = make_float4(max_s[c], sum, sum_r, 0.f);
           }
         }
-        ok = ok && mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, wctx);
+        ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
         named_barrier_sync(1 + set, 128);
         tc_fence_after();
 #pragma unroll 1
