@@ -49,27 +49,27 @@ def _fail_acc(msg: str) -> None:
     raise ValueError(f"dsa_evict.accumulate: {msg}")
 
 
-def _rows_of(name: str, t: torch.Tensor, shape: tuple, fail) -> None:
-    if t.dtype is not torch.float32 or t.shape != shape:
-        fail(f"{name} must be float32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.stride(1) != 1 or (shape[0] > 1 and t.stride(0) < shape[1]):
+def _rows_of(name: str, t: torch.Tensor, rows: int, width: int, fail) -> int:
+    """The pitch of a float32 [rows, width] tensor, in elements."""
+    if t.dtype is not torch.float32 or t.shape != (rows, width):
+        fail(f"{name} must be float32 [{rows}, {width}], got {t.dtype} {tuple(t.shape)}")
+    pitch, col = t.stride()
+    if col != 1 or (rows > 1 and pitch < width):
         fail(f"{name} must have contiguous rows that do not overlap (strides {t.stride()})")
+    return pitch if rows > 1 else width
 
 
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two [B, width] float32 tensors with contiguous rows share memory."""
-    lo, hi = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
-    apart = (hi.data_ptr() - lo.data_ptr()) // 4
-    pitch, width = _pitch(lo), lo.shape[1]
-    if apart >= (lo.shape[0] - 1) * pitch + width:
+def _overlap(rows: int, a: int, a_pitch: int, a_width: int, b: int, b_pitch: int, b_width: int) -> bool:
+    """Whether two float32 tensors of `rows` contiguous rows at the addresses a
+    and b (pitches and widths in elements) share memory."""
+    if a > b:
+        a, a_pitch, a_width, b, b_pitch, b_width = b, b_pitch, b_width, a, a_pitch, a_width
+    apart = (b - a) // 4
+    if apart >= (rows - 1) * a_pitch + a_width:
         return False
     # Interleaved rows of one buffer, such as its left and right columns.
-    at = apart % pitch
-    return _pitch(hi) != pitch or at < width or at + hi.shape[1] > pitch
+    at = apart % a_pitch
+    return a_pitch != b_pitch or at < a_width or at + b_width > a_pitch
 
 
 def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor,
@@ -81,26 +81,29 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
         tree.check_device(_fail_acc, q_nope=q_nope, lse=lse, acc=acc, out=out)
     if lse.dtype is not torch.float32 or lse.shape != (T, H):
         _fail_acc(f"lse must be float32 [{T}, {H}]")
-    _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_acc)
-    _rows_of("out", out, (B, max_pages * PAGE_SIZE), _fail_acc)
-    same = acc.data_ptr() == out.data_ptr() and _pitch(acc) == _pitch(out)
-    if not same and B > 0 and _overlap(acc, out):
+    width = max_pages * PAGE_SIZE
+    acc_pitch, out_pitch = _rows_of("acc", acc, B, width, _fail_acc), _rows_of("out", out, B, width, _fail_acc)
+    acc_ptr, out_ptr = acc.data_ptr(), out.data_ptr()
+    same = acc_ptr == out_ptr and acc_pitch == out_pitch
+    if not same and B > 0 and _overlap(B, acc_ptr, acc_pitch, width, out_ptr, out_pitch, width):
         _fail_acc("out must be acc itself or not overlap it")
     if isinstance(sm_scale, torch.Tensor):
-        sm_scale = float(sm_scale.item())
+        sm_scale = sm_scale.item()
     if B == 0:
         return
     if T == 0:
         if not same:
             out.copy_(acc)
         return
-    lse = lse.contiguous()
+    if not lse.is_contiguous():
+        lse = lse.contiguous()
     dev = q_nope.device
     cur = _native.current_stream(dev)
     ws = workspace.get(dev, "evict", _native.WORKSPACE_HEADER, cur)
-    st = _native.call_on(dev, _native.lib().dsa_tree_weights_run, *args, float(sm_scale), lse.data_ptr(),
-                         acc.data_ptr(), _pitch(acc), out.data_ptr(), _pitch(out), ws.data_ptr(), ws.numel(), cur)
-    _native.check(st, "dsa_tree_weights_run")
+    st = _native.call_on(dev, _native.lib().dsa_tree_weights_run, *args, sm_scale, lse.data_ptr(), acc_ptr, acc_pitch,
+                         out_ptr, out_pitch, ws.data_ptr(), ws.numel(), cur)
+    if st:
+        _native.check(st, "dsa_tree_weights_run")
     if tree._CHECK and not torch.cuda.is_current_stream_capturing():
         raise_on_device_status(dev)
 
@@ -127,12 +130,8 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
     if len(new_block_table.shape) != 2 or new_block_table.shape[0] != B or new_block_table.shape[1] < 1:
         _fail_run(f"new_block_table must be [{B}, new_max_pages]")
     new_pages = new_block_table.shape[1]
-    if ckv_cache.dtype is not torch.bfloat16 or kpe_cache.dtype is not torch.bfloat16:
-        _fail_run(f"ckv_cache and kpe_cache must be bfloat16, got {ckv_cache.dtype} and {kpe_cache.dtype}")
-    pages, ckv_page, ckv_row = tree._strides("ckv_cache", ckv_cache, tree.DIM_CKV, _fail_run)
-    kpe_pages, kpe_page, kpe_row = tree._strides("kpe_cache", kpe_cache, tree.DIM_KPE, _fail_run)
-    if kpe_pages != pages:
-        _fail_run("ckv_cache and kpe_cache must hold the same number of pages")
+    caches = tree.cache_layout(_fail_run, ckv_cache, kpe_cache)
+    pages = caches[-1]
     if k_index_cache_fp8 is not None:
         if k_index_cache_fp8.element_size() != 1 or not k_index_cache_fp8.is_contiguous():
             _fail_run("k_index_cache_fp8 must be a contiguous 1-byte tensor (written in place)")
@@ -151,30 +150,32 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
         _fail_run(f"a budget of {budget} tokens (keep.shape[1]) does not fit new_block_table's {new_pages} pages")
     if num_sink < 0 or num_recent < 0 or num_sink + num_recent > budget:
         _fail_run(f"num_sink {num_sink} and num_recent {num_recent} must fit the budget of {budget}")
-    _rows_of("acc", acc, (B, max_pages * PAGE_SIZE), _fail_run)
-    _rows_of("new_acc", new_acc, (B, new_pages * PAGE_SIZE), _fail_run)
-    if B > 0 and _overlap(acc, new_acc):
+    width, new_width = max_pages * PAGE_SIZE, new_pages * PAGE_SIZE
+    acc_pitch = _rows_of("acc", acc, B, width, _fail_run)
+    new_pitch = _rows_of("new_acc", new_acc, B, new_width, _fail_run)
+    acc_ptr, new_ptr = acc.data_ptr(), new_acc.data_ptr()
+    if B > 0 and _overlap(B, acc_ptr, acc_pitch, width, new_ptr, new_pitch, new_width):
         _fail_run("new_acc must not overlap acc")
     if B == 0:
         return
     if B > 65536 or max_pages > 1 << 24 or new_pages > 1 << 24:
         _fail_run(f"{B} requests of {max_pages} pages are more than one call takes")
-    sl = seq_lens.contiguous()
-    bt = tree._int32("block_table", block_table, _fail_run)
-    nbt = tree._int32("new_block_table", new_block_table, _fail_run)
+    sl = seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
+    bt = tree.int32_of("block_table", block_table, _fail_run)
+    nbt = tree.int32_of("new_block_table", new_block_table, _fail_run)
     dev = acc.device
     check = tree._CHECK and not torch.cuda.is_current_stream_capturing()
     if check:
         _check_new_pages(sl, bt, nbt, budget, pages)
     cur = _native.current_stream(dev)
     ws = workspace.get(dev, "evict", _native.WORKSPACE_HEADER, cur)
-    st = _native.call_on(dev, _native.lib().dsa_cache_evict_run, acc.data_ptr(), _pitch(acc), sl.data_ptr(),
-                         bt.data_ptr(), nbt.data_ptr(), B, max_pages, new_pages, ckv_cache.data_ptr(), ckv_page, ckv_row,
-                         kpe_cache.data_ptr(), kpe_page, kpe_row,
+    st = _native.call_on(dev, _native.lib().dsa_cache_evict_run, acc_ptr, acc_pitch, sl.data_ptr(), bt.data_ptr(),
+                         nbt.data_ptr(), B, max_pages, new_pages, *caches[:6],
                          None if k_index_cache_fp8 is None else k_index_cache_fp8.data_ptr(), pages, budget, num_sink,
-                         num_recent, keep.data_ptr(), new_seq_lens.data_ptr(), new_acc.data_ptr(), _pitch(new_acc),
-                         ws.data_ptr(), ws.numel(), cur)
-    _native.check(st, "dsa_cache_evict_run")
+                         num_recent, keep.data_ptr(), new_seq_lens.data_ptr(), new_ptr, new_pitch, ws.data_ptr(),
+                         ws.numel(), cur)
+    if st:
+        _native.check(st, "dsa_cache_evict_run")
     if check:
         raise_on_device_status(dev)
 

@@ -64,20 +64,25 @@ def masks_from_parents(parents) -> list:
     return [[w - (1 << 64) if w >> 63 else w for w in row] for row in rows]
 
 
-def _strides(name: str, t: torch.Tensor, width: int, fail) -> tuple:
-    """(pages, page stride, row stride) of a [pages, 64, width] bf16 cache, strides in bytes."""
-    shape = t.shape
-    if len(shape) != 3 or shape[1] != PAGE_SIZE or shape[2] != width:
-        fail(f"{name} must be [pages, {PAGE_SIZE}, {width}], got {tuple(shape)}")
-    pages = shape[0]
-    if pages < 1:
-        fail(f"{name} has no pages")
-    page, row, col = t.stride()
-    if pages == 1:  # a stride that is never taken
-        page = PAGE_SIZE * row
-    if col != 1 or row < width or page < row or row % 8 or page % 8 or t.data_ptr() % 16:
-        fail(f"{name} must have contiguous rows, 16-byte aligned (strides {t.stride()})")
-    return pages, 2 * page, 2 * row
+def cache_layout(fail, ckv_cache: torch.Tensor, kpe_cache: torch.Tensor) -> tuple:
+    """(ckv pointer, page and row stride in bytes, the same of kpe, pages) of the two caches."""
+    shape = ckv_cache.shape
+    pages = shape[0] if shape else 0
+    if pages < 1 or shape != (pages, PAGE_SIZE, DIM_CKV) or kpe_cache.shape != (pages, PAGE_SIZE, DIM_KPE):
+        fail(f"ckv_cache must be [pages, {PAGE_SIZE}, {DIM_CKV}] and kpe_cache [pages, {PAGE_SIZE}, {DIM_KPE}] with at "
+             f"least one page, got {tuple(shape)} and {tuple(kpe_cache.shape)}")
+    if ckv_cache.dtype is not torch.bfloat16 or kpe_cache.dtype is not torch.bfloat16:
+        fail(f"ckv_cache and kpe_cache must be bfloat16, got {ckv_cache.dtype} and {kpe_cache.dtype}")
+    cp, cr, cc = ckv_cache.stride()
+    kp, kr, kc = kpe_cache.stride()
+    if pages == 1:  # strides that are never taken
+        cp, kp = PAGE_SIZE * cr, PAGE_SIZE * kr
+    ckv, kpe = ckv_cache.data_ptr(), kpe_cache.data_ptr()
+    if cc != 1 or kc != 1 or cr < DIM_CKV or kr < DIM_KPE or cp < cr or kp < kr or (cp | cr | kp | kr) & 7 or \
+            (ckv | kpe) & 15:
+        fail(f"ckv_cache and kpe_cache must have contiguous rows, 16-byte aligned (strides {ckv_cache.stride()} and "
+             f"{kpe_cache.stride()})")
+    return ckv, 2 * cp, 2 * cr, kpe, 2 * kp, 2 * kr, pages
 
 
 def check_device(fail, **tensors) -> None:
@@ -101,21 +106,15 @@ def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_tabl
             tree_mask.get_device() != at:
         check_device(fail, q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache, prefix_lens=prefix_lens,
                      block_table=block_table, cu_drafts=cu_drafts, tree_mask=tree_mask)
-    bf16 = torch.bfloat16
-    if q_nope.dtype is not bf16 or q_pe.dtype is not bf16 or ckv_cache.dtype is not bf16 or kpe_cache.dtype is not bf16:
-        for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
-            if t.dtype is not bf16:
-                fail(f"{name} must be bfloat16, got {t.dtype}")
     shape = q_nope.shape
     if len(shape) != 3 or shape[2] != DIM_CKV or not 1 <= shape[1] <= MAX_HEADS:
         fail(f"q_nope must be [T, heads <= {MAX_HEADS}, {DIM_CKV}], got {tuple(shape)}")
     T, H, _ = shape
     if q_pe.shape != (T, H, DIM_KPE):
         fail(f"q_pe must be [{T}, {H}, {DIM_KPE}]")
-    pages, ckv_page, ckv_row = _strides("ckv_cache", ckv_cache, DIM_CKV, fail)
-    kpe_pages, kpe_page, kpe_row = _strides("kpe_cache", kpe_cache, DIM_KPE, fail)
-    if kpe_pages != pages:
-        fail("ckv_cache and kpe_cache must hold the same number of pages")
+    if q_nope.dtype is not torch.bfloat16 or q_pe.dtype is not torch.bfloat16:
+        fail(f"q_nope and q_pe must be bfloat16, got {q_nope.dtype} and {q_pe.dtype}")
+    caches = cache_layout(fail, ckv_cache, kpe_cache)
     shape = block_table.shape
     if len(shape) != 2 or shape[1] < 1:
         fail("block_table must be [B, max_pages]")
@@ -129,19 +128,22 @@ def check_rows(fail, q_nope, q_pe, ckv_cache, kpe_cache, prefix_lens, block_tabl
         fail(f"tree_mask must be int64 [{T}, words <= {MAX_MASK_WORDS}]")
     if T * H > 1 << 24 or B > 65536 or (T * H // 64 + B) * (max_pages + 3) > 1 << 30:
         fail(f"{T} drafts of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
-    qn, qp, pl, tm = q_nope.contiguous(), q_pe.contiguous(), prefix_lens.contiguous(), tree_mask.contiguous()
-    bt, cu = _int32("block_table", block_table, fail), _int32("cu_drafts", cu_drafts, fail)
-    args = (qn.data_ptr(), qp.data_ptr(), ckv_cache.data_ptr(), ckv_page, ckv_row, kpe_cache.data_ptr(), kpe_page, kpe_row,
-            pages, pl.data_ptr(), bt.data_ptr(), cu.data_ptr(), tm.data_ptr(), B, T, H, max_pages, shape[1])
+    qn = q_nope if q_nope.is_contiguous() else q_nope.contiguous()
+    qp = q_pe if q_pe.is_contiguous() else q_pe.contiguous()
+    pl = prefix_lens if prefix_lens.is_contiguous() else prefix_lens.contiguous()
+    tm = tree_mask if tree_mask.is_contiguous() else tree_mask.contiguous()
+    bt, cu = int32_of("block_table", block_table, fail), int32_of("cu_drafts", cu_drafts, fail)
+    args = (qn.data_ptr(), qp.data_ptr(), *caches, pl.data_ptr(), bt.data_ptr(), cu.data_ptr(), tm.data_ptr(), B, T, H,
+            max_pages, shape[1])
     return at, T, H, B, max_pages, args, (qn, qp, pl, bt, cu, tm)
 
 
-def _int32(name: str, t: torch.Tensor, fail) -> torch.Tensor:
+def int32_of(name: str, t: torch.Tensor, fail) -> torch.Tensor:
     if t.dtype is not torch.int32:
         if t.dtype is not torch.int64:
             fail(f"{name} must be int32 or int64")
         t = t.to(torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _fail(msg: str) -> None:
@@ -162,7 +164,7 @@ def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_c
                                             cu_drafts, tree_mask)
     if output.get_device() != at or lse.get_device() != at:
         check_device(_fail, q_nope=q_nope, output=output, lse=lse)
-    if output.dtype is not torch.bfloat16 or output.shape != q_nope.shape or not output.is_contiguous():
+    if output.dtype is not torch.bfloat16 or output.shape != (T, H, DIM_CKV) or not output.is_contiguous():
         _fail(f"output must be contiguous bfloat16 [{T}, {H}, {DIM_CKV}]")
     if lse.dtype is not torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
         _fail(f"lse must be contiguous float32 [{T}, {H}]")
@@ -173,9 +175,10 @@ def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_c
     dev = q_nope.device
     cur = _native.current_stream(dev)
     ws = workspace.get(dev, "tree", _workspace_bytes(dev), cur)
-    st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, float(sm_scale), output.data_ptr(),
-                         lse.data_ptr(), ws.data_ptr(), ws.numel(), cur)
-    _native.check(st, "dsa_tree_attention_run")
+    st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, sm_scale, output.data_ptr(), lse.data_ptr(),
+                         ws.data_ptr(), ws.numel(), cur)
+    if st:
+        _native.check(st, "dsa_tree_attention_run")
     if _CHECK and not torch.cuda.is_current_stream_capturing():
         raise_on_device_status(dev)
 

@@ -23,6 +23,9 @@ _lock = threading.Lock()
 
 def get(device: torch.device, name: str, nbytes: int, stream: int = 0) -> torch.Tensor:
     key = (device.index if device.index is not None else torch.cuda.current_device(), name, stream)
+    buf = _buffers.get(key)  # atomic; a buffer is entered once it is complete
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
     with _lock:
         buf = _buffers.get(key)
         if buf is None or buf.numel() < nbytes:

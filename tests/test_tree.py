@@ -55,19 +55,25 @@ def test_entry_points_refuse_cpu_tensors():
         evict.accumulate(**a, lse=torch.zeros(1), acc=torch.zeros(1), out=torch.zeros(1))
 
 
-def test_cache_strides():
+def test_cache_layout():
     def fail(msg):
         raise ValueError(msg)
 
     both = torch.zeros(3, 64, 576, dtype=torch.bfloat16)
-    assert tree._strides("ckv", both[:, :, :512], 512, fail) == (3, 2 * 64 * 576, 2 * 576)
-    assert tree._strides("kpe", both[:, :, 512:], 64, fail) == (3, 2 * 64 * 576, 2 * 576)
-    assert tree._strides("ckv", both[:1, :, :512], 512, fail) == (1, 2 * 64 * 576, 2 * 576)
-    for bad in (both[:, :, 4:516], both[:, :, :511], torch.zeros(3, 64, 580, dtype=torch.bfloat16)[:, :, :512],
-                both[:, :, :512].transpose(0, 1), both[:0, :, :512], both[:1, :, :512].expand(3, 64, 512),
-                both.flatten(0, 1)[:, :512]):
+    ckv, kpe = both[:, :, :512], both[:, :, 512:]
+    at = both.data_ptr()
+    assert tree.cache_layout(fail, ckv, kpe) == (at, 2 * 64 * 576, 2 * 576, at + 1024, 2 * 64 * 576, 2 * 576, 3)
+    one = tree.cache_layout(fail, ckv[:1], kpe[:1].contiguous())
+    assert one[1:3] == (2 * 64 * 576, 2 * 576) and one[4:] == (2 * 64 * 64, 128, 1)
+    wide = torch.zeros(3, 64, 580, dtype=torch.bfloat16)
+    for bad in ((both[:, :, 4:516], kpe), (both[:, :, :511], kpe), (wide[:, :, :512], kpe), (ckv.transpose(0, 1), kpe),
+                (ckv[:0], kpe[:0]), (ckv[:1].expand(3, 64, 512), kpe), (ckv.flatten(0, 1), kpe), (ckv, kpe[1:]),
+                (ckv, kpe.half()), (ckv.float(), kpe), (ckv, both[:, :, 8:72]), (torch.zeros(()), kpe)):
+        if bad[1].data_ptr() == at + 16:  # aligned, and allowed to lie within the other
+            tree.cache_layout(fail, *bad)
+            continue
         with pytest.raises(ValueError):
-            tree._strides("ckv", bad, 512, fail)
+            tree.cache_layout(fail, *bad)
 
 
 def evict_call(lib, requests=1, max_pages=4, new_pages=2, pages=9, budget=100, sink=4, recent=8, acc=16, acc_stride=256,
@@ -98,16 +104,16 @@ def test_weights_c_abi_refuses_bad_arguments(change, status):
 
 
 def test_overlapping_accumulators():
-    buf = torch.zeros(1000)
-    rows = lambda at, n, width, pitch: buf[at:].as_strided((n, width), (pitch, 1))  # noqa: E731
-    a = rows(0, 4, 64, 150)
-    assert not evict._overlap(a, rows(64, 4, 64, 150)) and not evict._overlap(rows(64, 4, 64, 150), a)
-    assert not evict._overlap(a, rows(514, 2, 64, 64))       # behind the last row
-    assert evict._overlap(a, rows(1, 4, 64, 150))
-    assert evict._overlap(a, rows(100, 4, 64, 150))          # wraps into the next row
-    assert evict._overlap(a, rows(64, 4, 64, 151))
-    assert evict._overlap(a, rows(513, 2, 64, 64))
-    assert not evict._overlap(rows(0, 1, 64, 7), rows(64, 1, 64, 7))
+    o = lambda at, n, width, pitch, at2, width2, pitch2: evict._overlap(  # noqa: E731
+        n, 4096 + 4 * at, pitch, width, 4096 + 4 * at2, pitch2, width2)
+    assert not o(0, 4, 64, 150, 64, 64, 150) and not o(64, 4, 64, 150, 0, 64, 150)
+    assert not o(0, 4, 64, 150, 514, 64, 64)       # behind the last row
+    assert o(0, 4, 64, 150, 513, 64, 64)
+    assert o(0, 4, 64, 150, 1, 64, 150)
+    assert o(0, 4, 64, 150, 100, 64, 150)          # wraps into the next row
+    assert o(0, 4, 64, 150, 64, 64, 151)
+    assert o(0, 4, 64, 150, 64, 87, 150) and not o(0, 4, 64, 150, 64, 86, 150)
+    assert not o(0, 1, 64, 64, 64, 64, 64) and o(0, 1, 64, 64, 63, 64, 64) and o(5, 2, 64, 64, 5, 64, 64)
 
 
 def test_evict_oracle():
