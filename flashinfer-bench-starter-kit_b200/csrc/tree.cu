@@ -846,8 +846,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
                 for (int h = 0; h < 2; ++h) {
                   const uint32_t at = tmem_base + lane_base + kColO + 64u * mb + 32u * set + 16u * h;
                   float o[16];
-                  tmem_ld16(at, o);
-                  tmem_wait_ld();
+                  tmem_ld16_wait(at, o);
 #pragma unroll
                   for (int c = 0; c < 16; ++c) o[c] *= factor_s[32 * set + 16 * h + c];
                   tmem_st16(at, o);
