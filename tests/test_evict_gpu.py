@@ -121,7 +121,9 @@ def test_neighbouring_floats_are_told_apart(cuda_device):
 
 
 def test_contexts_longer_than_the_cluster_can_hold(cuda_device):
-    c = Case([450_000, 300_000], 2000, cuda_device, seed=5, shared=True)
+    c = Case([450_000, 300_000], 2000, cuda_device, seed=5, shared=True)  # 16 CTAs a request: it fits
+    c.check(c.run(10, 500), 10, 500)
+    c = Case([450_000, *[70] * 78, 300_000], 2000, cuda_device, seed=5, shared=True)  # 2 CTAs: it does not
     c.check(c.run(10, 500), 10, 500)
 
 
