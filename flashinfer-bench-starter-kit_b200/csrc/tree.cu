@@ -860,7 +860,8 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             // anything; a zero weight would still turn an infinity or NaN
             // among them into NaN.  The logits have been read (S^T is done),
             // so such values are zeroed in the V tile; a row that does see
-            // one has its NaN from the logit.
+            // one has its NaN from the logit (or, where the logit is -inf,
+            // the weight 0 and nothing of the value).
 #pragma unroll
             for (int x = 0; x < kParts; ++x) ok = ok && mbar_wait(&kv_full[st * kParts + x], (i >> 1) & 1, wctx);
             const int from = s.r.prefix > t * kTok ? s.r.prefix - t * kTok : 0;

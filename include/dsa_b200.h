@@ -275,8 +275,9 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(void);
  * and (num_drafts * num_heads / 64 + num_requests) * (max_pages + 3) <= 2^30.
  * Masked cache rows may hold anything.  Data-dependent
  * errors: lengths that do not fit the table (clamped), drafts that do not fit
- * cu_drafts or the mask (left out): DSA_DEV_BAD_SEQ_LEN; page ids outside the
- * pool (their tokens are masked): DSA_DEV_BAD_PAGE. */
+ * cu_drafts or the mask (left out), a cu_drafts that decreases (the call then
+ * writes no row): DSA_DEV_BAD_SEQ_LEN; page ids outside the pool (their tokens
+ * are masked): DSA_DEV_BAD_PAGE. */
 DSA_API int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const void* ckv_cache,
                                    int64_t ckv_page_bytes, int64_t ckv_row_bytes,
                                    const void* kpe_cache, int64_t kpe_page_bytes,

@@ -139,6 +139,13 @@ def test_wide_tables_strided_weights_and_no_index_cache(cuda_device):
     assert (target[:, -1] == 5).all()
 
 
+def test_tables_and_lengths_in_other_layouts(cuda_device):
+    c = Case([900, 70, 300], 256, cuda_device, seed=41)
+    apart = lambda t: torch.stack((t, t), -1)[..., 0]  # noqa: E731  every second element
+    c.seq, c.table, c.new_table = apart(c.seq), apart(c.table.long()), apart(c.new_table.long())
+    c.check(c.run(4, 16), 4, 16)
+
+
 def test_strided_caches(cuda_device):
     c = Case([900, 400], 300, cuda_device, seed=7)
     both = torch.zeros(c.ckv.shape[0], 64, 576, dtype=torch.bfloat16)

@@ -282,6 +282,31 @@ def test_weights_in_place_repeat_and_skip_what_saw_nothing(cuda_device):
     assert torch.equal(view, out) and (strided[:, acc.shape[1]:] == 3).all()
 
 
+def test_inputs_in_other_layouts_give_the_same_bits(cuda_device):
+    c = Case([70, 900], [5, 3], 16, seed=31, device=cuda_device)
+    args = c.args()
+    out, lse = run(c, args)
+    _, acc, weights = weigh(c, args, lse=lse)
+    apart = lambda t: torch.stack((t, t), -1)[..., 0]  # noqa: E731  every second element
+    assert not any(apart(args[i]).is_contiguous() for i in (0, 1, 4, 7))
+    other = [apart(args[0]), apart(args[1]), args[2], args[3], apart(args[4]), apart(args[5].long()),
+             apart(args[6].long()), apart(args[7])]
+    o, l = run(c, other)
+    assert torch.equal(o, out) and torch.equal(l, lse)
+    assert torch.equal(weigh(c, other, acc=acc, lse=apart(lse))[2], weights)
+
+
+def test_a_page_that_a_request_has_twice_and_another_shares(cuda_device):
+    c = Case([200, 130], [3, 2], 16, seed=32, device=cuda_device)
+    c.table[0, 1] = c.table[0, 0]
+    c.table[1, 0] = c.table[0, 2]
+    c.check(*run(c))
+    lse, acc, out = weigh(c)
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    assert ((out.cpu().double() - want).abs() <= off).all()
+
+
 def test_no_drafts_at_all(cuda_device):
     c = Case([5, 70], [1, 1], 16, seed=22, device=cuda_device)
     args = c.args()
