@@ -12,11 +12,16 @@
 //   keys that share the boundary's bits, each added up in the first CTA's
 //   shared memory with the sums of every 32 bins: a warp of each CTA finds the
 //   boundary bin from those 64 sums and 32 bins, 384 bytes of remote reads
-//   (all 2048 bins from one SM took 4400 clocks a pass).  The kept positions then come out in order: a
+//   (all 2048 bins from one SM took 4400 clocks a pass).  The kept positions
+//   then come out in order: a
 //   token's place is the number kept before it, from ballots, a scan over
 //   the CTA's warps and the counts of the lower CTAs.
 // move_kernel: copies the kept tokens' rows of every cache to their new
-//   pages, 1288 B per token in and out; HBM-bound.
+//   pages, up to 1284 B per token in and out; HBM-bound.
+//
+// Measured, 32 requests of 32768-65536 tokens to 8192: select 28 us (latency of
+// its barriers and remote reads; 7 us for one request of 5001 to 1024), move
+// 106 us (262144 tokens, 673 MB, 6.3 TB/s).
 #include <mutex>
 
 #include "dsa_b200.h"
