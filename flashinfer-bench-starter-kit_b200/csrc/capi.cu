@@ -112,6 +112,7 @@ const char* dsa_b200_status_string(int status) {
     case DSA_ERR_CUDA: return "CUDA runtime error";
     case DSA_ERR_UNSUPPORTED_DEVICE: return "device is not sm_100 (B200)";
     case DSA_ERR_TENSOR_MAP: return "tensor map encoding failed";
+    case DSA_ERR_OVERLAP: return "an output shares memory with an input or another output";
     default: return "unknown status";
   }
 }

@@ -17,7 +17,9 @@
 //   token's place is the number kept before it, from ballots, a scan over
 //   the CTA's warps and the counts of the lower CTAs.
 // move_kernel: copies the kept tokens' rows of every cache to their new
-//   pages, up to 1284 B per token in and out; HBM-bound.
+//   pages, up to 1284 B per token in and out; HBM-bound.  It writes the new
+//   lengths too: they may take the old ones' place, which all of a cluster's
+//   threads read for themselves.
 //
 // Measured, 32 requests of 32768-65536 tokens to 8192: select 28 us (latency of
 // its barriers and remote reads; 7 us for one request of 5001 to 1024), move
@@ -102,7 +104,6 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   float* new_acc = p.new_acc + b * p.new_acc_stride;
   const int kept = L < p.budget ? L : p.budget;
   const int t0 = rank * kThreads + tid, step = ctas * kThreads;
-  if (t0 == 0) p.new_seq_lens[b] = kept;
   // Behind what is kept.
   for (int i = kept + t0; i < p.budget; i += step) keep[i] = -1;
   for (int i = kept + t0; i < p.new_max_pages * kPage; i += step) new_acc[i] = 0.f;
@@ -298,6 +299,10 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * kMoveWarps;
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * kMoveWarps + (threadIdx.x >> 5); w < all; w += step) {
     const int b = static_cast<int>(w / per_row), i0 = static_cast<int>(w % per_row) * kMoveTokens;
+    if (i0 == 0 && lane == 0) {
+      bool bad;  // reported by the select
+      p.new_seq_lens[b] = min(length_of(p, b, bad), p.budget);
+    }
     // Lane l looks up token l & 3 of the four.
     const int i = i0 + (lane & (kMoveTokens - 1));
     const int pos = i < p.budget ? __ldcg(p.keep + static_cast<int64_t>(b) * p.budget + i) : -1;
@@ -360,6 +365,28 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
   }
 }
 
+// Whether the float32 [rows, width] tensors at a and b, of the given pitches,
+// share memory.  Rows of one pitch may interleave, such as the left and right
+// columns of one buffer; of two pitches, their extents have to lie apart.
+bool rows_overlap(int64_t rows, const float* a, int64_t a_pitch, int64_t a_width, const float* b, int64_t b_pitch,
+                  int64_t b_width) {
+  if (reinterpret_cast<uintptr_t>(a) > reinterpret_cast<uintptr_t>(b)) {
+    const float* c = a;
+    a = b;
+    b = c;
+    int64_t x = a_pitch;
+    a_pitch = b_pitch;
+    b_pitch = x;
+    x = a_width;
+    a_width = b_width;
+    b_width = x;
+  }
+  const int64_t apart = static_cast<int64_t>((reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) / 4);
+  if (apart >= (rows - 1) * a_pitch + a_width) return false;
+  const int64_t at = apart % a_pitch;
+  return a_pitch != b_pitch || at < a_width || at + b_width > a_pitch;
+}
+
 // CTAs per request: as many as the cluster limit, the SMs (two 512-thread CTAs
 // each) and the table's width can use, down to 256 tokens a CTA.  One request of
 // 65536 tokens: 14.9 us with 16, 20.0 with 8; 8 of 3000-4096: 11.3 us, 15.5 with
@@ -412,6 +439,27 @@ extern "C" int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const i
        reinterpret_cast<uintptr_t>(new_acc)) & 3u)
     return DSA_ERR_MISALIGNED;
   if (workspace_bytes < kWorkspaceHeader) return DSA_ERR_WORKSPACE_TOO_SMALL;
+  // The kernels read their inputs while they write keep and new_acc; a
+  // request's length alone is read by nobody once its new one is written.
+  const size_t n = static_cast<size_t>(num_requests);
+  const int64_t width = static_cast<int64_t>(max_pages) * evict::kPage;
+  const int64_t new_width = static_cast<int64_t>(new_max_pages) * evict::kPage;
+  const struct {
+    const void* at;
+    size_t bytes;
+  } out[3] = {{keep, n * budget * 4}, {new_seq_lens, n * 4}, {new_acc, ((n - 1) * new_acc_stride + new_width) * 4}},
+    in[3] = {{seq_lens, n * 4}, {block_table, n * max_pages * 4}, {new_block_table, n * new_max_pages * 4}};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 3; ++j) {
+      if (i < j && ranges_overlap(out[i].at, out[i].bytes, out[j].at, out[j].bytes)) return DSA_ERR_OVERLAP;
+      const bool in_place = i == 1 && j == 0 && new_seq_lens == seq_lens;
+      if (!in_place && ranges_overlap(out[i].at, out[i].bytes, in[j].at, in[j].bytes)) return DSA_ERR_OVERLAP;
+    }
+  }
+  const size_t acc_bytes = static_cast<size_t>((num_requests - 1) * acc_stride + width) * 4;
+  if (ranges_overlap(keep, out[0].bytes, acc, acc_bytes) || ranges_overlap(new_seq_lens, out[1].bytes, acc, acc_bytes) ||
+      evict::rows_overlap(num_requests, acc, acc_stride, width, new_acc, new_acc_stride, new_width))
+    return DSA_ERR_OVERLAP;
   DeviceInfo info;
   int st = current_device_info(&info);
   if (st != DSA_OK) return st;

@@ -39,6 +39,11 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
+
 // Launches the indexer's top-2048 select over `rows` score rows (one CTA
 // each, programmatically after the kernel that wrote the scores): row b
 // reads scores[b], hist[b], seq_lens[b] and block-table row row_req[b]

@@ -17,6 +17,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().with_name("libdsa_b200.so")
 WORKSPACE_HEADER = 256  # bytes at the start of every workspace; the status word is the first of them
 
 DSA_OK = 0
+DSA_ERR_OVERLAP = 7
 DEV_BAD_SEQ_LEN = 0x1
 DEV_BAD_PAGE = 0x2
 DEV_BAD_INDEX = 0x4

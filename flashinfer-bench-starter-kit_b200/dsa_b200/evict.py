@@ -25,8 +25,8 @@ of largest ``acc`` (equal: the earlier; NaN is largest), ``budget`` in all; the
 others keep everything.  What is kept stays in order: position ``keep[r, i]``
 (ascending, then -1) becomes position i of ``new_block_table``'s row, in the ckv
 and kpe caches and, unless it is None, in the indexer's FP8 key cache.
-``new_seq_lens`` and ``new_acc`` (float32 ``[B, new_max_pages * 64]``, 0 behind the
-kept tokens) go with the new table.
+``new_seq_lens`` (which may be ``seq_lens`` itself) and ``new_acc`` (float32
+``[B, new_max_pages * 64]``, 0 behind the kept tokens) go with the new table.
 
 The new pages are pages of the same pool that no row of ``block_table`` uses; the
 old ones are not changed, so requests may share them, and the caller frees
@@ -175,6 +175,9 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
                          num_recent, keep.data_ptr(), new_seq_lens.data_ptr(), new_ptr, new_pitch, ws.data_ptr(),
                          ws.numel(), cur)
     if st:
+        if st == _native.DSA_ERR_OVERLAP:
+            _fail_run("keep, new_seq_lens and new_acc must share memory neither with one another nor with the inputs "
+                      "(new_seq_lens may be seq_lens itself)")
         _native.check(st, "dsa_cache_evict_run")
     if check:
         raise_on_device_status(dev)

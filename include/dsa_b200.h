@@ -55,6 +55,7 @@ extern "C" {
 #define DSA_ERR_CUDA                 4
 #define DSA_ERR_UNSUPPORTED_DEVICE   5
 #define DSA_ERR_TENSOR_MAP           6
+#define DSA_ERR_OVERLAP              7
 
 /* ---- sticky device status bits (first uint32 of each workspace) ------ */
 #define DSA_DEV_BAD_SEQ_LEN   0x1u  /* seq_len < 0 or > max_pages*64; clamped   */
@@ -330,11 +331,13 @@ DSA_API int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const voi
  *   k_index_cache_fp8 num_pages pages of 8448 bytes, or NULL
  *   keep              [num_requests, budget] int32: the kept positions,
  *                     ascending, then -1
- *   new_seq_lens      [num_requests] int32
+ *   new_seq_lens      [num_requests] int32; may be seq_lens itself
  *   new_acc           [num_requests, new_max_pages * 64] fp32, rows
  *                     new_acc_stride apart: acc of the kept tokens, then 0
  *
- * Token keep[r, i] becomes token i of the new table's row.  Data-dependent
+ * Token keep[r, i] becomes token i of the new table's row.  keep, new_seq_lens
+ * and new_acc share memory neither with one another nor with acc, the tables
+ * or (but for new_seq_lens in place) seq_lens: DSA_ERR_OVERLAP.  Data-dependent
  * errors: a seq_len outside [0, max_pages * 64] (clamped):
  * DSA_DEV_BAD_SEQ_LEN; a page outside the pool (its tokens are not moved):
  * DSA_DEV_BAD_PAGE.  The workspace holds only the status word (256 bytes). */

@@ -376,3 +376,57 @@ def test_a_whole_step_in_one_graph(cuda_device):
             assert int(got[1][b]) == len(k) and got[0][b, :len(k)].tolist() == k
             assert torch.equal(got[2][b, :len(k)], a[b, k])
         assert torch.allclose(a.sum(1), torch.tensor([32.0, 48.0]), rtol=1e-3)
+
+
+def test_lengths_in_place(cuda_device):
+    """new_seq_lens may be seq_lens: eager, and captured and replayed until
+    every request is within the budget."""
+    d = cuda_device
+    for seq, budget in (([5001, 70, 30000, 1999, 0], 515), ([9000] * 40, 63), ([650, 700] * 200, 130)):
+        c = Case(seq, budget, d, seed=51)
+        rest = dict(acc=c.acc.to(d), block_table=c.table.to(d), new_block_table=c.new_table.to(d), num_sink=3, num_recent=11)
+        for _ in range(5):
+            caches = dict(ckv_cache=c.ckv.to(d), kpe_cache=c.kpe.to(d), k_index_cache_fp8=c.index.to(d))
+            lens = c.seq.to(d)
+            keep = torch.full((len(seq), budget), 7, dtype=torch.int32, device=d)
+            acc = torch.full((len(seq), c.new_table.shape[1] * 64), 7.0, device=d)
+            evict.run(**rest, **caches, seq_lens=lens, keep=keep, new_seq_lens=lens, new_acc=acc)
+            torch.cuda.synchronize()
+            c.check({"ckv": caches["ckv_cache"].cpu(), "kpe": caches["kpe_cache"].cpu(),
+                     "index": caches["k_index_cache_fp8"].cpu(), "keep": keep.cpu(), "seq": lens.cpu(), "acc": acc.cpu()}, 3, 11)
+    lens.copy_(c.seq)
+    side = torch.cuda.Stream(d)
+    side.wait_stream(torch.cuda.current_stream(d))
+    with torch.cuda.stream(side):
+        evict.run(**rest, **caches, seq_lens=lens, keep=keep, new_seq_lens=lens, new_acc=acc)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            evict.run(**rest, **caches, seq_lens=lens, keep=keep, new_seq_lens=lens, new_acc=acc)
+    for grown in (1, 40, 500):  # as a decode loop lengthens them
+        lens.add_(grown)
+        lens.clamp_(max=c.table.shape[1] * 64)
+        want = lens.cpu()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(lens.cpu(), want.clamp(max=budget))
+        kept = otree.evict_reference(c.acc, want, budget, 3, 11)
+        for b, k in enumerate(kept):
+            assert keep[b, :len(k)].tolist() == k
+
+
+def test_outputs_over_inputs_are_refused(cuda_device):
+    d = cuda_device
+    c = Case([900, 400], 300, d, seed=52)
+    lens = torch.tensor([900, 400, 0], dtype=torch.int32, device=d)
+    table = c.table.to(d)
+    good = dict(acc=c.acc.to(d), seq_lens=lens[:2], block_table=table, new_block_table=c.new_table.to(d), ckv_cache=c.ckv.to(d),
+                kpe_cache=c.kpe.to(d), k_index_cache_fp8=c.index.to(d), num_sink=1, num_recent=1,
+                keep=torch.empty(2, 300, dtype=torch.int32, device=d), new_seq_lens=torch.empty(2, dtype=torch.int32, device=d),
+                new_acc=torch.empty(2, 320, device=d))
+    evict.run(**good)
+    for change in (dict(new_seq_lens=lens[1:]), dict(new_seq_lens=table.view(-1)[:2]), dict(new_seq_lens=good["keep"].view(-1)[3:5]),
+                   dict(keep=good["acc"].view(torch.int32).view(-1)[:600].view(2, 300)),
+                   dict(keep=good["new_acc"].view(torch.int32).view(-1)[:600].view(2, 300))):
+        with pytest.raises(ValueError, match="share memory"):
+            evict.run(**{**good, **change})
