@@ -15,9 +15,14 @@ summed over its rows and heads and added to the token's accumulator:
 
 ``acc`` and ``out`` are float32 ``[B, max_pages * 64]`` by position in the
 request (not by cache slot, so requests that share pages keep sums of their
-own); ``out`` may be ``acc``.  Every element of ``out`` is written.  To count
-accepted drafts only, pass their rows alone, with a ``cu_drafts`` and masks to
-match.  The sums run in a fixed order, so that results repeat.
+own); ``out`` may be ``acc``.  Every element of ``out`` is written.  The sums run
+in a fixed order, so that results repeat.
+
+To count accepted drafts only, give the others' rows an ``lse`` of -inf, for
+example ``lse.masked_fill(~accepted[:, None], -math.inf)``: such a row adds
+nothing.  (Leaving the rows out is another call: a draft's position is its
+place among its request's rows, so that accepted drafts 0 and 3 passed alone
+would be taken for the drafts at positions prefix and prefix + 1.)
 
 ``run``: a request with more than ``budget = keep.shape[1]`` tokens keeps its
 first ``num_sink``, its last ``num_recent`` and, of the tokens between them, those

@@ -267,7 +267,8 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(void);
  *   tree_mask     [num_drafts, mask_words] int64: bit j & 63 of word j / 64
  *                 is set if the draft sees its request's j-th draft (itself
  *                 and its ancestors, as a rule); 64 * mask_words drafts a
- *                 request at most
+ *                 request at most; bits of drafts that the request does not
+ *                 have are ignored
  *   output        [num_drafts, num_heads, 512] bf16
  *   lse           [num_drafts, num_heads] fp32, base-2 log-sum-exp of the
  *                 scaled logits; a row that sees nothing has -inf, output 0
@@ -296,7 +297,10 @@ DSA_API int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const v
  *                   2^(scaled logit - lse[i, h])
  * for every position k < max_pages * 64 (+ 0 behind a request's tokens).
  *
- *   lse           [num_drafts, num_heads] fp32, as the attention gave it
+ *   lse           [num_drafts, num_heads] fp32, as the attention gave it; a
+ *                 row with -inf adds nothing (so rows of rejected drafts are
+ *                 kept out; leaving them out of the arguments would move the
+ *                 positions of the drafts behind them)
  *   acc           [num_requests, max_pages * 64] fp32, rows acc_stride apart
  *   acc_out       likewise; may be acc itself, else the two do not overlap
  *

@@ -121,3 +121,25 @@ def test_evict_oracle():
     acc = torch.tensor([[3.0, 1.0, 2.0, 2.0, 0.0, 9.0], [float("nan"), 1, 5, 5, 5, 0]])
     assert otree.evict_reference(acc, torch.tensor([6, 5]), 3, 1, 1) == [[0, 2, 5], [0, 2, 4]]
     assert otree.evict_reference(acc, torch.tensor([6, 3]), 3, 0, 0) == [[0, 2, 5], [0, 1, 2]]
+
+
+def test_weights_of_accepted_drafts_alone():
+    """Rows of rejected drafts are kept out by an lse of -inf; rows that are
+    left out instead move the drafts behind them to other positions."""
+    import math
+
+    from oracle import tree as otree
+    g = torch.Generator().manual_seed(1)
+    normal = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)  # noqa: E731
+    qn, qp, ckv, kpe = normal(4, 2, 512), normal(4, 2, 64), normal(2, 64, 512), normal(2, 64, 64)
+    table = torch.tensor([[1, 0]])
+    mask = torch.tensor(tree.masks_from_parents([-1, 0, 0, 0]))
+    rest = (ckv, kpe, torch.tensor([70]), table)
+    lse = otree.tree_reference(qn, qp, *rest, torch.tensor([0, 4]), mask, 0.05)[1]
+    acc, accepted = torch.zeros(1, 128), torch.tensor([True, False, False, True])
+    kept_out = torch.where(accepted[:, None], lse, -math.inf)
+    new = otree.weights_reference(qn, qp, *rest, torch.tensor([0, 4]), mask, 0.05, kept_out, acc)[0]
+    assert abs(float(new.sum()) - 4) < 1e-9 and float(new[0, 73]) > 0 and (new[0, 71:73] == 0).all()
+    alone = otree.weights_reference(qn[accepted], qp[accepted], *rest, torch.tensor([0, 2]), mask[accepted], 0.05,
+                                    lse[accepted], acc)[0]
+    assert float(alone.sum()) < 4 - 1e-3

@@ -429,3 +429,23 @@ def test_refusals(cuda_device):
                     (lse, acc[:1].expand(2, -1), acc)):
         with pytest.raises(ValueError):
             evict.accumulate(**good, lse=l, acc=a, out=o)
+
+
+def test_weights_of_accepted_drafts_alone(cuda_device):
+    """Rejected rows get an lse of -inf; the accepted ones need not be the first."""
+    c = Case([130, 61, 2000], [4, 9, 6], 16, seed=41, device=cuda_device)
+    for b, parents in enumerate(([-1, 0, 0, 0], [-1, -1, 0, 1, 2, 2, 4, 3, 6], [-1, 0, 0, 1, 1, 3])):
+        c.mask[int(c.cu[b]):int(c.cu[b + 1])] = torch.tensor(tree.masks_from_parents(parents))
+    accepted = torch.zeros(19, dtype=torch.bool)
+    accepted[[0, 3, 4 + 0, 4 + 2, 4 + 4, 4 + 6, 4 + 8]] = True  # {0, 3}, {0, 2, 4, 6, 8} and none
+    args = c.args()
+    lse = run(c, args)[1].masked_fill(~accepted.to(cuda_device)[:, None], -math.inf)
+    acc = torch.zeros(3, args[5].shape[1] * 64, device=cuda_device)
+    out = weigh(c, args, acc=acc, lse=lse)[2].cpu()
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    assert ((out.double() - want).abs() <= off).all()
+    # An accepted row's weights sum to 2^(its lse - the given one); the test's own sum is in 64 bits.
+    lse_off = (torch.exp2(c.reference()[3]) - 1)[accepted].sum()
+    assert ((out.double().sum(1) - torch.tensor([2 * 16.0, 5 * 16.0, 0.0])).abs() <= off.sum(1) + lse_off).all()
+    assert (out[0, 133] > 0) and (out[0, 131:133] == 0).all() and (out[2] == 0).all()
