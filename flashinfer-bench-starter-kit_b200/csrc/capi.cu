@@ -64,6 +64,21 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return g_encode;
 }
 
+int encode(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base, const cuuint64_t* dims,
+           const cuuint64_t* strides, const cuuint32_t* box) {
+  const cuuint32_t estr[3] = {1, 1, 1};
+  auto once = [&]() {
+    return g_encode(map, dtype, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = once();
+  // The driver's call wants a current context, and a host thread has none
+  // before its first call of the runtime that needs one: this one may be it.
+  int dev;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = once();
+  return r == CUDA_SUCCESS ? DSA_OK : DSA_ERR_TENSOR_MAP;
+}
+
 }  // namespace
 
 int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
@@ -74,11 +89,7 @@ int encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_pitch_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? DSA_OK : DSA_ERR_TENSOR_MAP;
+  return encode(map, dtype, 2, base, dims, strides, box);
 }
 
 int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
@@ -90,11 +101,7 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
   cuuint64_t dims[3] = {inner, middle, outer};
   cuuint64_t strides[2] = {middle_pitch_bytes, outer_pitch_bytes};
   cuuint32_t box[3] = {box_inner, box_middle, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? DSA_OK : DSA_ERR_TENSOR_MAP;
+  return encode(map, dtype, 3, base, dims, strides, box);
 }
 
 }  // namespace dsa
