@@ -24,8 +24,10 @@ a row that sees nothing yields output 0 and lse -inf.
 * Query rows outside of ``[cu_drafts[0], cu_drafts[-1])`` are left as they are.
 * Lengths stay on the device; every launch goes to the current stream and can
   be captured into a CUDA graph (make one call on the capturing stream first,
-  so that its workspace exists).  Calls that overlap need different streams,
-  and graphs captured on one stream must not be replayed at the same time.
+  so that its workspace exists).  Calls that overlap need different streams;
+  threads may call on one stream, whose calls then run one after the other.
+  A graph uses the workspace of the stream that it was captured on: it must not
+  run beside another one captured there, nor beside calls on that stream.
 * Lengths that do not fit, page ids outside the pool and drafts that do not
   fit the mask set a sticky status bit (``device_status``), as for the other
   operators; with ``DSA_B200_CHECK=1`` each call synchronises and raises.

@@ -244,7 +244,8 @@ DSA_API int dsa_index_cache_write(const void* k, const int64_t* slot_mapping, in
  * same for every call: a 256-byte header, two fp32 records of 64 rows per SM
  * (39 MB in all) for contexts that several SMs share, and the call's list of
  * row groups (2.6 MB).  Zero-fill it once (its status word); nothing else in
- * it carries over from call to call. */
+ * it carries over from call to call.  Calls that may overlap on the device
+ * need a workspace each; threads may call with one workspace on one stream. */
 DSA_API size_t dsa_tree_attention_workspace_bytes(void);
 
 /* Attention of a tree of drafted tokens over the paged ckv / kpe cache

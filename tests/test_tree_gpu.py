@@ -449,3 +449,38 @@ def test_weights_of_accepted_drafts_alone(cuda_device):
     lse_off = (torch.exp2(c.reference()[3]) - 1)[accepted].sum()
     assert ((out.double().sum(1) - torch.tensor([2 * 16.0, 5 * 16.0, 0.0])).abs() <= off.sum(1) + lse_off).all()
     assert (out[0, 133] > 0) and (out[0, 131:133] == 0).all() and (out[2] == 0).all()
+
+
+def test_two_threads_on_one_stream(cuda_device, monkeypatch):
+    """A call is two launches that share the stream's records: another thread's
+    must not come between them."""
+    import threading
+
+    monkeypatch.setattr(tree, "_CHECK", False)
+    cases = [Case([4000, 900, 2500], [9, 2, 5], 16, seed=42, device=cuda_device),
+             Case([700, 6000, 64], [20, 3, 1], 8, seed=43, device=cuda_device)]
+    args = [c.args() for c in cases]
+    want = [run(c, a) for c, a in zip(cases, args)]
+    outs = [[c.outs() for _ in range(150)] for c in cases]
+    torch.cuda.synchronize()
+    start, errors = threading.Barrier(2), []
+
+    def calls(a, mine):
+        try:
+            start.wait()
+            for o in mine:
+                tree.run(*a, SCALE, *o)
+        except Exception as e:  # noqa: BLE001  raised below, in the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=calls, args=x) for x in zip(args, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert tree.device_status(cuda_device) == 0
+    for w, mine in zip(want, outs):
+        for o in mine:
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
