@@ -484,3 +484,56 @@ def test_two_threads_on_one_stream(cuda_device, monkeypatch):
     for w, mine in zip(want, outs):
         for o in mine:
             assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
+
+
+def test_back_to_back_and_concurrent_calls_without_waits(cuda_device, monkeypatch):
+    """Eager calls that nothing waits between: attention, weights and eviction
+    overlap the next launch on their stream, and those of another stream."""
+    monkeypatch.setattr(tree, "_CHECK", False)
+    cases = [Case([4000, 900, 2500], [9, 2, 5], 16, seed=44, device=cuda_device),
+             Case([700, 6000], [20, 3], 8, seed=45, device=cuda_device)]
+    args = [c.args() for c in cases]
+    state = []
+    for c, a in zip(cases, args):
+        out, lse = run(c, a)
+        _, acc, new = weigh(c, a, lse=lse)
+        B, budget = c.B, 256
+        caches = [torch.cat([t, torch.zeros(B * 4, *t.shape[1:], dtype=t.dtype, device=t.device)]) for t in a[2:4]]
+        fresh = (a[2].shape[0] + torch.arange(B * 4, device=cuda_device)).int().reshape(B, 4)
+        lens = (a[4] + a[6][1:] - a[6][:-1]).int()
+        keep, kept = (torch.empty(B, budget, dtype=torch.int32, device=cuda_device),
+                      torch.empty(B, dtype=torch.int32, device=cuda_device))
+        new2 = torch.empty(B, 256, device=cuda_device)
+
+        def step(a=a, c=c, caches=caches, out=out, lse=lse, acc=acc, new=new, lens=lens, fresh=fresh, keep=keep, kept=kept,
+                 new2=new2):
+            rows = (*a[:2], *caches, *a[4:], SCALE)
+            tree.run(*rows, out, lse)
+            evict.accumulate(*rows, lse, acc, new)
+            evict.run(new, lens, a[5], fresh, *caches, None, 3, 20, keep, kept, new2)
+
+        step()
+        torch.cuda.synchronize()
+        mine = [out, lse, new, keep, kept, new2, *caches]
+        state.append((step, mine, [t.clone() for t in mine]))
+        kept_ = otree.evict_reference(new.cpu(), lens.cpu(), budget, 3, 20)
+        assert all(keep[b, :len(k)].tolist() == k for b, k in enumerate(kept_))
+    streams = [torch.cuda.Stream(cuda_device) for _ in cases]
+    for s, (step, _, _) in zip(streams, state):
+        s.wait_stream(torch.cuda.current_stream(cuda_device))
+        with torch.cuda.stream(s):
+            step()  # the stream's workspaces exist
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, (_, mine, _) in zip(streams, state):
+            for t in mine[:6]:
+                t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, (step, _, _) in zip(streams, state):
+                with torch.cuda.stream(s):
+                    step()
+        torch.cuda.synchronize()
+        for _, mine, want in state:
+            assert all(torch.equal(x, y) for x, y in zip(mine, want))
+    assert tree.device_status(cuda_device) == 0 and evict.device_status(cuda_device) == 0
