@@ -131,3 +131,18 @@ def test_rows_that_see_nothing_for_whole_tiles(cuda_device):
     want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
                                         lse.cpu(), acc.cpu())
     assert ((new.cpu().double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("drafts,most", [(1, 16), (8, 8), (9, 8)])  # one group of rows, two, three; tiles a run
+def test_weights_over_many_runs_of_tiles(cuda_device, drafts, most):
+    n = 150 if drafts == 1 else 100
+    c = Pooled(lengths(n, 1100, 2500, 5), [drafts] * n, 16, 6, cuda_device)
+    pieces = list(c.pieces(0).values())
+    assert max(pieces) > most and any(p > most and p % most for p in pieces), pieces
+    lse, acc, out = weigh(c)
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    assert ((out.cpu().double() - want).abs() <= off).all()
+    twice = acc.clone()
+    weigh(c, acc=twice, lse=lse, out=twice)
+    assert torch.equal(twice, out)
