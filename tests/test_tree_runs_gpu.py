@@ -146,3 +146,43 @@ def test_weights_over_many_runs_of_tiles(cuda_device, drafts, most):
     twice = acc.clone()
     weigh(c, acc=twice, lse=lse, out=twice)
     assert torch.equal(twice, out)
+
+
+@pytest.mark.parametrize("requests,drafts,heads,bound", [
+    (3, 2, 16, 16),        # a row a block, 512 threads
+    (15, 2, 16, 32),       # a row a block
+    (25, 4, 16, 64),       # two rows
+    (50, 4, 16, 128),      # four
+    (60, 5, 24, 296),      # eight; drafts split between groups
+    (100, 4, 16, 296),     # eight
+    (300, 4, 16, None),    # by record
+])
+def test_every_form_of_the_join(cuda_device, requests, drafts, heads, bound):
+    """One request is much longer than the others, so that its groups have many
+    records; some requests begin or end within a slice."""
+    prefixes = lengths(requests - 1, 1, 300, 7)
+    prefixes.insert(requests // 3, 40_000 if requests > 100 else 20_000)
+    c = Pooled(prefixes, [drafts] * requests, heads, 8, cuda_device, variants=1 if requests > 100 else 2)
+    groups = requests * drafts * heads // 64 + requests
+    sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    tiers = [16, 32, 64, 128, 2 * sms]
+    assert next((t for t in tiers if groups <= t), None) == (2 * sms if bound == 296 else bound)
+    records = [k for k in c.pieces(LEAD) if k[1] == requests // 3 and k[2] == 0]
+    assert len(records) > 8, len(records)
+    out, lse = run(c)
+    c.check(out, lse)
+    c.check_rms(out)
+    again = run(c)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    # The long request alone: other slices, the same sums up to their roundings.
+    b = requests // 3
+    lo, hi = int(c.cu[b]), int(c.cu[b + 1])
+    alone = Pooled.__new__(Pooled)
+    alone.__dict__.update(c.__dict__, q_nope=c.q_nope[lo:hi], q_pe=c.q_pe[lo:hi], prefix=c.prefix[b:b + 1], B=1, T=hi - lo,
+                          table=c.table[b:b + 1], cu=c.cu[b:b + 2] - lo, mask=c.mask[lo:hi], drafts=[drafts])
+    o, l = run(alone)
+    bound_o, bound_l = c.reference()[2:]
+    assert ((o - out[lo:hi]).cpu().double().abs() <= 2 * bound_o[lo:hi]).all()
+    assert ((l - lse[lo:hi]).cpu().double().abs() <= 2 * bound_l[lo:hi]).all()
+    apart = (o.double() - out[lo:hi].double()).square().mean().sqrt()
+    assert apart <= 2 * math.sqrt(2) * 2.0 ** -8 * out[lo:hi].double().square().mean().sqrt()
