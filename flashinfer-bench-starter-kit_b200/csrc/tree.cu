@@ -1016,7 +1016,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
 // block y its rows y * rows_per_block ...  Each kParts-th of the block takes every
 // kParts-th record of a row, a thread four dims: the loads are latency-bound,
 // so many are in flight at once.
-constexpr int kJoinRows = 8;       // most rows per block
+constexpr int kJoinRows = 4;       // most rows per block
 constexpr int kJoinDepth = 8;      // records whose loads a thread has in flight
 
 template <int kParts>
@@ -1285,16 +1285,22 @@ extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, cons
   if (launch_programmatic(tree::tree_kernel<false>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
                           maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
     return DSA_ERR_CUDA;
-  // Up to 16 groups: a row a block of 512 threads, so that a long context's
-  // many records are read by many SMs with many loads in flight (1 request of
-  // 30000 tokens: 26.0 against 31.2 us with 256 threads).  More: a group has few
-  // records, and blocks of 128 threads and several rows cost less (40 requests
-  // of 1000-6000 tokens: 46.1 us; 48.7 with 256 threads, 56.1 with 512).
+  // Up to 10 groups (by their bound): a row a block of 512 threads, so that a
+  // long context's many records are read by many SMs with many loads in flight.
+  // More: a group has few records, and blocks of 128 threads and up to four
+  // rows cost less.  Whole calls in us, requests of 4 drafts x 16 heads with
+  // 2000-16000 tokens, from 64 groups on 1000-8000, at 200 500-6000:
+  //   groups            8    10    12    16    32    48    64    96   128   200
+  //   1 row, 512     26.2  25.0  28.8  32.7  50.0  67.5  63.3  86.1 107.5 127.9
+  //   1 row, 128     29.9  26.5  27.0  28.8  41.7  53.7  45.4  57.7  71.9  77.8
+  //   2 rows         35.9  31.0  31.0  32.9  43.2  53.5  44.0  55.6  68.7  73.3
+  //   4 rows         44.0  37.9  39.1  40.6  47.8  56.7  47.0  55.4  67.6  71.8
+  //   8 rows         61.9  55.9  56.1  57.5  57.8  64.5  54.1  61.2  72.2  73.7
   const int64_t groups = tree::groups_bound(num_drafts, num_heads, num_requests);
   const bool by_record = groups > 2 * info.num_sms;
   const unsigned int across = static_cast<unsigned int>(by_record ? 2 * info.num_sms : groups);
-  const int rows = across <= 32 ? 1 : (across <= 64 ? 2 : (across <= 128 ? 4 : tree::kJoinRows));
-  const bool deep = across <= 16;
+  const int rows = across <= 32 ? 1 : (across <= 96 ? 2 : tree::kJoinRows);
+  const bool deep = across <= 10;
   if (launch_programmatic(deep ? tree::combine_kernel<4> : tree::combine_kernel<1>, dim3(across, tree::kRows / rows),
                           dim3(deep ? 512 : 128), 0, s, prm, info.num_sms, rows, by_record) != cudaSuccess)
     return DSA_ERR_CUDA;

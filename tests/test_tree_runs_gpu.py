@@ -149,12 +149,13 @@ def test_weights_over_many_runs_of_tiles(cuda_device, drafts, most):
 
 
 @pytest.mark.parametrize("requests,drafts,heads,bound", [
-    (3, 2, 16, 16),        # a row a block, 512 threads
-    (15, 2, 16, 32),       # a row a block
-    (25, 4, 16, 64),       # two rows
-    (50, 4, 16, 128),      # four
-    (60, 5, 24, 296),      # eight; drafts split between groups
-    (100, 4, 16, 296),     # eight
+    (3, 2, 16, 10),        # a row a block, 512 threads
+    (9, 2, 16, 32),        # a row a block
+    (15, 2, 16, 32),
+    (25, 4, 16, 96),       # two rows
+    (50, 4, 16, 296),      # four
+    (60, 5, 24, 296),      # drafts split between groups
+    (100, 4, 16, 296),
     (300, 4, 16, None),    # by record
 ])
 def test_every_form_of_the_join(cuda_device, requests, drafts, heads, bound):
@@ -165,7 +166,7 @@ def test_every_form_of_the_join(cuda_device, requests, drafts, heads, bound):
     c = Pooled(prefixes, [drafts] * requests, heads, 8, cuda_device, variants=1 if requests > 100 else 2)
     groups = requests * drafts * heads // 64 + requests
     sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
-    tiers = [16, 32, 64, 128, 2 * sms]
+    tiers = [10, 32, 96, 2 * sms]
     assert next((t for t in tiers if groups <= t), None) == (2 * sms if bound == 296 else bound)
     records = [k for k in c.pieces(LEAD) if k[1] == requests // 3 and k[2] == 0]
     assert len(records) > 8, len(records)
