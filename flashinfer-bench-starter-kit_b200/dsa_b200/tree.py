@@ -13,8 +13,12 @@ sees the whole prefix and the drafts whose bits its row of ``tree_mask`` has
 its own bit set is plain dense decoding.
 
 Unlike ``dsa_b200.attention.run``, which reads 2048 selected slots, this reads
-every visible token.  ``lse`` is the base-2 log-sum-exp of the scaled logits;
-a row that sees nothing yields output 0 and lse -inf.
+every visible token.  The two are the same function where a draft sees at most
+2048 tokens (the indexer then selects them all); beyond, a model that decodes
+with the indexer's selection gets another distribution from dense rows, and its
+own drafts are verified by ``indexer.run_prefill`` and ``attention.run``.
+``lse`` is the base-2 log-sum-exp of the scaled logits; a row that sees nothing
+yields output 0 and lse -inf.
 
 * Any 1 to 128 heads; up to ``64 * tree_mask.shape[1]`` drafts per request.
 * ``ckv_cache`` ``[pages, 64, 512]`` and ``kpe_cache`` ``[pages, 64, 64]`` may be

@@ -254,6 +254,7 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(void);
  * cu_drafts[r] .. cu_drafts[r+1]-1, whose ckv / kpe rows lie in the cache
  * behind the prefix (position prefix + j for its j-th draft).  A draft sees
  * the whole prefix and those drafts of its request whose bits its mask has.
+ * Equal to indexer and sparse attention where a draft sees at most 2048 tokens.
  *
  *   q_nope        [num_drafts, num_heads, 512] bf16, contiguous
  *   q_pe          [num_drafts, num_heads, 64] bf16, contiguous

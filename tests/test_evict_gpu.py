@@ -430,3 +430,25 @@ def test_outputs_over_inputs_are_refused(cuda_device):
                    dict(keep=good["new_acc"].view(torch.int32).view(-1)[:600].view(2, 300))):
         with pytest.raises(ValueError, match="share memory"):
             evict.run(**{**good, **change})
+
+
+def test_dense_and_sparse_agree_up_to_the_selection_size(cuda_device):
+    """Where a draft sees at most 2048 tokens the indexer selects them all, and
+    tree attention is the sparse attention's function."""
+    d = cuda_device
+    lens = [2048, 1500, 63, 1]
+    dec = workloads.make_decode_inputs(lens, seed=53, device=d)
+    ix = dec.indexer
+    topk = torch.full((4, 2048), 7, dtype=torch.int32, device=d)
+    indexer.run(ix.q_index_fp8, ix.k_index_cache_fp8, ix.weights, ix.seq_lens, ix.block_table, topk)
+    so, sl = torch.empty(4, 16, 512, dtype=torch.bfloat16, device=d), torch.empty(4, 16, device=d)
+    attention.run(dec.q_nope, dec.q_pe, dec.ckv_cache, dec.kpe_cache, topk, dec.sm_scale, so, sl)
+    o, l = torch.empty_like(so), torch.empty_like(sl)
+    rows = (dec.q_nope, dec.q_pe, dec.ckv_cache, dec.kpe_cache, torch.tensor(lens, dtype=torch.int32, device=d) - 1,
+            ix.block_table, torch.arange(5, dtype=torch.int32, device=d), torch.ones(4, 1, dtype=torch.int64, device=d))
+    tree.run(*rows, dec.sm_scale, o, l)
+    host = [t.cpu() for t in rows]
+    ro, rl, bo, bl = otree.tree_reference(*host, dec.sm_scale)
+    assert ((o.cpu().double() - ro).abs() <= bo).all() and ((l.cpu().double() - rl).abs() <= bl).all()
+    # The sparse attention's own tolerance (its harness's) on the same values.
+    assert compare.harness_close(so.cpu(), ro.float(), 1e-2, 1e-2).ok and compare.harness_close(sl.cpu(), rl.float(), 1e-3, 1e-3).ok
