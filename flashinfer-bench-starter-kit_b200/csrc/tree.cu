@@ -867,7 +867,9 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
             // among them into NaN.  The logits have been read (S^T is done),
             // so such values are zeroed in the V tile; a row that does see
             // one has its NaN from the logit (or, where the logit is -inf,
-            // the weight 0 and nothing of the value).
+            // the weight 0 and nothing of the value; before the prefix's end,
+            // where nothing is zeroed, 0 times infinity: callers are told
+            // that this is not defined).
 #pragma unroll
             for (int x = 0; x < kParts; ++x) ok = ok && mbar_wait(&kv_full[st * kParts + x], (i >> 1) & 1, wctx);
             const int from = s.r.prefix > t * kTok ? s.r.prefix - t * kTok : 0;

@@ -25,6 +25,9 @@ yields output 0 and lse -inf.
   strided (pages and rows at multiples of 16 bytes), such as two slices of one
   ``[pages, 64, 576]`` cache; they are never copied.
 * Cache rows that a mask hides may hold anything, infinities and NaN included.
+  A visible row with NaN, or with an infinity that makes its logit +inf or NaN,
+  makes the output NaN.  If the logit is -inf, whether an infinity among its values
+  counts as 0 times infinity or as nothing is not defined.
 * Query rows outside of ``[cu_drafts[0], cu_drafts[-1])`` are left as they are.
 * Lengths stay on the device; every launch goes to the current stream and can
   be captured into a CUDA graph (make one call on the capturing stream first,

@@ -277,7 +277,8 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(void);
  *
  * 1 <= num_heads <= 128; num_drafts * num_heads <= 2^24, num_requests <= 65536
  * and (num_drafts * num_heads / 64 + num_requests) * (max_pages + 3) <= 2^30.
- * Masked cache rows may hold anything.  Data-dependent
+ * Masked cache rows may hold anything; whether a visible row with a logit of
+ * -inf adds 0 times its infinite values or nothing is not defined.  Data-dependent
  * errors: lengths that do not fit the table (clamped), drafts that do not fit
  * cu_drafts or the mask (left out), a cu_drafts that decreases (the call then
  * writes no row): DSA_DEV_BAD_SEQ_LEN; page ids outside the pool (their tokens

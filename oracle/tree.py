@@ -63,6 +63,8 @@ def tree_reference(q_nope, q_pe, ckv, kpe, prefix, table, cu, mask, scale):
         lo, hi, c, x, off = _request(q_nope, q_pe, ckv, kpe, prefix, table, cu, mask, scale, b)
         if hi <= lo:
             continue
+        # For masked rows.  Of a visible one a finite logit leaves nothing infinite; with a logit of
+        # -inf its infinities count as nothing here, which the operator does not define.
         c = torch.where(torch.isfinite(c), c, 0.0)
         top = x.amax(-1, keepdim=True) if x.shape[-1] else torch.full((*x.shape[:2], 1), -math.inf)
         top = torch.where(top == -math.inf, 0.0, top)
