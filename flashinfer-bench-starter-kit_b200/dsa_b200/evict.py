@@ -42,6 +42,8 @@ given twice, raises.  Streams, graphs and device status bits are as for
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _native, tree, workspace
@@ -92,8 +94,7 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
     same = acc_ptr == out_ptr and acc_pitch == out_pitch
     if not same and B > 0 and _overlap(B, acc_ptr, acc_pitch, width, out_ptr, out_pitch, width):
         _fail_acc("out must be acc itself or not overlap it")
-    if isinstance(sm_scale, torch.Tensor):
-        sm_scale = sm_scale.item()
+    sm_scale = float(sm_scale)
     if B == 0:
         return
     if T == 0:
@@ -153,6 +154,7 @@ def run(acc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, ne
     budget = keep.shape[1]
     if not 1 <= budget <= new_pages * PAGE_SIZE:
         _fail_run(f"a budget of {budget} tokens (keep.shape[1]) does not fit new_block_table's {new_pages} pages")
+    num_sink, num_recent = operator.index(num_sink), operator.index(num_recent)
     if num_sink < 0 or num_recent < 0 or num_sink + num_recent > budget:
         _fail_run(f"num_sink {num_sink} and num_recent {num_recent} must fit the budget of {budget}")
     width, new_width = max_pages * PAGE_SIZE, new_pages * PAGE_SIZE

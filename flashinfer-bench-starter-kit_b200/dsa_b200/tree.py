@@ -177,8 +177,7 @@ def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_c
         _fail(f"output must be contiguous bfloat16 [{T}, {H}, {DIM_CKV}]")
     if lse.dtype is not torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
         _fail(f"lse must be contiguous float32 [{T}, {H}]")
-    if isinstance(sm_scale, torch.Tensor):
-        sm_scale = sm_scale.item()
+    sm_scale = float(sm_scale)
     if T == 0 or B == 0:
         return
     dev = q_nope.device

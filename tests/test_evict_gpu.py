@@ -452,3 +452,25 @@ def test_dense_and_sparse_agree_up_to_the_selection_size(cuda_device):
     assert ((o.cpu().double() - ro).abs() <= bo).all() and ((l.cpu().double() - rl).abs() <= bl).all()
     # The sparse attention's own tolerance (its harness's) on the same values.
     assert compare.harness_close(so.cpu(), ro.float(), 1e-2, 1e-2).ok and compare.harness_close(sl.cpu(), rl.float(), 1e-3, 1e-3).ok
+
+
+def test_scalars_of_other_types(cuda_device):
+    """A scale and counts that are numpy's or tensors, as the sparse attention takes them."""
+    import numpy as np
+    d = cuda_device
+    dec = workloads.make_decode_inputs([900, 400], seed=54, device=d, pool_pages=64)
+    bt = dec.indexer.block_table
+    rows = (dec.q_nope, dec.q_pe, dec.ckv_cache, dec.kpe_cache, torch.tensor([899, 399], dtype=torch.int32, device=d), bt,
+            torch.arange(3, dtype=torch.int32, device=d), torch.ones(2, 1, dtype=torch.int64, device=d))
+    want = None
+    for scale in (0.0625, np.float32(0.0625), np.float64(0.0625), torch.tensor(0.0625), torch.tensor([0.0625], device=d)):
+        out, lse = torch.zeros(2, 16, 512, dtype=torch.bfloat16, device=d), torch.zeros(2, 16, device=d)
+        acc = torch.zeros(2, bt.shape[1] * 64, device=d)
+        tree.run(*rows, scale, out, lse)
+        evict.accumulate(*rows, scale, lse, acc, acc)
+        want = want or (out, lse, acc)
+        assert all(torch.equal(a, b) for a, b in zip(want, (out, lse, acc)))
+    c = Case([900, 400], 300, d, seed=55)
+    c.check(c.run(np.int64(4), torch.tensor(16)), 4, 16)
+    with pytest.raises(TypeError):
+        c.run(4.0, 16)
