@@ -59,16 +59,22 @@ _CHECK = os.environ.get("DSA_B200_CHECK", "0") not in ("", "0")
 _ws_bytes: dict = {}  # device index -> dsa_tree_attention_workspace_bytes
 
 
-def masks_from_parents(parents) -> list:
+def masks_from_parents(parents, words=None) -> list:
     """``tree_mask`` rows (lists of signed 64-bit words) of one request's drafts:
     ``parents[j]`` is the index of draft j's parent, below j, or -1 if it
-    follows the prefix directly.  Every draft sees its ancestors and itself."""
+    follows the prefix directly.  Every draft sees its ancestors and itself.
+    Rows have as many words as the drafts need, or ``words``: a batch's trees
+    need the largest one's."""
     bits = []
     for j, par in enumerate(parents):
         if not -1 <= par < j:
             raise ValueError(f"parents[{j}] is {par}: a parent comes before its children")
         bits.append((1 << j) | (bits[par] if par >= 0 else 0))
-    words = max(1, (len(bits) + 63) // 64)
+    need = max(1, (len(bits) + 63) // 64)
+    if words is None:
+        words = need
+    elif words < need:
+        raise ValueError(f"{len(bits)} drafts need {need} words, not {words}")
     rows = [[(m >> (64 * w)) & ((1 << 64) - 1) for w in range(words)] for m in bits]
     return [[w - (1 << 64) if w >> 63 else w for w in row] for row in rows]
 

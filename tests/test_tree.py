@@ -143,3 +143,12 @@ def test_weights_of_accepted_drafts_alone():
     alone = otree.weights_reference(qn[accepted], qp[accepted], *rest, torch.tensor([0, 2]), mask[accepted], 0.05,
                                     lse[accepted], acc)[0]
     assert float(alone.sum()) < 4 - 1e-3
+
+
+def test_masks_of_a_batch_have_the_words_of_its_largest_tree():
+    small, large = [-1, 0, 0], list(range(-1, 69))
+    rows = tree.masks_from_parents(small, words=2) + tree.masks_from_parents(large, words=2)
+    assert torch.tensor(rows).shape == (73, 2)
+    assert rows[:3] == [[1, 0], [3, 0], [5, 0]] and rows[3:] == tree.masks_from_parents(large)
+    with pytest.raises(ValueError, match="2 words"):
+        tree.masks_from_parents(large, words=1)

@@ -187,3 +187,21 @@ def test_every_form_of_the_join(cuda_device, requests, drafts, heads, bound):
     assert ((l - lse[lo:hi]).cpu().double().abs() <= 2 * bound_l[lo:hi]).all()
     apart = (o.double() - out[lo:hi].double()).square().mean().sqrt()
     assert apart <= 2 * math.sqrt(2) * 2.0 ** -8 * out[lo:hi].double().square().mean().sqrt()
+
+
+@pytest.mark.parametrize("prefixes,drafts,heads", [
+    ([1000, 77, 0], [300, 129, 65], 16),   # five words of mask, chains with branches
+    ([30], [1000], 3),                      # 16 words, drafts over 16 pages
+    ([5000], [512], 16),                    # a prompt's chunk
+])
+def test_more_than_64_drafts(cuda_device, prefixes, drafts, heads):
+    c = Pooled(prefixes, drafts, heads, 9, cuda_device)
+    if len(prefixes) == 1 and heads == 16:  # causal
+        c.mask = torch.tensor(tree.masks_from_parents(list(range(-1, drafts[0] - 1))))
+    out, lse = run(c)
+    c.check(out, lse)
+    c.check_rms(out)
+    lse, acc, new = weigh(c, lse=lse)
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    assert ((new.cpu().double() - want).abs() <= off).all()
