@@ -365,28 +365,6 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
   }
 }
 
-// Whether the float32 [rows, width] tensors at a and b, of the given pitches,
-// share memory.  Rows of one pitch may interleave, such as the left and right
-// columns of one buffer; of two pitches, their extents have to lie apart.
-bool rows_overlap(int64_t rows, const float* a, int64_t a_pitch, int64_t a_width, const float* b, int64_t b_pitch,
-                  int64_t b_width) {
-  if (reinterpret_cast<uintptr_t>(a) > reinterpret_cast<uintptr_t>(b)) {
-    const float* c = a;
-    a = b;
-    b = c;
-    int64_t x = a_pitch;
-    a_pitch = b_pitch;
-    b_pitch = x;
-    x = a_width;
-    a_width = b_width;
-    b_width = x;
-  }
-  const int64_t apart = static_cast<int64_t>((reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) / 4);
-  if (apart >= (rows - 1) * a_pitch + a_width) return false;
-  const int64_t at = apart % a_pitch;
-  return a_pitch != b_pitch || at < a_width || at + b_width > a_pitch;
-}
-
 // CTAs per request: as many as the cluster limit, the SMs (two 512-thread CTAs
 // each) and the table's width can use, down to 256 tokens a CTA.  One request of
 // 65536 tokens: 14.9 us with 16, 20.0 with 8; 8 of 3000-4096: 11.3 us, 15.5 with
@@ -458,7 +436,7 @@ extern "C" int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const i
   }
   const size_t acc_bytes = static_cast<size_t>((num_requests - 1) * acc_stride + width) * 4;
   if (ranges_overlap(keep, out[0].bytes, acc, acc_bytes) || ranges_overlap(new_seq_lens, out[1].bytes, acc, acc_bytes) ||
-      evict::rows_overlap(num_requests, acc, acc_stride, width, new_acc, new_acc_stride, new_width))
+      rows_overlap(num_requests, acc, acc_stride, width, new_acc, new_acc_stride, new_width))
     return DSA_ERR_OVERLAP;
   DeviceInfo info;
   int st = current_device_info(&info);

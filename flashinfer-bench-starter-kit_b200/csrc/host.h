@@ -44,6 +44,28 @@ inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t 
   return x < y ? y - x < a_bytes : x - y < b_bytes;
 }
 
+// Whether the float32 [rows, width] tensors at a and b, of the given pitches,
+// share memory.  Rows of one pitch may interleave, such as the left and right
+// columns of one buffer; of two pitches, their extents have to lie apart.
+inline bool rows_overlap(int64_t rows, const float* a, int64_t a_pitch, int64_t a_width, const float* b,
+                         int64_t b_pitch, int64_t b_width) {
+  if (reinterpret_cast<uintptr_t>(a) > reinterpret_cast<uintptr_t>(b)) {
+    const float* c = a;
+    a = b;
+    b = c;
+    int64_t x = a_pitch;
+    a_pitch = b_pitch;
+    b_pitch = x;
+    x = a_width;
+    a_width = b_width;
+    b_width = x;
+  }
+  const int64_t apart = static_cast<int64_t>((reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) / 4);
+  if (apart >= (rows - 1) * a_pitch + a_width) return false;
+  const int64_t at = apart % a_pitch;
+  return a_pitch != b_pitch || at < a_width || at + b_width > a_pitch;
+}
+
 // Launches the indexer's top-2048 select over `rows` score rows (one CTA
 // each, programmatically after the kernel that wrote the scores): row b
 // reads scores[b], hist[b], seq_lens[b] and block-table row row_req[b]

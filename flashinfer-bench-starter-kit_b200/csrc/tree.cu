@@ -1176,12 +1176,19 @@ inline bool sizes_ok(int64_t drafts, int64_t heads, int64_t requests) {
          drafts * heads <= kMaxRows;
 }
 
+struct Range {
+  const void* at;
+  size_t bytes;
+};
+
+// `more`: the attention's output and lse; the weights' accumulators and lse,
+// which is an input.
 int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64_t ckv_page, int64_t ckv_row,
                     const void* kpe, int64_t kpe_page, int64_t kpe_row, int64_t num_pages,
                     const int32_t* prefix_lens, const int32_t* block_table, const int32_t* cu, const int64_t* mask,
                     int32_t requests, int32_t drafts, int32_t heads, int32_t max_pages, int32_t mask_words,
-                    float sm_scale, void* workspace, size_t workspace_bytes, bool records, DeviceInfo* info,
-                    Params* prm, CUtensorMap (&maps)[4]) {
+                    float sm_scale, void* workspace, size_t workspace_bytes, bool records, const Range (&more)[2],
+                    DeviceInfo* info, Params* prm, CUtensorMap (&maps)[4]) {
   if (!q_nope || !q_pe || !ckv || !kpe || !prefix_lens || !block_table || !cu || !mask || !workspace)
     return DSA_ERR_INVALID_ARGUMENT;
   if (num_pages < 1 || num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || mask_words < 1 ||
@@ -1196,6 +1203,24 @@ int check_and_setup(const void* q_nope, const void* q_pe, const void* ckv, int64
        reinterpret_cast<uintptr_t>(cu)) & 3u)
     return DSA_ERR_MISALIGNED;
   if (reinterpret_cast<uintptr_t>(mask) & 7u) return DSA_ERR_MISALIGNED;
+  // Outputs lie apart from what other CTAs still read.  The attention's output
+  // may be q_nope: a group's rows are written behind its queries' last use, by
+  // the CTA that read them or by the join.
+  const size_t n = static_cast<size_t>(requests), rows_q = static_cast<size_t>(drafts) * heads;
+  const Range in[8] = {{q_nope, rows_q * kCkv * 2},
+                       {q_pe, rows_q * kKpe * 2},
+                       {ckv, static_cast<size_t>(num_pages - 1) * ckv_page + (kTok - 1) * ckv_row + kCkv * 2},
+                       {kpe, static_cast<size_t>(num_pages - 1) * kpe_page + (kTok - 1) * kpe_row + kKpe * 2},
+                       {prefix_lens, n * 4},
+                       {block_table, n * max_pages * 4},
+                       {cu, (n + 1) * 4},
+                       {mask, static_cast<size_t>(drafts) * mask_words * 8}};
+  if (ranges_overlap(more[0].at, more[0].bytes, more[1].at, more[1].bytes)) return DSA_ERR_OVERLAP;
+  for (int o = 0; o < (records ? 2 : 1); ++o)
+    for (int i = 0; i < 8; ++i)
+      if (ranges_overlap(more[o].at, more[o].bytes, in[i].at, in[i].bytes) &&
+          !(records && o == 0 && i == 0 && more[o].at == q_nope))
+        return DSA_ERR_OVERLAP;
   int st = current_device_info(info);
   if (st != DSA_OK) return st;
   if (static_cast<size_t>(kSmemBytes) > info->max_smem_optin || info->num_sms > kMaxCtas)
@@ -1275,10 +1300,12 @@ extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, cons
   DeviceInfo info;
   tree::Params prm;
   CUtensorMap maps[4];
+  const size_t rows_q = static_cast<size_t>(num_drafts) * num_heads;
   const int st = tree::check_and_setup(q_nope, q_pe, ckv_cache, ckv_page_bytes, ckv_row_bytes, kpe_cache,
                                        kpe_page_bytes, kpe_row_bytes, num_pages, prefix_lens, block_table, cu_drafts,
                                        tree_mask, num_requests, num_drafts, num_heads, max_pages, mask_words, sm_scale,
-                                       workspace, workspace_bytes, true, &info, &prm, maps);
+                                       workspace, workspace_bytes, true,
+                                       {{output, rows_q * tree::kCkv * 2}, {lse, rows_q * 4}}, &info, &prm, maps);
   if (st != DSA_OK) return st;
   prm.out = static_cast<__nv_bfloat16*>(output);
   prm.lse_out = lse;
@@ -1323,9 +1350,11 @@ extern "C" int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const 
   if (!lse || !acc || !acc_out) return DSA_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(acc) | reinterpret_cast<uintptr_t>(acc_out)) & 3u)
     return DSA_ERR_MISALIGNED;
-  if (max_pages < 1 || acc_stride < static_cast<int64_t>(max_pages) * tree::kTok ||
-      acc_out_stride < static_cast<int64_t>(max_pages) * tree::kTok || (acc == acc_out && acc_stride != acc_out_stride))
+  const int64_t width = static_cast<int64_t>(max_pages) * tree::kTok;
+  if (max_pages < 1 || acc_stride < width || acc_out_stride < width || (acc == acc_out && acc_stride != acc_out_stride))
     return DSA_ERR_INVALID_ARGUMENT;
+  if (acc != acc_out && rows_overlap(num_requests, acc, acc_stride, width, acc_out, acc_out_stride, width))
+    return DSA_ERR_OVERLAP;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (num_drafts == 0) {  // nothing to add
     if (acc != acc_out &&
@@ -1340,7 +1369,10 @@ extern "C" int dsa_tree_weights_run(const void* q_nope, const void* q_pe, const 
   const int st = tree::check_and_setup(q_nope, q_pe, ckv_cache, ckv_page_bytes, ckv_row_bytes, kpe_cache,
                                        kpe_page_bytes, kpe_row_bytes, num_pages, prefix_lens, block_table, cu_drafts,
                                        tree_mask, num_requests, num_drafts, num_heads, max_pages, mask_words, sm_scale,
-                                       workspace, workspace_bytes, false, &info, &prm, maps);
+                                       workspace, workspace_bytes, false,
+                                       {{acc_out, static_cast<size_t>((num_requests - 1) * acc_out_stride + width) * 4},
+                                        {lse, static_cast<size_t>(num_drafts) * num_heads * 4}},
+                                       &info, &prm, maps);
   if (st != DSA_OK) return st;
   prm.lse_in = lse;
   prm.acc = acc;

@@ -109,6 +109,8 @@ def accumulate(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor
     st = _native.call_on(dev, _native.lib().dsa_tree_weights_run, *args, sm_scale, lse.data_ptr(), acc_ptr, acc_pitch,
                          out_ptr, out_pitch, ws.data_ptr(), ws.numel(), cur)
     if st:
+        if st == _native.DSA_ERR_OVERLAP:
+            _fail_acc("out must share memory with no input but acc, which it may be")
         _native.check(st, "dsa_tree_weights_run")
     if tree._CHECK and not torch.cuda.is_current_stream_capturing():
         raise_on_device_status(dev)

@@ -28,6 +28,7 @@ yields output 0 and lse -inf.
   A visible row with NaN, or with an infinity that makes its logit +inf or NaN,
   makes the output NaN.  If the logit is -inf, whether an infinity among its values
   counts as 0 times infinity or as nothing is not defined.
+* ``output`` may be ``q_nope`` itself; other outputs over an input are refused.
 * Query rows outside of ``[cu_drafts[0], cu_drafts[-1])`` are left as they are.
 * Lengths stay on the device; every launch goes to the current stream and can
   be captured into a CUDA graph (make one call on the capturing stream first,
@@ -192,6 +193,8 @@ def run(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_cache: torch.Tensor, kpe_c
     st = _native.call_on(dev, _native.lib().dsa_tree_attention_run, *args, sm_scale, output.data_ptr(), lse.data_ptr(),
                          ws.data_ptr(), ws.numel(), cur)
     if st:
+        if st == _native.DSA_ERR_OVERLAP:
+            _fail("output and lse must share memory neither with each other nor with the inputs (output may be q_nope itself)")
         _native.check(st, "dsa_tree_attention_run")
     if _CHECK and not torch.cuda.is_current_stream_capturing():
         raise_on_device_status(dev)

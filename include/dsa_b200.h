@@ -271,10 +271,11 @@ DSA_API size_t dsa_tree_attention_workspace_bytes(void);
  *                 and its ancestors, as a rule); 64 * mask_words drafts a
  *                 request at most; bits of drafts that the request does not
  *                 have are ignored
- *   output        [num_drafts, num_heads, 512] bf16
+ *   output        [num_drafts, num_heads, 512] bf16; may be q_nope itself
  *   lse           [num_drafts, num_heads] fp32, base-2 log-sum-exp of the
  *                 scaled logits; a row that sees nothing has -inf, output 0
  *
+ * Outputs that share memory with anything else: DSA_ERR_OVERLAP.
  * 1 <= num_heads <= 128; num_drafts * num_heads <= 2^24, num_requests <= 65536
  * and (num_drafts * num_heads / 64 + num_requests) * (max_pages + 3) <= 2^30.
  * Masked cache rows may hold anything; whether a visible row with a logit of
@@ -305,7 +306,8 @@ DSA_API int dsa_tree_attention_run(const void* q_nope, const void* q_pe, const v
  *                 kept out; leaving them out of the arguments would move the
  *                 positions of the drafts behind them)
  *   acc           [num_requests, max_pages * 64] fp32, rows acc_stride apart
- *   acc_out       likewise; may be acc itself, else the two do not overlap
+ *   acc_out       likewise; may be acc itself, else it shares memory with no
+ *                 other argument (DSA_ERR_OVERLAP)
  *
  * The sums run in a fixed order (no atomics).  The workspace holds only the
  * status word (256 bytes). */

@@ -152,3 +152,41 @@ def test_masks_of_a_batch_have_the_words_of_its_largest_tree():
     assert rows[:3] == [[1, 0], [3, 0], [5, 0]] and rows[3:] == tree.masks_from_parents(large)
     with pytest.raises(ValueError, match="2 words"):
         tree.masks_from_parents(large, words=1)
+
+
+# name -> bytes, one behind the other: 3 requests of 4 pages, 5 drafts of 16 heads, one word of mask, 9 pages of cache
+SIZES = {"q_nope": 5 * 16 * 1024, "q_pe": 5 * 16 * 128, "ckv": 9 * 65536, "kpe": 9 * 8192, "prefix": 12, "table": 48, "cu": 16,
+         "pad": 4, "mask": 40, "lse": 5 * 16 * 4, "pad2": 8, "out": 5 * 16 * 1024, "acc": 3 * 4 * 256, "new": 3 * 4 * 256}
+AT, _end = {}, 1 << 20
+for _name, _bytes in SIZES.items():
+    AT[_name] = _end
+    _end += _bytes
+
+
+def placed(entry, **where):
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up: no launch may follow")
+    at = {k: P(v) for k, v in (AT | where).items()}
+    rows = (at["q_nope"], at["q_pe"], at["ckv"], 65536, 1024, at["kpe"], 8192, 128, 9, at["prefix"], at["table"], at["cu"],
+            at["mask"], 3, 5, 16, 4, 1, 0.1)
+    if entry == "attention":
+        return _native.lib().dsa_tree_attention_run(*rows, at["out"], at["lse"], P(16), 1 << 30, None)
+    return _native.lib().dsa_tree_weights_run(*rows, at["lse"], at["acc"], 256, at["new"], 256, P(16), 256, None)
+
+
+def test_outputs_beside_the_inputs_and_in_place_are_taken():
+    known = (1, 2, 3, _native.DSA_ERR_OVERLAP)  # only the device is missing
+    assert placed("attention") not in known and placed("attention", out=AT["q_nope"]) not in known
+    assert placed("weights") not in known and placed("weights", new=AT["acc"]) not in known
+
+
+@pytest.mark.parametrize("entry,out", [("attention", "out"), ("attention", "lse"), ("weights", "new")])
+@pytest.mark.parametrize("other", ["q_nope", "q_pe", "ckv", "kpe", "prefix", "table", "cu", "mask", "lse", "acc"])
+def test_outputs_over_inputs_are_refused(entry, out, other):
+    if other == out or (other, entry) == ("acc", "attention"):
+        pytest.skip("not an input of this call")
+    step = 16 if out == "out" else 4  # outputs keep their alignment
+    last = (AT[other] + SIZES[other] - 1) // step * step
+    first = -(-(AT[other] - SIZES[out] + 1) // step) * step
+    assert placed(entry, **{out: last}) == _native.DSA_ERR_OVERLAP
+    assert placed(entry, **{out: first}) == _native.DSA_ERR_OVERLAP

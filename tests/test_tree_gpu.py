@@ -537,3 +537,49 @@ def test_back_to_back_and_concurrent_calls_without_waits(cuda_device, monkeypatc
         for _, mine, want in state:
             assert all(torch.equal(x, y) for x, y in zip(mine, want))
     assert tree.device_status(cuda_device) == 0 and evict.device_status(cuda_device) == 0
+
+
+def test_rows_before_the_first_request_are_left(cuda_device):
+    c = Case([130, 0, 20], [5, 3, 2], 16, seed=46, device=cuda_device, tail=4)
+    for name in ("q_nope", "q_pe", "mask"):  # the four rows of no request go first
+        setattr(c, name, getattr(c, name).roll(4, 0))
+    c.cu = c.cu + 4
+    out, lse = run(c)
+    c.check(out, lse)  # the first rows too: NaN in the reference, left as they were
+    assert (out[:4] == 7).all() and (lse[:4] == 7).all()
+    lse, acc, new = weigh(c, lse=lse)
+    want, off = otree.weights_reference(c.q_nope, c.q_pe, c.ckv, c.kpe, c.prefix, c.table, c.cu, c.mask, SCALE,
+                                        lse.cpu(), acc.cpu())
+    assert ((new.cpu().double() - want).abs() <= off).all()
+
+
+def test_output_over_the_queries(cuda_device):
+    """A group's rows are written after its queries were read, by the CTA that
+    read them or by the join, so the output may take the queries' place."""
+    c = Case([3000, 500, 0, 64], [9, 2, 3, 30], 16, seed=47, device=cuda_device)
+    args = c.args()
+    out, lse = run(c, args)
+    for _ in range(5):
+        q = args[0].clone()
+        tree.run(q, *args[1:], SCALE, q, lse)
+        assert torch.equal(q, out)
+
+
+def test_outputs_over_inputs_are_refused(cuda_device):
+    c = Case([100, 20], [3, 2], 16, seed=48, device=cuda_device)
+    args = c.args()
+    out, lse = c.outs()
+    tree.run(*args, SCALE, out, lse)
+    acc = torch.zeros(2, args[5].shape[1] * 64, device=cuda_device)
+    shifted = torch.empty(6, 16, 512, dtype=torch.bfloat16, device=cuda_device)
+    shifted[:5] = args[0]
+    for q, o, l in ((shifted[:5], shifted[1:], lse), (args[0], args[2].view(-1)[:out.numel()].view(out.shape), lse),
+                    (args[0], out, out.view(torch.float32).view(-1)[:80].view(5, 16)),
+                    (args[0], out, args[0].view(torch.float32).view(-1)[:80].view(5, 16))):
+        with pytest.raises(ValueError, match="share memory"):
+            tree.run(q, *args[1:], SCALE, o, l)
+    big = torch.zeros(2 * acc.numel(), device=cuda_device)
+    for l, o in ((big[:80].view(5, 16), big[64:64 + acc.numel()].view(acc.shape)),
+                 (lse, args[3].view(torch.float32).view(-1)[:acc.numel()].view(acc.shape))):
+        with pytest.raises(ValueError, match="share"):
+            evict.accumulate(*args, SCALE, l, acc, o)
