@@ -5,6 +5,7 @@
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <mutex>
 
 namespace dsa {
 
@@ -80,6 +81,15 @@ int launch_topk_select(const float* scores, const unsigned int* hist, const int3
 // Arms the indexer's test fault (dsa_b200_test_inject with DSA_TEST_SKIP_READY):
 // kind << 56 | wait limit in ns, or 0 to disarm.
 void arm_indexer_test_fault(unsigned long long armed);
+
+// Held over the launches of a call that hand data on through the workspace:
+// threads that call on one stream take turns, so that no other call's launch
+// comes between two of them.  One lock for each of some sets of workspaces
+// (torch puts large ones at multiples of 2 MB).
+inline std::mutex g_turn[16];
+inline std::mutex& turn_of(const void* workspace) {
+  return g_turn[(reinterpret_cast<uintptr_t>(workspace) >> 21) % 16];
+}
 
 // Launches `kernel` on `stream` with programmatic stream serialization, so
 // its CTAs may be scheduled while the previous kernel on the stream drains

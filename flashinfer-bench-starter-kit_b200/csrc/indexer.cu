@@ -1238,6 +1238,7 @@ extern "C" int dsa_indexer_run(const void* q_index_fp8, const void* k_index_cach
   if (st != DSA_OK) return st;
 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const std::lock_guard<std::mutex> turn(turn_of(workspace));
   {
     // Launched normally: it starts after every earlier write to the inputs,
     // so the score kernel (launched programmatically after it) may read them

@@ -658,6 +658,7 @@ extern "C" int dsa_indexer_prefill_run(const void* q_index_fp8, const void* k_in
 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const std::lock_guard<std::mutex> turn(turn_of(workspace));
   if (cudaMemsetAsync(ws + lay.hist, 0, lay.scores - lay.hist, s) != cudaSuccess) return DSA_ERR_CUDA;
 
   const int cap = pf::group_cap(num_rows, num_requests);

@@ -1156,14 +1156,6 @@ combine_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
 std::once_flag g_once[64];
 int g_status[64];
 
-// The attention and its join are two launches that share the workspace's
-// records: threads that call on one stream take turns, so that no other call
-// comes between the two.  One lock for each of some sets of workspaces.
-std::mutex g_turn[16];
-inline std::mutex& turn_of(const void* workspace) {
-  return g_turn[(reinterpret_cast<uintptr_t>(workspace) >> 21) % 16];  // large blocks begin at multiples of 2 MB
-}
-
 struct Layout {
   size_t part_ml, part_o, plan, bytes;
 };
@@ -1323,7 +1315,7 @@ extern "C" int dsa_tree_attention_run(const void* q_nope, const void* q_pe, cons
   prm.out = static_cast<__nv_bfloat16*>(output);
   prm.lse_out = lse;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const std::lock_guard<std::mutex> turn(tree::turn_of(workspace));
+  const std::lock_guard<std::mutex> turn(turn_of(workspace));  // the attention and its join share the records
   if (launch_programmatic(tree::tree_kernel<false>, dim3(info.num_sms), dim3(tree::kThreads), tree::kSmemBytes, s,
                           maps[0], maps[1], maps[2], maps[3], prm) != cudaSuccess)
     return DSA_ERR_CUDA;

@@ -79,3 +79,46 @@ def test_tree_weights_and_eviction(cuda_device):
     new2, seq = torch.zeros(2, 320, device=cuda_device), prefix + 1
     twice(lambda: evict.run(new, seq, bt, fresh, dec.ckv_cache, dec.kpe_cache, None, 4, 32, keep, lens, new2),
           [keep, lens, new2])
+
+
+def test_two_threads_of_indexer_calls_on_one_stream(cuda_device):
+    """A call's launches hand histograms and scores on through the stream's
+    workspace: another thread's must not come between them."""
+    ix = [workloads.make_indexer_inputs(lens, pool_pages=256, seed=84 + k, device=cuda_device)
+          for k, lens in enumerate(([5000, 2500, 70], [3000, 9000, 2049]))]
+    pf = [workloads.make_prefill_inputs([2500 + 300 * k, 40], [4, 2], seed=86 + k, device=cuda_device) for k in range(2)]
+    topk = [[torch.zeros(n, 2048, dtype=torch.int32, device=cuda_device) for _ in range(101)] for n in (3, 3, 6, 6)]
+
+    def decode(k, out):
+        i = ix[k]
+        indexer.run(i.q_index_fp8, i.k_index_cache_fp8, i.weights, i.seq_lens, i.block_table, out)
+
+    def prefill(k, out):
+        p = pf[k]
+        indexer.run_prefill(p.q_index_fp8, p.k_index_cache_fp8, p.weights, p.seq_lens, p.block_table, p.cu_seqlens_q, out)
+
+    for k in range(2):
+        decode(k, topk[k][0])
+        prefill(k, topk[2 + k][0])
+    torch.cuda.synchronize()
+    start, errors = threading.Barrier(2), []
+
+    def calls(k):
+        try:
+            start.wait()
+            for n in range(1, 101):
+                decode(k, topk[k][n])
+                prefill(k, topk[2 + k][n])
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=calls, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert indexer.device_status(cuda_device) == 0
+    for rows in topk:
+        assert all(torch.equal(t, rows[0]) for t in rows[1:])
