@@ -36,10 +36,10 @@
 // no other can be partial) and joined by combine_kernel.
 //
 // Measured, attention with its join, one call a graph replay: 64 x 65536 tokens
-// with 4 drafts of 16 heads 784 us (4.84 GB, 6.2 TB/s: HBM-bound); 4 x 32768
-// with 64 drafts 357 us (0.80 PFLOP/s: the stages' hand-over and shared memory).
-// Back to back for a second the power cap makes those 961 and 429 us.  Weights:
-// 32 x 8192-65536 tokens 153 us (0.93 GB, 6.0 TB/s: HBM-bound).
+// with 4 drafts of 16 heads 798 us (4.84 GB, 6.1 TB/s: HBM-bound); 4 x 32768
+// with 64 drafts 360 us (0.80 PFLOP/s: the stages' hand-over and shared memory).
+// Back to back for a second the power cap makes those 963 and 434 us.  Weights:
+// 32 x 8192-65536 tokens 155 us (0.93 GB, 6.0 TB/s: HBM-bound).
 #include <cuda_bf16.h>
 
 #include <mutex>
