@@ -88,13 +88,15 @@ constexpr int kParts = 4;
 // The tensor core cuts its fp32 accumulator off below the last bit at every
 // step, always towards zero: after 36 steps a logit is about 5e-7 of itself too
 // small, which no sum over rows takes back.  The weights, which have nothing
-// coarser in them, sum each part apart and add the four in registers (TMEM has
-// the room: there is no O).  Weights of logits from 4 to 9 are 5.5e-7 off (rms)
-// then, 2.0e-6 before; 4 x 12000-16384 tokens with 32-40 drafts take 74.5 us
-// for 72.5, long contexts as long as before.  The attention rounds its weights
-// to bf16, beside which this is nothing.
-constexpr int kSumsS = 4;
-static_assert(kSumsS == kParts, "a sum for each part");
+// coarser in them, keep kSumsS sums of kSumSteps steps and add them in
+// registers (TMEM has the room: there is no O).  Weights of logits from 4 to 9
+// are 6.9e-7 off (rms) with three sums, 2.0e-6 with one, 1.0e-6 with two and
+// 5.5e-7 with four; 4 x 12000-16384 tokens with 32-40 drafts take 70.2, 68.0,
+// 70.1 and 75.7 us.  Long contexts take the same with any.  The attention rounds
+// its weights to bf16, beside which this is nothing.
+constexpr int kSumsS = 3;
+constexpr int kSumSteps = (kCkv + kKpe) / 16 / kSumsS;
+static_assert(kSumsS * kSumSteps * 16 == kCkv + kKpe, "equal sums");
 __device__ __forceinline__ constexpr uint32_t part_bytes(int x) {
   return (x == kParts - 1 ? 3 : 2) * kChunkBytes;
 }
@@ -587,7 +589,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
               // +8192 bytes per 64 columns, +32 per K16 step (>> 4)
               const uint32_t at = (k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2;
               if (kWeights)
-                umma_bf16(d + 64u * x, a + at, q_desc + at, idesc, k > 8 * x ? 1u : 0u);
+                umma_bf16(d + 64u * (k / kSumSteps), a + at, q_desc + at, idesc, k % kSumSteps > 0 ? 1u : 0u);
               else
                 umma_bf16(d, a + at, q_desc + at, idesc, k > 0 ? 1u : 0u);
             }
@@ -695,7 +697,7 @@ tree_kernel(const __grid_constant__ CUtensorMap ckv_map, const __grid_constant__
           ok = ok && mbar_wait(&s_full[st], (i >> 1) & 1, wctx);
           tc_fence_after();
           float v[16];
-          tmem_ld_16x32_sum4_wait(tmem_base + lane_base + kColS + 64u * kSumsS * st + 32u * set, v);
+          tmem_ld_16x32_sum3_wait(tmem_base + lane_base + kColS + 64u * kSumsS * st + 32u * set, v);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[st]);

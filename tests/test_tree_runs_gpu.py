@@ -210,10 +210,9 @@ def test_more_than_64_drafts(cuda_device, prefixes, drafts, heads):
 def test_logits_of_the_weights_are_not_shrunk(cuda_device):
     """The tensor core truncates its accumulator at each step of 16 products, by
     half a unit in the last place on average, at most 2^-24 of the partial sum.
-    Partial sums grow towards the logit in proportion to their steps, so that a
-    sum over parts of 8, 8, 8 and 12 steps shrinks it by at most
-    (3 * 8/36 * 4.5 + 12/36 * 6.5) 2^-24 = 3.1e-7 of itself (one of 36 steps:
-    at most 1.1e-6, 4.7e-7 as measured)."""
+    Partial sums grow towards the logit in proportion to their steps, so that
+    three sums of 12 steps shrink it by at most 6.5 * 2^-24 = 3.9e-7 of itself
+    (one of 36 steps: at most 1.1e-6, 4.7e-7 as measured)."""
     n = 40_000
     c = Pooled([n], [1], 1, 10, cuda_device, variants=1)
     acc = torch.zeros(1, c.table.shape[1] * 64, device=cuda_device)
@@ -221,4 +220,4 @@ def test_logits_of_the_weights_are_not_shrunk(cuda_device):
     k = torch.cat([c.ckv, c.kpe], -1)[c.table[0].long()].reshape(-1, 576)[:n].double()
     x = k @ torch.cat([c.q_nope, c.q_pe], -1).reshape(576).double() * (SCALE * otree.LOG2E)
     shrunk = -((out.log2() - x) * x).sum() / x.square().sum()  # the error's part along x
-    assert abs(float(shrunk)) <= (3 * 8 / 36 * 4.5 + 12 / 36 * 6.5) * 2.0 ** -24, float(shrunk)
+    assert abs(float(shrunk)) <= 6.5 * 2.0 ** -24, float(shrunk)
