@@ -15,8 +15,8 @@ its own bit set is plain dense decoding.
 Unlike ``dsa_b200.attention.run``, which reads 2048 selected slots, this reads
 every visible token.  The two are the same function where a draft sees at most
 2048 tokens (the indexer then selects them all); beyond, a model that decodes
-with the indexer's selection gets another distribution from dense rows, and its
-own drafts are verified by ``indexer.run_prefill`` and ``attention.run``.
+with the indexer's selection gets another distribution from dense rows, and a
+chain of its drafts is verified by ``indexer.run_prefill`` and ``attention.run``.
 ``lse`` is the base-2 log-sum-exp of the scaled logits; a row that sees nothing
 yields output 0 and lse -inf.
 
