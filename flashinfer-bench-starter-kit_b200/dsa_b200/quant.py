@@ -1,0 +1,185 @@
+"""The paged latent cache in 8 bits (destination-passing style): written with
+the latent's norm and the position part's rotation in one pass, read back as
+bf16 rows.
+
+    write(kv, slot_mapping, latent_cache, norm_weight=None, eps=1e-6,
+          positions=None, cos_sin=None, interleaved=False) -> None
+    read(latent_cache, block_table, starts, cu_rows, ckv, kpe) -> None
+
+``latent_cache`` takes the place of the bf16 ``ckv`` / ``kpe`` caches that
+``dsa_b200.attention`` and ``dsa_b200.tree`` read, at 644 bytes a token for 1152:
+pages of 41216 bytes (``PAGE_BYTES``; a contiguous 1-byte tensor of any shape)
+hold 64 x 512 float8_e4m3fn codes, 64 x 64 bf16 of the position part and 64
+float32 scales, one for each token, whose latent is code * scale.  Slots and
+block tables are those of the other caches.
+
+``write`` takes rows ``[N, 576]`` as a projection gives them (rows may be
+strided): the first 512 values c become
+    codes e4m3(448 t / max|t|) of t = c * norm_weight, and the scale
+    max|t| / 448 / sqrt(mean(c^2) + eps),
+the last 64 are rotated by their position's 32 angles (``cos_sin``: [positions,
+64] float32, cosines then sines; pairs (i, i + 32), or (2 i, 2 i + 1) with
+``interleaved``) and rounded to bf16.  Without ``norm_weight`` the latent is
+stored as given, without ``cos_sin`` the position part.  Negative slots are
+padding and skipped; a slot beyond the cache or a position beyond the table
+sets a status bit, and the token is not written.  A slot given twice in a call
+holds either of its tokens, or parts of both.  A latent with an infinity or NaN
+is stored as NaN throughout; one whose scale would be below 2^-126 as zeros.
+
+``read`` makes row ``cu_rows[r] + i`` of ``ckv`` [T, 512] and ``kpe`` [T, 64]
+(bf16, rows may be strided, such as the two parts of one [T, 576] buffer) the
+token at position ``starts[r] + i`` of request r.  Rows outside of
+``[cu_rows[0], cu_rows[-1])`` are left as they are; a row whose position or page
+does not exist is zeros and sets a status bit.
+
+Launches go to the current stream and can be captured into a CUDA graph (make
+one call on the capturing stream first).  ``device_status`` reads the sticky
+status bits; with ``DSA_B200_CHECK=1`` each call synchronises and raises.
+"""
+
+from __future__ import annotations
+
+import os
+
+import torch
+
+from . import _native, workspace
+from .tree import check_device, int32_of, read_status
+
+PAGE_SIZE = 64
+DIM_CKV = 512
+DIM_KPE = 64
+PAGE_BYTES = PAGE_SIZE * (DIM_CKV + 2 * DIM_KPE + 4)
+
+_CHECK = os.environ.get("DSA_B200_CHECK", "0") not in ("", "0")
+
+
+def _fail_write(msg: str) -> None:
+    raise ValueError(f"dsa_quant.write: {msg}")
+
+
+def _fail_read(msg: str) -> None:
+    raise ValueError(f"dsa_quant.read: {msg}")
+
+
+def _pages(fail, latent_cache: torch.Tensor) -> int:
+    nbytes = latent_cache.numel()
+    if latent_cache.element_size() != 1 or not latent_cache.is_contiguous() or nbytes % PAGE_BYTES or nbytes == 0:
+        fail(f"latent_cache must be a contiguous 1-byte tensor of pages of {PAGE_BYTES} bytes, at least one")
+    if latent_cache.data_ptr() & 15:
+        fail("latent_cache must be 16-byte aligned")
+    return nbytes // PAGE_BYTES
+
+
+def _rows(fail, name: str, t: torch.Tensor, rows, width: int) -> int:
+    """Bytes from row to row of a bf16 [rows, width] tensor."""
+    shape = t.shape
+    if t.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
+        fail(f"{name} must be bfloat16 [{'N' if rows is None else rows}, {width}], got {t.dtype} {tuple(shape)}")
+    pitch, step = t.stride()
+    if shape[0] <= 1:
+        pitch = width
+    if (step != 1 and width > 1) or pitch < width or pitch & 7 or t.data_ptr() & 15:
+        fail(f"{name} must have contiguous rows, 16-byte aligned (strides {t.stride()})")
+    return 2 * pitch
+
+
+def _int64_of(fail, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    if t.shape != (n,) or t.dtype not in (torch.int64, torch.int32):
+        fail(f"{name} must be int64 or int32 [{n}]")
+    if t.dtype is not torch.int64:
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _finish(status: int, entry: str, fail, dev: torch.device) -> None:
+    if status:
+        if status == _native.DSA_ERR_OVERLAP:
+            fail("what is written must share memory neither with an input nor with another output")
+        _native.check(status, entry)
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        raise_on_device_status(dev)
+
+
+def write(kv: torch.Tensor, slot_mapping: torch.Tensor, latent_cache: torch.Tensor, norm_weight: torch.Tensor = None,
+          eps: float = 1e-6, positions: torch.Tensor = None, cos_sin: torch.Tensor = None,
+          interleaved: bool = False) -> None:
+    at = kv.get_device()
+    if at < 0 or slot_mapping.get_device() != at or latent_cache.get_device() != at or \
+            any(t is not None and t.get_device() != at for t in (norm_weight, positions, cos_sin)):
+        check_device(_fail_write, kv=kv, slot_mapping=slot_mapping, latent_cache=latent_cache, norm_weight=norm_weight,
+                     positions=positions, cos_sin=cos_sin)
+    pitch = _rows(_fail_write, "kv", kv, None, DIM_CKV + DIM_KPE)
+    n = kv.shape[0]
+    slots = _int64_of(_fail_write, "slot_mapping", slot_mapping, n)
+    pages = _pages(_fail_write, latent_cache)
+    norm = 0
+    if norm_weight is not None:
+        if norm_weight.dtype is not torch.bfloat16 or norm_weight.shape != (DIM_CKV,) or not norm_weight.is_contiguous() or \
+                norm_weight.data_ptr() & 15:
+            _fail_write(f"norm_weight must be contiguous bfloat16 [{DIM_CKV}], 16-byte aligned")
+        norm = norm_weight.data_ptr()
+    if (positions is None) != (cos_sin is None):
+        _fail_write("positions and cos_sin come together")
+    pos, angles, most = None, 0, 0
+    if positions is not None:
+        pos = _int64_of(_fail_write, "positions", positions, n)
+        if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != DIM_KPE or cos_sin.shape[0] < 1 or \
+                not cos_sin.is_contiguous() or cos_sin.data_ptr() & 7:
+            _fail_write(f"cos_sin must be contiguous float32 [positions, {DIM_KPE}]")
+        angles, most = cos_sin.data_ptr(), cos_sin.shape[0]
+    if n >= 1 << 31:
+        _fail_write(f"{n} tokens are more than one call takes")
+    if n == 0:
+        return
+    dev = kv.device
+    cur = _native.current_stream(dev)
+    ws = workspace.get(dev, "quant_rows", _native.WORKSPACE_HEADER, cur)
+    st = _native.call_on(dev, _native.lib().dsa_latent_cache_write, kv.data_ptr(), pitch, slots.data_ptr(), n, norm,
+                         float(eps), pos.data_ptr() if pos is not None else 0, angles, most, int(bool(interleaved)),
+                         latent_cache.data_ptr(), pages, ws.data_ptr(), cur)
+    _finish(st, "dsa_latent_cache_write", _fail_write, dev)
+
+
+def read(latent_cache: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, cu_rows: torch.Tensor,
+         ckv: torch.Tensor, kpe: torch.Tensor) -> None:
+    at = latent_cache.get_device()
+    if at < 0 or block_table.get_device() != at or starts.get_device() != at or cu_rows.get_device() != at or \
+            ckv.get_device() != at or kpe.get_device() != at:
+        check_device(_fail_read, latent_cache=latent_cache, block_table=block_table, starts=starts, cu_rows=cu_rows,
+                     ckv=ckv, kpe=kpe)
+    pages = _pages(_fail_read, latent_cache)
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        _fail_read("block_table must be [B, max_pages]")
+    B, max_pages = shape
+    if starts.shape != (B,) or cu_rows.shape != (B + 1,):
+        _fail_read(f"starts must be [{B}] and cu_rows [{B + 1}]")
+    ckv_pitch = _rows(_fail_read, "ckv", ckv, None, DIM_CKV)
+    T = ckv.shape[0]
+    kpe_pitch = _rows(_fail_read, "kpe", kpe, T, DIM_KPE)
+    bt, st, cu = (int32_of(name, t, _fail_read) for name, t in
+                  (("block_table", block_table), ("starts", starts), ("cu_rows", cu_rows)))
+    if T >= 1 << 31:
+        _fail_read(f"{T} rows are more than one call takes")
+    if T == 0 or B == 0:
+        return
+    dev = latent_cache.device
+    cur = _native.current_stream(dev)
+    ws = workspace.get(dev, "quant_rows", _native.WORKSPACE_HEADER, cur)
+    status = _native.call_on(dev, _native.lib().dsa_latent_cache_read, latent_cache.data_ptr(), pages, bt.data_ptr(),
+                             st.data_ptr(), cu.data_ptr(), B, max_pages, T, ckv.data_ptr(), ckv_pitch, kpe.data_ptr(),
+                             kpe_pitch, ws.data_ptr(), cur)
+    _finish(status, "dsa_latent_cache_read", _fail_read, dev)
+
+
+def device_status(device: torch.device, clear: bool = True) -> int:
+    """OR of the sticky status bits of every workspace of these operators on
+    `device` (synchronises)."""
+    return read_status(device, "quant_rows", clear) | read_status(device, "quant", clear)
+
+
+def raise_on_device_status(device: torch.device) -> None:
+    bits = device_status(device, clear=True)
+    if bits:
+        raise _native.DsaError(f"dsa_quant: {_native.describe_device_status(bits)} (status bits {bits:#x})")

@@ -77,6 +77,9 @@ extern "C" {
 #define DSA_ATTN_HEADS       16
 #define DSA_CKV_DIM          512
 #define DSA_KPE_DIM          64
+/* A page of the 8-bit latent cache: 64 x 512 e4m3 codes (ckv), then 64 x 64 bf16
+ * (kpe), then 64 fp32 scales, one for each token: a latent is code * scale. */
+#define DSA_LATENT_PAGE_BYTES 41216
 
 /* Version of this ABI (bumped on any signature change). */
 DSA_API int dsa_b200_abi_version(void);
@@ -359,6 +362,57 @@ DSA_API int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const int3
                                 int32_t num_sink, int32_t num_recent, int32_t* keep,
                                 int32_t* new_seq_lens, float* new_acc, int64_t new_acc_stride,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Writes new tokens into the paged latent cache in 8 bits, with the latent's norm
+ * and the rotation of the position part in the same pass.  With c the first 512
+ * and e the last 64 values of a token's row:
+ *   t = c * norm_weight,  r = 1 / sqrt(mean(c^2) + eps),  M = max |t|
+ *   codes = e4m3(448 t / M) to nearest even,  scale = r M / 448
+ *   e: (a, b) -> (a cos - b sin, b cos + a sin) for its 32 pairs
+ *
+ *   kv             num_tokens rows of 576 bf16, kv_row_bytes apart (a multiple of
+ *                  16, the base 16-byte aligned)
+ *   slot_mapping   [num_tokens] int64 global slot ids (page * 64 + token);
+ *                  negative: padding, skipped.  What a slot holds that is given
+ *                  twice in one call is not defined.
+ *   norm_weight    [512] bf16, 16-byte aligned; NULL: no norm (t = c, r = 1)
+ *   positions      [num_tokens] int64, with cos_sin [max_positions, 64] fp32: 32
+ *                  cosines, then 32 sines of a position's angles; both NULL: no
+ *                  rotation
+ *   interleaved    non-zero: the pairs are (2 i, 2 i + 1); zero: (i, i + 32)
+ *   latent_cache   num_pages pages of DSA_LATENT_PAGE_BYTES, 16-byte aligned
+ *   status         optional device word (NULL: none): DSA_DEV_BAD_INDEX is OR-ed
+ *                  in for a slot >= num_pages * 64 or a position outside of the
+ *                  table; such a token is not written
+ *
+ * A row with an infinity or NaN in its latent is stored as NaN throughout, one
+ * whose scale would be below 2^-126 as zeros.  A cache that shares memory with an
+ * input: DSA_ERR_OVERLAP. */
+DSA_API int dsa_latent_cache_write(const void* kv, int64_t kv_row_bytes, const int64_t* slot_mapping,
+                                   int32_t num_tokens, const void* norm_weight, float eps,
+                                   const int64_t* positions, const float* cos_sin, int64_t max_positions,
+                                   int32_t interleaved, void* latent_cache, int64_t num_pages,
+                                   uint32_t* status, void* stream);
+
+/* Reads ranges of cached tokens back: row cu_rows[r] + i becomes the token at
+ * position starts[r] + i of request r, ckv as bf16(code * scale), kpe as it is.
+ *
+ *   block_table    [num_requests, max_pages] int32
+ *   starts         [num_requests] int32
+ *   cu_rows        [num_requests + 1] int32, ascending; rows outside of
+ *                  [cu_rows[0], cu_rows[num_requests]) are left as they are
+ *   ckv, kpe       num_rows rows of 512 and 64 bf16, 16-byte aligned and
+ *                  multiples of 16 bytes apart (they may be columns of one buffer)
+ *   status         device word: DSA_DEV_BAD_SEQ_LEN for a position outside of the
+ *                  table, DSA_DEV_BAD_PAGE for a page outside of the pool; such a
+ *                  row is written as zeros
+ *
+ * Outputs that share memory with anything else: DSA_ERR_OVERLAP. */
+DSA_API int dsa_latent_cache_read(const void* latent_cache, int64_t num_pages,
+                                  const int32_t* block_table, const int32_t* starts,
+                                  const int32_t* cu_rows, int32_t num_requests, int32_t max_pages,
+                                  int32_t num_rows, void* ckv, int64_t ckv_row_bytes, void* kpe,
+                                  int64_t kpe_row_bytes, uint32_t* status, void* stream);
 
 /* Copies the sticky device status word of `workspace` to *status_out
  * (synchronising `stream`), and zeroes it when `clear` is non-zero.

@@ -1,0 +1,80 @@
+"""The latent cache in 8 bits, in 64 bits and byte by byte from the layout of a
+page (TEST INFRASTRUCTURE ONLY): written, read, and attention over it.
+
+A page of 64 tokens is 41216 bytes: 64 x 512 e4m3 codes, 64 x 64 bf16, 64 fp32
+scales.  ``write`` gives the codes that exact arithmetic gives (the quotients are
+of integers of at most 19 and 16 bits, so float64 rounds none of them across a
+border of e4m3) and scales and rotated values in 64 bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+PAGE, CKV, KPE = 64, 512, 64
+PAGE_BYTES = 41216
+LOG2E = 1.4426950408889634
+
+
+def pieces(cache: torch.Tensor):
+    """Codes [pages, 64, 512] (uint8), kpe [pages, 64, 64] (bf16), scales [pages, 64]: views of a uint8 cache."""
+    flat = cache.view(torch.uint8).reshape(-1, PAGE_BYTES)
+    return (flat[:, :PAGE * CKV].unflatten(1, (PAGE, CKV)),
+            flat[:, PAGE * CKV:PAGE * (CKV + 2 * KPE)].view(torch.bfloat16).unflatten(1, (PAGE, KPE)),
+            flat[:, PAGE * (CKV + 2 * KPE):].view(torch.float32))
+
+
+def e4m3(x: torch.Tensor) -> torch.Tensor:
+    """Bytes of float64 values rounded to nearest even (|x| <= 448; NaN is 0x7F), by their definition."""
+    a = x.abs()
+    e = torch.floor(torch.log2(torch.where(a > 0, a, 2.0 ** -6))).clamp(min=-6)
+    for _ in range(2):  # log2 may be off by one step at a power of two
+        e = torch.where(a < 2.0 ** e, e - 1, torch.where(a >= 2.0 ** (e + 1), e + 1, e)).clamp(min=-6)
+    steps = torch.round(a / 2.0 ** (e - 3))  # torch rounds halves to even
+    code = ((e + 6) * 8 + steps).to(torch.int64)  # the implicit bit is the 8 of the steps; a carry moves the exponent
+    code = torch.where(torch.isnan(x), 0x7F, torch.where(torch.signbit(x), code | 0x80, code))
+    return code.to(torch.uint8)
+
+
+def value(code: torch.Tensor) -> torch.Tensor:
+    """float64 values of e4m3 bytes."""
+    c = code.to(torch.int64)
+    e, m = (c >> 3) & 15, c & 7
+    v = torch.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e.double() - 10))
+    v = torch.where((c & 0x7F) == 0x7F, math.nan, v)
+    return torch.where(c >= 128, -v, v)
+
+
+def write_rows(kv, norm=None, eps=1e-6, positions=None, cos_sin=None, interleaved=False):
+    """(codes uint8 [N, 512], scales, kpe), scales and kpe in float64 unrounded, of bf16 rows [N, 576]."""
+    c, e = kv[:, :CKV].double(), kv[:, CKV:].double()
+    t = c if norm is None else c * norm.double()
+    r = torch.ones(len(kv), dtype=torch.float64) if norm is None else 1 / torch.sqrt((c * c).mean(1) + eps)
+    top = t.abs().amax(1)
+    scale = top * r / 448
+    small = ~(scale >= 2.0 ** -126)
+    broken = ~torch.isfinite(t).all(1)
+    code = e4m3(448 * t / torch.where(small | broken, 1.0, top)[:, None].clamp(min=1e-300))
+    code[small] = 0
+    code[broken] = 0x7F
+    scale = torch.where(small | broken, 1.0, scale)
+    if positions is not None:
+        cos, sin = cos_sin[positions].double().chunk(2, 1)
+        a, b = (e[:, 0::2], e[:, 1::2]) if interleaved else e.chunk(2, 1)
+        x, y = a * cos - b * sin, b * cos + a * sin
+        e = torch.stack([x, y], 2).flatten(1) if interleaved else torch.cat([x, y], 1)
+    return code, scale, e
+
+
+def rows(cache: torch.Tensor, slot: torch.Tensor):
+    """(latents, position parts) of slots, float64."""
+    codes, kpe, scales = pieces(cache)
+    p, t = slot // PAGE, slot % PAGE
+    return value(codes[p, t]) * scales[p, t].double()[:, None], kpe[p, t].double()
+
+
+def bf16(x: torch.Tensor) -> torch.Tensor:
+    """A float64 tensor that float32 holds exactly, or nearly: rounded through it to bf16."""
+    return x.float().bfloat16()
