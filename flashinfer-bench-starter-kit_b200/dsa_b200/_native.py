@@ -62,6 +62,8 @@ SIGNATURES = {
                                               ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int64, _P, _P]),
     "dsa_latent_cache_read": (ctypes.c_int, [_P, ctypes.c_int64, _P, _P, _P, ctypes.c_int32, ctypes.c_int32,
                                              ctypes.c_int32, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P]),
+    "dsa_verify_run": (ctypes.c_int, [_P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P, _P, _P, _P, ctypes.c_int32,
+                                      ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P, _P]),
     "dsa_b200_test_inject": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
 }
 

@@ -414,6 +414,44 @@ DSA_API int dsa_latent_cache_read(const void* latent_cache, int64_t num_pages,
                                   int32_t num_rows, void* ckv, int64_t ckv_row_bytes, void* kpe,
                                   int64_t kpe_row_bytes, uint32_t* status, void* stream);
 
+/* Verifies drafted tokens against the target's probabilities, from given random
+ * numbers, and draws the token that follows.  Request r has the rows
+ * cu_drafts[r] .. cu_drafts[r+1]-1: its last certain token, then drafts, a tree by
+ * their parents.  From row 0 on, the children of a row are looked at in their
+ * order; child x is accepted with probability min(1, p'(x) / q(x)), p' being the
+ * target's distribution after the row, from which each rejection takes q away:
+ *   c = 0, R = 1;  accepted: u q(x) R < max(p(x) - c q(x), 0)
+ *   rejected:      c += R, R = sum max(p - c q, 0)
+ * The walk goes on at an accepted row.  Where it ends, the next token is the first
+ * whose running sum of max(p - c q, 0) exceeds sample_u of the whole (of p, if the
+ * whole is 0; -1 if that is 0 or NaN too).  All in 64 bits.
+ *
+ *   target_probs   num_rows rows of vocab fp32, target_stride values apart: the
+ *                  target's distribution after each row
+ *   draft_probs    likewise: what the children of each row were drawn from; NULL:
+ *                  q is 1 at the drafted token, a rejected x is struck out of p
+ *   draft_tokens   [num_rows] int32 (row 0's is not read)
+ *   parents        [num_rows] int32, in the request; below the row's own place
+ *   cu_drafts      [num_requests + 1] int32
+ *   accept_u       [num_rows] fp32, sample_u [num_requests] fp32, in [0, 1)
+ *   path           [num_requests, path_width] int32: the accepted rows' places in
+ *                  the request, then -1; the walk ends when it is full
+ *   num_accepted   [num_requests] int32
+ *   next_token     [num_requests] int32
+ *   status         device word: DSA_DEV_BAD_SEQ_LEN for cu_drafts that do not fit (the
+ *                  request is taken as empty) and requests of over 4096 rows (cut
+ *                  off there), DSA_DEV_BAD_INDEX for tokens outside of the vocabulary
+ *                  (never accepted)
+ *
+ * num_rows <= 2^24, num_requests <= 65536, vocab <= 2^28, path_width <= 65536.
+ * Outputs that share memory with anything else: DSA_ERR_OVERLAP. */
+DSA_API int dsa_verify_run(const float* target_probs, int64_t target_stride, const float* draft_probs,
+                           int64_t draft_stride, const int32_t* draft_tokens, const int32_t* parents,
+                           const int32_t* cu_drafts, const float* accept_u, const float* sample_u,
+                           int32_t num_requests, int32_t num_rows, int32_t vocab, int32_t path_width,
+                           int32_t* path, int32_t* num_accepted, int32_t* next_token,
+                           uint32_t* status, void* stream);
+
 /* Copies the sticky device status word of `workspace` to *status_out
  * (synchronising `stream`), and zeroes it when `clear` is non-zero.
  * No counterpart in the reference, which has no error channel
