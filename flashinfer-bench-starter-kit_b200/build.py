@@ -19,7 +19,7 @@ REPO = ROOT.parent
 CSRC = ROOT / "csrc"
 OUT = ROOT / "dsa_b200" / "libdsa_b200.so"
 SOURCES = ["capi.cu", "indexer.cu", "attention.cu", "noalloc.cu", "cache_write.cu", "prefill.cu",
-           "tree.cu", "evict.cu", "quant.cu", "verify.cu"]
+           "tree.cu", "evict.cu", "quant.cu", "quant_attention.cu", "verify.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

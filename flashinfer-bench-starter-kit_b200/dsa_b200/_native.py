@@ -62,6 +62,12 @@ SIGNATURES = {
                                               ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int64, _P, _P]),
     "dsa_latent_cache_read": (ctypes.c_int, [_P, ctypes.c_int64, _P, _P, _P, ctypes.c_int32, ctypes.c_int32,
                                              ctypes.c_int32, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P]),
+    "dsa_latent_attention_workspace_bytes": (ctypes.c_size_t, []),
+    "dsa_latent_attention_run": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _P, _P, _P, ctypes.c_int32, ctypes.c_int32,
+                                                ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _P, ctypes.c_size_t,
+                                                _P]),
+    "dsa_latent_sparse_attention_run": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _P, ctypes.c_int32, ctypes.c_int32,
+                                                       ctypes.c_int32, ctypes.c_float, _P, _P, _P, ctypes.c_size_t, _P]),
     "dsa_verify_run": (ctypes.c_int, [_P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P, _P, _P, _P, ctypes.c_int32,
                                       ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P, _P]),
     "dsa_b200_test_inject": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),

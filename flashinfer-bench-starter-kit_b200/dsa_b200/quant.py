@@ -1,10 +1,14 @@
 """The paged latent cache in 8 bits (destination-passing style): written with
 the latent's norm and the position part's rotation in one pass, read back as
-bf16 rows.
+bf16 rows, and attended to.
 
     write(kv, slot_mapping, latent_cache, norm_weight=None, eps=1e-6,
           positions=None, cos_sin=None, interleaved=False) -> None
     read(latent_cache, block_table, starts, cu_rows, ckv, kpe) -> None
+    attend(q_nope, q_pe, latent_cache, seq_lens, block_table, cu_rows, sm_scale,
+           output, lse) -> None
+    attend_sparse(q_nope, q_pe, latent_cache, sparse_indices, sm_scale, output,
+                  lse) -> None
 
 ``latent_cache`` takes the place of the bf16 ``ckv`` / ``kpe`` caches that
 ``dsa_b200.attention`` and ``dsa_b200.tree`` read, at 644 bytes a token for 1152:
@@ -32,6 +36,21 @@ token at position ``starts[r] + i`` of request r.  Rows outside of
 ``[cu_rows[0], cu_rows[-1])`` are left as they are; a row whose position or page
 does not exist is zeros and sets a status bit.
 
+``attend`` reads everything a request has cached, as ``dsa_b200.tree.run`` does
+of the bf16 caches: with ``cu_rows`` None one row per request (plain decoding);
+else request r has the rows ``cu_rows[r] .. cu_rows[r+1]-1`` of ``q_nope`` / ``q_pe``,
+its last tokens (a chain of drafts, written to the cache before), and row j of n
+sees the first ``seq_lens[r] - n + 1 + j`` tokens.  ``attend_sparse`` reads the slots
+of ``sparse_indices`` [T, K] (-1: none), as ``dsa_b200.attention.run`` does.  Both take
+1 to 128 heads; ``lse`` is the base-2 log-sum-exp of the scaled logits; a row that
+sees nothing yields output 0 and lse -inf.  Tokens that no row sees may hold
+anything; a visible one with NaN makes the output NaN.  ``output`` may be ``q_nope``
+itself; other outputs over an input are refused.  Queries are used as they are
+(their products with the codes are exact), softmax weights to 2^-9 of each.
+
+Calls that overlap need different streams; threads may call on one stream.  A
+captured graph uses the workspace of the stream that it was captured on: it must
+not run beside another one captured there, nor beside calls on that stream.
 Launches go to the current stream and can be captured into a CUDA graph (make
 one call on the capturing stream first).  ``device_status`` reads the sticky
 status bits; with ``DSA_B200_CHECK=1`` each call synchronises and raises.
@@ -49,9 +68,11 @@ from .tree import check_device, int32_of, read_status
 PAGE_SIZE = 64
 DIM_CKV = 512
 DIM_KPE = 64
+MAX_HEADS = 128
 PAGE_BYTES = PAGE_SIZE * (DIM_CKV + 2 * DIM_KPE + 4)
 
 _CHECK = os.environ.get("DSA_B200_CHECK", "0") not in ("", "0")
+_ws_bytes: dict = {}  # device index -> dsa_latent_attention_workspace_bytes
 
 
 def _fail_write(msg: str) -> None:
@@ -60,6 +81,14 @@ def _fail_write(msg: str) -> None:
 
 def _fail_read(msg: str) -> None:
     raise ValueError(f"dsa_quant.read: {msg}")
+
+
+def _fail_attend(msg: str) -> None:
+    raise ValueError(f"dsa_quant.attend: {msg}")
+
+
+def _fail_sparse(msg: str) -> None:
+    raise ValueError(f"dsa_quant.attend_sparse: {msg}")
 
 
 def _pages(fail, latent_cache: torch.Tensor) -> int:
@@ -171,6 +200,95 @@ def read(latent_cache: torch.Tensor, block_table: torch.Tensor, starts: torch.Te
                              st.data_ptr(), cu.data_ptr(), B, max_pages, T, ckv.data_ptr(), ckv_pitch, kpe.data_ptr(),
                              kpe_pitch, ws.data_ptr(), cur)
     _finish(status, "dsa_latent_cache_read", _fail_read, dev)
+
+
+def _queries(fail, q_nope, q_pe, output, lse) -> tuple:
+    shape = q_nope.shape
+    if len(shape) != 3 or shape[2] != DIM_CKV or not 1 <= shape[1] <= MAX_HEADS:
+        fail(f"q_nope must be [T, heads <= {MAX_HEADS}, {DIM_CKV}], got {tuple(shape)}")
+    T, H, _ = shape
+    if q_pe.shape != (T, H, DIM_KPE):
+        fail(f"q_pe must be [{T}, {H}, {DIM_KPE}]")
+    if q_nope.dtype is not torch.bfloat16 or q_pe.dtype is not torch.bfloat16:
+        fail(f"q_nope and q_pe must be bfloat16, got {q_nope.dtype} and {q_pe.dtype}")
+    if output.dtype is not torch.bfloat16 or output.shape != shape or not output.is_contiguous():
+        fail(f"output must be contiguous bfloat16 [{T}, {H}, {DIM_CKV}]")
+    if lse.dtype is not torch.float32 or lse.shape != (T, H) or not lse.is_contiguous():
+        fail(f"lse must be contiguous float32 [{T}, {H}]")
+    if T * H > 1 << 24:
+        fail(f"{T} rows of {H} heads are more than one call takes")
+    return T, H, q_nope if q_nope.is_contiguous() else q_nope.contiguous(), q_pe if q_pe.is_contiguous() else q_pe.contiguous()
+
+
+def _workspace(dev: torch.device, cur: int) -> torch.Tensor:
+    n = _ws_bytes.get(dev.index)
+    if n is None:
+        n = _ws_bytes[dev.index] = _native.call_on(dev, _native.lib().dsa_latent_attention_workspace_bytes)
+    return workspace.get(dev, "quant", n, cur)
+
+
+def attend(q_nope: torch.Tensor, q_pe: torch.Tensor, latent_cache: torch.Tensor, seq_lens: torch.Tensor,
+           block_table: torch.Tensor, cu_rows, sm_scale, output: torch.Tensor, lse: torch.Tensor) -> None:
+    at = q_nope.get_device()
+    if at < 0 or q_pe.get_device() != at or latent_cache.get_device() != at or seq_lens.get_device() != at or \
+            block_table.get_device() != at or (cu_rows is not None and cu_rows.get_device() != at) or \
+            output.get_device() != at or lse.get_device() != at:
+        check_device(_fail_attend, q_nope=q_nope, q_pe=q_pe, latent_cache=latent_cache, seq_lens=seq_lens,
+                     block_table=block_table, cu_rows=cu_rows, output=output, lse=lse)
+    T, H, qn, qp = _queries(_fail_attend, q_nope, q_pe, output, lse)
+    pages = _pages(_fail_attend, latent_cache)
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        _fail_attend("block_table must be [B, max_pages]")
+    B, max_pages = shape
+    if seq_lens.shape != (B,):
+        _fail_attend(f"seq_lens must be int32 [{B}]")
+    if cu_rows is None:
+        if T != B:
+            _fail_attend(f"without cu_rows there is one row for each of the {B} requests, not {T}")
+    elif cu_rows.shape != (B + 1,):
+        _fail_attend(f"cu_rows must be int32 [{B + 1}] (one more than block_table rows)")
+    if B > 65536 or (T * H // 16 + B) * (max_pages // 2 + 3) > 1 << 30:
+        _fail_attend(f"{T} rows of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
+    bt, sl = int32_of("block_table", block_table, _fail_attend), int32_of("seq_lens", seq_lens, _fail_attend)
+    cu = int32_of("cu_rows", cu_rows, _fail_attend) if cu_rows is not None else None
+    sm_scale = float(sm_scale)
+    if T == 0 or B == 0:
+        return
+    dev = q_nope.device
+    cur = _native.current_stream(dev)
+    ws = _workspace(dev, cur)
+    st = _native.call_on(dev, _native.lib().dsa_latent_attention_run, qn.data_ptr(), qp.data_ptr(), latent_cache.data_ptr(),
+                         pages, sl.data_ptr(), bt.data_ptr(), cu.data_ptr() if cu is not None else 0, B, T, H, max_pages,
+                         sm_scale, output.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), cur)
+    _finish(st, "dsa_latent_attention_run", _fail_attend, dev)
+
+
+def attend_sparse(q_nope: torch.Tensor, q_pe: torch.Tensor, latent_cache: torch.Tensor, sparse_indices: torch.Tensor,
+                  sm_scale, output: torch.Tensor, lse: torch.Tensor) -> None:
+    at = q_nope.get_device()
+    if at < 0 or q_pe.get_device() != at or latent_cache.get_device() != at or sparse_indices.get_device() != at or \
+            output.get_device() != at or lse.get_device() != at:
+        check_device(_fail_sparse, q_nope=q_nope, q_pe=q_pe, latent_cache=latent_cache, sparse_indices=sparse_indices,
+                     output=output, lse=lse)
+    T, H, qn, qp = _queries(_fail_sparse, q_nope, q_pe, output, lse)
+    pages = _pages(_fail_sparse, latent_cache)
+    shape = sparse_indices.shape
+    if len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= 65536:
+        _fail_sparse(f"sparse_indices must be [{T}, 1 to 65536]")
+    if pages > 0x7FFFFFFF // PAGE_SIZE:
+        _fail_sparse("latent_cache has more slots than an index can name")
+    idx = int32_of("sparse_indices", sparse_indices, _fail_sparse)
+    sm_scale = float(sm_scale)
+    if T == 0:
+        return
+    dev = q_nope.device
+    cur = _native.current_stream(dev)
+    ws = _workspace(dev, cur)
+    st = _native.call_on(dev, _native.lib().dsa_latent_sparse_attention_run, qn.data_ptr(), qp.data_ptr(),
+                         latent_cache.data_ptr(), pages, idx.data_ptr(), T, H, shape[1], sm_scale, output.data_ptr(),
+                         lse.data_ptr(), ws.data_ptr(), ws.numel(), cur)
+    _finish(st, "dsa_latent_sparse_attention_run", _fail_sparse, dev)
 
 
 def device_status(device: torch.device, clear: bool = True) -> int:

@@ -414,6 +414,57 @@ DSA_API int dsa_latent_cache_read(const void* latent_cache, int64_t num_pages,
                                   int32_t num_rows, void* ckv, int64_t ckv_row_bytes, void* kpe,
                                   int64_t kpe_row_bytes, uint32_t* status, void* stream);
 
+/* Bytes of device workspace the two calls below need on this device, the same for
+ * every call: a 256-byte header, two fp32 records of 32 rows per SM (19 MB) and the
+ * call's list of row groups (9 MB).  Zero-fill it once (its status word); nothing
+ * else in it carries over.  Calls that may overlap on the device need a workspace
+ * each; threads may call with one workspace on one stream. */
+DSA_API size_t dsa_latent_attention_workspace_bytes(void);
+
+/* Attention over everything a request has in the latent cache in 8 bits: of single
+ * tokens (decoding), or of the last rows of each request (chains of drafts, whose
+ * own tokens are in the cache), each of which sees the tokens up to its own.
+ *
+ *   q_nope         [num_rows, num_heads, 512] bf16, contiguous
+ *   q_pe           [num_rows, num_heads, 64] bf16, contiguous
+ *   latent_cache   num_pages pages of DSA_LATENT_PAGE_BYTES
+ *   seq_lens       [num_requests] int32: cached tokens, the rows' own among them
+ *   block_table    [num_requests, max_pages] int32
+ *   cu_rows        [num_requests + 1] int32: request r has the rows cu_rows[r] ..
+ *                  cu_rows[r+1]-1; row j of n sees seq_lens[r] - n + 1 + j tokens.
+ *                  Rows outside of [cu_rows[0], cu_rows[num_requests]) are left as
+ *                  they are.  NULL: row r is request r's only one
+ *   output         [num_rows, num_heads, 512] bf16; may be q_nope itself
+ *   lse            [num_rows, num_heads] fp32, base-2 log-sum-exp of the scaled
+ *                  logits; a row that sees nothing has -inf, output 0
+ *
+ * 1 <= num_heads <= 128; num_rows * num_heads <= 2^24, num_requests <= 65536 and
+ * (num_rows * num_heads / 16 + num_requests) * (max_pages / 2 + 3) <= 2^30.  Tokens
+ * that no row sees may hold anything; a visible one with NaN makes the output NaN.
+ * Outputs that share memory with anything else: DSA_ERR_OVERLAP.  Data-dependent
+ * errors: lengths that do not fit the table (clamped), cu_rows that do not fit
+ * (the request is left out; decreasing: the call writes no row): DSA_DEV_BAD_SEQ_LEN;
+ * page ids outside the pool (their tokens are masked): DSA_DEV_BAD_PAGE. */
+DSA_API int dsa_latent_attention_run(const void* q_nope, const void* q_pe, const void* latent_cache,
+                                     int64_t num_pages, const int32_t* seq_lens,
+                                     const int32_t* block_table, const int32_t* cu_rows,
+                                     int32_t num_requests, int32_t num_rows, int32_t num_heads,
+                                     int32_t max_pages, float sm_scale, void* output, float* lse,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over selected slots (as dsa_attention_run, of the cache in 8 bits).
+ *
+ *   sparse_indices [num_rows, topk] int32 slots, -1: none; topk <= 65536.  A slot
+ *                  that is given twice counts twice.
+ *
+ * Indices outside of [-1, num_pages * 64): DSA_DEV_BAD_INDEX, taken as -1. */
+DSA_API int dsa_latent_sparse_attention_run(const void* q_nope, const void* q_pe,
+                                            const void* latent_cache, int64_t num_pages,
+                                            const int32_t* sparse_indices, int32_t num_rows,
+                                            int32_t num_heads, int32_t topk, float sm_scale,
+                                            void* output, float* lse, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+
 /* Verifies drafted tokens against the target's probabilities, from given random
  * numbers, and draws the token that follows.  Request r has the rows
  * cu_drafts[r] .. cu_drafts[r+1]-1: its last certain token, then drafts, a tree by

@@ -78,3 +78,59 @@ def rows(cache: torch.Tensor, slot: torch.Tensor):
 def bf16(x: torch.Tensor) -> torch.Tensor:
     """A float64 tensor that float32 holds exactly, or nearly: rounded through it to bf16."""
     return x.float().bfloat16()
+
+
+def _softmax(q_nope, q_pe, c, e, see, scale):
+    """(output, lse and their bounds) of one row's heads over tokens c, e [n, ...] of which `see` [n] are visible."""
+    H = q_nope.shape[0]
+    c, e = c[see], e[see]
+    if len(c) == 0:
+        z = torch.zeros(H, CKV, dtype=torch.float64)
+        return z, torch.full((H,), -math.inf, dtype=torch.float64), z, torch.zeros(H, dtype=torch.float64)
+    q, r = q_nope.double(), q_pe.double()
+    x = (q @ c.T + r @ e.T) * (scale * LOG2E)
+    off = (q.abs() @ c.abs().T + r.abs() @ e.abs().T) * (600 * 2.0 ** -23 * abs(scale) * LOG2E)
+    lse = torch.logsumexp(x / LOG2E, 1) * LOG2E
+    move = off.amax(1)
+    w = torch.exp2(x - lse[:, None])
+    out = w @ c
+    err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -9 + 2.0 ** -20) * w
+    bound = err @ c.abs() + 2.0 ** -22 * w.amax(1, keepdim=True) * c.abs().sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
+    return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
+
+
+def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
+    """(output, lse, output bound, lse bound), float64; rows of no request are NaN.
+
+    * A logit is a sum of 512 products, scaled, and of 64 more, accumulated in fp32 in an order that is not known, in two
+      parts of the query, with the scale's and the parts' own roundings: off by at most 600 * 2^-23 of the sum of the
+      magnitudes (2^-23, not 2^-24, for accumulators that truncate).
+    * The lse moves by at most the largest of these, the exponential's and the sum's errors (2^-18 is far above both) and
+      one rounding; a weight by ln 2 times its logit's and the lse's error.
+    * A weight is the sum of three parts of 3 bits each, every one to nearest: within 2^-9 of itself, and, where it is far
+      below the largest, within half the smallest step of the parts' type (2^-17 of weights that are scaled to 2^8 or
+      more for the largest one: 2^-25, taken as 2^-22).  The output is rounded to bf16, 2^-8 of itself.
+    """
+    T, H = q_nope.shape[:2]
+    out = torch.full((T, H, CKV), math.nan, dtype=torch.float64)
+    lse = torch.full((T, H), math.nan, dtype=torch.float64)
+    bo, bl = torch.zeros_like(out), torch.zeros_like(lse)
+    for b in range(len(seq_lens)):
+        lo, hi = (b, b + 1) if cu is None else (int(cu[b]), int(cu[b + 1]))
+        L = int(seq_lens[b])
+        pos = torch.arange(L)
+        c, e = rows(cache, table[b].long()[pos // PAGE] * PAGE + pos % PAGE)
+        for i in range(lo, hi):
+            out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, pos < L - (hi - 1 - i), scale)
+    return out, lse, bo, bl
+
+
+def sparse_reference(q_nope, q_pe, cache, picked, scale):
+    """The same for rows of slots, -1: none."""
+    T, H = q_nope.shape[:2]
+    out, lse = torch.zeros(T, H, CKV, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    bo, bl = torch.zeros_like(out), torch.zeros_like(lse)
+    for i in range(T):
+        c, e = rows(cache, picked[i].long().clamp(min=0))
+        out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, picked[i] >= 0, scale)
+    return out, lse, bo, bl
