@@ -6,10 +6,32 @@
 //   x_k = scale * (s_k (q_nope . c_k) + q_pe . e_k)
 //   lse = log2 sum_k 2^(x_k log2 e),   out = sum_k 2^(x_k log2 e - lse) s_k c_k
 //
-// This first form is the plain one: one CTA per query row and 16 heads, a warp
-// per head, tiles of 16 tokens in shared memory, everything in fp32.
+// The codes go to the tensor core as they are: a token's scale is taken out of
+// both products.  For that the other operands have to be 8 bits too, and are, in
+// parts that add up to what they were:
+//   q_nope f = a + b / 16 with a, b e4m3 and f a power of two for each row (its
+//     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
+//     b the other 4: the parts are exact down to 2^-22 of the row's largest.
+//   w = p s (weight by scale) = a + b + c with e5m2 parts, each to nearest: 3 + 3
+//     + 3 bits, within 2^-9 of w, over the range of the type (2^31).  Weights in
+//     bf16, as a bf16 product would take them, are within 2^-8.
+// Per tile of 128 tokens and group of R rows (token, head)
+//   S^T[128, 2R] = C[128, 512] . [a b]^T    16 x (M128 N2R K32, e4m3)
+//   E^T[128, R]  = E[128, 64] . (q_pe f)^T   4 x (M128 NR K16, bf16)
+//   O^T[512, 3R] += C^T[512, 128] . [a b c]^T   4 x 4 x (M128 N3R K32, e4m3 x e5m2)
+// so the parts lie along N, which costs the tensor core nothing up to N = 64: it
+// is fed at 128 bytes of A a clock.  A tile's 82 KB cross shared memory once in,
+// and once and a half out, against three and a half times for bf16 copies of it
+// (225 KB, 1750 clocks, where its share of the HBM rate takes 3500).
+//
+// Units of work are (request, group, tile), cut into equal contiguous slices, one
+// per CTA; slices' pieces that do not cover their group's whole context are
+// written as fp32 records (slot 0: at the slice's start, slot 1: at its end) and
+// joined by join_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
+
+#include <mutex>
 
 #include "dsa_b200.h"
 #include "host.h"
@@ -18,16 +40,67 @@
 namespace dsa {
 namespace qattn {
 
-constexpr int kCkv = DSA_CKV_DIM;
-constexpr int kKpe = DSA_KPE_DIM;
+constexpr int kCkv = DSA_CKV_DIM;            // 512
+constexpr int kKpe = DSA_KPE_DIM;            // 64
 constexpr int kPage = DSA_PAGE_SIZE;
 constexpr int kPageBytes = DSA_LATENT_PAGE_BYTES;
 constexpr int kKpeAt = kPage * kCkv;
 constexpr int kScaleAt = kKpeAt + kPage * kKpe * 2;
-constexpr int kTile = 16;
-constexpr int kHeads = 16;
+constexpr int kTok = 128;                    // tokens per tile: two pages
+constexpr int kBlockBytes = kTok * 128;      // 16384: 128 dims of a tile's codes, or its position part
+constexpr int kParts = 4;                    // blocks of codes
+constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
+constexpr int kSoftWarps = 8;                // warps 0-7: two sets of four, half of the columns each
+constexpr int kLoadWarp = 8;                 // dense: TMA
+constexpr int kLogitWarp = 9;                // S^T, E^T (owns TMEM)
+constexpr int kValueWarp = 10;               // O^T
+constexpr int kQueryWarp = 12;               // 12-15: queries into parts
+constexpr int kGatherWarp = 16;              // sparse: 16-23, two groups of four, one for each stage
+constexpr int kDenseThreads = 512;
+constexpr int kSparseThreads = 768;
+constexpr int kTmemCols = 512;
+constexpr float kRescaleThreshold = 4.0f;    // log2 units, see the softmax warps
+constexpr float kScaleGrowth = 8.0f;
+constexpr float kUnit = 256.0f;              // of weights: 2^4 x 8 x 256 = 2^15 is the largest, e5m2 goes to 57344
+constexpr int kMostRows = 32;
+
+// Largest and small layouts: R = 16 rows with two buffers of queries and of S^T,
+// or 32 with one.
+template <int kR>
+struct Shape {
+  static constexpr int kCols = kR / 2;                   // columns (rows of Q) of a softmax thread
+  static constexpr int kQBufs = kR == 16 ? 2 : 1;
+  static constexpr int kSBufs = kR == 16 ? 2 : 1;
+  static constexpr int kQBlock = 2 * kR * 128;           // 128 dims of both parts
+  static constexpr int kQBytes = kParts * kQBlock + kR * 128;
+  static constexpr uint32_t kColS = 0;                   // a: 0, b: R, e: 2R of each buffer
+  static constexpr uint32_t kColO = kSBufs * 3 * kR;     // 4 blocks of 128 dims x 3R columns
+  static_assert(kColO + kParts * 3 * kR <= kTmemCols, "TMEM");
+  static constexpr uint32_t kIdescS = idesc_make(0, 0, false, false, 128, 2 * kR);
+  static constexpr uint32_t kIdescE = idesc_make(1, 1, false, false, 128, kR);
+  static constexpr uint32_t kIdescO = idesc_make(0, 1, true, true, 128, 3 * kR);  // e4m3 codes, e5m2 weights
+};
+
+constexpr int kOffQ = 2 * kStageBytes;                 // 163840
+constexpr int kOffP = kOffQ + 36864;                   // either shape's queries
+static_assert(Shape<16>::kQBufs * Shape<16>::kQBytes == 36864 && Shape<32>::kQBytes == 36864, "queries");
+constexpr int kOffScale = kOffP + kTok * 128;          // [2][128]
+constexpr int kOffBar = kOffScale + 2 * kTok * 4;
+constexpr int kOffMisc = kOffBar + 256;
+constexpr int kOffRed = kOffMisc + 128;                // [2 sets][4 warps][16], planning: warp sums
+constexpr int kOffFactor = kOffRed + 512;              // [32]
+constexpr int kOffMax = kOffFactor + 128;              // [32]
+constexpr int kOffMost = kOffMax + 128;                // [2][4] largest scales
+constexpr int kOffC = kOffMost + 32;                   // [2][32] logits' factors
+constexpr int kSmemBytes = 1024 + kOffC + 256;
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+
 constexpr int kMaxRequests = 65536;
-constexpr int64_t kMaxRows = 1 << 24;  // rows x heads
+constexpr int64_t kMaxRows = 1 << 24;          // rows x heads
+constexpr int64_t kMaxUnits = 1 << 30;
+constexpr int kMaxCtas = 256;
+constexpr int kPlanGroups = 2 * kMaxCtas;      // the plan: groups of the records, then first row and rows of each group
+constexpr int kPartFloats = kMostRows * kCkv;
 
 struct Params {
   const __nv_bfloat16* q_nope;
@@ -44,133 +117,1074 @@ struct Params {
   __nv_bfloat16* out;
   float* lse;
   unsigned int* status;
+  unsigned long long wait_limit_ns;
+  float* part_o;            // [2 * grid][kMostRows][512]
+  float2* part_ml;          // [2 * grid][kMostRows]: m, l
+  int* plan;
 };
 
-__device__ __forceinline__ float fp8(uint8_t x) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(x, __NV_E4M3);
-  return __half2float(*reinterpret_cast<const __half*>(&h));
+struct Request {
+  int row0, n;              // first row, rows (tokens)
+  int length;               // cached tokens; row j of n sees length - n + 1 + j
+  int rows, groups, tiles;  // (token, head) rows
+  int span;                 // units per group: its tiles and kLead more for its start
+};
+
+// What starting a group costs, in tiles.
+constexpr int kLead = 2;
+
+template <int kR, bool kSparse>
+__device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
+  Request r;
+  bad = false;
+  if (kSparse) {
+    r.row0 = b;
+    r.n = 1;
+    r.length = p.topk;
+  } else {
+    const int cap = p.max_pages * kPage;
+    r.row0 = b;
+    r.n = 1;
+    if (p.cu != nullptr) {
+      const int lo = p.cu[b], hi = p.cu[b + 1];
+      r.row0 = lo;
+      r.n = hi - lo;
+      if (lo < 0 || hi < lo || hi > p.num_rows) {
+        r.n = 0;
+        bad = true;
+      }
+    }
+    r.length = p.seq_lens[b];
+    if (r.length < 0 || r.length > cap) {
+      r.length = r.length < 0 ? 0 : cap;
+      bad = true;
+    }
+  }
+  r.rows = r.n * p.heads;
+  r.groups = (r.rows + kR - 1) / kR;
+  // A row that sees nothing is written by a tile whose tokens are all masked.
+  r.tiles = r.n == 0 ? 0 : max(1, (r.length + kTok - 1) / kTok);
+  r.span = r.n == 0 ? 0 : r.tiles + kLead;
+  return r;
 }
 
-__global__ void __launch_bounds__(32 * kHeads)
-plain_kernel(const Params p) {
+// CTA c of `ctas` has the units [start(c), start(c+1)), start(c) = floor(total c / ctas).
+__device__ __forceinline__ int slice_start(int total, int c, int ctas) {
+  const int q = total / ctas;
+  return q * c + (total - q * ctas) * c / ctas;
+}
+
+struct Start {
+  int b, first, first_group;  // request, its first unit and group over all requests
+  Request r;
+  int group, unit;
+};
+
+// A run of tiles of one group.
+struct Segment {
+  int b, group, t0, t1, group_index;
+  Request r;
+  bool whole;  // covers the group's whole context
+  int slot;    // of its record if it does not
+};
+
+template <int kR, bool kSparse>
+struct Walker {
+  const Params& p;
+  int u, u0, u1, b, first, first_group;
+  Request r;
+  int group, unit;
+
+  __device__ Walker(const Params& prm, int u0_, int u1_, const Start& st)
+      : p(prm), u(u0_), u0(u0_), u1(u1_), b(st.b), first(st.first), first_group(st.first_group) {
+    if (u0 >= u1) return;
+    r = st.r;
+    group = st.group;
+    unit = st.unit;
+  }
+  __device__ bool leave() {  // to the next request that has units in the slice
+    for (;;) {
+      first += r.groups * r.span;
+      first_group += r.groups;
+      ++b;
+      if (b >= p.num_requests || first >= u1) return false;
+      bool bad;
+      r = load_request<kR, kSparse>(p, b, bad);
+      if (r.tiles == 0) continue;
+      group = unit = 0;
+      return true;
+    }
+  }
+  __device__ bool next(Segment& s) {
+    while (u < u1) {
+      s.b = b;
+      s.r = r;
+      s.group = group;
+      s.group_index = first_group + group;
+      const int len = min(r.span - unit, u1 - u);
+      s.t0 = unit < kLead ? 0 : unit - kLead;
+      s.t1 = unit + len - kLead;
+      s.whole = s.t0 == 0 && s.t1 == r.tiles;
+      s.slot = u == u0 ? 0 : 1;
+      u += len;
+      unit = 0;
+      if (u < u1 && ++group == r.groups && !leave()) u = u1;
+      if (s.t1 > s.t0) return true;  // else a slice's end within the lead
+    }
+    return false;
+  }
+};
+
+// kN consecutive columns of 32 lanes, and for the logits three such blocks, with
+// the wait for them in the same statement.
+template <int kN>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t at, float (&v)[kN]) {
+  if constexpr (kN == 16) {
+    tmem_ld16_wait(at, v);
+  } else {
+    uint32_t r[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+
+template <int kN>
+__device__ __forceinline__ void tmem_st_cols(uint32_t at, const float (&v)[kN]) {
+  if constexpr (kN == 16) {
+    tmem_st16(at, v);
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+  }
+}
+
+template <int kN>
+__device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[kN], float (&b)[kN],
+                                              float (&c)[kN]) {
+  uint32_t r[3 * kN];
+  if constexpr (kN == 16) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%48];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%49];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47}, [%50];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+          "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+          "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47])
+        : "r"(a0), "r"(b0), "r"(c0)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23])
+        : "r"(a0), "r"(b0), "r"(c0)
+        : "memory");
+  }
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    a[i] = __uint_as_float(r[i]);
+    b[i] = __uint_as_float(r[kN + i]);
+    c[i] = __uint_as_float(r[2 * kN + i]);
+  }
+}
+
+// 16 bytes with cp.async, or zeros.
+__device__ __forceinline__ void cp_async16_or_zeros(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+
+// A value's upper three bits, to nearest: what e5m2 keeps of it, where it is normal there.
+__device__ __forceinline__ float three_bits(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x00100000u) & 0xFFE00000u);
+}
+__device__ __forceinline__ uint32_t e5m2x4(const float* v) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E5M2);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E5M2);
+  return lo | (hi << 16);
+}
+
+template <int kR, bool kSparse>
+__global__ void __launch_bounds__(kSparse ? kSparseThreads : kDenseThreads, 1)
+attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap kpe_map, const Params p) {
+  using Sh = Shape<kR>;
+  constexpr int C = Sh::kCols;
+  constexpr int kThreads = kSparse ? kSparseThreads : kDenseThreads;
+  constexpr int kWarps = kThreads / 32;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_mem = smem + kOffQ;
+  uint8_t* p_mem = smem + kOffP;
+  float* scale_s = reinterpret_cast<float*>(smem + kOffScale);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint64_t* kv_full = bars;                // [2 stages][kParts]; sparse: the last of each only
+  uint64_t* kv_free = bars + 2 * kParts;   // [2][kParts]: the block's part of O^T is done
+  uint64_t* q_full = bars + 4 * kParts;    // [2]
+  uint64_t* q_empty = q_full + 2;          // [2]
+  uint64_t* s_full = q_full + 4;           // [2]
+  uint64_t* s_empty = q_full + 6;          // [2]
+  uint64_t* p_full = q_full + 8;
+  uint64_t* o_empty = q_full + 9;
+  uint64_t* drain = q_full + 10;           // [2]
+  constexpr int kBars = 4 * kParts + 12;
+  static_assert(kBars * 8 <= kOffMisc - kOffBar, "barriers");
+  auto pv_done = [&](int i) { return &kv_free[(i & 1) * kParts + kParts - 1]; };
+  int* misc = reinterpret_cast<int*>(smem + kOffMisc);
+  uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(misc);
+  int* abort_flag = misc + 1;
+  Start* found = reinterpret_cast<Start*>(misc + 2);
+  static_assert(8 + sizeof(Start) <= kOffRed - kOffMisc, "misc");
+  float* red = reinterpret_cast<float*>(smem + kOffRed);
+  int* warp_sums = reinterpret_cast<int*>(red);  // planning: units, groups of each warp
+  static_assert(2 * kWarps * 4 <= 512, "warp sums");
+  float* factor_s = reinterpret_cast<float*>(smem + kOffFactor);
+  float* max_s = reinterpret_cast<float*>(smem + kOffMax);
+  float* most_s = reinterpret_cast<float*>(smem + kOffMost);
+  float* c_s = reinterpret_cast<float*>(smem + kOffC);
+
+  const int tid = threadIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int lane = tid & 31;
+
+  if (tid == 0) {
+    for (int x = 0; x < kBars; ++x) mbar_init(&bars[x], 1);
+    for (int s = 0; s < 2; ++s) {
+      if (kSparse) mbar_init(&kv_full[s * kParts + kParts - 1], 4);
+      mbar_init(&q_full[s], 4);
+      mbar_init(&q_empty[s], 1 + kSoftWarps);
+      mbar_init(&s_empty[s], kSoftWarps);
+    }
+    mbar_init(p_full, kSoftWarps);
+    mbar_init(o_empty, kSoftWarps);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (!kSparse && warp == kLoadWarp && elect_one()) {
+    prefetch_tensor_map(&codes_map);
+    prefetch_tensor_map(&kpe_map);
+  }
+  if (warp == kLogitWarp) tmem_alloc(tmem_base_smem, kTmemCols);
+  griddep_launch_dependents();
   griddep_wait();
-  __shared__ float tile[kTile][kCkv + kKpe];
-  __shared__ int64_t where[kTile];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = blockIdx.x, head = blockIdx.y * kHeads + warp;
-  int tokens = p.topk;
-  const int32_t* table = nullptr;
-  if (p.picked == nullptr) {
-    int r = row;
-    int len;
-    if (p.cu != nullptr) {
-      bool decreasing = p.cu[0] < 0 || p.cu[p.num_requests] > p.num_rows;
-      for (int k = tid; k < p.num_requests; k += blockDim.x) decreasing |= p.cu[k + 1] < p.cu[k];
-      if (__syncthreads_or(decreasing)) {
-        if (tid == 0) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
-        return;
-      }
-      if (row < p.cu[0] || row >= p.cu[p.num_requests]) return;
-      int lo = 0, hi = p.num_requests;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.cu[mid] <= row) lo = mid;
-        else hi = mid;
-      }
-      r = lo;
-      len = p.seq_lens[r];
-      if (len < 0 || len > p.max_pages * kPage) {
-        if (tid == 0) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
-        len = len < 0 ? 0 : p.max_pages * kPage;
-      }
-      len -= p.cu[r + 1] - 1 - row;
-    } else {
-      len = p.seq_lens[r];
-      if (len < 0 || len > p.max_pages * kPage) {
-        if (tid == 0) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
-        len = len < 0 ? 0 : p.max_pages * kPage;
+
+  // ---- plan: total units, and the request that holds this slice's first one.
+  const int ctas = gridDim.x;
+  const bool keeper = blockIdx.x == 0;  // writes the groups for join_kernel
+  int2* groups_out = reinterpret_cast<int2*>(p.plan + kPlanGroups);
+  int total = 0;
+  if constexpr (kSparse) {
+    bool bad;
+    const Request r = load_request<kR, true>(p, 0, bad);
+    total = p.num_rows * r.groups * r.span;  // every row alike
+    if (keeper)
+      for (int x = tid; x < p.num_rows * r.groups; x += kThreads)
+        groups_out[x] = make_int2(x / r.groups * p.heads + x % r.groups * kR, min(kR, r.rows - x % r.groups * kR));
+    if (tid == 0) {
+      const int u0 = slice_start(total, blockIdx.x, ctas);
+      const int b = u0 / (r.groups * r.span), in = u0 - b * r.groups * r.span;
+      Request mine = r;
+      mine.row0 = b;
+      *found = Start{b, b * r.groups * r.span, b * r.groups, mine, in / r.span, in % r.span};
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  } else {
+    // Every CTA sums all requests (one or two loads a thread for ordinary
+    // batches) instead of waiting for a planning launch.
+    const int per = (p.num_requests + kThreads - 1) / kThreads;
+    const int b_lo = min(tid * per, p.num_requests), b_hi = min(b_lo + per, p.num_requests);
+    int units = 0, groups = 0;
+    bool any_bad = false, decreasing = false;
+    Request mine;  // the thread's first (for ordinary batches its only) request
+    for (int b = b_lo; b < b_hi; ++b) {
+      bool bad;
+      const Request r = load_request<kR, false>(p, b, bad);
+      if (b == b_lo) mine = r;
+      if (p.cu != nullptr) decreasing |= p.cu[b + 1] < p.cu[b];
+      units += r.groups * r.span;
+      groups += r.groups;
+      any_bad |= bad;
+    }
+    if (any_bad && keeper) atomicOr(p.status, DSA_DEV_BAD_SEQ_LEN);
+    int iu = units, ig = groups;  // inclusive over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, iu, o), c = __shfl_up_sync(0xffffffffu, ig, o);
+      if (lane >= o) {
+        iu += a;
+        ig += c;
       }
     }
-    tokens = max(len, 0);
-    table = p.block_table + static_cast<int64_t>(r) * p.max_pages;
-  }
-  float q[18], o[16], m = -INFINITY, l = 0.f;
+    if (lane == 31) {
+      warp_sums[warp] = iu;
+      warp_sums[kWarps + warp] = ig;
+    }
+    tc_fence_before();
+    // Where cu_rows decreases, requests could share rows, and the sums exceed
+    // what the host checked: such a call does nothing.
+    const bool nothing = __syncthreads_or(decreasing);
+    tc_fence_after();
+    int before = iu - units, gbefore = ig - groups;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) o[k] = 0.f;
-  if (head < p.heads) {
-    const int64_t at = static_cast<int64_t>(row) * p.heads + head;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) q[k] = __bfloat162float(p.q_nope[at * kCkv + lane + 32 * k]);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) q[16 + k] = __bfloat162float(p.q_pe[at * kKpe + lane + 32 * k]);
-  }
-  for (int t0 = 0; t0 < tokens; t0 += kTile) {
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) {
+        before += warp_sums[w];
+        gbefore += warp_sums[kWarps + w];
+      }
+      total += warp_sums[w];
+    }
+    if (nothing) total = units = 0;
+    const int u0 = slice_start(total, blockIdx.x, ctas);
+    if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
+      for (int b = b_lo; b < b_hi; ++b) {
+        bool bad;
+        const Request r = b == b_lo ? mine : load_request<kR, false>(p, b, bad);
+        const int un = r.groups * r.span;
+        if (u0 >= before && u0 < before + un) {
+          const int group = (u0 - before) / r.span;
+          *found = Start{b, before, gbefore, r, group, u0 - before - group * r.span};
+        }
+        if (keeper)
+          for (int g = 0; g < r.groups; ++g)
+            groups_out[gbefore + g] = make_int2(r.row0 * p.heads + g * kR, min(kR, r.rows - g * kR));
+        before += un;
+        gbefore += r.groups;
+      }
+    }
     __syncthreads();
-    if (tid < kTile) {
-      int64_t w = -1;
-      const int t = t0 + tid;
-      if (t < tokens) {
-        int64_t slot;
-        if (p.picked != nullptr) {
-          slot = p.picked[static_cast<int64_t>(row) * p.topk + t];
-          if (slot < -1 || slot >= static_cast<int64_t>(p.num_pages) * kPage) {
-            atomicOr(p.status, DSA_DEV_BAD_INDEX);
-            slot = -1;
+  }
+  const int u0 = slice_start(total, blockIdx.x, ctas), u1 = slice_start(total, blockIdx.x + 1, ctas);
+  const uint32_t tmem_base = *tmem_base_smem;
+  const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
+  Walker<kR, kSparse> walk(p, u0, u1, *found);
+  Segment s;
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads (dense)
+    if (!kSparse && elect_one()) {
+      int i = 0;
+      int parts = 0;  // issued
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        const int32_t* row = p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+        // A page outside of the pool or behind the tokens reads as zeros (a box
+        // outside of the tensor is filled with them); its tokens are masked.
+        auto page_at = [&](int x) {
+          const int page = x * kPage < s.r.length ? row[x] : -1;
+          return page < 0 || page >= p.num_pages ? p.num_pages : page;
+        };
+        int n0 = page_at(2 * s.t0), n1 = page_at(2 * s.t0 + 1);
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int p0 = n0, p1 = n1;
+          if (t + 1 < s.t1) {
+            n0 = page_at(2 * t + 2);
+            n1 = page_at(2 * t + 3);
+          }
+          const int st = i & 1;
+          uint8_t* dst = smem + st * kStageBytes;
+#pragma unroll
+          for (int x = 0; x < kParts; ++x) {
+            ok = ok && mbar_wait(&kv_free[st * kParts + x], ((i >> 1) & 1) ^ 1, wctx);
+            if (!ok) break;
+            uint64_t* bar = &kv_full[st * kParts + x];
+            mbar_arrive_expect_tx(bar, x == kParts - 1 ? 2 * kBlockBytes + kTok * 4 : kBlockBytes);
+            tma_load_3d(dst + x * kBlockBytes, &codes_map, bar, 128 * x, 0, p0);
+            tma_load_3d(dst + x * kBlockBytes + kBlockBytes / 2, &codes_map, bar, 128 * x, 0, p1);
+            if (x == kParts - 1) {
+              tma_load_3d(dst + kParts * kBlockBytes, &kpe_map, bar, 0, 0, p0);
+              tma_load_3d(dst + kParts * kBlockBytes + kBlockBytes / 2, &kpe_map, bar, 0, 0, p1);
+              const uint8_t* s0 = p.cache + static_cast<int64_t>(p0 < p.num_pages ? p0 : 0) * kPageBytes + kScaleAt;
+              const uint8_t* s1 = p.cache + static_cast<int64_t>(p1 < p.num_pages ? p1 : 0) * kPageBytes + kScaleAt;
+              bulk_load(scale_s + st * kTok, s0, kPage * 4, bar);
+              bulk_load(scale_s + st * kTok + kPage, s1, kPage * 4, bar);
+            }
+            ++parts;
+          }
+          if (!ok) break;
+        }
+      }
+      // Copies still in flight (after an abort) land before the CTA exits: of
+      // each part the last two, whose phases nothing refills.
+      for (int x = 0; x < kParts; ++x) {
+        const int tiles = (parts + kParts - 1 - x) / kParts;
+        for (int k = tiles - 1; k >= 0 && k >= tiles - 2; --k)
+          mbar_drain(&kv_full[(k & 1) * kParts + x], (k >> 1) & 1, p.status);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kLogitWarp) {
+    // ------------------------------------------------------------ S^T and E^T
+    if (elect_one()) {
+      const uint64_t k_desc = sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t q_desc = sdesc_sw128(smem_u32(q_mem), 16, 1024);
+      int i = 0, segs = 0;
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        const int qb = segs % Sh::kQBufs;
+        const uint64_t bq = q_desc + qb * (Sh::kQBytes >> 4);
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1, sb = i % Sh::kSBufs;
+          const uint64_t a = k_desc + st * (kStageBytes >> 4);
+          const uint32_t d = tmem_base + Sh::kColS + 3u * kR * sb;
+          ok = mbar_wait(&s_empty[sb], ((i / Sh::kSBufs) & 1) ^ 1, wctx);
+          if (t == s.t0) ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
+#pragma unroll
+          for (int x = 0; x < kParts; ++x) {
+            if (!kSparse || x == 0)
+              ok = ok && mbar_wait(&kv_full[st * kParts + (kSparse ? kParts - 1 : x)], (i >> 1) & 1, wctx);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // +32 bytes per K32 step
+              umma_f8(d, a + x * (kBlockBytes >> 4) + 2 * k, bq + x * (Sh::kQBlock >> 4) + 2 * k, Sh::kIdescS,
+                      x + k > 0 ? 1u : 0u);
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(d + 2u * kR, a + kParts * (kBlockBytes >> 4) + 2 * k, bq + kParts * (Sh::kQBlock >> 4) + 2 * k,
+                      Sh::kIdescE, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[sb]);
+          if (t == s.t1 - 1) umma_commit(&q_empty[qb]);
+        }
+        ++segs;
+      }
+      umma_commit(&drain[0]);
+      mbar_drain(&drain[0], 0, p.status);
+    }
+    __syncwarp();
+  } else if (warp == kValueWarp) {
+    // ------------------------------------------------------------ O^T
+    if (elect_one()) {
+      const uint64_t v_desc = sdesc_sw128(smem_u32(smem), kBlockBytes, 1024);
+      const uint64_t p_desc = sdesc_sw128(smem_u32(p_mem), kBlockBytes, 1024);
+      int i = 0, segs = 0;
+      bool ok = true;
+      while (ok && walk.next(s)) {
+        for (int t = s.t0; t < s.t1; ++t, ++i) {
+          const int st = i & 1;
+          if (t == s.t0) ok = mbar_wait(o_empty, (segs & 1) ^ 1, wctx);
+          ok = ok && mbar_wait(p_full, i & 1, wctx);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t more = t == s.t0 ? 0u : 1u;
+          const uint64_t a = v_desc + st * (kStageBytes >> 4);
+#pragma unroll
+          for (int mb = 0; mb < kParts; ++mb) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // a K32 step is 32 token rows of 128 bytes
+              umma_f8(tmem_base + Sh::kColO + 3u * kR * mb, a + mb * (kBlockBytes >> 4) + kk * (4096 >> 4),
+                      p_desc + kk * (4096 >> 4), Sh::kIdescO, kk > 0 ? 1u : more);
+            umma_commit(&kv_free[st * kParts + mb]);
+          }
+        }
+        ++segs;
+      }
+      umma_commit(&drain[1]);
+      mbar_drain(&drain[1], 0, p.status);
+    }
+    __syncwarp();
+  } else if (warp >= kQueryWarp && warp < kQueryWarp + 4) {
+    // ------------------------------------------------------------ queries
+    // A warp takes every fourth row of the group: lane l its dims 16 l .. +15.
+    constexpr int kEach = kR / 4;
+    int segs = 0;
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      const int qb = segs % Sh::kQBufs;
+      const int rows = min(kR, s.r.rows - s.group * kR);
+      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
+      uint8_t* to = q_mem + qb * Sh::kQBytes;
+#pragma unroll 1
+      for (int j0 = 0; j0 < kEach; j0 += 4) {
+        uint4 raw[4][2], pe[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = warp - kQueryWarp + 4 * (j0 + j);
+          raw[j][0] = raw[j][1] = pe[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.q_nope + (row_q + r) * kCkv) + 2 * lane;
+            raw[j][0] = src[0];
+            raw[j][1] = src[1];
+            if (lane < 8) pe[j] = *(reinterpret_cast<const uint4*>(p.q_pe + (row_q + r) * kKpe) + lane);
+          }
+        }
+        if (j0 == 0)  // all lanes leave together
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&q_empty[qb], ((segs / Sh::kQBufs) & 1) ^ 1, wctx));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = warp - kQueryWarp + 4 * (j0 + j);
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[j]);
+          uint32_t most = 0u;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) most = max(most, max((x[k] << 16) & 0x7FFFFFFFu, x[k] & 0x7FFF0000u));
+          most = __reduce_max_sync(0xffffffffu, most);
+          // f = 2^7 over the largest value's power of two, at most 2^30: the
+          // logits of queries below that are 0 to all purposes.
+          const int exponent = most == 0u || most >= 0x7F800000u ? 127 : min(max(261 - static_cast<int>(most >> 23), 1), 157);
+          const float f = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
+          uint32_t pa[4], pb[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t a4 = 0u, b4 = 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = x[2 * k + h];
+              const float2 v = make_float2(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
+              const __nv_fp8x2_storage_t a2 = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+              const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(a2, __NV_E4M3);
+              const float2 af = __half22float2(*reinterpret_cast<const __half2*>(&back));
+              const __nv_fp8x2_storage_t b2 = __nv_cvt_float2_to_fp8x2(
+                  make_float2((v.x - af.x) * 16.f, (v.y - af.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+              a4 |= static_cast<uint32_t>(a2) << (16 * h);
+              b4 |= static_cast<uint32_t>(b2) << (16 * h);
+            }
+            pa[k] = a4;
+            pb[k] = b4;
+          }
+          if (most >= 0x7F800000u) {  // an infinity or NaN: the row's logits are NaN
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pa[k] = pb[k] = 0x7F7F7F7Fu;
+          }
+          uint8_t* at = to + (lane >> 3) * Sh::kQBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+          if (ok) {
+            *reinterpret_cast<uint4*>(at) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
+            *reinterpret_cast<uint4*>(at + kR * 128) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
+            if (lane < 8) {
+              uint32_t* y = reinterpret_cast<uint32_t*>(&pe[j]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[k] << 16) * f,
+                                                               __uint_as_float(y[k] & 0xFFFF0000u) * f);
+                y[k] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              *reinterpret_cast<uint4*>(to + kParts * Sh::kQBlock + r * 128 + ((lane ^ (r & 7)) << 4)) = pe[j];
+            }
+            if (lane == 0) c_s[qb * kMostRows + r] = p.scale_log2 / f;
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[qb]);
+      ++segs;
+    }
+  } else if (kSparse && warp >= kGatherWarp) {
+    // ------------------------------------------------------------ gather (sparse)
+    // Four warps for each stage; a warp copies 32 of its tile's tokens, 16 bytes
+    // a lane: a token's codes with one instruction, four position parts with one.
+    const int group = (warp - kGatherWarp) >> 2, quarter = (warp - kGatherWarp) & 3;
+    int i = 0;
+    bool ok = true;
+    while (ok && walk.next(s)) {
+      const int32_t* row = p.picked + static_cast<int64_t>(s.b) * p.topk;
+      for (int t = s.t0; t < s.t1; ++t, ++i) {
+        if ((i & 1) != group) continue;
+        const int pos = t * kTok + 32 * quarter + lane;
+        int slot = pos < p.topk ? row[pos] : -1;
+        if (slot < -1 || slot >= p.num_pages * kPage) {
+          atomicOr(p.status, DSA_DEV_BAD_INDEX);
+          slot = -1;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[group * kParts + kParts - 1], ((i >> 1) & 1) ^ 1, wctx));
+        if (!ok) break;
+        const uint32_t to = smem_u32(smem + group * kStageBytes);
+#pragma unroll 8
+        for (int n = 0; n < 32; ++n) {
+          const int x = __shfl_sync(0xffffffffu, slot, n);
+          const int r = 32 * quarter + n;
+          const uint8_t* src = p.cache + static_cast<int64_t>(max(x, 0) >> 6) * kPageBytes + (max(x, 0) & 63) * kCkv + 16 * lane;
+          cp_async16_or_zeros(to + (lane >> 3) * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src, x >= 0);
+        }
+#pragma unroll
+        for (int n = 0; n < 32; n += 4) {
+          const int x = __shfl_sync(0xffffffffu, slot, n + (lane >> 3));
+          const int r = 32 * quarter + n + (lane >> 3);
+          const uint8_t* src = p.cache + static_cast<int64_t>(max(x, 0) >> 6) * kPageBytes + kKpeAt + (max(x, 0) & 63) * (kKpe * 2) + 16 * (lane & 7);
+          cp_async16_or_zeros(to + kParts * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src, x >= 0);
+        }
+        cp_async4_or_zeros(smem_u32(scale_s + group * kTok + 32 * quarter + lane),
+                           p.cache + static_cast<int64_t>(max(slot, 0) >> 6) * kPageBytes + kScaleAt + 4 * (max(slot, 0) & 63),
+                           slot >= 0);
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[group * kParts + kParts - 1]);
+      }
+    }
+  } else if (warp < kSoftWarps) {
+    // ------------------------------------------------------------ softmax
+    // Set `set` of four warps has the columns C set .. + C - 1 (rows of Q); in it
+    // thread (sp, lane) has token 32 sp + lane.
+    const int set = warp >> 2, sp = warp & 3;
+    const int tok = 32 * sp + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(32 * sp) << 16;
+    const int e = tid & 127;  // thread of the set
+    float* red_set = red + 64 * set;  // [4][16]
+    int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
+    if (tid == 0) group_of[0] = group_of[1] = -1;
+    int i = 0, segs = 0;
+    bool ok = true;
+    // Online softmax in base 2.  A column's running max m is the same in every
+    // thread that has it.  It moves only when some token of the tile exceeds it
+    // by more than kRescaleThreshold (always at a segment's first tile), which
+    // one OR-barrier per tile tells the set; only then is the tile's max reduced
+    // over the tokens and O rescaled.  Weights by scales are taken relative to
+    // `ref`, the largest scale of the first tile, which moves in the same way
+    // when a scale exceeds it more than kScaleGrowth times.
+    while (walk.next(s)) {
+      const int qb = segs % Sh::kQBufs;
+      const int rows = min(kR, s.r.rows - s.group * kR);
+      float c[C], minus[C], l[C];  // minus: -m, or 0 while the column has seen nothing
+      uint32_t unset = 0;          // columns that have seen nothing yet
+      float ref = 0.f, by_ref = 0.f;
+      ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const bool in = C * set + k < rows;
+        c[k] = c_s[qb * kMostRows + C * set + k];
+        minus[k] = in ? 0.f : -INFINITY;  // no row of the group: all weights 0
+        l[k] = 0.f;
+        if (in) unset |= 1u << k;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[qb]);
+      const int sure = s.r.length - s.r.n + 1;  // tokens that every row sees
+      const int32_t* bt = kSparse ? p.picked + static_cast<int64_t>(s.b) * p.topk
+                                  : p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+      // Dense: the token's page; sparse: its slot.  -1 behind the context.
+      auto place = [&](int t) {
+        const int pos = t * kTok + tok;
+        return pos < s.r.length ? bt[kSparse ? pos : pos / kPage] : -1;
+      };
+      const int places = kSparse ? p.num_pages * kPage : p.num_pages;
+      int next_place = place(s.t0);
+      for (int t = s.t0; t < s.t1; ++t, ++i) {
+        const int st = i & 1, sb = i % Sh::kSBufs;
+        const int pos = t * kTok + tok;
+        const int at_place = next_place;
+        if (t + 1 < s.t1) next_place = place(t + 1);
+        const bool hidden = at_place < 0 || at_place >= places;  // seen by no row
+        const bool tail = !kSparse && (t + 1) * kTok > sure;
+        if (!kSparse && hidden && pos < s.r.length && (e & 63) == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
+        ok = ok && mbar_wait(&kv_full[st * kParts + kParts - 1], (i >> 1) & 1, wctx);
+        const float scale = scale_s[st * kTok + tok];
+        ok = ok && mbar_wait(&s_full[sb], (i / Sh::kSBufs) & 1, wctx);
+        tc_fence_after();
+        float x[C], d[C];
+        {
+          float b[C], pe[C];
+          const uint32_t at = tmem_base + lane_base + Sh::kColS + 3u * kR * sb + C * set;
+          tmem_ld_three<C>(at, at + kR, at + 2 * kR, x, b, pe);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[sb]);
+#pragma unroll
+          for (int k = 0; k < C; ++k) x[k] = fmaf(fmaf(b[k], 0.0625f, x[k]), scale, pe[k]);
+        }
+        uint32_t see = hidden ? 0u : 0xFFFFFFFFu;  // columns that see the token
+        if (tail && !hidden && pos >= sure) {
+          int row = s.group * kR + C * set;
+          int draft = row / p.heads, left = (draft + 1) * p.heads - row;
+          see = 0u;
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            if (pos < sure + draft) see |= 1u << k;
+            if (--left == 0) {
+              ++draft;
+              left = p.heads;
+            }
+          }
+        }
+        auto differences = [&]() {
+#pragma unroll
+          for (int k = 0; k < C; ++k) d[k] = fmaf(x[k], c[k], minus[k]);
+          if (see != 0xFFFFFFFFu) {
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+              if (!((see >> k) & 1)) d[k] = -INFINITY;
+          }
+        };
+        differences();
+        float most = d[0];
+#pragma unroll
+        for (int k = 1; k < C; ++k) most = fmaxf(most, d[k]);
+        if (named_barrier_or(1 + set, 128,
+                             unset != 0 || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const float v = d[k] - minus[k];
+            const uint32_t key = __reduce_max_sync(0xffffffffu, float_order_key(v == v ? v : -INFINITY));
+            if (lane == k) red_set[16 * sp + k] = float_from_order_key(key);
+          }
+          const uint32_t sk = __float_as_uint(scale);
+          const uint32_t largest = __reduce_max_sync(0xffffffffu, !hidden && sk < 0x7F800000u ? sk : 0u);
+          if (lane == 0) most_s[4 * set + sp] = __uint_as_float(largest);
+          named_barrier_sync(1 + set, 128);
+          float shrink = 1.f;
+          {
+            const float* m4 = most_s + 4 * set;
+            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            if (mt > kScaleGrowth * ref) {
+              shrink = ref == 0.f ? 1.f : ref / mt;  // scales of 0 so far: O is 0
+              ref = mt;
+              by_ref = mt < 1e-35f ? 0.f : kUnit / mt;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const float mt = fmaxf(fmaxf(red_set[k], red_set[16 + k]), fmaxf(red_set[32 + k], red_set[48 + k]));
+            const bool first = (unset >> k) & 1;
+            float alpha = 1.f;
+            if (first ? mt != -INFINITY : mt > kRescaleThreshold - minus[k]) {
+              alpha = first ? 0.f : exp2f(-minus[k] - mt);
+              minus[k] = -mt;
+              unset &= ~(1u << k);
+            }
+            l[k] *= alpha;
+            if (sp == 0 && lane == k) factor_s[C * set + k] = alpha * shrink;
+          }
+          differences();
+          named_barrier_sync(1 + set, 128);
+          if (t > s.t0) {
+            // O holds PV(i - 1) before it is rescaled.
+            ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
+            tc_fence_after();
+#pragma unroll 1
+            for (int y = 0; y < kParts * 3; ++y) {  // block and part
+              const uint32_t at = tmem_base + lane_base + Sh::kColO + kR * y + C * set;
+              float o[C];
+              tmem_ld_cols<C>(at, o);
+#pragma unroll
+              for (int k = 0; k < C; ++k) o[k] *= factor_s[C * set + k];
+              tmem_st_cols<C>(at, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (tail) {
+          // Tokens that some row does not see may hold anything; a zero weight
+          // would still turn a NaN code of theirs into NaN.  Their logits have
+          // been read (S^T is done), so such codes are zeroed; a row that does
+          // see one has its NaN from the logit.
+#pragma unroll
+          for (int y = 0; y < kParts; ++y) ok = ok && mbar_wait(&kv_full[st * kParts + y], (i >> 1) & 1, wctx);
+          const int from = max(sure - t * kTok, 0);
+          for (int q = tid; q < (kTok - from) * 32; q += 32 * kSoftWarps) {
+            uint4* at = reinterpret_cast<uint4*>(smem + st * kStageBytes + ((q >> 3) & 3) * kBlockBytes +
+                                                 (from + (q >> 5)) * 128 + (q & 7) * 16);
+            uint4 w = *at;
+            uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+            bool changed = false;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const uint32_t nan = ((ww[z] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+              ww[z] &= ~((nan >> 7) * 0xFFu);
+              changed |= nan != 0u;
+            }
+            if (changed) *at = w;
+          }
+        }
+        // Weights, and their products with the scale in three parts.
+        const float by = hidden ? 0.f : scale * by_ref;
+        uint32_t pa[C / 4], pb[C / 4], pc[C / 4];
+#pragma unroll
+        for (int k4 = 0; k4 < C / 4; ++k4) {
+          float a[4], b[4], r[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const int k = 4 * k4 + z;
+            const float w = ex2_approx(d[k]);  // d is -inf (weight 0) or NaN (kept) in a column that has seen nothing
+            l[k] += w;
+            float ws = w * by;
+            if (tail && !((see >> k) & 1)) ws = 0.f;  // `by` may be anything
+            a[z] = three_bits(ws);
+            r[z] = ws - a[z];
+            b[z] = three_bits(r[z]);
+            r[z] -= b[z];
+          }
+          pa[k4] = e5m2x4(a);
+          pb[k4] = e5m2x4(b);
+          pc[k4] = e5m2x4(r);
+        }
+        // P was last read by PV(i - 1).
+        if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
+        {
+          // One 128-byte row per token, 16-byte pieces swizzled by token & 7.
+          uint8_t* at = p_mem + tok * 128;
+          auto piece = [&](int x) { return at + ((x ^ (tok & 7)) << 4); };
+          if constexpr (C == 16) {
+            *reinterpret_cast<uint4*>(piece(set)) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
+            *reinterpret_cast<uint4*>(piece(2 + set)) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
+            *reinterpret_cast<uint4*>(piece(4 + set)) = make_uint4(pc[0], pc[1], pc[2], pc[3]);
+          } else {
+            *reinterpret_cast<uint2*>(piece(0) + 8 * set) = make_uint2(pa[0], pa[1]);
+            *reinterpret_cast<uint2*>(piece(1) + 8 * set) = make_uint2(pb[0], pb[1]);
+            *reinterpret_cast<uint2*>(piece(2) + 8 * set) = make_uint2(pc[0], pc[1]);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+      }
+      ++segs;
+
+      // ---- the segment's end: denominators over the tokens (while the last PV
+      // runs), then O.
+      {
+        // Over the warp's tokens: at each step a lane keeps half of its columns
+        // and sends the others.
+        int k0 = 0;  // the column that is left
+#pragma unroll
+        for (int half = C / 2, o = 16; half >= 1; half /= 2, o /= 2) {
+          const bool up = lane & o;
+#pragma unroll
+          for (int k = 0; k < half; ++k) {
+            const float send = up ? l[k] : l[k + half];
+            l[k] = (up ? l[k + half] : l[k]) + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+          if (up) k0 += half;
+        }
+#pragma unroll
+        for (int o = 16 / C; o >= 1; o /= 2) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        red_set[16 * sp + k0] = l[0];
+      }
+      if (sp == 0) {
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+          if (lane == k) max_s[C * set + k] = (unset >> k) & 1 ? -INFINITY : -minus[k];
+      }
+      named_barrier_sync(1 + set, 128);
+      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
+      const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + s.slot;
+      if (tid == 0 && !s.whole) group_of[s.slot] = s.group_index;
+      if (e < C) {
+        const int col = C * set + e;
+        const float sum = (red_set[e] + red_set[16 + e]) + (red_set[32 + e] + red_set[48 + e]);
+        const float unit = by_ref == 0.f ? 0.f : ref * (1.f / kUnit);
+        if (s.whole) {
+          factor_s[col] = sum == 0.f ? 0.f : unit / sum;
+          if (col < rows) p.lse[row_q + col] = sum == 0.f ? -INFINITY : max_s[col] + log2f(sum);
+        } else {
+          factor_s[col] = unit;
+          p.part_ml[rec * kMostRows + col] = make_float2(max_s[col], sum);
+        }
+      }
+      ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
+      named_barrier_sync(1 + set, 128);
+      tc_fence_after();
+#pragma unroll 1
+      for (int mb = 0; mb < kParts; ++mb) {
+        const int dim = 128 * mb + 32 * sp + lane;
+        float o[C];
+        {
+          float b[C], r[C];
+          const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
+          tmem_ld_three<C>(at, at + kR, at + 2 * kR, o, b, r);
+#pragma unroll
+          for (int k = 0; k < C; ++k) o[k] = ((o[k] + b[k]) + r[k]) * factor_s[C * set + k];
+        }
+        if (s.whole) {
+          // Neighbouring lanes swap halves, so that each stores two dims of one row.
+          const bool odd = lane & 1;
+          __nv_bfloat16* out = p.out + row_q * kCkv + (dim & ~1);
+#pragma unroll
+          for (int k = 0; k < C; k += 2) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? o[k] : o[k + 1], 1);
+            const int row = C * set + k + (odd ? 1 : 0);
+            if (row < rows)
+              *reinterpret_cast<__nv_bfloat162*>(out + static_cast<int64_t>(row) * kCkv) =
+                  odd ? __floats2bfloat162_rn(got, o[k + 1]) : __floats2bfloat162_rn(o[k], got);
           }
         } else {
-          const int page = table[t / kPage];
-          slot = static_cast<int64_t>(page) * kPage + t % kPage;
-          if (page < 0 || page >= p.num_pages) {
-            atomicOr(p.status, DSA_DEV_BAD_PAGE);
-            slot = -1;
-          }
+          float* to = p.part_o + rec * kPartFloats + C * set * kCkv + dim;
+#pragma unroll
+          for (int k = 0; k < C; ++k)
+            if (C * set + k < rows) to[k * kCkv] = o[k];
         }
-        if (slot >= 0) w = slot;
       }
-      where[tid] = w;
-    }
-    __syncthreads();
-    for (int t = warp; t < kTile; t += kHeads) {
-      if (where[t] < 0) continue;
-      const uint8_t* page = p.cache + where[t] / kPage * kPageBytes;
-      const int in = static_cast<int>(where[t] % kPage);
-      const float s = *reinterpret_cast<const float*>(page + kScaleAt + 4 * in);
-      for (int k = lane; k < kCkv; k += 32) tile[t][k] = s * fp8(page[in * kCkv + k]);
-      for (int k = lane; k < kKpe; k += 32)
-        tile[t][kCkv + k] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(page + kKpeAt)[in * kKpe + k]);
-    }
-    __syncthreads();
-    if (head < p.heads) {
-      for (int t = 0; t < kTile; ++t) {
-        if (where[t] < 0) continue;
-        float x = 0.f;
-#pragma unroll
-        for (int k = 0; k < 18; ++k) x = fmaf(q[k], tile[t][lane + 32 * k], x);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-        x *= p.scale_log2;
-        const float top = fmaxf(m, x);
-        if (!(x <= m)) {  // NaN too
-          const float a = m == -INFINITY ? 0.f : exp2f(m - top);
-          l *= a;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] *= a;
-          m = top;
-        }
-        const float w = x == -INFINITY ? 0.f : exp2f(x - m);
-        l += w;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = fmaf(w, tile[t][lane + 32 * k], o[k]);
-      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
     }
   }
-  if (head < p.heads) {
-    const int64_t at = static_cast<int64_t>(row) * p.heads + head;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) p.out[at * kCkv + lane + 32 * k] = __float2bfloat16_rn(o[k] * inv);
-    if (lane == 0) p.lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kLogitWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
   }
+}
+
+// Joins the records of a group that several slices share: per row
+//   M = max m_i, L = sum l_i 2^(m_i - M), lse = M + log2 L, out = sum O_i 2^(m_i - M) / L,
+// in an order that the slices alone give.  Block x has the group x, or where
+// groups outnumber records the group of record x if x is its first one; block y
+// its rows y * rows_per_block ...  Each kSplit-th of the block takes every
+// kSplit-th record of a row, a thread four dims, many loads in flight.
+constexpr int kJoinRows = 4;       // most rows per block
+constexpr int kJoinDepth = 8;      // records whose loads a thread has in flight
+
+template <int kSplit>
+__global__ void __launch_bounds__(128 * kSplit)
+join_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
+  griddep_wait();
+  constexpr int kThreads = 128 * kSplit;
+  constexpr int kLooks = 2 * kMaxCtas / kThreads;  // records a thread looks at
+  __shared__ int recs[2 * kMaxCtas];
+  __shared__ float weight[kJoinRows][2 * kMaxCtas];
+  __shared__ int warp_count[kLooks][kThreads / 32];
+  __shared__ float4 other[kSplit > 1 ? kSplit - 1 : 1][kCkv / 4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int x = blockIdx.x;
+  const int group = by_record ? __ldcg(p.plan + x) : x;
+  int mine[kLooks];
+#pragma unroll
+  for (int k = 0; k < kLooks; ++k) {
+    const int r = tid + k * kThreads;
+    mine[k] = r < 2 * ctas ? __ldcg(p.plan + r) : -1;
+  }
+  if (group < 0) return;
+  const int2 info = __ldcg(reinterpret_cast<const int2*>(p.plan + kPlanGroups) + group);
+  unsigned int votes[kLooks];
+#pragma unroll
+  for (int k = 0; k < kLooks; ++k) {
+    votes[k] = __ballot_sync(0xffffffffu, mine[k] == group);
+    if (lane == 0) warp_count[k][warp] = __popc(votes[k]);
+  }
+  __syncthreads();
+  int count = 0;
+#pragma unroll
+  for (int k = 0; k < kLooks; ++k) {
+    int at = count + __popc(votes[k] & ((1u << lane) - 1u));
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) at += warp_count[k][w];
+      count += warp_count[k][w];
+    }
+    if (mine[k] == group) recs[at] = tid + k * kThreads;
+  }
+  __syncthreads();
+  if (count == 0 || (by_record && recs[0] != x)) return;  // written whole; or another block's
+  const int y0 = blockIdx.y * rows_per_block;
+  const int rows = min(rows_per_block, info.y - y0);
+  if (rows <= 0) return;
+  // The first records' loads of the first row need no weights: they go first.
+  const int part = tid >> 7, d4 = tid & 127;
+  const float4* src = reinterpret_cast<const float4*>(p.part_o) + y0 * (kCkv / 4) + d4;
+  float4 v[kJoinDepth];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < kJoinDepth; ++j)
+      if (k0 + kSplit * j < count)
+        v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + kSplit * j]) * (kPartFloats / 4));
+  };
+  load(part);
+  for (int y = warp; y < rows; y += kThreads / 32) {
+    float M = -INFINITY, L = 0.f;
+    const float2* ml = p.part_ml + y0 + y;
+    for (int k = lane; k < count; k += 32) {
+      const float m = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kMostRows].x);
+      M = fmaxf(M, m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int k = lane; k < count; k += 32) {
+      const float2 q = __ldcg(ml + static_cast<int64_t>(recs[k]) * kMostRows);
+      // NaN sums have a place even where the max of what is left of a piece is -inf.
+      const float w = q.x == -INFINITY ? (q.y == q.y ? 0.f : q.y) : exp2f(q.x - M);
+      L = fmaf(q.y, w, L);
+      weight[y][k] = w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    __syncwarp();
+    for (int k = lane; k < count; k += 32) weight[y][k] *= inv;
+    if (lane == 0) p.lse[info.x + y0 + y] = L == 0.f ? -INFINITY : M + log2f(L);
+  }
+  __syncthreads();
+  for (int y = 0; y < rows; ++y) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = part; k0 < count; k0 += kSplit * kJoinDepth) {
+      if (y > 0 || k0 > part) load(k0);
+#pragma unroll
+      for (int j = 0; j < kJoinDepth; ++j) {
+        if (k0 + kSplit * j < count) {
+          const float w = weight[y][k0 + kSplit * j];
+          acc.x = fmaf(v[j].x, w, acc.x);
+          acc.y = fmaf(v[j].y, w, acc.y);
+          acc.z = fmaf(v[j].z, w, acc.z);
+          acc.w = fmaf(v[j].w, w, acc.w);
+        }
+      }
+    }
+    src += kCkv / 4;
+    if (part > 0) other[part - 1][d4] = acc;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int k = 0; k < kSplit - 1; ++k) {
+        const float4 o = other[k][d4];
+        acc.x += o.x;
+        acc.y += o.y;
+        acc.z += o.z;
+        acc.w += o.w;
+      }
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x, acc.y), __floats2bfloat162_rn(acc.z, acc.w)};
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(info.x) + y0 + y) * kCkv + 4 * d4) =
+          *reinterpret_cast<const uint2*>(h);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ host
+std::once_flag g_once[64];
+int g_status[64];
+
+struct Layout {
+  size_t part_ml, part_o, plan, bytes;
+};
+
+// Upper bound of the groups of R rows of all requests.
+inline int64_t groups_bound(int64_t rows, int64_t heads, int64_t requests, int r) { return rows * heads / r + requests; }
+
+// The same for every call that is accepted, so that a workspace never has to
+// move (a captured graph would go on using the old one).
+inline Layout layout(int sms) {
+  Layout a;
+  a.part_ml = kWorkspaceHeader;
+  a.part_o = a.part_ml + static_cast<size_t>(2 * sms) * kMostRows * sizeof(float2);
+  a.plan = a.part_o + static_cast<size_t>(2 * sms) * kPartFloats * sizeof(float);
+  a.bytes = a.plan + (kPlanGroups + 2 * static_cast<size_t>(groups_bound(kMaxRows, 1, kMaxRequests, 16))) * sizeof(int);
+  return a;
 }
 
 struct Range {
@@ -191,9 +1205,59 @@ int check_outputs(const void* output, const float* lse, size_t rows_q, const Ran
   return DSA_OK;
 }
 
-int launch(const Params& p, cudaStream_t s) {
-  if (launch_programmatic(plain_kernel, dim3(p.num_rows, (p.heads + kHeads - 1) / kHeads), dim3(32 * kHeads), 0, s, p) !=
-          cudaSuccess ||
+int setup(const DeviceInfo& info) {
+  if (static_cast<size_t>(kSmemBytes) > info.max_smem_optin || info.num_sms > kMaxCtas) return DSA_ERR_UNSUPPORTED_DEVICE;
+  std::call_once(g_once[info.device], [&]() {
+    auto large = [](const void* f) {
+      return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
+    };
+    g_status[info.device] = large(reinterpret_cast<const void*>(attend_kernel<16, false>)) &&
+                                    large(reinterpret_cast<const void*>(attend_kernel<32, false>)) &&
+                                    large(reinterpret_cast<const void*>(attend_kernel<16, true>))
+                                ? DSA_OK
+                                : DSA_ERR_CUDA;
+  });
+  return g_status[info.device];
+}
+
+// The attention and its join; `p` without what the workspace gives.
+int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaStream_t s) {
+  CUtensorMap maps[2] = {};
+  const bool sparse = p.picked != nullptr;
+  if (!sparse) {
+    int st = encode_tmap_3d(&maps[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.cache, kCkv, kPage, p.num_pages, kCkv, kPageBytes,
+                            128, kPage);
+    if (st != DSA_OK) return st;
+    st = encode_tmap_3d(&maps[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache + kKpeAt, kKpe, kPage, p.num_pages, kKpe * 2,
+                        kPageBytes, kKpe, kPage);
+    if (st != DSA_OK) return st;
+  }
+  const Layout a = layout(info.num_sms);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.status = reinterpret_cast<unsigned int*>(ws);
+  p.wait_limit_ns = kWaitLimitNs;
+  p.part_ml = reinterpret_cast<float2*>(ws + a.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + a.part_o);
+  p.plan = reinterpret_cast<int*>(ws + a.plan);
+  const std::lock_guard<std::mutex> turn(turn_of(workspace));  // the attention and its join share the records
+  const dim3 grid(info.num_sms);
+  cudaError_t err;
+  if (sparse)
+    err = launch_programmatic(attend_kernel<16, true>, grid, dim3(kSparseThreads), kSmemBytes, s, maps[0], maps[1], p);
+  else if (wide)
+    err = launch_programmatic(attend_kernel<32, false>, grid, dim3(kDenseThreads), kSmemBytes, s, maps[0], maps[1], p);
+  else
+    err = launch_programmatic(attend_kernel<16, false>, grid, dim3(kDenseThreads), kSmemBytes, s, maps[0], maps[1], p);
+  if (err != cudaSuccess) return DSA_ERR_CUDA;
+  const int r = wide ? 32 : 16;
+  const int64_t groups = sparse ? static_cast<int64_t>(p.num_rows) * ((p.heads + r - 1) / r)
+                                : groups_bound(p.num_rows, p.heads, p.num_requests, r);
+  const bool by_record = groups > 2 * info.num_sms;
+  const unsigned int across = static_cast<unsigned int>(by_record ? 2 * info.num_sms : groups);
+  const int rows = across <= 32 ? 1 : (across <= 96 ? 2 : kJoinRows);
+  const bool deep = across <= 10;
+  if (launch_programmatic(deep ? join_kernel<4> : join_kernel<1>, dim3(across, r / rows), dim3(deep ? 512 : 128), 0, s, p,
+                          info.num_sms, rows, by_record) != cudaSuccess ||
       cudaGetLastError() != cudaSuccess)
     return DSA_ERR_CUDA;
   return DSA_OK;
@@ -204,7 +1268,12 @@ int launch(const Params& p, cudaStream_t s) {
 
 using namespace dsa;
 
-extern "C" size_t dsa_latent_attention_workspace_bytes(void) { return kWorkspaceHeader; }
+extern "C" size_t dsa_latent_attention_workspace_bytes(void) {
+  DeviceInfo info;
+  // Without a usable device, size for the largest SM count of the family.
+  const int sms = current_device_info(&info) == DSA_OK ? info.num_sms : 160;
+  return qattn::layout(sms).bytes;
+}
 
 extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, const void* latent_cache, int64_t num_pages,
                                         const int32_t* seq_lens, const int32_t* block_table, const int32_t* cu_rows,
@@ -217,6 +1286,8 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   if (num_rows == 0 || num_requests == 0) return DSA_OK;
   if (!q_nope || !q_pe || !latent_cache || !seq_lens || !block_table || !output || !lse || !workspace || num_pages < 1 ||
       num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || (!cu_rows && num_rows != num_requests))
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (qattn::groups_bound(num_rows, num_heads, num_requests, 16) * (max_pages / 2 + 1 + qattn::kLead) > qattn::kMaxUnits)
     return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(latent_cache) || !aligned16(output) || !aligned16(workspace) ||
       ((reinterpret_cast<uintptr_t>(seq_lens) | reinterpret_cast<uintptr_t>(block_table) |
@@ -233,7 +1304,8 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   if (st != DSA_OK) return st;
   DeviceInfo info;
   if ((st = current_device_info(&info)) != DSA_OK) return st;
-  if (workspace_bytes < dsa_latent_attention_workspace_bytes()) return DSA_ERR_WORKSPACE_TOO_SMALL;
+  if ((st = qattn::setup(info)) != DSA_OK) return st;
+  if (workspace_bytes < qattn::layout(info.num_sms).bytes) return DSA_ERR_WORKSPACE_TOO_SMALL;
   qattn::Params p{};
   p.q_nope = static_cast<const __nv_bfloat16*>(q_nope);
   p.q_pe = static_cast<const __nv_bfloat16*>(q_pe);
@@ -249,8 +1321,9 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.lse = lse;
-  p.status = static_cast<unsigned int*>(workspace);
-  return qattn::launch(p, reinterpret_cast<cudaStream_t>(stream));
+  // Groups of 16 rows or 32: 32 where requests have more than 16 rows, since a group reads the whole context.
+  const bool wide = static_cast<int64_t>(num_rows) * num_heads > 16 * static_cast<int64_t>(num_requests);
+  return qattn::launch(p, info, wide, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q_pe, const void* latent_cache,
@@ -259,6 +1332,9 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
                                                void* workspace, size_t workspace_bytes, void* stream) {
   if (num_rows < 0 || num_heads < 1 || num_heads > 128 || static_cast<int64_t>(num_rows) * num_heads > qattn::kMaxRows ||
       topk < 1 || topk > 65536)
+    return DSA_ERR_INVALID_ARGUMENT;
+  const int64_t groups = static_cast<int64_t>(num_rows) * ((num_heads + 15) / 16);
+  if (groups > qattn::kMaxRows / 16 || groups * ((topk + qattn::kTok - 1) / qattn::kTok + qattn::kLead) > qattn::kMaxUnits)
     return DSA_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return DSA_OK;
   if (!q_nope || !q_pe || !latent_cache || !sparse_indices || !output || !lse || !workspace || num_pages < 1 ||
@@ -276,7 +1352,8 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
   if (st != DSA_OK) return st;
   DeviceInfo info;
   if ((st = current_device_info(&info)) != DSA_OK) return st;
-  if (workspace_bytes < dsa_latent_attention_workspace_bytes()) return DSA_ERR_WORKSPACE_TOO_SMALL;
+  if ((st = qattn::setup(info)) != DSA_OK) return st;
+  if (workspace_bytes < qattn::layout(info.num_sms).bytes) return DSA_ERR_WORKSPACE_TOO_SMALL;
   qattn::Params p{};
   p.q_nope = static_cast<const __nv_bfloat16*>(q_nope);
   p.q_pe = static_cast<const __nv_bfloat16*>(q_pe);
@@ -284,11 +1361,11 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
   p.num_pages = static_cast<int>(num_pages);
   p.picked = sparse_indices;
   p.topk = topk;
+  p.num_requests = num_rows;
   p.num_rows = num_rows;
   p.heads = num_heads;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.lse = lse;
-  p.status = static_cast<unsigned int*>(workspace);
-  return qattn::launch(p, reinterpret_cast<cudaStream_t>(stream));
+  return qattn::launch(p, info, false, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
