@@ -29,6 +29,7 @@
 // written as fp32 records (slot 0: at the slice's start, slot 1: at its end) and
 // joined by join_kernel.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <mutex>
@@ -50,25 +51,27 @@ constexpr int kTok = 128;                    // tokens per tile: two pages
 constexpr int kBlockBytes = kTok * 128;      // 16384: 128 dims of a tile's codes, or its position part
 constexpr int kParts = 4;                    // blocks of codes
 constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
-constexpr int kSoftWarps = 8;                // warps 0-7: two sets of four, half of the columns each
-constexpr int kLoadWarp = 8;                 // dense: TMA
-constexpr int kLogitWarp = 9;                // S^T, E^T (owns TMEM)
-constexpr int kValueWarp = 10;               // O^T
-constexpr int kQueryWarp = 12;               // 12-15: queries into parts
-constexpr int kGatherWarp = 16;              // sparse: 16-23, two groups of four, one for each stage
-constexpr int kDenseThreads = 512;
-constexpr int kSparseThreads = 768;
+constexpr int kCols = 8;                     // columns (rows of Q) of a softmax thread
+constexpr int kQueryWarps = 4;               // queries into parts
+constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
-constexpr float kRescaleThreshold = 4.0f;    // log2 units, see the softmax warps
-constexpr float kScaleGrowth = 8.0f;
-constexpr float kUnit = 256.0f;              // of weights: 2^4 x 8 x 256 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kRescaleThreshold = 6.0f;    // log2 units, see the softmax warps
+constexpr float kScaleGrowth = 4.0f;
+constexpr float kUnit = 128.0f;              // of weights: 2^6 x 4 x 128 = 2^15 is the largest, e5m2 goes to 57344
 constexpr int kMostRows = 32;
 
-// Largest and small layouts: R = 16 rows with two buffers of queries and of S^T,
-// or 32 with one.
-template <int kR>
+// R = 16 rows with two buffers of queries and of S^T, or 32 with one.  Softmax
+// warps come in sets of four, which have 8 columns each and a token a thread.
+template <int kR, bool kSparse>
 struct Shape {
-  static constexpr int kCols = kR / 2;                   // columns (rows of Q) of a softmax thread
+  static constexpr int kSets = kR / kCols;
+  static constexpr int kSoftWarps = 4 * kSets;
+  static constexpr int kLoadWarp = kSoftWarps;           // dense: TMA
+  static constexpr int kLogitWarp = kSoftWarps + 1;      // S^T, E^T (owns TMEM)
+  static constexpr int kValueWarp = kSoftWarps + 2;      // O^T
+  static constexpr int kQueryWarp = kSoftWarps + 4;
+  static constexpr int kGatherWarp = kQueryWarp + kQueryWarps;
+  static constexpr int kThreads = 32 * (kGatherWarp + (kSparse ? kGatherWarps : 0));
   static constexpr int kQBufs = kR == 16 ? 2 : 1;
   static constexpr int kSBufs = kR == 16 ? 2 : 1;
   static constexpr int kQBlock = 2 * kR * 128;           // 128 dims of both parts
@@ -83,15 +86,16 @@ struct Shape {
 
 constexpr int kOffQ = 2 * kStageBytes;                 // 163840
 constexpr int kOffP = kOffQ + 36864;                   // either shape's queries
-static_assert(Shape<16>::kQBufs * Shape<16>::kQBytes == 36864 && Shape<32>::kQBytes == 36864, "queries");
+static_assert(Shape<16, false>::kQBufs * Shape<16, false>::kQBytes == 36864 && Shape<32, false>::kQBytes == 36864,
+              "queries");
 constexpr int kOffScale = kOffP + kTok * 128;          // [2][128]
 constexpr int kOffBar = kOffScale + 2 * kTok * 4;
 constexpr int kOffMisc = kOffBar + 256;
-constexpr int kOffRed = kOffMisc + 128;                // [2 sets][4 warps][16], planning: warp sums
+constexpr int kOffRed = kOffMisc + 128;                // [4 sets][4 warps][8], planning: warp sums
 constexpr int kOffFactor = kOffRed + 512;              // [32]
-constexpr int kOffMax = kOffFactor + 128;              // [32]
-constexpr int kOffMost = kOffMax + 128;                // [2][4] largest scales
-constexpr int kOffC = kOffMost + 32;                   // [2][32] logits' factors
+constexpr int kOffMax = kOffFactor + 128;              // [32] running maxima
+constexpr int kOffMost = kOffMax + 128;                // [4][4] largest scales
+constexpr int kOffC = kOffMost + 64;                   // [2][32] logits' factors
 constexpr int kSmemBytes = 1024 + kOffC + 256;
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
@@ -235,77 +239,67 @@ struct Walker {
   }
 };
 
-// kN consecutive columns of 32 lanes, and for the logits three such blocks, with
-// the wait for them in the same statement.
-template <int kN>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t at, float (&v)[kN]) {
-  if constexpr (kN == 16) {
-    tmem_ld16_wait(at, v);
-  } else {
-    uint32_t r[8];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-        : "r"(at)
-        : "memory");
+// Three blocks of 8 consecutive columns of 32 lanes, with the wait for them in
+// the same statement.
+__device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[8], float (&b)[8],
+                                              float (&c)[8]) {
+  uint32_t r[24];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23])
+      : "r"(a0), "r"(b0), "r"(c0)
+      : "memory");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-  }
-}
-
-template <int kN>
-__device__ __forceinline__ void tmem_st_cols(uint32_t at, const float (&v)[kN]) {
-  if constexpr (kN == 16) {
-    tmem_st16(at, v);
-  } else {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
-                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
-                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
-                 : "memory");
-  }
-}
-
-template <int kN>
-__device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[kN], float (&b)[kN],
-                                              float (&c)[kN]) {
-  uint32_t r[3 * kN];
-  if constexpr (kN == 16) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%48];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%49];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47}, [%50];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-          "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-          "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47])
-        : "r"(a0), "r"(b0), "r"(c0)
-        : "memory");
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23])
-        : "r"(a0), "r"(b0), "r"(c0)
-        : "memory");
-  }
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
+  for (int i = 0; i < 8; ++i) {
     a[i] = __uint_as_float(r[i]);
-    b[i] = __uint_as_float(r[kN + i]);
-    c[i] = __uint_as_float(r[2 * kN + i]);
+    b[i] = __uint_as_float(r[8 + i]);
+    c[i] = __uint_as_float(r[16 + i]);
   }
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t at, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+               "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+               "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+               : "memory");
+}
+
+// Eight values of each lane reduced over the warp: at each step a lane keeps half
+// of its columns and sends the others.  Lanes end with column `k`'s result.
+template <typename Op>
+__device__ __forceinline__ float over_tokens(float (&v)[8], int lane, int& k, Op op) {
+  k = 0;
+#pragma unroll
+  for (int half = 4, o = 16; half >= 1; half /= 2, o /= 2) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < half; ++j) {
+      const float send = up ? v[j] : v[j + half];
+      v[j] = op(up ? v[j + half] : v[j], __shfl_xor_sync(0xffffffffu, send, o));
+    }
+    if (up) k += half;
+  }
+  v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 2));
+  v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
+  return v[0];
+}
+
+__device__ __forceinline__ void load8(const float* from, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+  v[0] = a.x;
+  v[1] = a.y;
+  v[2] = a.z;
+  v[3] = a.w;
+  v[4] = b.x;
+  v[5] = b.y;
+  v[6] = b.z;
+  v[7] = b.w;
 }
 
 // 16 bytes with cp.async, or zeros.
@@ -327,12 +321,14 @@ __device__ __forceinline__ uint32_t e5m2x4(const float* v) {
 }
 
 template <int kR, bool kSparse>
-__global__ void __launch_bounds__(kSparse ? kSparseThreads : kDenseThreads, 1)
+__global__ void __launch_bounds__(Shape<kR, kSparse>::kThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap kpe_map, const Params p) {
-  using Sh = Shape<kR>;
-  constexpr int C = Sh::kCols;
-  constexpr int kThreads = kSparse ? kSparseThreads : kDenseThreads;
+  using Sh = Shape<kR, kSparse>;
+  constexpr int C = kCols;
+  constexpr int kThreads = Sh::kThreads;
   constexpr int kWarps = kThreads / 32;
+  constexpr int kSoftWarps = Sh::kSoftWarps, kLoadWarp = Sh::kLoadWarp, kLogitWarp = Sh::kLogitWarp;
+  constexpr int kValueWarp = Sh::kValueWarp, kQueryWarp = Sh::kQueryWarp, kGatherWarp = Sh::kGatherWarp;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -373,7 +369,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     for (int x = 0; x < kBars; ++x) mbar_init(&bars[x], 1);
     for (int s = 0; s < 2; ++s) {
       if (kSparse) mbar_init(&kv_full[s * kParts + kParts - 1], 4);
-      mbar_init(&q_full[s], 4);
+      mbar_init(&q_full[s], kQueryWarps);
       mbar_init(&q_empty[s], 1 + kSoftWarps);
       mbar_init(&s_empty[s], kSoftWarps);
     }
@@ -608,10 +604,10 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       mbar_drain(&drain[1], 0, p.status);
     }
     __syncwarp();
-  } else if (warp >= kQueryWarp && warp < kQueryWarp + 4) {
+  } else if (warp >= kQueryWarp && warp < kQueryWarp + kQueryWarps) {
     // ------------------------------------------------------------ queries
     // A warp takes every fourth row of the group: lane l its dims 16 l .. +15.
-    constexpr int kEach = kR / 4;
+    constexpr int kEach = kR / kQueryWarps;
     int segs = 0;
     bool ok = true;
     while (ok && walk.next(s)) {
@@ -653,13 +649,15 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             uint32_t a4 = 0u, b4 = 0u;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+              // In half precision: its 11 bits hold q f down to 2^-24.
               const uint32_t w = x[2 * k + h];
-              const float2 v = make_float2(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
-              const __nv_fp8x2_storage_t a2 = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
-              const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(a2, __NV_E4M3);
-              const float2 af = __half22float2(*reinterpret_cast<const __half2*>(&back));
-              const __nv_fp8x2_storage_t b2 = __nv_cvt_float2_to_fp8x2(
-                  make_float2((v.x - af.x) * 16.f, (v.y - af.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+              const __half2 v = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
+              const __nv_fp8x2_storage_t a2 =
+                  __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(v), __NV_SATFINITE, __NV_E4M3);
+              const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(a2, __NV_E4M3));
+              const __half2 rest = __hmul2(__hsub2(v, back), __floats2half2_rn(16.f, 16.f));
+              const __nv_fp8x2_storage_t b2 =
+                  __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(rest), __NV_SATFINITE, __NV_E4M3);
               a4 |= static_cast<uint32_t>(a2) << (16 * h);
               b4 |= static_cast<uint32_t>(b2) << (16 * h);
             }
@@ -738,21 +736,24 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     }
   } else if (warp < kSoftWarps) {
     // ------------------------------------------------------------ softmax
-    // Set `set` of four warps has the columns C set .. + C - 1 (rows of Q); in it
-    // thread (sp, lane) has token 32 sp + lane.
+    // Set `set` of four warps has the columns 8 set .. 8 set + 7 (rows of Q); in
+    // it thread (sp, lane) has token 32 sp + lane.
     const int set = warp >> 2, sp = warp & 3;
     const int tok = 32 * sp + lane;
     const uint32_t lane_base = static_cast<uint32_t>(32 * sp) << 16;
     const int e = tid & 127;  // thread of the set
-    float* red_set = red + 64 * set;  // [4][16]
+    float* red_set = red + 4 * C * set;  // [4][8]
+    float* my_max = max_s + C * set;
+    float* my_factor = factor_s + C * set;
     int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
     if (tid == 0) group_of[0] = group_of[1] = -1;
     int i = 0, segs = 0;
     bool ok = true;
     // Online softmax in base 2.  A column's running max m is the same in every
-    // thread that has it.  It moves only when some token of the tile exceeds it
-    // by more than kRescaleThreshold (always at a segment's first tile), which
-    // one OR-barrier per tile tells the set; only then is the tile's max reduced
+    // thread that has it (-inf: it has seen nothing; +inf: no row of the group,
+    // all weights 0).  It moves only when some token of the tile exceeds it by
+    // more than kRescaleThreshold (always at a segment's first tile), which one
+    // OR-barrier per tile tells the set; only then is the tile's max reduced
     // over the tokens and O rescaled.  Weights by scales are taken relative to
     // `ref`, the largest scale of the first tile, which moves in the same way
     // when a scale exceeds it more than kScaleGrowth times.
@@ -760,16 +761,15 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       const int qb = segs % Sh::kQBufs;
       const int rows = min(kR, s.r.rows - s.group * kR);
       float c[C], minus[C], l[C];  // minus: -m, or 0 while the column has seen nothing
-      uint32_t unset = 0;          // columns that have seen nothing yet
+      bool unset = C * set < rows;  // some column has seen nothing yet
       float ref = 0.f, by_ref = 0.f;
+      if (e < C) my_max[e] = C * set + e < rows ? -INFINITY : INFINITY;
       ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
+      load8(c_s + qb * kMostRows + C * set, c);
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        const bool in = C * set + k < rows;
-        c[k] = c_s[qb * kMostRows + C * set + k];
-        minus[k] = in ? 0.f : -INFINITY;  // no row of the group: all weights 0
+        minus[k] = C * set + k < rows ? 0.f : -INFINITY;
         l[k] = 0.f;
-        if (in) unset |= 1u << k;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[qb]);
@@ -799,7 +799,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         {
           float b[C], pe[C];
           const uint32_t at = tmem_base + lane_base + Sh::kColS + 3u * kR * sb + C * set;
-          tmem_ld_three<C>(at, at + kR, at + 2 * kR, x, b, pe);
+          tmem_ld_three(at, at + kR, at + 2 * kR, x, b, pe);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[sb]);
@@ -820,68 +820,76 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             }
           }
         }
-        auto differences = [&]() {
 #pragma unroll
-          for (int k = 0; k < C; ++k) d[k] = fmaf(x[k], c[k], minus[k]);
-          if (see != 0xFFFFFFFFu) {
+        for (int k = 0; k < C; ++k) d[k] = fmaf(x[k], c[k], minus[k]);
+        if (see != 0xFFFFFFFFu) {
 #pragma unroll
-            for (int k = 0; k < C; ++k)
-              if (!((see >> k) & 1)) d[k] = -INFINITY;
-          }
-        };
-        differences();
-        float most = d[0];
-#pragma unroll
-        for (int k = 1; k < C; ++k) most = fmaxf(most, d[k]);
+          for (int k = 0; k < C; ++k)
+            if (!((see >> k) & 1)) d[k] = -INFINITY;
+        }
+        float most = fmaxf(fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])), fmaxf(fmaxf(d[4], d[5]), fmaxf(d[6], d[7])));
         if (named_barrier_or(1 + set, 128,
-                             unset != 0 || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
+                             unset || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
+          int col;
+          {
+            float v[C];
 #pragma unroll
-          for (int k = 0; k < C; ++k) {
-            const float v = d[k] - minus[k];
-            const uint32_t key = __reduce_max_sync(0xffffffffu, float_order_key(v == v ? v : -INFINITY));
-            if (lane == k) red_set[16 * sp + k] = float_from_order_key(key);
+            for (int k = 0; k < C; ++k) v[k] = (see >> k) & 1 ? x[k] * c[k] : -INFINITY;
+            // (fmaxf passes over NaN, which moves no maximum.)
+            const float mt = over_tokens(v, lane, col, [](float a, float b) { return fmaxf(a, b); });
+            red_set[C * sp + col] = mt == mt ? mt : -INFINITY;
           }
           const uint32_t sk = __float_as_uint(scale);
           const uint32_t largest = __reduce_max_sync(0xffffffffu, !hidden && sk < 0x7F800000u ? sk : 0u);
           if (lane == 0) most_s[4 * set + sp] = __uint_as_float(largest);
           named_barrier_sync(1 + set, 128);
+          const float4 m4 = *reinterpret_cast<const float4*>(most_s + 4 * set);
+          const float largest4 = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
           float shrink = 1.f;
-          {
-            const float* m4 = most_s + 4 * set;
-            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            if (mt > kScaleGrowth * ref) {
-              shrink = ref == 0.f ? 1.f : ref / mt;  // scales of 0 so far: O is 0
-              ref = mt;
-              by_ref = mt < 1e-35f ? 0.f : kUnit / mt;
-            }
+          if (largest4 > kScaleGrowth * ref) {
+            shrink = ref == 0.f ? 1.f : ref / largest4;  // scales of 0 so far: O is 0
+            ref = largest4;
+            by_ref = largest4 < 1e-35f ? 0.f : kUnit / largest4;
           }
+          if (sp == 0) {
+            const float mt = fmaxf(fmaxf(red_set[col], red_set[C + col]), fmaxf(red_set[2 * C + col], red_set[3 * C + col]));
+            const float m = my_max[col];
+            const bool moves = mt > m + kRescaleThreshold;
+            __syncwarp();
+            if (moves) my_max[col] = mt;
+            my_factor[col] = moves ? exp2f(m - mt) : 1.f;  // 0 when m was -inf
+          }
+          named_barrier_sync(1 + set, 128);
+          float alpha[C];
+          load8(my_factor, alpha);
+          load8(my_max, minus);
+          unset = false;
 #pragma unroll
           for (int k = 0; k < C; ++k) {
-            const float mt = fmaxf(fmaxf(red_set[k], red_set[16 + k]), fmaxf(red_set[32 + k], red_set[48 + k]));
-            const bool first = (unset >> k) & 1;
-            float alpha = 1.f;
-            if (first ? mt != -INFINITY : mt > kRescaleThreshold - minus[k]) {
-              alpha = first ? 0.f : exp2f(-minus[k] - mt);
-              minus[k] = -mt;
-              unset &= ~(1u << k);
-            }
-            l[k] *= alpha;
-            if (sp == 0 && lane == k) factor_s[C * set + k] = alpha * shrink;
+            unset |= minus[k] == -INFINITY;
+            minus[k] = minus[k] == -INFINITY ? 0.f : -minus[k];
+            l[k] *= alpha[k];
+            alpha[k] *= shrink;
+            d[k] = (see >> k) & 1 ? fmaf(x[k], c[k], minus[k]) : -INFINITY;
           }
-          differences();
-          named_barrier_sync(1 + set, 128);
           if (t > s.t0) {
             // O holds PV(i - 1) before it is rescaled.
             ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
             tc_fence_after();
 #pragma unroll 1
-            for (int y = 0; y < kParts * 3; ++y) {  // block and part
-              const uint32_t at = tmem_base + lane_base + Sh::kColO + kR * y + C * set;
-              float o[C];
-              tmem_ld_cols<C>(at, o);
+            for (int mb = 0; mb < kParts; ++mb) {
+              const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
+              float o[C], o1[C], o2[C];
+              tmem_ld_three(at, at + kR, at + 2 * kR, o, o1, o2);
 #pragma unroll
-              for (int k = 0; k < C; ++k) o[k] *= factor_s[C * set + k];
-              tmem_st_cols<C>(at, o);
+              for (int k = 0; k < C; ++k) {
+                o[k] *= alpha[k];
+                o1[k] *= alpha[k];
+                o2[k] *= alpha[k];
+              }
+              tmem_st8(at, o);
+              tmem_st8(at + kR, o1);
+              tmem_st8(at + 2 * kR, o2);
             }
             tmem_wait_st();
           }
@@ -934,18 +942,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         // P was last read by PV(i - 1).
         if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
         {
-          // One 128-byte row per token, 16-byte pieces swizzled by token & 7.
+          // One 128-byte row per token: column n of part x at byte x R + n, 16-byte pieces swizzled by token & 7.
           uint8_t* at = p_mem + tok * 128;
-          auto piece = [&](int x) { return at + ((x ^ (tok & 7)) << 4); };
-          if constexpr (C == 16) {
-            *reinterpret_cast<uint4*>(piece(set)) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
-            *reinterpret_cast<uint4*>(piece(2 + set)) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
-            *reinterpret_cast<uint4*>(piece(4 + set)) = make_uint4(pc[0], pc[1], pc[2], pc[3]);
-          } else {
-            *reinterpret_cast<uint2*>(piece(0) + 8 * set) = make_uint2(pa[0], pa[1]);
-            *reinterpret_cast<uint2*>(piece(1) + 8 * set) = make_uint2(pb[0], pb[1]);
-            *reinterpret_cast<uint2*>(piece(2) + 8 * set) = make_uint2(pc[0], pc[1]);
-          }
+          auto to = [&](int byte) { return reinterpret_cast<uint2*>(at + (((byte >> 4) ^ (tok & 7)) << 4) + (byte & 8)); };
+          *to(C * set) = make_uint2(pa[0], pa[1]);
+          *to(kR + C * set) = make_uint2(pb[0], pb[1]);
+          *to(2 * kR + C * set) = make_uint2(pc[0], pc[1]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -957,27 +959,9 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       // ---- the segment's end: denominators over the tokens (while the last PV
       // runs), then O.
       {
-        // Over the warp's tokens: at each step a lane keeps half of its columns
-        // and sends the others.
-        int k0 = 0;  // the column that is left
-#pragma unroll
-        for (int half = C / 2, o = 16; half >= 1; half /= 2, o /= 2) {
-          const bool up = lane & o;
-#pragma unroll
-          for (int k = 0; k < half; ++k) {
-            const float send = up ? l[k] : l[k + half];
-            l[k] = (up ? l[k + half] : l[k]) + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-          if (up) k0 += half;
-        }
-#pragma unroll
-        for (int o = 16 / C; o >= 1; o /= 2) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-        red_set[16 * sp + k0] = l[0];
-      }
-      if (sp == 0) {
-#pragma unroll
-        for (int k = 0; k < C; ++k)
-          if (lane == k) max_s[C * set + k] = (unset >> k) & 1 ? -INFINITY : -minus[k];
+        int col;
+        const float sum = over_tokens(l, lane, col, [](float a, float b) { return a + b; });
+        red_set[C * sp + col] = sum;
       }
       named_barrier_sync(1 + set, 128);
       const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
@@ -985,7 +969,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       if (tid == 0 && !s.whole) group_of[s.slot] = s.group_index;
       if (e < C) {
         const int col = C * set + e;
-        const float sum = (red_set[e] + red_set[16 + e]) + (red_set[32 + e] + red_set[48 + e]);
+        const float sum = (red_set[e] + red_set[C + e]) + (red_set[2 * C + e] + red_set[3 * C + e]);
         const float unit = by_ref == 0.f ? 0.f : ref * (1.f / kUnit);
         if (s.whole) {
           factor_s[col] = sum == 0.f ? 0.f : unit / sum;
@@ -1005,7 +989,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         {
           float b[C], r[C];
           const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
-          tmem_ld_three<C>(at, at + kR, at + 2 * kR, o, b, r);
+          tmem_ld_three(at, at + kR, at + 2 * kR, o, b, r);
 #pragma unroll
           for (int k = 0; k < C; ++k) o[k] = ((o[k] + b[k]) + r[k]) * factor_s[C * set + k];
         }
@@ -1243,11 +1227,11 @@ int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaSt
   const dim3 grid(info.num_sms);
   cudaError_t err;
   if (sparse)
-    err = launch_programmatic(attend_kernel<16, true>, grid, dim3(kSparseThreads), kSmemBytes, s, maps[0], maps[1], p);
+    err = launch_programmatic(attend_kernel<16, true>, grid, dim3(Shape<16, true>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
   else if (wide)
-    err = launch_programmatic(attend_kernel<32, false>, grid, dim3(kDenseThreads), kSmemBytes, s, maps[0], maps[1], p);
+    err = launch_programmatic(attend_kernel<32, false>, grid, dim3(Shape<32, false>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
   else
-    err = launch_programmatic(attend_kernel<16, false>, grid, dim3(kDenseThreads), kSmemBytes, s, maps[0], maps[1], p);
+    err = launch_programmatic(attend_kernel<16, false>, grid, dim3(Shape<16, false>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
   if (err != cudaSuccess) return DSA_ERR_CUDA;
   const int r = wide ? 32 : 16;
   const int64_t groups = sparse ? static_cast<int64_t>(p.num_rows) * ((p.heads + r - 1) / r)
