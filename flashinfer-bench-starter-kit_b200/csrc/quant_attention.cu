@@ -12,9 +12,10 @@
 //   q_nope f = a + b / 16 with a, b e4m3 and f a power of two for each row (its
 //     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
 //     b the other 4: the parts are exact down to 2^-22 of the row's largest.
-//   w = p s (weight by scale) = a + b + c with e5m2 parts, each to nearest: 3 + 3
-//     + 3 bits, within 2^-9 of w, over the range of the type (2^31).  Weights in
-//     bf16, as a bf16 product would take them, are within 2^-8.
+//   w = p s (weight by scale) = a + b + c with e5m2 parts of w in half precision,
+//     each to nearest: 3 + 3 + 3 bits, within 2^-9 of it (and it within 2^-11 of
+//     w), over the range of the type (2^31).  Weights in bf16, as a bf16 product
+//     would take them, are within 2^-8.
 // Per tile of 128 tokens and group of R rows (token, head)
 //   S^T[128, 2R] = C[128, 512] . [a b]^T    16 x (M128 N2R K32, e4m3)
 //   E^T[128, R]  = E[128, 64] . (q_pe f)^T   4 x (M128 NR K16, bf16)
@@ -94,7 +95,8 @@ constexpr int kOffMisc = kOffBar + 256;
 constexpr int kOffRed = kOffMisc + 128;                // [4 sets][4 warps][8], planning: warp sums
 constexpr int kOffFactor = kOffRed + 512;              // [32]
 constexpr int kOffMax = kOffFactor + 128;              // [32] running maxima
-constexpr int kOffMost = kOffMax + 128;                // [4][4] largest scales
+constexpr int kOffMinus = kOffMax + 128;               // [32] what is added to logits
+constexpr int kOffMost = kOffMinus + 128;              // [4][4] largest scales
 constexpr int kOffC = kOffMost + 64;                   // [2][32] logits' factors
 constexpr int kSmemBytes = 1024 + kOffC + 256;
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
@@ -310,14 +312,25 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-// A value's upper three bits, to nearest: what e5m2 keeps of it, where it is normal there.
-__device__ __forceinline__ float three_bits(float x) {
-  return __uint_as_float((__float_as_uint(x) + 0x00100000u) & 0xFFE00000u);
-}
-__device__ __forceinline__ uint32_t e5m2x4(const float* v) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E5M2);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E5M2);
-  return lo | (hi << 16);
+// Eight weights (at most 2^15) into their three e5m2 parts, in half precision:
+// rounded to its 11 bits, then each part to nearest.  An e5m2 value is the upper
+// byte of the same value in half precision.
+__device__ __forceinline__ void in_parts(const float (&w)[8], uint2& a, uint2& b, uint2& c) {
+  uint32_t part[3][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    __half2 h = __floats2half2_rn(w[2 * k], w[2 * k + 1]);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E5M2);
+      part[x][k] = two;
+      const uint32_t back = __byte_perm(two, 0u, 0x1404);
+      if (x < 2) h = __hsub2(h, *reinterpret_cast<const __half2*>(&back));  // exact
+    }
+  }
+  a = make_uint2(__byte_perm(part[0][0], part[0][1], 0x5410), __byte_perm(part[0][2], part[0][3], 0x5410));
+  b = make_uint2(__byte_perm(part[1][0], part[1][1], 0x5410), __byte_perm(part[1][2], part[1][3], 0x5410));
+  c = make_uint2(__byte_perm(part[2][0], part[2][1], 0x5410), __byte_perm(part[2][2], part[2][3], 0x5410));
 }
 
 template <int kR, bool kSparse>
@@ -330,8 +343,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   constexpr int kSoftWarps = Sh::kSoftWarps, kLoadWarp = Sh::kLoadWarp, kLogitWarp = Sh::kLogitWarp;
   constexpr int kValueWarp = Sh::kValueWarp, kQueryWarp = Sh::kQueryWarp, kGatherWarp = Sh::kGatherWarp;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset: the compiler still knows it as shared)
   uint8_t* q_mem = smem + kOffQ;
   uint8_t* p_mem = smem + kOffP;
   float* scale_s = reinterpret_cast<float*>(smem + kOffScale);
@@ -358,6 +370,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   static_assert(2 * kWarps * 4 <= 512, "warp sums");
   float* factor_s = reinterpret_cast<float*>(smem + kOffFactor);
   float* max_s = reinterpret_cast<float*>(smem + kOffMax);
+  float* minus_s = reinterpret_cast<float*>(smem + kOffMinus);
   float* most_s = reinterpret_cast<float*>(smem + kOffMost);
   float* c_s = reinterpret_cast<float*>(smem + kOffC);
 
@@ -744,6 +757,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     const int e = tid & 127;  // thread of the set
     float* red_set = red + 4 * C * set;  // [4][8]
     float* my_max = max_s + C * set;
+    float* my_minus = minus_s + C * set;  // -m, or 0 where m is -inf
     float* my_factor = factor_s + C * set;
     int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
     if (tid == 0) group_of[0] = group_of[1] = -1;
@@ -760,19 +774,15 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     while (walk.next(s)) {
       const int qb = segs % Sh::kQBufs;
       const int rows = min(kR, s.r.rows - s.group * kR);
-      float c[C], minus[C], l[C];  // minus: -m, or 0 while the column has seen nothing
+      float l[C];
       bool unset = C * set < rows;  // some column has seen nothing yet
       float ref = 0.f, by_ref = 0.f;
+      // (The first tile's values from minus_s count for nothing: its maxima are taken anyway.)
       if (e < C) my_max[e] = C * set + e < rows ? -INFINITY : INFINITY;
       ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
-      load8(c_s + qb * kMostRows + C * set, c);
+      const float* my_c = c_s + qb * kMostRows + C * set;
 #pragma unroll
-      for (int k = 0; k < C; ++k) {
-        minus[k] = C * set + k < rows ? 0.f : -INFINITY;
-        l[k] = 0.f;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[qb]);
+      for (int k = 0; k < C; ++k) l[k] = 0.f;
       const int sure = s.r.length - s.r.n + 1;  // tokens that every row sees
       const int32_t* bt = kSparse ? p.picked + static_cast<int64_t>(s.b) * p.topk
                                   : p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
@@ -795,38 +805,38 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         const float scale = scale_s[st * kTok + tok];
         ok = ok && mbar_wait(&s_full[sb], (i / Sh::kSBufs) & 1, wctx);
         tc_fence_after();
-        float x[C], d[C];
+        float x[C];  // logits
         {
-          float b[C], pe[C];
+          float b[C], pe[C], c[C];
+          load8(my_c, c);
           const uint32_t at = tmem_base + lane_base + Sh::kColS + 3u * kR * sb + C * set;
           tmem_ld_three(at, at + kR, at + 2 * kR, x, b, pe);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[sb]);
 #pragma unroll
-          for (int k = 0; k < C; ++k) x[k] = fmaf(fmaf(b[k], 0.0625f, x[k]), scale, pe[k]);
+          for (int k = 0; k < C; ++k) x[k] = fmaf(fmaf(b[k], 0.0625f, x[k]), scale, pe[k]) * c[k];
         }
-        uint32_t see = hidden ? 0u : 0xFFFFFFFFu;  // columns that see the token
-        if (tail && !hidden && pos >= sure) {
+        if (t == s.t1 - 1) {  // the queries' factors have been read
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_empty[qb]);
+        }
+        if (__any_sync(0xffffffffu, hidden || (tail && pos >= sure))) {
           int row = s.group * kR + C * set;
           int draft = row / p.heads, left = (draft + 1) * p.heads - row;
-          see = 0u;
 #pragma unroll
           for (int k = 0; k < C; ++k) {
-            if (pos < sure + draft) see |= 1u << k;
+            if (hidden || (tail && pos >= sure + draft)) x[k] = -INFINITY;
             if (--left == 0) {
               ++draft;
               left = p.heads;
             }
           }
         }
+        float d[C];
+        load8(my_minus, d);
 #pragma unroll
-        for (int k = 0; k < C; ++k) d[k] = fmaf(x[k], c[k], minus[k]);
-        if (see != 0xFFFFFFFFu) {
-#pragma unroll
-          for (int k = 0; k < C; ++k)
-            if (!((see >> k) & 1)) d[k] = -INFINITY;
-        }
+        for (int k = 0; k < C; ++k) d[k] += x[k];
         float most = fmaxf(fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])), fmaxf(fmaxf(d[4], d[5]), fmaxf(d[6], d[7])));
         if (named_barrier_or(1 + set, 128,
                              unset || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
@@ -834,7 +844,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           {
             float v[C];
 #pragma unroll
-            for (int k = 0; k < C; ++k) v[k] = (see >> k) & 1 ? x[k] * c[k] : -INFINITY;
+            for (int k = 0; k < C; ++k) v[k] = x[k];
             // (fmaxf passes over NaN, which moves no maximum.)
             const float mt = over_tokens(v, lane, col, [](float a, float b) { return fmaxf(a, b); });
             red_set[C * sp + col] = mt == mt ? mt : -INFINITY;
@@ -856,21 +866,24 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             const float m = my_max[col];
             const bool moves = mt > m + kRescaleThreshold;
             __syncwarp();
-            if (moves) my_max[col] = mt;
+            const float now = moves ? mt : m;
+            my_max[col] = now;
+            my_minus[col] = now == -INFINITY ? 0.f : -now;
             my_factor[col] = moves ? exp2f(m - mt) : 1.f;  // 0 when m was -inf
           }
           named_barrier_sync(1 + set, 128);
           float alpha[C];
-          load8(my_factor, alpha);
-          load8(my_max, minus);
+          load8(my_max, alpha);
           unset = false;
 #pragma unroll
+          for (int k = 0; k < C; ++k) unset |= alpha[k] == -INFINITY;
+          load8(my_factor, alpha);
+          load8(my_minus, d);
+#pragma unroll
           for (int k = 0; k < C; ++k) {
-            unset |= minus[k] == -INFINITY;
-            minus[k] = minus[k] == -INFINITY ? 0.f : -minus[k];
             l[k] *= alpha[k];
             alpha[k] *= shrink;
-            d[k] = (see >> k) & 1 ? fmaf(x[k], c[k], minus[k]) : -INFINITY;
+            d[k] += x[k];
           }
           if (t > s.t0) {
             // O holds PV(i - 1) before it is rescaled.
@@ -917,37 +930,27 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             if (changed) *at = w;
           }
         }
-        // Weights, and their products with the scale in three parts.
-        const float by = hidden ? 0.f : scale * by_ref;
-        uint32_t pa[C / 4], pb[C / 4], pc[C / 4];
+        // Weights (of d = -inf, 0; NaN stays), and their products with the scale in
+        // three parts.  Scales that are no number have made the logits NaN, and with
+        // them l, where they are seen; here they count as 0.
+        const float by = !hidden && scale < INFINITY ? scale * by_ref : 0.f;
+        uint2 pa, pb, pc;
 #pragma unroll
-        for (int k4 = 0; k4 < C / 4; ++k4) {
-          float a[4], b[4], r[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const int k = 4 * k4 + z;
-            const float w = ex2_approx(d[k]);  // d is -inf (weight 0) or NaN (kept) in a column that has seen nothing
-            l[k] += w;
-            float ws = w * by;
-            if (tail && !((see >> k) & 1)) ws = 0.f;  // `by` may be anything
-            a[z] = three_bits(ws);
-            r[z] = ws - a[z];
-            b[z] = three_bits(r[z]);
-            r[z] -= b[z];
-          }
-          pa[k4] = e5m2x4(a);
-          pb[k4] = e5m2x4(b);
-          pc[k4] = e5m2x4(r);
+        for (int k = 0; k < C; ++k) {
+          d[k] = ex2_approx(d[k]);
+          l[k] += d[k];
+          d[k] *= by;
         }
+        in_parts(d, pa, pb, pc);
         // P was last read by PV(i - 1).
         if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
         {
           // One 128-byte row per token: column n of part x at byte x R + n, 16-byte pieces swizzled by token & 7.
           uint8_t* at = p_mem + tok * 128;
           auto to = [&](int byte) { return reinterpret_cast<uint2*>(at + (((byte >> 4) ^ (tok & 7)) << 4) + (byte & 8)); };
-          *to(C * set) = make_uint2(pa[0], pa[1]);
-          *to(kR + C * set) = make_uint2(pb[0], pb[1]);
-          *to(2 * kR + C * set) = make_uint2(pc[0], pc[1]);
+          *to(C * set) = pa;
+          *to(kR + C * set) = pb;
+          *to(2 * kR + C * set) = pc;
         }
         fence_proxy_async_smem();
         tc_fence_before();

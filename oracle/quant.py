@@ -80,10 +80,16 @@ def bf16(x: torch.Tensor) -> torch.Tensor:
     return x.float().bfloat16()
 
 
-def _softmax(q_nope, q_pe, c, e, see, scale):
-    """(output, lse and their bounds) of one row's heads over tokens c, e [n, ...] of which `see` [n] are visible."""
+def scales_of(cache: torch.Tensor, slot: torch.Tensor) -> torch.Tensor:
+    return pieces(cache)[2][slot // PAGE, slot % PAGE].double()
+
+
+def _softmax(q_nope, q_pe, c, e, scales, see, scale):
+    """(output, lse and their bounds) of one row's heads over tokens c, e [n, ...] of these scales, of which `see` [n] are
+    visible."""
     H = q_nope.shape[0]
-    c, e = c[see], e[see]
+    largest = scales[torch.isfinite(scales)].max() if torch.isfinite(scales).any() else 0.0
+    c, e, scales = c[see], e[see], scales[see]
     if len(c) == 0:
         z = torch.zeros(H, CKV, dtype=torch.float64)
         return z, torch.full((H,), -math.inf, dtype=torch.float64), z, torch.zeros(H, dtype=torch.float64)
@@ -94,8 +100,9 @@ def _softmax(q_nope, q_pe, c, e, see, scale):
     move = off.amax(1)
     w = torch.exp2(x - lse[:, None])
     out = w @ c
-    err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -9 + 2.0 ** -20) * w
-    bound = err @ c.abs() + 2.0 ** -22 * w.amax(1, keepdim=True) * c.abs().sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
+    err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -19) * w
+    codes = torch.where(scales[:, None] == 0, 0.0, c.abs() / scales[:, None])
+    bound = err @ c.abs() + 2.0 ** -23 * largest * w.amax(1, keepdim=True) * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
     return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
 
 
@@ -107,9 +114,12 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
       magnitudes (2^-23, not 2^-24, for accumulators that truncate).
     * The lse moves by at most the largest of these, the exponential's and the sum's errors (2^-18 is far above both) and
       one rounding; a weight by ln 2 times its logit's and the lse's error.
-    * A weight is the sum of three parts of 3 bits each, every one to nearest: within 2^-9 of itself, and, where it is far
-      below the largest, within half the smallest step of the parts' type (2^-17 of weights that are scaled to 2^8 or
-      more for the largest one: 2^-25, taken as 2^-22).  The output is rounded to bf16, 2^-8 of itself.
+    * A weight is rounded to half precision (2^-11 of itself), then split into three parts of 3 bits each, every one to
+      nearest: within 2^-9 (1 + 2^-11), as each leaves at most 2^-3 of what it is given.  Where it is far below the largest,
+      it is within half the smallest step of the parts' type, 2^-17 (and of half precision, 2^-25): of weights times scales
+      over `ref` / 128, where ref is at most the largest scale of the context, and relative to a maximum that is at most
+      the true one.  Each token's code may so count 2^-23.9 times the largest scale times the largest weight too much or
+      too little.  The output is rounded to bf16, 2^-8 of itself.
     """
     T, H = q_nope.shape[:2]
     out = torch.full((T, H, CKV), math.nan, dtype=torch.float64)
@@ -119,9 +129,10 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
         lo, hi = (b, b + 1) if cu is None else (int(cu[b]), int(cu[b + 1]))
         L = int(seq_lens[b])
         pos = torch.arange(L)
-        c, e = rows(cache, table[b].long()[pos // PAGE] * PAGE + pos % PAGE)
+        slot = table[b].long()[pos // PAGE] * PAGE + pos % PAGE
+        c, e = rows(cache, slot)
         for i in range(lo, hi):
-            out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, pos < L - (hi - 1 - i), scale)
+            out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, scales_of(cache, slot), pos < L - (hi - 1 - i), scale)
     return out, lse, bo, bl
 
 
@@ -131,6 +142,7 @@ def sparse_reference(q_nope, q_pe, cache, picked, scale):
     out, lse = torch.zeros(T, H, CKV, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
     bo, bl = torch.zeros_like(out), torch.zeros_like(lse)
     for i in range(T):
-        c, e = rows(cache, picked[i].long().clamp(min=0))
-        out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, picked[i] >= 0, scale)
+        slot = picked[i].long().clamp(min=0)
+        c, e = rows(cache, slot)
+        out[i], lse[i], bo[i], bl[i] = _softmax(q_nope[i], q_pe[i], c, e, scales_of(cache, slot), picked[i] >= 0, scale)
     return out, lse, bo, bl

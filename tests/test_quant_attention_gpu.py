@@ -213,7 +213,7 @@ def test_reports_and_masks_what_does_not_fit(cuda_device):
     see[128:192] = False
     pos = torch.arange(300)
     slot = c.table[0].long().clamp(max=c.cache.shape[0] - 1)[pos // 64] * 64 + pos % 64
-    ro, rl, bo, bl = oq._softmax(c.q_nope[0], c.q_pe[0], *oq.rows(c.cache, slot), see, SCALE)
+    ro, rl, bo, bl = oq._softmax(c.q_nope[0], c.q_pe[0], *oq.rows(c.cache, slot), oq.scales_of(c.cache, slot), see, SCALE)
     compare(out[0].cpu(), lse[0].cpu(), ro, rl, bo, bl)
     c = Dense([300, 90], None, 16, seed=24)
     c.seq[1] = 10 ** 6
