@@ -65,143 +65,145 @@ struct WriteParams {
   unsigned int* status;       // or nullptr
 };
 
-// A warp takes kTok tokens at a time, a lane values 8 l .. 8 l + 7 and 256 + 8 l
-// .. of the latent (16-byte loads, 8-byte stores, each of a warp's in one piece)
-// and the pair 2 l, 2 l + 1 of the position part.  All loads of the kTok tokens
-// are made before any is used.
-template <int kTok>
-__global__ void __launch_bounds__(32 * kWarps)
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Warps walk the tokens kTok at a time; of a token a lane has the values 8 l ..
+// 8 l + 7 and 256 + 8 l .. of the latent (16-byte loads, 8-byte stores, each of a
+// warp's in one piece) and the pair 2 l, 2 l + 1 of the position part.  A token
+// costs about 230 instructions (200003 tokens: 60 us at the HBM rate, 41 us to
+// issue), so what matters is warps enough to overlap the two: two tokens a warp
+// in 80 registers and 24 warps an SM, against four tokens in 159 registers and 8
+// warps (185 us).  Weights are held as 7/8 = 448 / 2^9 of their value (exact).
+constexpr int kTok = 2;
+constexpr int kBlocksPerSm = 3;
+
+__global__ void __launch_bounds__(32 * kWarps, kBlocksPerSm)
 write_kernel(const WriteParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int stride = gridDim.x * kWarps * kTok;
-  uint4 wraw[2] = {make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u),
-                   make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)};  // ones
-  if (p.norm != nullptr) {
-    wraw[0] = *reinterpret_cast<const uint4*>(p.norm + 8 * lane);
-    wraw[1] = *reinterpret_cast<const uint4*>(p.norm + 256 + 8 * lane);
+  float w78[16];
+  {
+    uint4 raw[2] = {make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u),
+                    make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)};  // ones
+    if (p.norm != nullptr) {
+      raw[0] = *reinterpret_cast<const uint4*>(p.norm + 8 * lane);
+      raw[1] = *reinterpret_cast<const uint4*>(p.norm + 256 + 8 * lane);
+    }
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 w = bf16x2(x[k]);
+      w78[2 * k] = w.x * (kMostCode / 512.f);
+      w78[2 * k + 1] = w.y * (kMostCode / 512.f);
+    }
   }
-  const uint32_t* w32 = reinterpret_cast<const uint32_t*>(wraw);
-  const int64_t stride64 = stride;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps * kTok;
   for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kTok; t0 < p.num_tokens;
-       t0 += stride64) {
-    const int n = p.num_tokens - t0 < kTok ? static_cast<int>(p.num_tokens - t0) : kTok;
+       t0 += stride) {
     uint4 raw[kTok][2];
     uint32_t pe[kTok];
+    int64_t slot[kTok];
+    float2 cs[kTok], sn[kTok];
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      if (i < n) {
+      const bool in = t0 + i < p.num_tokens;
+      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      pe[i] = 0u;
+      slot[i] = -1;
+      cs[i] = sn[i] = make_float2(0.f, 0.f);
+      if (in) {
         const uint8_t* row = p.kv + (t0 + i) * p.kv_row;
+        slot[i] = p.slots[t0 + i];
+        int64_t pos = 0;
+        if (p.positions != nullptr) pos = p.positions[t0 + i];
         raw[i][0] = *reinterpret_cast<const uint4*>(row + 16 * lane);
         raw[i][1] = *reinterpret_cast<const uint4*>(row + 512 + 16 * lane);
         pe[i] = *reinterpret_cast<const uint32_t*>(row + 2 * kCkv + 4 * lane);
-      } else {
-        raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
-        pe[i] = 0u;
-      }
-    }
-    // Lane i has what is token i's own: where it goes, its position.
-    int64_t slot = -1, pos = 0;
-    if (lane < n) {
-      slot = p.slots[t0 + lane];
-      bool bad = slot >= p.num_slots;
-      if (p.positions != nullptr) {
-        pos = p.positions[t0 + lane];
-        bad |= slot >= 0 && (pos < 0 || pos >= p.max_positions);
-      }
-      if (bad) {
-        slot = -1;
-        if (p.status != nullptr) atomicOr(p.status, DSA_DEV_BAD_INDEX);
-      }
-    }
-    // cos and sin: of the pair's frequency (interleaved), or of the two
-    // frequencies 2 l, 2 l + 1 (mod 32) that the lane's values have.
-    float2 cs[kTok], sn[kTok];
-    if (p.positions != nullptr) {
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, slot >= 0 ? pos : 0, i);
-        if (i < n) {
-          const float* row = p.cos_sin + at * kKpe;
+        bool bad = slot[i] >= p.num_slots;
+        if (p.positions != nullptr) {
+          const bool outside = pos < 0 || pos >= p.max_positions;
+          bad |= slot[i] >= 0 && outside;
+          // cos and sin: of the pair's frequency (interleaved), or of the two
+          // frequencies 2 l, 2 l + 1 (mod 32) that the lane's values have.
+          const float* angles = p.cos_sin + (outside ? 0 : pos) * kKpe;
           if (p.interleaved) {
-            cs[i] = make_float2(row[lane], 0.f);
-            sn[i] = make_float2(row[32 + lane], 0.f);
+            cs[i].x = angles[lane];
+            sn[i].x = angles[32 + lane];
           } else {
-            cs[i] = *reinterpret_cast<const float2*>(row + 2 * (lane & 15));
-            sn[i] = *reinterpret_cast<const float2*>(row + 32 + 2 * (lane & 15));
+            cs[i] = *reinterpret_cast<const float2*>(angles + 2 * (lane & 15));
+            sn[i] = *reinterpret_cast<const float2*>(angles + 32 + 2 * (lane & 15));
           }
+        }
+        if (bad) {
+          slot[i] = -1;
+          if (lane == 0 && p.status != nullptr) atomicOr(p.status, DSA_DEV_BAD_INDEX);
         }
       }
     }
-    float sum[kTok];
-    uint32_t most[kTok];  // bits of the largest |t|: their order is that of the values, NaN on top
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
+      if (slot[i] < 0) continue;  // the whole warp
       const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[i]);
-      float s = 0.f;
-      uint32_t m = 0u;
+      float t[16];  // 7/8 c w, exact
+      float sum = 0.f, most = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float2 c = bf16x2(x[k]), w = bf16x2(w32[k]);
-        s = fmaf(c.x, c.x, s);
-        s = fmaf(c.y, c.y, s);
-        m = max(m, max(__float_as_uint(c.x * w.x) & 0x7FFFFFFFu, __float_as_uint(c.y * w.y) & 0x7FFFFFFFu));
+        const float2 c = bf16x2(x[k]);
+        sum = fmaf(c.x, c.x, sum);
+        sum = fmaf(c.y, c.y, sum);
+        t[2 * k] = c.x * w78[2 * k];
+        t[2 * k + 1] = c.y * w78[2 * k + 1];
+        most = max3_nan(most, fabsf(t[2 * k]), fabsf(t[2 * k + 1]));
       }
-      sum[i] = s;
-      most[i] = __reduce_max_sync(0xffffffffu, m);
-    }
-    if (p.norm != nullptr) {
+      // The order of non-negative floats is that of their bits, NaN on top.
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      if (p.norm != nullptr) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-        for (int i = 0; i < kTok; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const int64_t to = __shfl_sync(0xffffffffu, slot, i);
-      if (to < 0) continue;
-      const int64_t page = to / kPage;
-      const int row = static_cast<int>(to - page * kPage);
-      uint8_t* base = p.cache + page * kPageBytes;
-      const float M = __uint_as_float(most[i]);
-      const float r = p.norm != nullptr ? 1.f / sqrtf(fmaf(sum[i], 1.f / kCkv, p.eps)) : 1.f;
-      float scale = M * r / kMostCode;
+      const float r = p.norm != nullptr ? 1.f / sqrtf(fmaf(sum, 1.f / kCkv, p.eps)) : 1.f;
+      // M / 2^9, M = max |c w|: exact again; the row's scale.
+      float D = __fdiv_rn(__uint_as_float(top), kMostCode);
+      float scale = D * (512.f / kMostCode) * r;
       uint32_t code[4];
-      if (most[i] >= 0x7F800000u) {  // an infinity or NaN: the whole row is NaN
+      if (top >= 0x7F800000u) {  // an infinity or NaN: the whole row is NaN
         scale = 1.f;
         code[0] = code[1] = code[2] = code[3] = 0x7F7F7F7Fu;
       } else if (!(scale >= kLeastScale)) {  // zeros, or too small for a scale
         scale = 1.f;
         code[0] = code[1] = code[2] = code[3] = 0u;
       } else {
-        // Powers of two bring M to [1, 2), exactly; then 448 t / M as the
-        // correctly rounded reciprocal and an FMA-corrected quotient (P.
-        // Markstein, IBM J. Res. Dev. 34(1), 1990: equal to IEEE division here;
-        // what underflows is far below half of the smallest code).
-        const int exponent = static_cast<int>(most[i] >> 23);  // biased; 0: M is subnormal
-        const float by = __uint_as_float(static_cast<uint32_t>(min(max(254 - exponent, 1), 254)) << 23);
-        const float Mn = M * by, rcp = __frcp_rn(Mn), by448 = by;
-        const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[i]);
+        if (D < 1e-18f || D > 1e18f) {  // by a power of two, so that no reciprocal or quotient leaves the range
+          const float by = D < 1.f ? 1.8446744073709552e19f : 5.421010862427522e-20f;  // 2^64, 2^-64
+          D *= by;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) t[k] *= by;
+        }
+        // t / D = 448 c w / M as the correctly rounded reciprocal and an FMA-corrected
+        // quotient (P. Markstein, IBM J. Res. Dev. 34(1), 1990: equal to IEEE
+        // division here; what underflows is far below half of the smallest code).
+        const float rcp = __frcp_rn(D);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float v[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 c = bf16x2(x[2 * k + h]), w = bf16x2(w32[2 * k + h]);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const float t = (z ? c.y * w.y : c.x * w.x) * by448 * kMostCode;  // exact: 19 bits
-              const float q = __fmul_rn(t, rcp);
-              v[2 * h + z] = __fmaf_rn(__fmaf_rn(-q, Mn, t), rcp, q);
-            }
+          for (int z = 0; z < 4; ++z) {
+            const float q = __fmul_rn(t[4 * k + z], rcp);
+            v[z] = __fmaf_rn(__fmaf_rn(-q, D, t[4 * k + z]), rcp, q);
           }
           const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
           const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
           code[k] = lo | (hi << 16);
         }
       }
+      const int64_t page = slot[i] / kPage;
+      const int row = static_cast<int>(slot[i] - page * kPage);
+      uint8_t* base = p.cache + page * kPageBytes;
       uint8_t* codes = base + row * kCkv;
       *reinterpret_cast<uint2*>(codes + 8 * lane) = make_uint2(code[0], code[1]);
       *reinterpret_cast<uint2*>(codes + 256 + 8 * lane) = make_uint2(code[2], code[3]);
@@ -253,20 +255,21 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int n, int row, int
   return lo;
 }
 
-template <int kTok>
+constexpr int kReadTok = 4;
+
 __global__ void __launch_bounds__(32 * kWarps)
 read_kernel(const ReadParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kTok;
+  const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kReadTok;
   if (row0 >= p.num_rows) return;
   int r = request_of(p.cu, p.num_requests, row0, lane);
   // Lane i resolves row i: its page's first byte and its row in it; -1: zeros, -2: not written.
   int64_t at = -2;
   int in_page = 0;
   const int mine = row0 + lane;
-  if (lane < kTok && mine < p.num_rows && mine >= p.cu[0] && mine < p.cu[p.num_requests]) {
+  if (lane < kReadTok && mine < p.num_rows && mine >= p.cu[0] && mine < p.cu[p.num_requests]) {
     while (r + 1 < p.num_requests && p.cu[r + 1] <= mine) ++r;
     const int64_t pos = static_cast<int64_t>(p.starts[r]) + (mine - p.cu[r]);
     at = -1;
@@ -281,12 +284,12 @@ read_kernel(const ReadParams p) {
         at = static_cast<int64_t>(page) * kPageBytes;
     }
   }
-  uint2 code[kTok][2];
-  uint32_t pe[kTok];
-  float scale[kTok];
-  bool write[kTok];
+  uint2 code[kReadTok][2];
+  uint32_t pe[kReadTok];
+  float scale[kReadTok];
+  bool write[kReadTok];
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
+  for (int i = 0; i < kReadTok; ++i) {
     const int64_t a = __shfl_sync(0xffffffffu, at, i);
     const int row = __shfl_sync(0xffffffffu, in_page, i);
     write[i] = a != -2;
@@ -302,7 +305,7 @@ read_kernel(const ReadParams p) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
+  for (int i = 0; i < kReadTok; ++i) {
     if (!write[i]) continue;
     uint8_t* to = p.ckv + static_cast<int64_t>(row0 + i) * p.ckv_row;
     const uint32_t x[4] = {code[i][0].x, code[i][0].y, code[i][1].x, code[i][1].y};
@@ -354,10 +357,10 @@ extern "C" int dsa_latent_cache_write(const void* kv, int64_t kv_row_bytes, cons
                              static_cast<const __nv_bfloat16*>(norm_weight), eps, positions, cos_sin, max_positions,
                              interleaved, static_cast<uint8_t*>(latent_cache), num_pages * quant::kPage,
                              reinterpret_cast<unsigned int*>(status)};
-  constexpr int kTok = 4;
-  const int64_t blocks = (static_cast<int64_t>(num_tokens) + quant::kWarps * kTok - 1) / (quant::kWarps * kTok);
-  if (launch_programmatic(quant::write_kernel<kTok>, dim3(static_cast<unsigned int>(blocks)), dim3(32 * quant::kWarps), 0,
-                          reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess ||
+  const int64_t need = (static_cast<int64_t>(num_tokens) + quant::kWarps * quant::kTok - 1) / (quant::kWarps * quant::kTok);
+  const int64_t most = static_cast<int64_t>(info.num_sms) * quant::kBlocksPerSm;
+  if (launch_programmatic(quant::write_kernel, dim3(static_cast<unsigned int>(need < most ? need : most)),
+                          dim3(32 * quant::kWarps), 0, reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess ||
       cudaGetLastError() != cudaSuccess)
     return DSA_ERR_CUDA;
   return DSA_OK;
@@ -400,9 +403,9 @@ extern "C" int dsa_latent_cache_read(const void* latent_cache, int64_t num_pages
                             cu_rows, num_requests, max_pages, num_rows, static_cast<uint8_t*>(ckv),
                             static_cast<uint8_t*>(kpe), ckv_row_bytes, kpe_row_bytes,
                             reinterpret_cast<unsigned int*>(status)};
-  constexpr int kTok = 4;
-  const int64_t blocks = (static_cast<int64_t>(num_rows) + quant::kWarps * kTok - 1) / (quant::kWarps * kTok);
-  if (launch_programmatic(quant::read_kernel<kTok>, dim3(static_cast<unsigned int>(blocks)), dim3(32 * quant::kWarps), 0,
+  constexpr int kRows = quant::kWarps * quant::kReadTok;
+  const int64_t blocks = (static_cast<int64_t>(num_rows) + kRows - 1) / kRows;
+  if (launch_programmatic(quant::read_kernel, dim3(static_cast<unsigned int>(blocks)), dim3(32 * quant::kWarps), 0,
                           reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess ||
       cudaGetLastError() != cudaSuccess)
     return DSA_ERR_CUDA;
