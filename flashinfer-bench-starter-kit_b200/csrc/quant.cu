@@ -71,15 +71,23 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return y;
 }
 
-// Warps walk the tokens kTok at a time; of a token a lane has the values 8 l ..
-// 8 l + 7 and 256 + 8 l .. of the latent (16-byte loads, 8-byte stores, each of a
-// warp's in one piece) and the pair 2 l, 2 l + 1 of the position part.  A token
-// costs about 230 instructions (200003 tokens: 60 us at the HBM rate, 41 us to
-// issue), so what matters is warps enough to overlap the two: two tokens a warp
-// in 80 registers and 24 warps an SM, against four tokens in 159 registers and 8
-// warps (185 us).  Weights are held as 7/8 = 448 / 2^9 of their value (exact).
-constexpr int kTok = 2;
+// Warps walk the tokens; of a token a lane has the values 8 l .. 8 l + 7 and 256
+// + 8 l .. of the latent (16-byte loads, 8-byte stores, each of a warp's in one
+// piece) and the pair 2 l, 2 l + 1 of the position part.  A warp loads its next
+// token before it works on the one it has: 24 warps an SM of 79 registers have
+// 33 KB on their way.  About 200 instructions a token.  200003 tokens with norm
+// and rotation: 74 us, 5.4 TB/s (60 us at the copy's rate); without the load
+// ahead 86, two tokens a warp 88, four in 159 registers (8 warps an SM) 185; two
+// blocks an SM 88, four (spilling) 98.
 constexpr int kBlocksPerSm = 3;
+
+// What a lane loads of a token.
+struct TokenPart {
+  uint4 c[2];
+  uint32_t pe;
+  float2 cs, sn;
+  int64_t slot;
+};
 
 __global__ void __launch_bounds__(32 * kWarps, kBlocksPerSm)
 write_kernel(const WriteParams p) {
@@ -102,53 +110,63 @@ write_kernel(const WriteParams p) {
       w78[2 * k + 1] = w.y * (kMostCode / 512.f);
     }
   }
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps * kTok;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kTok; t0 < p.num_tokens;
-       t0 += stride) {
-    uint4 raw[kTok][2];
-    uint32_t pe[kTok];
-    int64_t slot[kTok];
-    float2 cs[kTok], sn[kTok];
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const bool in = t0 + i < p.num_tokens;
-      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
-      pe[i] = 0u;
-      slot[i] = -1;
-      cs[i] = sn[i] = make_float2(0.f, 0.f);
-      if (in) {
-        const uint8_t* row = p.kv + (t0 + i) * p.kv_row;
-        slot[i] = p.slots[t0 + i];
-        int64_t pos = 0;
-        if (p.positions != nullptr) pos = p.positions[t0 + i];
-        raw[i][0] = *reinterpret_cast<const uint4*>(row + 16 * lane);
-        raw[i][1] = *reinterpret_cast<const uint4*>(row + 512 + 16 * lane);
-        pe[i] = *reinterpret_cast<const uint32_t*>(row + 2 * kCkv + 4 * lane);
-        bool bad = slot[i] >= p.num_slots;
-        if (p.positions != nullptr) {
-          const bool outside = pos < 0 || pos >= p.max_positions;
-          bad |= slot[i] >= 0 && outside;
-          // cos and sin: of the pair's frequency (interleaved), or of the two
-          // frequencies 2 l, 2 l + 1 (mod 32) that the lane's values have.
-          const float* angles = p.cos_sin + (outside ? 0 : pos) * kKpe;
-          if (p.interleaved) {
-            cs[i].x = angles[lane];
-            sn[i].x = angles[32 + lane];
-          } else {
-            cs[i] = *reinterpret_cast<const float2*>(angles + 2 * (lane & 15));
-            sn[i] = *reinterpret_cast<const float2*>(angles + 32 + 2 * (lane & 15));
-          }
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps;
+  int64_t t_next = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  // Lane x has slot and position of the warp's x-th token from here on, so that
+  // no load waits for another but once in 32 tokens.
+  int64_t lane_slot = -1, lane_pos = 0;
+  int turn = 0;
+  auto load = [&]() {
+    if (turn == 0) {
+      const int64_t at = t_next + lane * stride;
+      lane_slot = -1;
+      lane_pos = 0;
+      if (at < p.num_tokens) {
+        lane_slot = p.slots[at];
+        if (p.positions != nullptr) lane_pos = p.positions[at];
+        const bool outside = p.positions != nullptr && (lane_pos < 0 || lane_pos >= p.max_positions);
+        if (lane_slot >= p.num_slots || (lane_slot >= 0 && outside)) {
+          lane_slot = -1;
+          if (p.status != nullptr) atomicOr(p.status, DSA_DEV_BAD_INDEX);
         }
-        if (bad) {
-          slot[i] = -1;
-          if (lane == 0 && p.status != nullptr) atomicOr(p.status, DSA_DEV_BAD_INDEX);
+        if (outside) lane_pos = 0;
+      }
+    }
+    TokenPart n;
+    n.c[0] = n.c[1] = make_uint4(0u, 0u, 0u, 0u);
+    n.pe = 0u;
+    n.cs = n.sn = make_float2(0.f, 0.f);
+    n.slot = __shfl_sync(0xffffffffu, lane_slot, turn);
+    if (n.slot >= 0) {
+      const uint8_t* row = p.kv + t_next * p.kv_row;
+      n.c[0] = *reinterpret_cast<const uint4*>(row + 16 * lane);
+      n.c[1] = *reinterpret_cast<const uint4*>(row + 512 + 16 * lane);
+      n.pe = *reinterpret_cast<const uint32_t*>(row + 2 * kCkv + 4 * lane);
+      if (p.positions != nullptr) {
+        // cos and sin: of the pair's frequency (interleaved), or of the two
+        // frequencies 2 l, 2 l + 1 (mod 32) that the lane's values have.
+        const float* angles = p.cos_sin + __shfl_sync(0xffffffffu, lane_pos, turn) * kKpe;
+        if (p.interleaved) {
+          n.cs.x = angles[lane];
+          n.sn.x = angles[32 + lane];
+        } else {
+          n.cs = *reinterpret_cast<const float2*>(angles + 2 * (lane & 15));
+          n.sn = *reinterpret_cast<const float2*>(angles + 32 + 2 * (lane & 15));
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (slot[i] < 0) continue;  // the whole warp
-      const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[i]);
+    turn = (turn + 1) & 31;
+    t_next += stride;
+    return n;
+  };
+  if (t_next >= p.num_tokens) return;
+  TokenPart next = load();
+  for (;;) {
+    const TokenPart now = next;
+    const bool more = t_next < p.num_tokens;
+    if (more) next = load();
+    if (now.slot >= 0) {  // the whole warp
+      const uint32_t* x = reinterpret_cast<const uint32_t*>(now.c);
       float t[16];  // 7/8 c w, exact
       float sum = 0.f, most = 0.f;
 #pragma unroll
@@ -166,9 +184,11 @@ write_kernel(const WriteParams p) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-      const float r = p.norm != nullptr ? 1.f / sqrtf(fmaf(sum, 1.f / kCkv, p.eps)) : 1.f;
-      // M / 2^9, M = max |c w|: exact again; the row's scale.
-      float D = __fdiv_rn(__uint_as_float(top), kMostCode);
+      const float r = p.norm != nullptr ? rsqrtf(fmaf(sum, 1.f / kCkv, p.eps)) : 1.f;
+      // M / 2^9 with M = max |c w|, and the row's scale.  That quotient is exact:
+      // a first one, its remainder by one FMA, and the sum of both rounded.
+      const float top7 = __uint_as_float(top), first = top7 * (1.f / kMostCode);
+      float D = fmaf(fmaf(-first, kMostCode, top7), 1.f / kMostCode, first);
       float scale = D * (512.f / kMostCode) * r;
       uint32_t code[4];
       if (top >= 0x7F800000u) {  // an infinity or NaN: the whole row is NaN
@@ -184,10 +204,11 @@ write_kernel(const WriteParams p) {
 #pragma unroll
           for (int k = 0; k < 16; ++k) t[k] *= by;
         }
-        // t / D = 448 c w / M as the correctly rounded reciprocal and an FMA-corrected
-        // quotient (P. Markstein, IBM J. Res. Dev. 34(1), 1990: equal to IEEE
-        // division here; what underflows is far below half of the smallest code).
-        const float rcp = __frcp_rn(D);
+        // t / D = 448 c w / M in the same way: within 2^-44 of itself before it is
+        // rounded, so exact where it is a border of e4m3 (what underflows is far
+        // below half of the smallest code).
+        float rcp;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(D));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float v[4];
@@ -201,28 +222,29 @@ write_kernel(const WriteParams p) {
           code[k] = lo | (hi << 16);
         }
       }
-      const int64_t page = slot[i] / kPage;
-      const int row = static_cast<int>(slot[i] - page * kPage);
+      const int64_t page = now.slot / kPage;
+      const int row = static_cast<int>(now.slot - page * kPage);
       uint8_t* base = p.cache + page * kPageBytes;
       uint8_t* codes = base + row * kCkv;
       *reinterpret_cast<uint2*>(codes + 8 * lane) = make_uint2(code[0], code[1]);
       *reinterpret_cast<uint2*>(codes + 256 + 8 * lane) = make_uint2(code[2], code[3]);
       if (lane == 0) *reinterpret_cast<float*>(base + kScaleAt + 4 * row) = scale;
-      uint32_t rotated = pe[i];
+      uint32_t rotated = now.pe;
       if (p.positions != nullptr) {
-        const float2 v = bf16x2(pe[i]);
+        const float2 v = bf16x2(now.pe);
         if (p.interleaved) {
-          rotated = to_bf16x2(fmaf(v.x, cs[i].x, -(v.y * sn[i].x)), fmaf(v.y, cs[i].x, v.x * sn[i].x));
+          rotated = to_bf16x2(fmaf(v.x, now.cs.x, -(v.y * now.sn.x)), fmaf(v.y, now.cs.x, v.x * now.sn.x));
         } else {
           // Lanes 0-15 have the first halves a of the pairs, lanes 16-31 the
           // second ones b: a cos - b sin, and b cos + a sin.
-          const float2 o = bf16x2(__shfl_xor_sync(0xffffffffu, pe[i], 16));
+          const float2 o = bf16x2(__shfl_xor_sync(0xffffffffu, now.pe, 16));
           const float sign = lane < 16 ? -1.f : 1.f;
-          rotated = to_bf16x2(fmaf(v.x, cs[i].x, sign * (o.x * sn[i].x)), fmaf(v.y, cs[i].y, sign * (o.y * sn[i].y)));
+          rotated = to_bf16x2(fmaf(v.x, now.cs.x, sign * (o.x * now.sn.x)), fmaf(v.y, now.cs.y, sign * (o.y * now.sn.y)));
         }
       }
       *reinterpret_cast<uint32_t*>(base + kKpeAt + row * kKpe * 2 + 4 * lane) = rotated;
     }
+    if (!more) break;
   }
 }
 
@@ -357,7 +379,7 @@ extern "C" int dsa_latent_cache_write(const void* kv, int64_t kv_row_bytes, cons
                              static_cast<const __nv_bfloat16*>(norm_weight), eps, positions, cos_sin, max_positions,
                              interleaved, static_cast<uint8_t*>(latent_cache), num_pages * quant::kPage,
                              reinterpret_cast<unsigned int*>(status)};
-  const int64_t need = (static_cast<int64_t>(num_tokens) + quant::kWarps * quant::kTok - 1) / (quant::kWarps * quant::kTok);
+  const int64_t need = (static_cast<int64_t>(num_tokens) + quant::kWarps - 1) / quant::kWarps;
   const int64_t most = static_cast<int64_t>(info.num_sms) * quant::kBlocksPerSm;
   if (launch_programmatic(quant::write_kernel, dim3(static_cast<unsigned int>(need < most ? need : most)),
                           dim3(32 * quant::kWarps), 0, reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess ||
