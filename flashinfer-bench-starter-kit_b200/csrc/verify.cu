@@ -103,14 +103,27 @@ __device__ __forceinline__ double left_of(float p, float q, double c) {
   return w <= 0.0 ? 0.0 : w;  // NaN stays
 }
 
-// Weights of the four values from v on; `struck`: whether any child's token may
+// The same before the maximum, for whole rows, where conversions to 64 bits would
+// bound it (one takes 8 clocks of its unit): q is widened by three integer
+// instructions instead.  Exact for normal numbers; what is below 2^-126, 0 among
+// it, comes out between 2^-127 and 2^-126 and takes that much too much from p.
+__device__ __forceinline__ double difference(float p, float q, double c) {
+  const uint32_t b = __float_as_uint(q);
+  const double wide = __hiloint2double(static_cast<int>((b >> 3) + 0x38000000u), static_cast<int>(b << 29));
+  return fma(-c, wide, static_cast<double>(p));
+}
+
+// Weights of the four values from v on, doubled where q counts (max(w, 0) is half
+// of w + |w|, which takes no selection); `struck`: whether any child's token may
 // lie in the warp's segment.
 __device__ __forceinline__ void weights(const Left& s, float4 p, float4 q, int v, bool struck, double (&w)[4]) {
   if (s.q != nullptr && s.c != 0.0) {
-    w[0] = left_of(p.x, q.x, s.c);
-    w[1] = left_of(p.y, q.y, s.c);
-    w[2] = left_of(p.z, q.z, s.c);
-    w[3] = left_of(p.w, q.w, s.c);
+    w[0] = difference(p.x, q.x, s.c);
+    w[1] = difference(p.y, q.y, s.c);
+    w[2] = difference(p.z, q.z, s.c);
+    w[3] = difference(p.w, q.w, s.c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] += fabs(w[e]);
     return;
   }
   w[0] = p.x;
@@ -128,7 +141,7 @@ __device__ __forceinline__ void weights(const Left& s, float4 p, float4 q, int v
   }
 }
 
-// Sum of the weights of the warp's segment [from, to), in every lane.
+// Sum of these over the warp's segment [from, to), in every lane.
 template <bool kWide>
 __device__ double segment_sum(const Left& s, int from, int to, int vocab, bool struck) {
   const int lane = threadIdx.x & 31;
@@ -298,7 +311,7 @@ verify_kernel(const Params p) {
     double w = r.p;
     if (p.draft != nullptr) {
       if (open) {
-        R = exchange(segment_sum<kWide>(left(c, 0), from, to, p.vocab, false));
+        R = 0.5 * exchange(segment_sum<kWide>(left(c, 0), from, to, p.vocab, false));
         open = false;
       }
       w = left_of(r.p, r.q, c);
@@ -377,9 +390,9 @@ verify_kernel(const Params p) {
 // CTAs per request: enough that each SM has about two, at most one for every
 // 2048 values of the vocabulary.
 int cluster_for(int requests, int vocab, int sms) {
-  int c = 1;
-  while (c < kMaxCluster && 2 * c * requests <= 4 * sms && c * 2048 < vocab) c *= 2;
-  return c;
+  const int fit = 2 * sms / requests, fill = (vocab + 2047) / 2048;
+  const int c = fit < fill ? fit : fill;
+  return c < 1 ? 1 : (c < kMaxCluster ? c : kMaxCluster);
 }
 
 }  // namespace verify
