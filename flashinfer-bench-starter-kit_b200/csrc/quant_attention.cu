@@ -53,7 +53,6 @@ constexpr int kBlockBytes = kTok * 128;      // 16384: 128 dims of a tile's code
 constexpr int kParts = 4;                    // blocks of codes
 constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
 constexpr int kCols = 8;                     // columns (rows of Q) of a softmax thread
-constexpr int kQueryWarps = 4;               // queries into parts
 constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
 constexpr float kRescaleThreshold = 6.0f;    // log2 units, see the softmax warps
@@ -67,12 +66,16 @@ template <int kR, bool kSparse>
 struct Shape {
   static constexpr int kSets = kR / kCols;
   static constexpr int kSoftWarps = 4 * kSets;
-  static constexpr int kLoadWarp = kSoftWarps;           // dense: TMA
-  static constexpr int kLogitWarp = kSoftWarps + 1;      // S^T, E^T (owns TMEM)
-  static constexpr int kValueWarp = kSoftWarps + 2;      // O^T
-  static constexpr int kQueryWarp = kSoftWarps + 4;
-  static constexpr int kGatherWarp = kQueryWarp + kQueryWarps;
-  static constexpr int kThreads = 32 * (kGatherWarp + (kSparse ? kGatherWarps : 0));
+  static constexpr int kLogitWarp = kSoftWarps;          // S^T, E^T (owns TMEM)
+  static constexpr int kValueWarp = kSoftWarps + 1;      // O^T
+  static constexpr int kQueryWarps = kSparse ? 2 : 4;    // queries into parts
+  static constexpr int kQueryWarp = kSoftWarps + 2;
+  static constexpr int kLoadWarp = kQueryWarp + kQueryWarps;    // dense: TMA
+  static constexpr int kGatherWarp = kQueryWarp + kQueryWarps;  // sparse
+  static constexpr int kThreads = 32 * (kSparse ? kGatherWarp + kGatherWarps : kLoadWarp + 1);
+  // Warps that take queries at the first segment.
+  static constexpr int kFirstWarps = kQueryWarps + kSoftWarps;
+  static_assert(kFirstWarps % kQueryWarps == 0, "arrivals at q_full");
   static constexpr int kQBufs = kR == 16 ? 2 : 1;
   static constexpr int kSBufs = kR == 16 ? 2 : 1;
   static constexpr int kQBlock = 2 * kR * 128;           // 128 dims of both parts
@@ -241,6 +244,11 @@ struct Walker {
   }
 };
 
+// `count` arrivals at once.
+__device__ __forceinline__ void mbar_arrive_many(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+
 // Three blocks of 8 consecutive columns of 32 lanes, with the wait for them in
 // the same statement.
 __device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[8], float (&b)[8],
@@ -342,6 +350,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   constexpr int kWarps = kThreads / 32;
   constexpr int kSoftWarps = Sh::kSoftWarps, kLoadWarp = Sh::kLoadWarp, kLogitWarp = Sh::kLogitWarp;
   constexpr int kValueWarp = Sh::kValueWarp, kQueryWarp = Sh::kQueryWarp, kGatherWarp = Sh::kGatherWarp;
+  constexpr int kQueryWarps = Sh::kQueryWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset: the compiler still knows it as shared)
   uint8_t* q_mem = smem + kOffQ;
@@ -382,7 +391,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     for (int x = 0; x < kBars; ++x) mbar_init(&bars[x], 1);
     for (int s = 0; s < 2; ++s) {
       if (kSparse) mbar_init(&kv_full[s * kParts + kParts - 1], 4);
-      mbar_init(&q_full[s], kQueryWarps);
+      mbar_init(&q_full[s], Sh::kFirstWarps);
       mbar_init(&q_empty[s], 1 + kSoftWarps);
       mbar_init(&s_empty[s], kSoftWarps);
     }
@@ -492,9 +501,106 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   Walker<kR, kSparse> walk(p, u0, u1, *found);
   Segment s;
 
-  if (warp == kLoadWarp) {
+  // ------------------------------------------------------------ queries into parts
+  // The query warps do it for all segments, a segment ahead of the softmax where
+  // there are two buffers; at the first one the softmax warps, which have nothing
+  // to do yet, take their share of the rows.  Lane l has a row's dims 16 l .. +15.
+  if (warp < kSoftWarps || (warp >= kQueryWarp && warp < kQueryWarp + kQueryWarps)) {
+    const bool helper = warp < kSoftWarps;
+    Walker<kR, kSparse> ahead = walk;
+    int segs = 0;
+    bool ok = true;
+    while (ok && ahead.next(s)) {
+      const int qb = segs % Sh::kQBufs;
+      const int rows = min(kR, s.r.rows - s.group * kR);
+      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
+      const int step = segs == 0 ? Sh::kFirstWarps : kQueryWarps;
+      uint8_t* to = q_mem + qb * Sh::kQBytes;
+      struct Raw {
+        uint4 c[2], pe;
+      };
+      auto load = [&](int r) {
+        Raw x;
+        x.c[0] = x.c[1] = x.pe = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.q_nope + (row_q + r) * kCkv) + 2 * lane;
+          x.c[0] = src[0];
+          x.c[1] = src[1];
+          if (lane < 8) x.pe = *(reinterpret_cast<const uint4*>(p.q_pe + (row_q + r) * kKpe) + lane);
+        }
+        return x;
+      };
+      int r = helper ? warp : warp - kQueryWarp + step - kQueryWarps;
+      Raw first = load(r), second = load(r + step);
+      // All lanes leave together.
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((segs / Sh::kQBufs) & 1) ^ 1, wctx));
+#pragma unroll 1
+      for (; ok && r < kR; r += step) {
+        const uint32_t x[8] = {first.c[0].x, first.c[0].y, first.c[0].z, first.c[0].w,
+                               first.c[1].x, first.c[1].y, first.c[1].z, first.c[1].w};
+        const uint4 now_pe = first.pe;
+        first = second;
+        second = load(r + 2 * step);  // two rows ahead
+        uint32_t most = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = max(most, max((x[k] << 16) & 0x7FFFFFFFu, x[k] & 0x7FFF0000u));
+        most = __reduce_max_sync(0xffffffffu, most);
+        // f = 2^7 over the largest value's power of two, at most 2^30: the
+        // logits of queries below that are 0 to all purposes.
+        const int exponent = most == 0u || most >= 0x7F800000u ? 127 : min(max(261 - static_cast<int>(most >> 23), 1), 157);
+        const float f = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
+        uint32_t pa[4], pb[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t a4 = 0u, b4 = 0u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // In half precision: its 11 bits hold q f down to 2^-24.
+            const uint32_t w = x[2 * k + h];
+            const __half2 v = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
+            const __nv_fp8x2_storage_t a2 =
+                __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(v), __NV_SATFINITE, __NV_E4M3);
+            const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(a2, __NV_E4M3));
+            const __half2 rest = __hmul2(__hsub2(v, back), __floats2half2_rn(16.f, 16.f));
+            const __nv_fp8x2_storage_t b2 =
+                __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(rest), __NV_SATFINITE, __NV_E4M3);
+            a4 |= static_cast<uint32_t>(a2) << (16 * h);
+            b4 |= static_cast<uint32_t>(b2) << (16 * h);
+          }
+          pa[k] = a4;
+          pb[k] = b4;
+        }
+        if (most >= 0x7F800000u) {  // an infinity or NaN: the row's logits are NaN
+#pragma unroll
+          for (int k = 0; k < 4; ++k) pa[k] = pb[k] = 0x7F7F7F7Fu;
+        }
+        uint8_t* at = to + (lane >> 3) * Sh::kQBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(at) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
+        *reinterpret_cast<uint4*>(at + kR * 128) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
+        if (lane < 8) {
+          uint32_t y[4] = {now_pe.x, now_pe.y, now_pe.z, now_pe.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[k] << 16) * f,
+                                                           __uint_as_float(y[k] & 0xFFFF0000u) * f);
+            y[k] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *reinterpret_cast<uint4*>(to + kParts * Sh::kQBlock + r * 128 + ((lane ^ (r & 7)) << 4)) =
+              make_uint4(y[0], y[1], y[2], y[3]);
+        }
+        if (lane == 0) c_s[qb * kMostRows + r] = p.scale_log2 / f;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_many(&q_full[qb], segs == 0 ? 1 : Sh::kFirstWarps / kQueryWarps);
+      ++segs;
+      if (helper) break;
+    }
+  }
+
+  if (!kSparse && warp == kLoadWarp) {
     // ------------------------------------------------------------ loads (dense)
-    if (!kSparse && elect_one()) {
+    if (elect_one()) {
       int i = 0;
       int parts = 0;  // issued
       bool ok = true;
@@ -617,93 +723,6 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       mbar_drain(&drain[1], 0, p.status);
     }
     __syncwarp();
-  } else if (warp >= kQueryWarp && warp < kQueryWarp + kQueryWarps) {
-    // ------------------------------------------------------------ queries
-    // A warp takes every fourth row of the group: lane l its dims 16 l .. +15.
-    constexpr int kEach = kR / kQueryWarps;
-    int segs = 0;
-    bool ok = true;
-    while (ok && walk.next(s)) {
-      const int qb = segs % Sh::kQBufs;
-      const int rows = min(kR, s.r.rows - s.group * kR);
-      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
-      uint8_t* to = q_mem + qb * Sh::kQBytes;
-#pragma unroll 1
-      for (int j0 = 0; j0 < kEach; j0 += 4) {
-        uint4 raw[4][2], pe[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = warp - kQueryWarp + 4 * (j0 + j);
-          raw[j][0] = raw[j][1] = pe[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows) {
-            const uint4* src = reinterpret_cast<const uint4*>(p.q_nope + (row_q + r) * kCkv) + 2 * lane;
-            raw[j][0] = src[0];
-            raw[j][1] = src[1];
-            if (lane < 8) pe[j] = *(reinterpret_cast<const uint4*>(p.q_pe + (row_q + r) * kKpe) + lane);
-          }
-        }
-        if (j0 == 0)  // all lanes leave together
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(&q_empty[qb], ((segs / Sh::kQBufs) & 1) ^ 1, wctx));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = warp - kQueryWarp + 4 * (j0 + j);
-          const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[j]);
-          uint32_t most = 0u;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) most = max(most, max((x[k] << 16) & 0x7FFFFFFFu, x[k] & 0x7FFF0000u));
-          most = __reduce_max_sync(0xffffffffu, most);
-          // f = 2^7 over the largest value's power of two, at most 2^30: the
-          // logits of queries below that are 0 to all purposes.
-          const int exponent = most == 0u || most >= 0x7F800000u ? 127 : min(max(261 - static_cast<int>(most >> 23), 1), 157);
-          const float f = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
-          uint32_t pa[4], pb[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t a4 = 0u, b4 = 0u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              // In half precision: its 11 bits hold q f down to 2^-24.
-              const uint32_t w = x[2 * k + h];
-              const __half2 v = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
-              const __nv_fp8x2_storage_t a2 =
-                  __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(v), __NV_SATFINITE, __NV_E4M3);
-              const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(a2, __NV_E4M3));
-              const __half2 rest = __hmul2(__hsub2(v, back), __floats2half2_rn(16.f, 16.f));
-              const __nv_fp8x2_storage_t b2 =
-                  __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(rest), __NV_SATFINITE, __NV_E4M3);
-              a4 |= static_cast<uint32_t>(a2) << (16 * h);
-              b4 |= static_cast<uint32_t>(b2) << (16 * h);
-            }
-            pa[k] = a4;
-            pb[k] = b4;
-          }
-          if (most >= 0x7F800000u) {  // an infinity or NaN: the row's logits are NaN
-#pragma unroll
-            for (int k = 0; k < 4; ++k) pa[k] = pb[k] = 0x7F7F7F7Fu;
-          }
-          uint8_t* at = to + (lane >> 3) * Sh::kQBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-          if (ok) {
-            *reinterpret_cast<uint4*>(at) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
-            *reinterpret_cast<uint4*>(at + kR * 128) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
-            if (lane < 8) {
-              uint32_t* y = reinterpret_cast<uint32_t*>(&pe[j]);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[k] << 16) * f,
-                                                               __uint_as_float(y[k] & 0xFFFF0000u) * f);
-                y[k] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-              *reinterpret_cast<uint4*>(to + kParts * Sh::kQBlock + r * 128 + ((lane ^ (r & 7)) << 4)) = pe[j];
-            }
-            if (lane == 0) c_s[qb * kMostRows + r] = p.scale_log2 / f;
-          }
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[qb]);
-      ++segs;
-    }
   } else if (kSparse && warp >= kGatherWarp) {
     // ------------------------------------------------------------ gather (sparse)
     // Four warps for each stage; a warp copies 32 of its tile's tokens, 16 bytes
