@@ -12,9 +12,10 @@
 //   q_nope f = a + b / 16 with a, b e4m3 and f a power of two for each row (its
 //     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
 //     b the other 4: the parts are exact down to 2^-22 of the row's largest.
-//   w = p s (weight by scale) = a + b + c with e5m2 parts of w in half precision,
-//     each to nearest: 3 + 3 + 3 bits, within 2^-9 of it (and it within 2^-11 of
-//     w), over the range of the type (2^31).  Weights in bf16, as a bf16 product
+//   w = p s (weight by scale) = a + b / 8 + c / 64 with e5m2 parts of w in half
+//     precision, each to nearest: 3 + 3 + 3 bits, within 2^-9 of it (and it within
+//     2^-11 of w) from 2^15 down to 2^-14, and within 2^-23 below: many light
+//     tokens beside a heavy one still count.  Weights in bf16, as a bf16 product
 //     would take them, are within 2^-8.
 // Per tile of 128 tokens and group of R rows (token, head)
 //   S^T[128, 2R] = C[128, 512] . [a b]^T    16 x (M128 N2R K32, e4m3)
@@ -55,9 +56,9 @@ constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
 constexpr int kCols = 8;                     // columns (rows of Q) of a softmax thread
 constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
-constexpr float kRescaleThreshold = 6.0f;    // log2 units, see the softmax warps
+constexpr float kRescaleThreshold = 8.0f;    // log2 units, see the softmax warps
 constexpr float kScaleGrowth = 4.0f;
-constexpr float kUnit = 128.0f;              // of weights: 2^6 x 4 x 128 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kUnit = 32.0f;               // of weights: 2^8 x 4 x 32 = 2^15 is the largest, e5m2 goes to 57344
 constexpr int kMostRows = 32;
 
 // R = 16 rows with two buffers of queries and of S^T, or 32 with one.  Softmax
@@ -320,9 +321,9 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-// Eight weights (at most 2^15) into their three e5m2 parts, in half precision:
-// rounded to its 11 bits, then each part to nearest.  An e5m2 value is the upper
-// byte of the same value in half precision.
+// Eight weights (at most 2^15) into their three e5m2 parts a + b / 8 + c / 64, in
+// half precision: rounded to its 11 bits, then each part to nearest.  An e5m2
+// value is the upper byte of the same value in half precision.
 __device__ __forceinline__ void in_parts(const float (&w)[8], uint2& a, uint2& b, uint2& c) {
   uint32_t part[3][4];
 #pragma unroll
@@ -333,7 +334,8 @@ __device__ __forceinline__ void in_parts(const float (&w)[8], uint2& a, uint2& b
       const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E5M2);
       part[x][k] = two;
       const uint32_t back = __byte_perm(two, 0u, 0x1404);
-      if (x < 2) h = __hsub2(h, *reinterpret_cast<const __half2*>(&back));  // exact
+      // What is left, exactly, times 8: at most 2^12 x 8.
+      if (x < 2) h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&back)), __floats2half2_rn(8.f, 8.f));
     }
   }
   a = make_uint2(__byte_perm(part[0][0], part[0][1], 0x5410), __byte_perm(part[0][2], part[0][3], 0x5410));
@@ -1013,7 +1015,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
           tmem_ld_three(at, at + kR, at + 2 * kR, o, b, r);
 #pragma unroll
-          for (int k = 0; k < C; ++k) o[k] = ((o[k] + b[k]) + r[k]) * factor_s[C * set + k];
+          for (int k = 0; k < C; ++k) o[k] = fmaf(fmaf(r[k], 0.125f, b[k]), 0.125f, o[k]) * factor_s[C * set + k];
         }
         if (s.whole) {
           // Neighbouring lanes swap halves, so that each stores two dims of one row.

@@ -102,7 +102,7 @@ def _softmax(q_nope, q_pe, c, e, scales, see, scale):
     out = w @ c
     err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -19) * w
     codes = torch.where(scales[:, None] == 0, 0.0, c.abs() / scales[:, None])
-    bound = err @ c.abs() + 2.0 ** -23 * largest * w.amax(1, keepdim=True) * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
+    bound = err @ c.abs() + 2.0 ** -27 * largest * w.amax(1, keepdim=True) * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
     return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
 
 
@@ -116,10 +116,10 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
       one rounding; a weight by ln 2 times its logit's and the lse's error.
     * A weight is rounded to half precision (2^-11 of itself), then split into three parts of 3 bits each, every one to
       nearest: within 2^-9 (1 + 2^-11), as each leaves at most 2^-3 of what it is given.  Where it is far below the largest,
-      it is within half the smallest step of the parts' type, 2^-17 (and of half precision, 2^-25): of weights times scales
-      over `ref` / 128, where ref is at most the largest scale of the context, and relative to a maximum that is at most
-      the true one.  Each token's code may so count 2^-23.9 times the largest scale times the largest weight too much or
-      too little.  The output is rounded to bf16, 2^-8 of itself.
+      it is within half the smallest step of the third part, 2^-17 / 64 (and of half precision, 2^-25): of weights times
+      scales over `ref` / 32, where ref is at most the largest scale of the context, and relative to a maximum that is at
+      most the true one.  Each token's code may so count 2^-27.6 times the largest scale times the largest weight too much
+      or too little.  The output is rounded to bf16, 2^-8 of itself.
     """
     T, H = q_nope.shape[:2]
     out = torch.full((T, H, CKV), math.nan, dtype=torch.float64)
