@@ -124,6 +124,7 @@ struct Params {
   int topk;
   int num_requests, num_rows, heads, max_pages;
   float scale_log2;
+  double by_ctas;           // 1 / CTAs
   __nv_bfloat16* out;
   float* lse;
   unsigned int* status;
@@ -178,10 +179,11 @@ __device__ __forceinline__ Request load_request(const Params& p, int b, bool& ba
   return r;
 }
 
-// CTA c of `ctas` has the units [start(c), start(c+1)), start(c) = floor(total c / ctas).
-__device__ __forceinline__ int slice_start(int total, int c, int ctas) {
-  const int q = total / ctas;
-  return q * c + (total - q * ctas) * c / ctas;
+// CTA c of `ctas` has the units [start(c), start(c+1)), start(c) = floor(total c /
+// ctas); by_ctas is 1 / ctas.  In 64-bit floating point the quotient is within
+// 2^-14 of what it is exactly, of which 1 / ctas is more than 2^-9.
+__device__ __forceinline__ int slice_start(int total, int c, double by_ctas) {
+  return static_cast<int>(fma(static_cast<double>(total) * c, by_ctas, 1.0 / 1024.0));
 }
 
 struct Start {
@@ -411,7 +413,6 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   griddep_wait();
 
   // ---- plan: total units, and the request that holds this slice's first one.
-  const int ctas = gridDim.x;
   const bool keeper = blockIdx.x == 0;  // writes the groups for join_kernel
   int2* groups_out = reinterpret_cast<int2*>(p.plan + kPlanGroups);
   int total = 0;
@@ -423,7 +424,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       for (int x = tid; x < p.num_rows * r.groups; x += kThreads)
         groups_out[x] = make_int2(x / r.groups * p.heads + x % r.groups * kR, min(kR, r.rows - x % r.groups * kR));
     if (tid == 0) {
-      const int u0 = slice_start(total, blockIdx.x, ctas);
+      const int u0 = slice_start(total, blockIdx.x, p.by_ctas);
       const int b = u0 / (r.groups * r.span), in = u0 - b * r.groups * r.span;
       Request mine = r;
       mine.row0 = b;
@@ -478,7 +479,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       total += warp_sums[w];
     }
     if (nothing) total = units = 0;
-    const int u0 = slice_start(total, blockIdx.x, ctas);
+    const int u0 = slice_start(total, blockIdx.x, p.by_ctas);
     if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
       for (int b = b_lo; b < b_hi; ++b) {
         bool bad;
@@ -497,7 +498,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     }
     __syncthreads();
   }
-  const int u0 = slice_start(total, blockIdx.x, ctas), u1 = slice_start(total, blockIdx.x + 1, ctas);
+  const int u0 = slice_start(total, blockIdx.x, p.by_ctas), u1 = slice_start(total, blockIdx.x + 1, p.by_ctas);
   const uint32_t tmem_base = *tmem_base_smem;
   const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
   Walker<kR, kSparse> walk(p, u0, u1, *found);
@@ -890,7 +891,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             const float now = moves ? mt : m;
             my_max[col] = now;
             my_minus[col] = now == -INFINITY ? 0.f : -now;
-            my_factor[col] = moves ? exp2f(m - mt) : 1.f;  // 0 when m was -inf
+            my_factor[col] = moves ? ex2_approx(m - mt) : 1.f;  // 0 when m was -inf
           }
           named_barrier_sync(1 + set, 128);
           float alpha[C];
@@ -1244,6 +1245,7 @@ int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaSt
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.status = reinterpret_cast<unsigned int*>(ws);
   p.wait_limit_ns = kWaitLimitNs;
+  p.by_ctas = 1.0 / info.num_sms;
   p.part_ml = reinterpret_cast<float2*>(ws + a.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + a.part_o);
   p.plan = reinterpret_cast<int*>(ws + a.plan);
