@@ -138,11 +138,17 @@ struct Request {
   int row0, n;              // first row, rows (tokens)
   int length;               // cached tokens; row j of n sees length - n + 1 + j
   int rows, groups, tiles;  // (token, head) rows
-  int span;                 // units per group: its tiles and kLead more for its start
+  int span;                 // units per group: its tiles and kLead<kR> more for its start
 };
 
-// What starting a group costs, in tiles.
-constexpr int kLead = 2;
+// What starting a group costs, in tiles (of 16 rows; of 32, whose tiles take longer
+// but whose start and end do as well): requests of 1000-3000 tokens, 64 of one row
+// of 16 heads 30.1 us at 1, 29.6 at 2, 30.6 at 3, 31.3 at 4; 64 of four rows of
+// 300-900 tokens 31.3, 31.2, 29.7, 29.6; 4 of 128 heads and 4000-12000 tokens 28.4,
+// 26.9, 25.6, 25.7.
+template <int kR>
+constexpr int kLead = kR == 16 ? 2 : 3;
+constexpr int kMostLead = 3;
 
 template <int kR, bool kSparse>
 __device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
@@ -175,13 +181,13 @@ __device__ __forceinline__ Request load_request(const Params& p, int b, bool& ba
   r.groups = (r.rows + kR - 1) / kR;
   // A row that sees nothing is written by a tile whose tokens are all masked.
   r.tiles = r.n == 0 ? 0 : max(1, (r.length + kTok - 1) / kTok);
-  r.span = r.n == 0 ? 0 : r.tiles + kLead;
+  r.span = r.n == 0 ? 0 : r.tiles + kLead<kR>;
   return r;
 }
 
 // CTA c of `ctas` has the units [start(c), start(c+1)), start(c) = floor(total c /
-// ctas); by_ctas is 1 / ctas.  In 64-bit floating point the quotient is within
-// 2^-14 of what it is exactly, of which 1 / ctas is more than 2^-9.
+// ctas); by_ctas is 1 / ctas.  In 64-bit floating point the quotient, at most 2^30,
+// is within 2^-21 of the exact one, whose fraction is a multiple of 1 / 256 or more.
 __device__ __forceinline__ int slice_start(int total, int c, double by_ctas) {
   return static_cast<int>(fma(static_cast<double>(total) * c, by_ctas, 1.0 / 1024.0));
 }
@@ -234,8 +240,8 @@ struct Walker {
       s.group = group;
       s.group_index = first_group + group;
       const int len = min(r.span - unit, u1 - u);
-      s.t0 = unit < kLead ? 0 : unit - kLead;
-      s.t1 = unit + len - kLead;
+      s.t0 = unit < kLead<kR> ? 0 : unit - kLead<kR>;
+      s.t1 = unit + len - kLead<kR>;
       s.whole = s.t0 == 0 && s.t1 == r.tiles;
       s.slot = u == u0 ? 0 : 1;
       u += len;
@@ -1297,7 +1303,7 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   if (!q_nope || !q_pe || !latent_cache || !seq_lens || !block_table || !output || !lse || !workspace || num_pages < 1 ||
       num_pages > 0x7FFFFFFE || max_pages < 1 || max_pages > (1 << 24) || (!cu_rows && num_rows != num_requests))
     return DSA_ERR_INVALID_ARGUMENT;
-  if (qattn::groups_bound(num_rows, num_heads, num_requests, 16) * (max_pages / 2 + 1 + qattn::kLead) > qattn::kMaxUnits)
+  if (qattn::groups_bound(num_rows, num_heads, num_requests, 16) * (max_pages / 2 + 1 + qattn::kMostLead) > qattn::kMaxUnits)
     return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned16(q_nope) || !aligned16(q_pe) || !aligned16(latent_cache) || !aligned16(output) || !aligned16(workspace) ||
       ((reinterpret_cast<uintptr_t>(seq_lens) | reinterpret_cast<uintptr_t>(block_table) |
@@ -1344,7 +1350,7 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
       topk < 1 || topk > 65536)
     return DSA_ERR_INVALID_ARGUMENT;
   const int64_t groups = static_cast<int64_t>(num_rows) * ((num_heads + 15) / 16);
-  if (groups > qattn::kMaxRows / 16 || groups * ((topk + qattn::kTok - 1) / qattn::kTok + qattn::kLead) > qattn::kMaxUnits)
+  if (groups > qattn::kMaxRows / 16 || groups * ((topk + qattn::kTok - 1) / qattn::kTok + qattn::kMostLead) > qattn::kMaxUnits)
     return DSA_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return DSA_OK;
   if (!q_nope || !q_pe || !latent_cache || !sparse_indices || !output || !lse || !workspace || num_pages < 1 ||

@@ -248,7 +248,7 @@ def attend(q_nope: torch.Tensor, q_pe: torch.Tensor, latent_cache: torch.Tensor,
             _fail_attend(f"without cu_rows there is one row for each of the {B} requests, not {T}")
     elif cu_rows.shape != (B + 1,):
         _fail_attend(f"cu_rows must be int32 [{B + 1}] (one more than block_table rows)")
-    if B > 65536 or (T * H // 16 + B) * (max_pages // 2 + 3) > 1 << 30:
+    if B > 65536 or (T * H // 16 + B) * (max_pages // 2 + 4) > 1 << 30:
         _fail_attend(f"{T} rows of {H} heads over {B} requests of {max_pages} pages are more than one call takes")
     bt, sl = int32_of("block_table", block_table, _fail_attend), int32_of("seq_lens", seq_lens, _fail_attend)
     cu = int32_of("cu_rows", cu_rows, _fail_attend) if cu_rows is not None else None
@@ -277,7 +277,7 @@ def attend_sparse(q_nope: torch.Tensor, q_pe: torch.Tensor, latent_cache: torch.
     if len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= 65536:
         _fail_sparse(f"sparse_indices must be [{T}, 1 to 65536]")
     groups = T * ((H + 15) // 16)
-    if groups > 1 << 20 or groups * (shape[1] // 128 + 3) > 1 << 30:
+    if groups > 1 << 20 or groups * (shape[1] // 128 + 4) > 1 << 30:
         _fail_sparse(f"{T} rows of {H} heads over {shape[1]} slots are more than one call takes")
     if pages > 0x7FFFFFFF // PAGE_SIZE:
         _fail_sparse("latent_cache has more slots than an index can name")

@@ -439,7 +439,7 @@ DSA_API size_t dsa_latent_attention_workspace_bytes(void);
  *                  logits; a row that sees nothing has -inf, output 0
  *
  * 1 <= num_heads <= 128; num_rows * num_heads <= 2^24, num_requests <= 65536 and
- * (num_rows * num_heads / 16 + num_requests) * (max_pages / 2 + 3) <= 2^30.  Tokens
+ * (num_rows * num_heads / 16 + num_requests) * (max_pages / 2 + 4) <= 2^30.  Tokens
  * that no row sees may hold anything; a visible one with NaN makes the output NaN.
  * Outputs that share memory with anything else: DSA_ERR_OVERLAP.  Data-dependent
  * errors: lengths that do not fit the table (clamped), cu_rows that do not fit
@@ -457,7 +457,7 @@ DSA_API int dsa_latent_attention_run(const void* q_nope, const void* q_pe, const
  *   sparse_indices [num_rows, topk] int32 slots, -1: none; topk <= 65536.  A slot
  *                  that is given twice counts twice.
  *
- * num_rows * ceil(num_heads / 16) <= 2^20 and that times (topk / 128 + 3) <= 2^30.
+ * num_rows * ceil(num_heads / 16) <= 2^20 and that times (topk / 128 + 4) <= 2^30.
  * Indices outside of [-1, num_pages * 64): DSA_DEV_BAD_INDEX, taken as -1. */
 DSA_API int dsa_latent_sparse_attention_run(const void* q_nope, const void* q_pe,
                                             const void* latent_cache, int64_t num_pages,
