@@ -102,7 +102,8 @@ constexpr int kOffMax = kOffFactor + 128;              // [32] running maxima
 constexpr int kOffMinus = kOffMax + 128;               // [32] what is added to logits
 constexpr int kOffMost = kOffMinus + 128;              // [4][4] largest scales
 constexpr int kOffC = kOffMost + 64;                   // [2][32] logits' factors
-constexpr int kSmemBytes = 1024 + kOffC + 256;
+constexpr int kOffInfo = kOffC + 256;                  // what the softmax warps need of the segments, 4 in turn
+constexpr int kSmemBytes = 1024 + kOffInfo + 4 * 48;
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 constexpr int kMaxRequests = 65536;
@@ -205,6 +206,13 @@ struct Segment {
   bool whole;  // covers the group's whole context
   int slot;    // of its record if it does not
 };
+
+// The same as the softmax warps read it from shared memory, where it takes none of
+// their registers.  t0 == t1: the end.
+struct SegmentInfo {
+  int b, t0, t1, row_q, rows, length, n, group, group_index, whole, slot, unused;
+};
+static_assert(sizeof(SegmentInfo) == 48, "segment");
 
 template <int kR, bool kSparse>
 struct Walker {
@@ -392,6 +400,8 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   float* minus_s = reinterpret_cast<float*>(smem + kOffMinus);
   float* most_s = reinterpret_cast<float*>(smem + kOffMost);
   float* c_s = reinterpret_cast<float*>(smem + kOffC);
+  // Entry x & 3 is written again behind q_empty of segment x + 2, at which all softmax warps are done with segment x.
+  SegmentInfo* info_s = reinterpret_cast<SegmentInfo*>(smem + kOffInfo);
 
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -518,11 +528,11 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     const bool helper = warp < kSoftWarps;
     Walker<kR, kSparse> ahead = walk;
     int segs = 0;
-    bool ok = true;
-    while (ok && ahead.next(s)) {
+    for (;;) {
+      const bool more = ahead.next(s);
       const int qb = segs % Sh::kQBufs;
-      const int rows = min(kR, s.r.rows - s.group * kR);
-      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
+      const int rows = more ? min(kR, s.r.rows - s.group * kR) : 0;
+      const int64_t row_q = more ? static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR : 0;
       const int step = segs == 0 ? Sh::kFirstWarps : kQueryWarps;
       uint8_t* to = q_mem + qb * Sh::kQBytes;
       struct Raw {
@@ -542,9 +552,15 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       int r = helper ? warp : warp - kQueryWarp + step - kQueryWarps;
       Raw first = load(r), second = load(r + step);
       // All lanes leave together.
-      ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((segs / Sh::kQBufs) & 1) ^ 1, wctx));
+      if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((segs / Sh::kQBufs) & 1) ^ 1, wctx))) break;
+      if (warp == kQueryWarp && lane == 0) {
+        SegmentInfo x = {};
+        if (more)
+          x = SegmentInfo{s.b, s.t0, s.t1, static_cast<int>(row_q), rows, s.r.length, s.r.n, s.group, s.group_index, s.whole, s.slot, 0};
+        info_s[segs & 3] = x;
+      }
 #pragma unroll 1
-      for (; ok && r < kR; r += step) {
+      for (; more && r < kR; r += step) {
         const uint32_t x[8] = {first.c[0].x, first.c[0].y, first.c[0].z, first.c[0].w,
                                first.c[1].x, first.c[1].y, first.c[1].z, first.c[1].w};
         const uint4 now_pe = first.pe;
@@ -603,7 +619,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive_many(&q_full[qb], segs == 0 ? 1 : Sh::kFirstWarps / kQueryWarps);
       ++segs;
-      if (helper) break;
+      if (helper || !more) break;
     }
   }
 
@@ -799,36 +815,40 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     // over the tokens and O rescaled.  Weights by scales are taken relative to
     // `ref`, the largest scale of the first tile, which moves in the same way
     // when a scale exceeds it more than kScaleGrowth times.
-    while (walk.next(s)) {
+    for (;;) {
       const int qb = segs % Sh::kQBufs;
-      const int rows = min(kR, s.r.rows - s.group * kR);
+      ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
+      // All warps of the set leave together.
+      if (!named_barrier_and(1 + set, 128, ok)) break;
+      const SegmentInfo& seg = info_s[segs & 3];
+      const int t0 = seg.t0, t1 = seg.t1, rows = seg.rows, length = seg.length;
+      if (t0 == t1) break;
       float l[C];
       bool unset = C * set < rows;  // some column has seen nothing yet
       float ref = 0.f, by_ref = 0.f;
       // (The first tile's values from minus_s count for nothing: its maxima are taken anyway.)
       if (e < C) my_max[e] = C * set + e < rows ? -INFINITY : INFINITY;
-      ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
       const float* my_c = c_s + qb * kMostRows + C * set;
 #pragma unroll
       for (int k = 0; k < C; ++k) l[k] = 0.f;
-      const int sure = s.r.length - s.r.n + 1;  // tokens that every row sees
-      const int32_t* bt = kSparse ? p.picked + static_cast<int64_t>(s.b) * p.topk
-                                  : p.block_table + static_cast<int64_t>(s.b) * p.max_pages;
+      const int sure = length - seg.n + 1;  // tokens that every row sees
+      const int32_t* bt = kSparse ? p.picked + static_cast<int64_t>(seg.b) * p.topk
+                                  : p.block_table + static_cast<int64_t>(seg.b) * p.max_pages;
       // Dense: the token's page; sparse: its slot.  -1 behind the context.
       auto place = [&](int t) {
         const int pos = t * kTok + tok;
-        return pos < s.r.length ? bt[kSparse ? pos : pos / kPage] : -1;
+        return pos < length ? bt[kSparse ? pos : pos / kPage] : -1;
       };
       const int places = kSparse ? p.num_pages * kPage : p.num_pages;
-      int next_place = place(s.t0);
-      for (int t = s.t0; t < s.t1; ++t, ++i) {
+      int next_place = place(t0);
+      for (int t = t0; t < t1; ++t, ++i) {
         const int st = i & 1, sb = i % Sh::kSBufs;
         const int pos = t * kTok + tok;
         const int at_place = next_place;
-        if (t + 1 < s.t1) next_place = place(t + 1);
+        if (t + 1 < t1) next_place = place(t + 1);
         const bool hidden = at_place < 0 || at_place >= places;  // seen by no row
         const bool tail = !kSparse && (t + 1) * kTok > sure;
-        if (!kSparse && hidden && pos < s.r.length && (e & 63) == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
+        if (!kSparse && hidden && pos < length && (e & 63) == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
         ok = ok && mbar_wait(&kv_full[st * kParts + kParts - 1], (i >> 1) & 1, wctx);
         const float scale = scale_s[st * kTok + tok];
         ok = ok && mbar_wait(&s_full[sb], (i / Sh::kSBufs) & 1, wctx);
@@ -845,12 +865,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 #pragma unroll
           for (int k = 0; k < C; ++k) x[k] = fmaf(fmaf(b[k], 0.0625f, x[k]), scale, pe[k]) * c[k];
         }
-        if (t == s.t1 - 1) {  // the queries' factors have been read
+        if (t == t1 - 1) {  // the queries' factors have been read
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_empty[qb]);
         }
         if (__any_sync(0xffffffffu, hidden || (tail && pos >= sure))) {
-          int row = s.group * kR + C * set;
+          int row = seg.group * kR + C * set;
           int draft = row / p.heads, left = (draft + 1) * p.heads - row;
 #pragma unroll
           for (int k = 0; k < C; ++k) {
@@ -913,7 +933,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             alpha[k] *= shrink;
             d[k] += x[k];
           }
-          if (t > s.t0) {
+          if (t > t0) {
             // O holds PV(i - 1) before it is rescaled.
             ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
             tc_fence_after();
@@ -995,14 +1015,14 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         red_set[C * sp + col] = sum;
       }
       named_barrier_sync(1 + set, 128);
-      const int64_t row_q = static_cast<int64_t>(s.r.row0) * p.heads + s.group * kR;
-      const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + s.slot;
-      if (tid == 0 && !s.whole) group_of[s.slot] = s.group_index;
+      const int64_t row_q = seg.row_q;
+      const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + seg.slot;
+      if (tid == 0 && !seg.whole) group_of[seg.slot] = seg.group_index;
       if (e < C) {
         const int col = C * set + e;
         const float sum = (red_set[e] + red_set[C + e]) + (red_set[2 * C + e] + red_set[3 * C + e]);
         const float unit = by_ref == 0.f ? 0.f : ref * (1.f / kUnit);
-        if (s.whole) {
+        if (seg.whole) {
           factor_s[col] = sum == 0.f ? 0.f : unit / sum;
           if (col < rows) p.lse[row_q + col] = sum == 0.f ? -INFINITY : max_s[col] + log2f(sum);
         } else {
@@ -1024,7 +1044,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 #pragma unroll
           for (int k = 0; k < C; ++k) o[k] = fmaf(fmaf(r[k], 0.125f, b[k]), 0.125f, o[k]) * factor_s[C * set + k];
         }
-        if (s.whole) {
+        if (seg.whole) {
           // Neighbouring lanes swap halves, so that each stores two dims of one row.
           const bool odd = lane & 1;
           __nv_bfloat16* out = p.out + row_q * kCkv + (dim & ~1);
