@@ -1370,8 +1370,8 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
       topk < 1 || topk > 65536)
     return DSA_ERR_INVALID_ARGUMENT;
   const int64_t groups = static_cast<int64_t>(num_rows) * ((num_heads + 15) / 16);
-  if (groups > qattn::kMaxRows / 16 || groups * ((topk + qattn::kTok - 1) / qattn::kTok + qattn::kMostLead) > qattn::kMaxUnits)
-    return DSA_ERR_INVALID_ARGUMENT;
+  static_assert(qattn::kMaxRows / 16 * (65536 / qattn::kTok + qattn::kMostLead) <= qattn::kMaxUnits, "units");
+  if (groups > qattn::kMaxRows / 16) return DSA_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return DSA_OK;
   if (!q_nope || !q_pe || !latent_cache || !sparse_indices || !output || !lse || !workspace || num_pages < 1 ||
       num_pages > 0x7FFFFFFF / qattn::kPage)

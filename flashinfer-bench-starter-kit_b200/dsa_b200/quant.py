@@ -276,8 +276,7 @@ def attend_sparse(q_nope: torch.Tensor, q_pe: torch.Tensor, latent_cache: torch.
     shape = sparse_indices.shape
     if len(shape) != 2 or shape[0] != T or not 1 <= shape[1] <= 65536:
         _fail_sparse(f"sparse_indices must be [{T}, 1 to 65536]")
-    groups = T * ((H + 15) // 16)
-    if groups > 1 << 20 or groups * (shape[1] // 128 + 4) > 1 << 30:
+    if T * ((H + 15) // 16) > 1 << 20:
         _fail_sparse(f"{T} rows of {H} heads over {shape[1]} slots are more than one call takes")
     if pages > 0x7FFFFFFF // PAGE_SIZE:
         _fail_sparse("latent_cache has more slots than an index can name")

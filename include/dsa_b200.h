@@ -457,7 +457,7 @@ DSA_API int dsa_latent_attention_run(const void* q_nope, const void* q_pe, const
  *   sparse_indices [num_rows, topk] int32 slots, -1: none; topk <= 65536.  A slot
  *                  that is given twice counts twice.
  *
- * num_rows * ceil(num_heads / 16) <= 2^20 and that times (topk / 128 + 4) <= 2^30.
+ * num_rows * ceil(num_heads / 16) <= 2^20.
  * Indices outside of [-1, num_pages * 64): DSA_DEV_BAD_INDEX, taken as -1. */
 DSA_API int dsa_latent_sparse_attention_run(const void* q_nope, const void* q_pe,
                                             const void* latent_cache, int64_t num_pages,
