@@ -1085,6 +1085,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 // kSplit-th record of a row, a thread four dims, many loads in flight.
 constexpr int kJoinRows = 4;       // most rows per block
 constexpr int kJoinDepth = 8;      // records whose loads a thread has in flight
+constexpr int kJoinFew = 4;        // records of a row that are loaded for all of the block's rows at once
 
 template <int kSplit>
 __global__ void __launch_bounds__(128 * kSplit)
@@ -1130,28 +1131,46 @@ join_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
   const int y0 = blockIdx.y * rows_per_block;
   const int rows = min(rows_per_block, info.y - y0);
   if (rows <= 0) return;
-  // The first records' loads of the first row need no weights: they go first.
+  // The loads that need no weights go first: all rows' where they have few
+  // records, or the first records of the first row.
   const int part = tid >> 7, d4 = tid & 127;
   const float4* src = reinterpret_cast<const float4*>(p.part_o) + y0 * (kCkv / 4) + d4;
-  float4 v[kJoinDepth];
+  constexpr int kHeld = kSplit == 1 ? kJoinRows * kJoinFew : kJoinDepth;
+  static_assert(kHeld >= kJoinDepth, "loads");
+  const bool few = kSplit == 1 && count <= kJoinFew;
+  float4 v[kHeld];
   auto load = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < kJoinDepth; ++j)
       if (k0 + kSplit * j < count)
         v[j] = __ldcg(src + static_cast<int64_t>(recs[k0 + kSplit * j]) * (kPartFloats / 4));
   };
-  load(part);
+  if (few) {
+#pragma unroll
+    for (int k = 0; k < kJoinFew; ++k) {
+      if (k < count) {
+        const float4* from = src + static_cast<int64_t>(recs[k]) * (kPartFloats / 4);
+#pragma unroll
+        for (int y = 0; y < kHeld / kJoinFew; ++y)
+          if (y < rows) v[y * kJoinFew + k] = __ldcg(from + y * (kCkv / 4));
+      }
+    }
+  } else {
+    load(part);
+  }
   for (int y = warp; y < rows; y += kThreads / 32) {
     float M = -INFINITY, L = 0.f;
     const float2* ml = p.part_ml + y0 + y;
+    float2 first = make_float2(-INFINITY, 0.f);  // of the lane's first record
     for (int k = lane; k < count; k += 32) {
-      const float m = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kMostRows].x);
-      M = fmaxf(M, m);
+      const float2 q = __ldcg(&ml[static_cast<int64_t>(recs[k]) * kMostRows]);
+      if (k == lane) first = q;
+      M = fmaxf(M, q.x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     for (int k = lane; k < count; k += 32) {
-      const float2 q = __ldcg(ml + static_cast<int64_t>(recs[k]) * kMostRows);
+      const float2 q = k == lane ? first : __ldcg(ml + static_cast<int64_t>(recs[k]) * kMostRows);
       // NaN sums have a place even where the max of what is left of a piece is -inf.
       const float w = q.x == -INFINITY ? (q.y == q.y ? 0.f : q.y) : exp2f(q.x - M);
       L = fmaf(q.y, w, L);
@@ -1165,38 +1184,48 @@ join_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
     if (lane == 0) p.lse[info.x + y0 + y] = L == 0.f ? -INFINITY : M + log2f(L);
   }
   __syncthreads();
+  auto add = [](float4& acc, const float4& x, float w) {
+    acc.x = fmaf(x.x, w, acc.x);
+    acc.y = fmaf(x.y, w, acc.y);
+    acc.z = fmaf(x.z, w, acc.z);
+    acc.w = fmaf(x.w, w, acc.w);
+  };
+  auto store = [&](const float4& acc, int y) {
+    const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x, acc.y), __floats2bfloat162_rn(acc.z, acc.w)};
+    *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(info.x) + y0 + y) * kCkv + 4 * d4) =
+        *reinterpret_cast<const uint2*>(h);
+  };
+  if (few) {
+#pragma unroll
+    for (int y = 0; y < kHeld / kJoinFew; ++y) {
+      if (y < rows) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kJoinFew; ++k)
+          if (k < count) add(acc, v[y * kJoinFew + k], weight[y][k]);
+        store(acc, y);
+      }
+    }
+    return;
+  }
   for (int y = 0; y < rows; ++y) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = part; k0 < count; k0 += kSplit * kJoinDepth) {
       if (y > 0 || k0 > part) load(k0);
 #pragma unroll
-      for (int j = 0; j < kJoinDepth; ++j) {
-        if (k0 + kSplit * j < count) {
-          const float w = weight[y][k0 + kSplit * j];
-          acc.x = fmaf(v[j].x, w, acc.x);
-          acc.y = fmaf(v[j].y, w, acc.y);
-          acc.z = fmaf(v[j].z, w, acc.z);
-          acc.w = fmaf(v[j].w, w, acc.w);
-        }
-      }
+      for (int j = 0; j < kJoinDepth; ++j)
+        if (k0 + kSplit * j < count) add(acc, v[j], weight[y][k0 + kSplit * j]);
     }
     src += kCkv / 4;
-    if (part > 0) other[part - 1][d4] = acc;
-    __syncthreads();
-    if (part == 0) {
+    if (kSplit > 1) {
+      if (part > 0) other[part - 1][d4] = acc;
+      __syncthreads();
 #pragma unroll
-      for (int k = 0; k < kSplit - 1; ++k) {
-        const float4 o = other[k][d4];
-        acc.x += o.x;
-        acc.y += o.y;
-        acc.z += o.z;
-        acc.w += o.w;
-      }
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x, acc.y), __floats2bfloat162_rn(acc.z, acc.w)};
-      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(info.x) + y0 + y) * kCkv + 4 * d4) =
-          *reinterpret_cast<const uint2*>(h);
+      for (int k = 0; k < kSplit - 1; ++k)
+        if (part == 0) add(acc, other[k][d4], 1.f);
+      __syncthreads();
     }
-    __syncthreads();
+    if (part == 0) store(acc, y);
   }
 }
 
