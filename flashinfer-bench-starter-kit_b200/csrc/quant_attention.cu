@@ -53,7 +53,6 @@ constexpr int kTok = 128;                    // tokens per tile: two pages
 constexpr int kBlockBytes = kTok * 128;      // 16384: 128 dims of a tile's codes, or its position part
 constexpr int kParts = 4;                    // blocks of codes
 constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
-constexpr int kCols = 8;                     // columns (rows of Q) of a softmax thread
 constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units, see the softmax warps
@@ -65,6 +64,7 @@ constexpr int kMostRows = 32;
 // warps come in sets of four, which have 8 columns each and a token a thread.
 template <int kR, bool kSparse>
 struct Shape {
+  static constexpr int kCols = kR / 2;                       // columns (rows of Q) of a softmax thread
   static constexpr int kSets = kR / kCols;
   static constexpr int kSoftWarps = 4 * kSets;
   static constexpr int kLogitWarp = kSoftWarps;          // S^T, E^T (owns TMEM)
@@ -76,7 +76,7 @@ struct Shape {
   static constexpr int kThreads = 32 * (kSparse ? kGatherWarp + kGatherWarps : kLoadWarp + 1);
   // Warps that take queries at the first segment.
   static constexpr int kFirstWarps = kQueryWarps + kSoftWarps;
-  static_assert(kFirstWarps % kQueryWarps == 0, "arrivals at q_full");
+  static_assert(kFirstWarps % kQueryWarps == 0 && (kCols == 8 || kCols == 16), "shape");
   static constexpr int kQBufs = kR == 16 ? 2 : 1;
   static constexpr int kSBufs = kR == 16 ? 2 : 1;
   static constexpr int kQBlock = 2 * kR * 128;           // 128 dims of both parts
@@ -96,7 +96,7 @@ static_assert(Shape<16, false>::kQBufs * Shape<16, false>::kQBytes == 36864 && S
 constexpr int kOffScale = kOffP + kTok * 128;          // [2][128]
 constexpr int kOffBar = kOffScale + 2 * kTok * 4;
 constexpr int kOffMisc = kOffBar + 256;
-constexpr int kOffRed = kOffMisc + 128;                // [4 sets][4 warps][8], planning: warp sums
+constexpr int kOffRed = kOffMisc + 128;                // [sets][4 warps][columns], planning: warp sums
 constexpr int kOffFactor = kOffRed + 512;              // [32]
 constexpr int kOffMax = kOffFactor + 128;              // [32] running maxima
 constexpr int kOffMinus = kOffMax + 128;               // [32] what is added to logits
@@ -266,8 +266,8 @@ __device__ __forceinline__ void mbar_arrive_many(uint64_t* bar, uint32_t count) 
   asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
 
-// Three blocks of 8 consecutive columns of 32 lanes, with the wait for them in
-// the same statement.
+// Three blocks of 8 or 16 consecutive columns of 32 lanes, with the wait for them
+// in the same statement.
 __device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[8], float (&b)[8],
                                               float (&c)[8]) {
   uint32_t r[24];
@@ -289,7 +289,35 @@ __device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t
   }
 }
 
-__device__ __forceinline__ void tmem_st8(uint32_t at, const float (&v)[8]) {
+__device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t c0, float (&a)[16], float (&b)[16],
+                                              float (&c)[16]) {
+  uint32_t r[48];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%48];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%49];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47}, [%50];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47])
+      : "r"(a0), "r"(b0), "r"(c0)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    a[i] = __uint_as_float(r[i]);
+    b[i] = __uint_as_float(r[16 + i]);
+    c[i] = __uint_as_float(r[32 + i]);
+  }
+}
+
+__device__ __forceinline__ void tmem_st(uint32_t at, const float (&v)[16]) { tmem_st16(at, v); }
+__device__ __forceinline__ void tmem_st(uint32_t at, const float (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
                "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
                "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
@@ -297,13 +325,13 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const float (&v)[8]) {
                : "memory");
 }
 
-// Eight values of each lane reduced over the warp: at each step a lane keeps half
-// of its columns and sends the others.  Lanes end with column `k`'s result.
-template <typename Op>
-__device__ __forceinline__ float over_tokens(float (&v)[8], int lane, int& k, Op op) {
+// kN values of each lane reduced over the warp: at each step a lane keeps half of
+// its columns and sends the others.  Lanes end with column `k`'s result.
+template <int kN, typename Op>
+__device__ __forceinline__ float over_tokens(float (&v)[kN], int lane, int& k, Op op) {
   k = 0;
 #pragma unroll
-  for (int half = 4, o = 16; half >= 1; half /= 2, o /= 2) {
+  for (int half = kN / 2, o = 16; half >= 1; half /= 2, o /= 2) {
     const bool up = lane & o;
 #pragma unroll
     for (int j = 0; j < half; ++j) {
@@ -312,21 +340,21 @@ __device__ __forceinline__ float over_tokens(float (&v)[8], int lane, int& k, Op
     }
     if (up) k += half;
   }
-  v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 2));
-  v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
+#pragma unroll
+  for (int o = 16 / kN; o >= 1; o /= 2) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
   return v[0];
 }
 
-__device__ __forceinline__ void load8(const float* from, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
-  v[0] = a.x;
-  v[1] = a.y;
-  v[2] = a.z;
-  v[3] = a.w;
-  v[4] = b.x;
-  v[5] = b.y;
-  v[6] = b.z;
-  v[7] = b.w;
+template <int kN>
+__device__ __forceinline__ void load_cols(const float* from, float (&v)[kN]) {
+#pragma unroll
+  for (int k = 0; k < kN / 4; ++k) {
+    const float4 x = reinterpret_cast<const float4*>(from)[k];
+    v[4 * k] = x.x;
+    v[4 * k + 1] = x.y;
+    v[4 * k + 2] = x.z;
+    v[4 * k + 3] = x.w;
+  }
 }
 
 // 16 bytes with cp.async, or zeros.
@@ -340,7 +368,7 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
 // Eight weights (at most 2^15) into their three e5m2 parts a + b / 8 + c / 64, in
 // half precision: rounded to its 11 bits, then each part to nearest.  An e5m2
 // value is the upper byte of the same value in half precision.
-__device__ __forceinline__ void in_parts(const float (&w)[8], uint2& a, uint2& b, uint2& c) {
+__device__ __forceinline__ void in_parts(const float* w, uint2& a, uint2& b, uint2& c) {
   uint32_t part[3][4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -363,7 +391,7 @@ template <int kR, bool kSparse>
 __global__ void __launch_bounds__(Shape<kR, kSparse>::kThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap kpe_map, const Params p) {
   using Sh = Shape<kR, kSparse>;
-  constexpr int C = kCols;
+  constexpr int C = Sh::kCols;
   constexpr int kThreads = Sh::kThreads;
   constexpr int kWarps = kThreads / 32;
   constexpr int kSoftWarps = Sh::kSoftWarps, kLoadWarp = Sh::kLoadWarp, kLogitWarp = Sh::kLogitWarp;
@@ -799,7 +827,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     const int tok = 32 * sp + lane;
     const uint32_t lane_base = static_cast<uint32_t>(32 * sp) << 16;
     const int e = tid & 127;  // thread of the set
-    float* red_set = red + 4 * C * set;  // [4][8]
+    float* red_set = red + 4 * C * set;  // [4][C]
     float* my_max = max_s + C * set;
     float* my_minus = minus_s + C * set;  // -m, or 0 where m is -inf
     float* my_factor = factor_s + C * set;
@@ -856,7 +884,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         float x[C];  // logits
         {
           float b[C], pe[C], c[C];
-          load8(my_c, c);
+          load_cols(my_c, c);
           const uint32_t at = tmem_base + lane_base + Sh::kColS + 3u * kR * sb + C * set;
           tmem_ld_three(at, at + kR, at + 2 * kR, x, b, pe);
           tc_fence_before();
@@ -882,10 +910,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           }
         }
         float d[C];
-        load8(my_minus, d);
+        load_cols(my_minus, d);
 #pragma unroll
         for (int k = 0; k < C; ++k) d[k] += x[k];
-        float most = fmaxf(fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])), fmaxf(fmaxf(d[4], d[5]), fmaxf(d[6], d[7])));
+        float most = fmaxf(d[0], d[1]);
+#pragma unroll
+        for (int k = 2; k < C; k += 2) most = fmaxf(most, fmaxf(d[k], d[k + 1]));
         if (named_barrier_or(1 + set, 128,
                              unset || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
           int col;
@@ -921,12 +951,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           }
           named_barrier_sync(1 + set, 128);
           float alpha[C];
-          load8(my_max, alpha);
+          load_cols(my_max, alpha);
           unset = false;
 #pragma unroll
           for (int k = 0; k < C; ++k) unset |= alpha[k] == -INFINITY;
-          load8(my_factor, alpha);
-          load8(my_minus, d);
+          load_cols(my_factor, alpha);
+          load_cols(my_minus, d);
 #pragma unroll
           for (int k = 0; k < C; ++k) {
             l[k] *= alpha[k];
@@ -948,9 +978,9 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
                 o1[k] *= alpha[k];
                 o2[k] *= alpha[k];
               }
-              tmem_st8(at, o);
-              tmem_st8(at + kR, o1);
-              tmem_st8(at + 2 * kR, o2);
+              tmem_st(at, o);
+              tmem_st(at + kR, o1);
+              tmem_st(at + 2 * kR, o2);
             }
             tmem_wait_st();
           }
@@ -982,23 +1012,30 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         // three parts.  Scales that are no number have made the logits NaN, and with
         // them l, where they are seen; here they count as 0.
         const float by = !hidden && scale < INFINITY ? scale * by_ref : 0.f;
-        uint2 pa, pb, pc;
+        uint2 pa[C / 8], pb[C / 8], pc[C / 8];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
           d[k] = ex2_approx(d[k]);
           l[k] += d[k];
           d[k] *= by;
         }
-        in_parts(d, pa, pb, pc);
+#pragma unroll
+        for (int k = 0; k < C / 8; ++k) in_parts(d + 8 * k, pa[k], pb[k], pc[k]);
         // P was last read by PV(i - 1).
         if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
         {
           // One 128-byte row per token: column n of part x at byte x R + n, 16-byte pieces swizzled by token & 7.
           uint8_t* at = p_mem + tok * 128;
-          auto to = [&](int byte) { return reinterpret_cast<uint2*>(at + (((byte >> 4) ^ (tok & 7)) << 4) + (byte & 8)); };
-          *to(C * set) = pa;
-          *to(kR + C * set) = pb;
-          *to(2 * kR + C * set) = pc;
+          auto put = [&](int byte, const uint2(&v)[C / 8]) {
+            uint8_t* to = at + (((byte >> 4) ^ (tok & 7)) << 4) + (byte & 8);
+            if constexpr (C == 16)
+              *reinterpret_cast<uint4*>(to) = make_uint4(v[0].x, v[0].y, v[C / 8 - 1].x, v[C / 8 - 1].y);
+            else
+              *reinterpret_cast<uint2*>(to) = v[0];
+          };
+          put(C * set, pa);
+          put(kR + C * set, pb);
+          put(2 * kR + C * set, pc);
         }
         fence_proxy_async_smem();
         tc_fence_before();
