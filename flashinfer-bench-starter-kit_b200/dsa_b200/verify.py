@@ -53,14 +53,12 @@ def _fail(msg: str) -> None:
     raise ValueError(f"dsa_verify.run: {msg}")
 
 
-def _probs(name: str, t: torch.Tensor, shape) -> int:
+def _pitch(name: str, t: torch.Tensor, rows: int, vocab: int) -> int:
     """Values from row to row."""
-    if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] < 1 or (shape is not None and t.shape != shape):
-        _fail(f"{name} must be float32 {'[T, V]' if shape is None else list(shape)}, got {t.dtype} {tuple(t.shape)}")
     pitch, step = t.stride()
-    if t.shape[0] <= 1:
-        pitch = max(pitch, t.shape[1])
-    if (step != 1 and t.shape[1] > 1) or pitch < t.shape[1]:
+    if rows <= 1:
+        pitch = max(pitch, vocab)
+    if (step != 1 and vocab > 1) or pitch < vocab:
         _fail(f"{name} must have contiguous rows (strides {t.stride()})")
     return pitch
 
@@ -68,6 +66,7 @@ def _probs(name: str, t: torch.Tensor, shape) -> int:
 def run(target_probs: torch.Tensor, draft_probs, draft_tokens: torch.Tensor, parents: torch.Tensor,
         cu_drafts: torch.Tensor, accept_u: torch.Tensor, sample_u: torch.Tensor, path: torch.Tensor,
         num_accepted: torch.Tensor, next_token: torch.Tensor) -> None:
+    # Every message is formatted only on failure: this runs once per step, and small batches wait for the host.
     at = target_probs.get_device()
     if at < 0 or (draft_probs is not None and draft_probs.get_device() != at) or draft_tokens.get_device() != at or \
             parents.get_device() != at or cu_drafts.get_device() != at or accept_u.get_device() != at or \
@@ -76,30 +75,37 @@ def run(target_probs: torch.Tensor, draft_probs, draft_tokens: torch.Tensor, par
         check_device(_fail, target_probs=target_probs, draft_probs=draft_probs, draft_tokens=draft_tokens, parents=parents,
                      cu_drafts=cu_drafts, accept_u=accept_u, sample_u=sample_u, path=path, num_accepted=num_accepted,
                      next_token=next_token)
-    pitch = _probs("target_probs", target_probs, None)
-    T, V = target_probs.shape
+    shape = target_probs.shape
+    if target_probs.dtype is not torch.float32 or len(shape) != 2 or shape[1] < 1:
+        _fail(f"target_probs must be float32 [T, V], got {target_probs.dtype} {tuple(shape)}")
+    T, V = shape
+    pitch = _pitch("target_probs", target_probs, T, V)
     draft, draft_pitch = 0, 0
     if draft_probs is not None:
-        draft_pitch = _probs("draft_probs", draft_probs, target_probs.shape)
-        draft = draft_probs.data_ptr()
-    if draft_tokens.shape != (T,) or parents.shape != (T,):
+        if draft_probs.dtype is not torch.float32 or draft_probs.shape != shape:
+            _fail(f"draft_probs must be float32 [{T}, {V}], got {draft_probs.dtype} {tuple(draft_probs.shape)}")
+        draft, draft_pitch = draft_probs.data_ptr(), _pitch("draft_probs", draft_probs, T, V)
+    one = (T,)
+    if draft_tokens.shape != one or parents.shape != one:
         _fail(f"draft_tokens and parents must be [{T}]")
     if cu_drafts.dim() != 1 or cu_drafts.shape[0] < 1:
         _fail("cu_drafts must be [B + 1]")
     B = cu_drafts.shape[0] - 1
-    if accept_u.dtype is not torch.float32 or accept_u.shape != (T,) or sample_u.dtype is not torch.float32 or \
-            sample_u.shape != (B,):
+    each = (B,)
+    if accept_u.dtype is not torch.float32 or accept_u.shape != one or sample_u.dtype is not torch.float32 or \
+            sample_u.shape != each:
         _fail(f"accept_u must be float32 [{T}] and sample_u float32 [{B}]")
-    if path.dtype is not torch.int32 or path.dim() != 2 or path.shape[0] != B or path.shape[1] < 1 or not path.is_contiguous():
+    shape = path.shape
+    if path.dtype is not torch.int32 or len(shape) != 2 or shape[0] != B or shape[1] < 1 or not path.is_contiguous():
         _fail(f"path must be contiguous int32 [{B}, at least 1]")
-    for name, t in (("num_accepted", num_accepted), ("next_token", next_token)):
-        if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
-            _fail(f"{name} must be contiguous int32 [{B}]")
-    W = path.shape[1]
+    W = shape[1]
+    if num_accepted.dtype is not torch.int32 or num_accepted.shape != each or not num_accepted.is_contiguous() or \
+            next_token.dtype is not torch.int32 or next_token.shape != each or not next_token.is_contiguous():
+        _fail(f"num_accepted and next_token must be contiguous int32 [{B}]")
     if T > 1 << 24 or B > 65536 or V > 1 << 28 or W > 1 << 16:
         _fail(f"{T} rows of {B} requests over {V} tokens, paths of {W}, are more than one call takes")
-    tok, par, cu = (int32_of(name, t, _fail) for name, t in
-                    (("draft_tokens", draft_tokens), ("parents", parents), ("cu_drafts", cu_drafts)))
+    tok, par, cu = (int32_of("draft_tokens", draft_tokens, _fail), int32_of("parents", parents, _fail),
+                    int32_of("cu_drafts", cu_drafts, _fail))
     au = accept_u if accept_u.is_contiguous() else accept_u.contiguous()
     su = sample_u if sample_u.is_contiguous() else sample_u.contiguous()
     if B == 0:
