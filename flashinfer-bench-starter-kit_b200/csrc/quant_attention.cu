@@ -30,6 +30,15 @@
 // per CTA; slices' pieces that do not cover their group's whole context are
 // written as fp32 records (slot 0: at the slice's start, slot 1: at its end) and
 // joined by join_kernel.
+//
+// Measured, attention with its join in replayed graphs: one row of 16 heads over
+// 64 x 65536 tokens 406-412 us (2.70 GB, 6.6 TB/s: HBM-bound; 434-466 back to back
+// under the power cap); 16 x 4096-16384 tokens, 1-4 rows 37 us (96 MB: start, end
+// and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 62 us (35
+// GFLOP: the softmax warps' chain of 2400 clocks a tile, where the products take
+// 1400); 300 x 2048 selected slots of 16 heads 93 us (406 MB; a kernel that only
+// reads these rows takes 87: half-kilobyte pieces at random).  About 8 us are a
+// call's start (plan, page ids, first tile, its maxima) and end, 3.5-9 its join.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -55,16 +64,23 @@ constexpr int kParts = 4;                    // blocks of codes
 constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
 constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
-constexpr float kRescaleThreshold = 8.0f;    // log2 units, see the softmax warps
+// A rescale of O costs its tile some 2300 clocks, and of two sets whichever needs one
+// holds up the other: at a threshold of 8 log2 units 2 of 34 tiles need one (normal
+// logits of spread 2.5, scales spread by e^0.3), at 6 four, at 4 six.
+constexpr float kRescaleThreshold = 8.0f;
 constexpr float kScaleGrowth = 4.0f;
 constexpr float kUnit = 32.0f;               // of weights: 2^8 x 4 x 32 = 2^15 is the largest, e5m2 goes to 57344
 constexpr int kMostRows = 32;
 
 // R = 16 rows with two buffers of queries and of S^T, or 32 with one.  Softmax
-// warps come in sets of four, which have 8 columns each and a token a thread.
+// warps come in two sets of four, which have half of the columns each and a token
+// a thread.
 template <int kR, bool kSparse>
 struct Shape {
-  static constexpr int kCols = kR / 2;                       // columns (rows of Q) of a softmax thread
+  // Columns (rows of Q) of a softmax thread.  32 rows as four sets of 8 columns, 16
+  // warps in 80 registers, take 63.6 us for 62 (128 heads), 31.7 for 29.9 (16 x 2
+  // rows of 16 heads, 4000-12000 tokens): what a warp does once a tile is half of it.
+  static constexpr int kCols = kR / 2;
   static constexpr int kSets = kR / kCols;
   static constexpr int kSoftWarps = 4 * kSets;
   static constexpr int kLogitWarp = kSoftWarps;          // S^T, E^T (owns TMEM)
@@ -821,7 +837,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     }
   } else if (warp < kSoftWarps) {
     // ------------------------------------------------------------ softmax
-    // Set `set` of four warps has the columns 8 set .. 8 set + 7 (rows of Q); in
+    // Set `set` of four warps has the columns C set .. C set + C - 1 (rows of Q); in
     // it thread (sp, lane) has token 32 sp + lane.
     const int set = warp >> 2, sp = warp & 3;
     const int tok = 32 * sp + lane;
@@ -1423,7 +1439,9 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.lse = lse;
-  // Groups of 16 rows or 32: 32 where requests have more than 16 rows, since a group reads the whole context.
+  // Groups of 16 rows or 32: 32 where requests have more than 16 rows on average, since a group reads the whole context.
+  // Graph replays in us, 16 rows against 32: 64 x 1000-3000 tokens of two rows of 16 heads 38.9 and 37.1, of 64 x 300-900
+  // of four 34.0 and 31.2, of one row of 128 heads and 64 x 500-1500 tokens 64.2 and 57.0.
   const bool wide = static_cast<int64_t>(num_rows) * num_heads > 16 * static_cast<int64_t>(num_requests);
   return qattn::launch(p, info, wide, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
