@@ -8,6 +8,10 @@ Operators (destination-passing, same signatures as the reference solutions):
 * ``dsa_b200.attention.run(q_nope, q_pe, ckv_cache, kpe_cache, sparse_indices,
   sm_scale, output, lse)``
 
+Next to them: ``tree`` and ``evict`` (trees of drafts, bounded caches), ``quant`` (the
+latent cache in 8 bits and attention over it), ``verify`` (drafts against the
+target's probabilities), ``cache`` (the indexer's keys).
+
 The kernels live in libdsa_b200.so (C ABI: include/dsa_b200.h); there is no
 CPU or library fallback.
 """
