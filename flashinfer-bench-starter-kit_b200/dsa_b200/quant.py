@@ -41,8 +41,8 @@ of the bf16 caches: with ``cu_rows`` None one row per request (plain decoding);
 else request r has the rows ``cu_rows[r] .. cu_rows[r+1]-1`` of ``q_nope`` / ``q_pe``,
 its last tokens (a chain of drafts, written to the cache before), and row j of n
 sees the first ``seq_lens[r] - n + 1 + j`` tokens.  ``attend_sparse`` reads the slots
-of ``sparse_indices`` [T, K] (-1: none), as ``dsa_b200.attention.run`` does.  Both take
-1 to 128 heads; ``lse`` is the base-2 log-sum-exp of the scaled logits; a row that
+of ``sparse_indices`` [T, K] (-1: none; a slot given twice counts twice), as
+``dsa_b200.attention.run`` does.  Both take 1 to 128 heads; ``lse`` is the base-2 log-sum-exp of the scaled logits; a row that
 sees nothing yields output 0 and lse -inf.  Tokens that no row sees may hold
 anything; a visible one with NaN makes the output NaN.  ``output`` may be ``q_nope``
 itself; other outputs over an input are refused.  Queries are used as they are
