@@ -62,7 +62,6 @@ constexpr int kTok = 128;                    // tokens per tile: two pages
 constexpr int kBlockBytes = kTok * 128;      // 16384: 128 dims of a tile's codes, or its position part
 constexpr int kParts = 4;                    // blocks of codes
 constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
-constexpr int kGatherWarps = 8;              // sparse: two groups of four, one for each stage
 constexpr int kTmemCols = 512;
 // A rescale of O costs its tile some 2300 clocks, and of two sets whichever needs one
 // holds up the other: at a threshold of 8 log2 units 2 of 34 tiles need one (normal
@@ -89,6 +88,9 @@ struct Shape {
   static constexpr int kQueryWarp = kSoftWarps + 2;
   static constexpr int kLoadWarp = kQueryWarp + kQueryWarps;    // dense: TMA
   static constexpr int kGatherWarp = kQueryWarp + kQueryWarps;  // sparse
+  // Two groups, one for each stage: four warps each, or two for 32 rows, whose softmax
+  // warps need the registers (with four 188 bytes spill; 64 rows of 128 heads 111.6 us for 106.3).
+  static constexpr int kGatherWarps = kR == 16 ? 8 : 4;
   static constexpr int kThreads = 32 * (kSparse ? kGatherWarp + kGatherWarps : kLoadWarp + 1);
   // Warps that take queries at the first segment.
   static constexpr int kFirstWarps = kQueryWarps + kSoftWarps;
@@ -454,7 +456,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   if (tid == 0) {
     for (int x = 0; x < kBars; ++x) mbar_init(&bars[x], 1);
     for (int s = 0; s < 2; ++s) {
-      if (kSparse) mbar_init(&kv_full[s * kParts + kParts - 1], 4);
+      if (kSparse) mbar_init(&kv_full[s * kParts + kParts - 1], Sh::kGatherWarps / 2);
       mbar_init(&q_full[s], Sh::kFirstWarps);
       mbar_init(&q_empty[s], 1 + kSoftWarps);
       mbar_init(&s_empty[s], kSoftWarps);
@@ -794,41 +796,49 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     __syncwarp();
   } else if (kSparse && warp >= kGatherWarp) {
     // ------------------------------------------------------------ gather (sparse)
-    // Four warps for each stage; a warp copies 32 of its tile's tokens, 16 bytes
-    // a lane: a token's codes with one instruction, four position parts with one.
-    const int group = (warp - kGatherWarp) >> 2, quarter = (warp - kGatherWarp) & 3;
+    // A group of warps for each stage; a warp copies 32 of its tile's tokens at a
+    // time, 16 bytes a lane: a token's codes with one instruction, four position
+    // parts with one.
+    constexpr int kEach = Sh::kGatherWarps / 2, kTurns = kTok / 32 / kEach;
+    const int group = (warp - kGatherWarp) / kEach, part = (warp - kGatherWarp) % kEach;
     int i = 0;
     bool ok = true;
     while (ok && walk.next(s)) {
       const int32_t* row = p.picked + static_cast<int64_t>(s.b) * p.topk;
       for (int t = s.t0; t < s.t1; ++t, ++i) {
         if ((i & 1) != group) continue;
-        const int pos = t * kTok + 32 * quarter + lane;
-        int slot = pos < p.topk ? row[pos] : -1;
-        if (slot < -1 || slot >= p.num_pages * kPage) {
-          atomicOr(p.status, DSA_DEV_BAD_INDEX);
-          slot = -1;
+        int slots[kTurns];
+#pragma unroll
+        for (int c = 0; c < kTurns; ++c) {
+          const int pos = t * kTok + 32 * (part * kTurns + c) + lane;
+          slots[c] = pos < p.topk ? row[pos] : -1;
+          if (slots[c] < -1 || slots[c] >= p.num_pages * kPage) {
+            atomicOr(p.status, DSA_DEV_BAD_INDEX);
+            slots[c] = -1;
+          }
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[group * kParts + kParts - 1], ((i >> 1) & 1) ^ 1, wctx));
         if (!ok) break;
         const uint32_t to = smem_u32(smem + group * kStageBytes);
-#pragma unroll 8
-        for (int n = 0; n < 32; ++n) {
-          const int x = __shfl_sync(0xffffffffu, slot, n);
-          const int r = 32 * quarter + n;
-          const uint8_t* src = p.cache + static_cast<int64_t>(max(x, 0) >> 6) * kPageBytes + (max(x, 0) & 63) * kCkv + 16 * lane;
-          cp_async16_or_zeros(to + (lane >> 3) * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src, x >= 0);
-        }
 #pragma unroll
-        for (int n = 0; n < 32; n += 4) {
-          const int x = __shfl_sync(0xffffffffu, slot, n + (lane >> 3));
-          const int r = 32 * quarter + n + (lane >> 3);
-          const uint8_t* src = p.cache + static_cast<int64_t>(max(x, 0) >> 6) * kPageBytes + kKpeAt + (max(x, 0) & 63) * (kKpe * 2) + 16 * (lane & 7);
-          cp_async16_or_zeros(to + kParts * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src, x >= 0);
+        for (int c = 0; c < kTurns; ++c) {
+          const int first = 32 * (part * kTurns + c), slot = slots[c];
+          auto page = [&](int x) { return p.cache + static_cast<int64_t>(max(x, 0) >> 6) * kPageBytes; };
+#pragma unroll 8
+          for (int n = 0; n < 32; ++n) {
+            const int x = __shfl_sync(0xffffffffu, slot, n), r = first + n;
+            cp_async16_or_zeros(to + (lane >> 3) * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
+                                page(x) + (max(x, 0) & 63) * kCkv + 16 * lane, x >= 0);
+          }
+#pragma unroll
+          for (int n = 0; n < 32; n += 4) {
+            const int x = __shfl_sync(0xffffffffu, slot, n + (lane >> 3)), r = first + n + (lane >> 3);
+            cp_async16_or_zeros(to + kParts * kBlockBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
+                                page(x) + kKpeAt + (max(x, 0) & 63) * (kKpe * 2) + 16 * (lane & 7), x >= 0);
+          }
+          cp_async4_or_zeros(smem_u32(scale_s + group * kTok + first + lane),
+                             page(slot) + kScaleAt + 4 * (max(slot, 0) & 63), slot >= 0);
         }
-        cp_async4_or_zeros(smem_u32(scale_s + group * kTok + 32 * quarter + lane),
-                           p.cache + static_cast<int64_t>(max(slot, 0) >> 6) * kPageBytes + kScaleAt + 4 * (max(slot, 0) & 63),
-                           slot >= 0);
         cp_async_wait_all();
         fence_proxy_async_smem();
         __syncwarp();
@@ -1330,7 +1340,8 @@ int setup(const DeviceInfo& info) {
     };
     g_status[info.device] = large(reinterpret_cast<const void*>(attend_kernel<16, false>)) &&
                                     large(reinterpret_cast<const void*>(attend_kernel<32, false>)) &&
-                                    large(reinterpret_cast<const void*>(attend_kernel<16, true>))
+                                    large(reinterpret_cast<const void*>(attend_kernel<16, true>)) &&
+                                    large(reinterpret_cast<const void*>(attend_kernel<32, true>))
                                 ? DSA_OK
                                 : DSA_ERR_CUDA;
   });
@@ -1360,7 +1371,9 @@ int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaSt
   const std::lock_guard<std::mutex> turn(turn_of(workspace));  // the attention and its join share the records
   const dim3 grid(info.num_sms);
   cudaError_t err;
-  if (sparse)
+  if (sparse && wide)
+    err = launch_programmatic(attend_kernel<32, true>, grid, dim3(Shape<32, true>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
+  else if (sparse)
     err = launch_programmatic(attend_kernel<16, true>, grid, dim3(Shape<16, true>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
   else if (wide)
     err = launch_programmatic(attend_kernel<32, false>, grid, dim3(Shape<32, false>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
@@ -1487,5 +1500,12 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.lse = lse;
-  return qattn::launch(p, info, false, workspace, reinterpret_cast<cudaStream_t>(stream));
+  // Groups of 16 heads or 32: 32 where a row has more than 16 and groups of 16 make more than 8 tiles an SM.  A group
+  // gathers its row's slots anew; where there are few, the shorter start and end of 16 win.  Graph replays in us, 16
+  // against 32, 2048 slots, rows x heads (tiles an SM at 16): 4 x 32 (0.9) 11.9 and 14.0, 16 x 64 (6.9) 24.7 and 24.9,
+  // 8 x 128 (6.9) 24.4 and 24.8, 64 x 24 (14) 45.0 and 41.0, 64 x 32 (14) 44.8 and 43.3, 64 x 64 (28) 75.0 and 62.3,
+  // 64 x 128 (55) 129.6 and 106.3.
+  const int64_t tiles = groups * ((topk + qattn::kTok - 1) / qattn::kTok);
+  const bool wide = num_heads > 16 && tiles > 8 * static_cast<int64_t>(info.num_sms);
+  return qattn::launch(p, info, wide, workspace, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -253,6 +253,9 @@ def sparse_case(T, heads, topk, pages, seed, holes=0.0, empty=()):
     (1, 16, 2048, 40, 0.0, ()), (3, 16, 2048, 70, 0.3, (1,)), (2, 16, 1, 1, 0.0, ()), (2, 16, 127, 3, 0.1, ()), (2, 16, 128, 3, 0.0, ()),
     (4, 1, 129, 9, 0.5, (0, 3)), (5, 33, 300, 20, 0.2, ()), (2, 128, 2048, 50, 0.9, ()), (160, 16, 2048, 500, 0.1, (7, 150)),
     (700, 8, 64, 30, 0.95, ()), (1, 16, 65536, 900, 0.0, ()),
+    # rows of more than 16 heads that make many tiles
+    (75, 17, 1111, 60, 0.1, (0, 40)), (40, 33, 2048, 300, 0.0, ()), (20, 128, 1025, 90, 0.7, (19,)), (161, 128, 64, 30, 0.2, ()),
+    (2, 24, 65536, 900, 0.1, ()),
 ])
 def test_sparse(cuda_device, T, heads, topk, pages, holes, empty):
     case = sparse_case(T, heads, topk, pages, T + topk, holes, empty)
