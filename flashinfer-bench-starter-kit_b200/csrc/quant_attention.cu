@@ -29,7 +29,8 @@
 // Units of work are (request, group, tile), cut into equal contiguous slices, one
 // per CTA; slices' pieces that do not cover their group's whole context are
 // written as fp32 records (slot 0: at the slice's start, slot 1: at its end) and
-// joined by join_kernel.
+// joined by join_kernel.  Small calls give each group to a cluster of CTAs, which
+// join their pieces through shared memory (together_for).
 //
 // Measured, attention with its join in replayed graphs: one row of 16 heads over
 // 64 x 65536 tokens 406-412 us (2.70 GB, 6.6 TB/s: HBM-bound; 434-466 back to back
@@ -168,6 +169,7 @@ struct Request {
 template <int kR>
 constexpr int kLead = kR == 16 ? 2 : 3;
 constexpr int kMostLead = 3;
+constexpr int kMostTogether = 8;             // CTAs of a cluster that share a group
 
 template <int kR, bool kSparse>
 __device__ __forceinline__ Request load_request(const Params& p, int b, bool& bad) {
@@ -383,6 +385,25 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
+__device__ __forceinline__ uint32_t in_cluster(const void* mine, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float2 ld_cluster(const float2* mine, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_cluster(mine, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster(const float4* mine, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(in_cluster(mine, rank))
+               : "memory");
+  return v;
+}
+
 // Eight weights (at most 2^15) into their three e5m2 parts a + b / 8 + c / 64, in
 // half precision: rounded to its 11 bits, then each part to nearest.  An e5m2
 // value is the upper byte of the same value in half precision.
@@ -405,7 +426,9 @@ __device__ __forceinline__ void in_parts(const float* w, uint2& a, uint2& b, uin
   c = make_uint2(__byte_perm(part[2][0], part[2][1], 0x5410), __byte_perm(part[2][2], part[2][3], 0x5410));
 }
 
-template <int kR, bool kSparse>
+// kTogether: each cluster of CTAs has one group, whose tiles they share alike and
+// whose pieces they join through shared memory.
+template <int kR, bool kSparse, bool kTogether>
 __global__ void __launch_bounds__(Shape<kR, kSparse>::kThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap kpe_map, const Params p) {
   using Sh = Shape<kR, kSparse>;
@@ -446,6 +469,11 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   float* minus_s = reinterpret_cast<float*>(smem + kOffMinus);
   float* most_s = reinterpret_cast<float*>(smem + kOffMost);
   float* c_s = reinterpret_cast<float*>(smem + kOffC);
+  // kTogether: the CTA's piece, over the first stage: O over the codes once its last
+  // product is done, m and l over the position part, which the last logits have used.
+  float* together_o = reinterpret_cast<float*>(smem);  // [kR][512]
+  float2* together_ml = reinterpret_cast<float2*>(smem + kParts * kBlockBytes);
+  static_assert(kR * kCkv * 4 <= kParts * kBlockBytes, "a piece");
   // Entry x & 3 is written again behind q_empty of segment x + 2, at which all softmax warps are done with segment x.
   SegmentInfo* info_s = reinterpret_cast<SegmentInfo*>(smem + kOffInfo);
 
@@ -475,17 +503,27 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   griddep_wait();
 
   // ---- plan: total units, and the request that holds this slice's first one.
+  // (kTogether: the total of groups, and the request that holds the cluster's.)
+  const unsigned int ctas = kTogether ? cluster_size() : 1u;
+  const int rank = kTogether ? static_cast<int>(cluster_rank()) : 0;
+  const int cluster = static_cast<int>(blockIdx.x / ctas);
+  auto first_tile = [&](int tiles, int of) { return static_cast<int>(static_cast<unsigned int>(tiles) * of / ctas); };  // < 2^27
   const bool keeper = blockIdx.x == 0;  // writes the groups for join_kernel
   int2* groups_out = reinterpret_cast<int2*>(p.plan + kPlanGroups);
   int total = 0;
   if constexpr (kSparse) {
     bool bad;
     const Request r = load_request<kR, true>(p, 0, bad);
-    total = p.num_rows * r.groups * r.span;  // every row alike
-    if (keeper)
+    total = p.num_rows * r.groups * (kTogether ? 1 : r.span);  // every row alike
+    if (!kTogether && keeper)
       for (int x = tid; x < p.num_rows * r.groups; x += kThreads)
         groups_out[x] = make_int2(x / r.groups * p.heads + x % r.groups * kR, min(kR, r.rows - x % r.groups * kR));
-    if (tid == 0) {
+    if (kTogether && tid == 0) {
+      const int b = cluster / r.groups;
+      Request mine = r;
+      mine.row0 = b;
+      *found = Start{b, 0, 0, mine, cluster - b * r.groups, kLead<kR> + first_tile(r.tiles, rank)};
+    } else if (tid == 0) {
       const int u0 = slice_start(total, blockIdx.x, p.by_ctas);
       const int b = u0 / (r.groups * r.span), in = u0 - b * r.groups * r.span;
       Request mine = r;
@@ -508,7 +546,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       const Request r = load_request<kR, false>(p, b, bad);
       if (b == b_lo) mine = r;
       if (p.cu != nullptr) decreasing |= p.cu[b + 1] < p.cu[b];
-      units += r.groups * r.span;
+      units += r.groups * (kTogether ? 1 : r.span);
       groups += r.groups;
       any_bad |= bad;
     }
@@ -541,17 +579,19 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       total += warp_sums[w];
     }
     if (nothing) total = units = 0;
-    const int u0 = slice_start(total, blockIdx.x, p.by_ctas);
-    if (!nothing && (keeper || (u0 >= before && u0 < before + units))) {
+    const int u0 = kTogether ? cluster : slice_start(total, blockIdx.x, p.by_ctas);
+    if (!nothing && ((!kTogether && keeper) || (u0 >= before && u0 < before + units))) {
       for (int b = b_lo; b < b_hi; ++b) {
         bool bad;
         const Request r = b == b_lo ? mine : load_request<kR, false>(p, b, bad);
-        const int un = r.groups * r.span;
-        if (u0 >= before && u0 < before + un) {
+        const int un = r.groups * (kTogether ? 1 : r.span);
+        if (kTogether && u0 >= before && u0 < before + un) {
+          *found = Start{b, 0, 0, r, u0 - before, kLead<kR> + first_tile(r.tiles, rank)};
+        } else if (u0 >= before && u0 < before + un) {
           const int group = (u0 - before) / r.span;
           *found = Start{b, before, gbefore, r, group, u0 - before - group * r.span};
         }
-        if (keeper)
+        if (!kTogether && keeper)
           for (int g = 0; g < r.groups; ++g)
             groups_out[gbefore + g] = make_int2(r.row0 * p.heads + g * kR, min(kR, r.rows - g * kR));
         before += un;
@@ -560,7 +600,13 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     }
     __syncthreads();
   }
-  const int u0 = slice_start(total, blockIdx.x, p.by_ctas), u1 = slice_start(total, blockIdx.x + 1, p.by_ctas);
+  int u0 = 0, u1 = 0;
+  if constexpr (kTogether) {
+    if (cluster < total) u1 = first_tile(found->r.tiles, rank + 1) - first_tile(found->r.tiles, rank);
+  } else {
+    u0 = slice_start(total, blockIdx.x, p.by_ctas);
+    u1 = slice_start(total, blockIdx.x + 1, p.by_ctas);
+  }
   const uint32_t tmem_base = *tmem_base_smem;
   const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
   Walker<kR, kSparse> walk(p, u0, u1, *found);
@@ -858,7 +904,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     float* my_minus = minus_s + C * set;  // -m, or 0 where m is -inf
     float* my_factor = factor_s + C * set;
     int* group_of = p.plan + 2 * blockIdx.x;  // of this CTA's records
-    if (tid == 0) group_of[0] = group_of[1] = -1;
+    if (!kTogether && tid == 0) group_of[0] = group_of[1] = -1;
     int i = 0, segs = 0;
     bool ok = true;
     // Online softmax in base 2.  A column's running max m is the same in every
@@ -1080,7 +1126,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       named_barrier_sync(1 + set, 128);
       const int64_t row_q = seg.row_q;
       const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + seg.slot;
-      if (tid == 0 && !seg.whole) group_of[seg.slot] = seg.group_index;
+      if (!kTogether && tid == 0 && !seg.whole) group_of[seg.slot] = seg.group_index;
       if (e < C) {
         const int col = C * set + e;
         const float sum = (red_set[e] + red_set[C + e]) + (red_set[2 * C + e] + red_set[3 * C + e]);
@@ -1090,7 +1136,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           if (col < rows) p.lse[row_q + col] = sum == 0.f ? -INFINITY : max_s[col] + log2f(sum);
         } else {
           factor_s[col] = unit;
-          p.part_ml[rec * kMostRows + col] = make_float2(max_s[col], sum);
+          (kTogether ? together_ml : p.part_ml + rec * kMostRows)[col] = make_float2(max_s[col], sum);
         }
       }
       ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
@@ -1120,7 +1166,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
                   odd ? __floats2bfloat162_rn(got, o[k + 1]) : __floats2bfloat162_rn(o[k], got);
           }
         } else {
-          float* to = p.part_o + rec * kPartFloats + C * set * kCkv + dim;
+          float* to = (kTogether ? together_o : p.part_o + rec * kPartFloats) + C * set * kCkv + dim;
 #pragma unroll
           for (int k = 0; k < C; ++k)
             if (C * set + k < rows) to[k * kCkv] = o[k];
@@ -1133,10 +1179,56 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   }
 
   tc_fence_before();
-  __syncthreads();
+  if constexpr (kTogether)
+    cluster_sync();
+  else
+    __syncthreads();
   if (warp == kLogitWarp) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
+  }
+  if constexpr (kTogether) {
+    // The pieces as join_kernel joins records, in the order of the ranks; a CTA has
+    // its share of the rows' 16-byte pieces.
+    if (ctas > 1 && cluster < total && found->r.tiles > 1) {  // else written whole
+      const Start& st = *found;
+      const int rows = min(kR, st.r.rows - st.group * kR), tiles = st.r.tiles;
+      const int64_t row_q = static_cast<int64_t>(st.r.row0) * p.heads + st.group * kR;
+      const int all = rows * (kCkv / 4), each = (all + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+      for (int x = rank * each + tid; x < min((rank + 1) * each, all); x += kThreads) {
+        const int y = x / (kCkv / 4), d4 = x % (kCkv / 4);
+        float2 ml[kMostTogether];
+        float4 o[kMostTogether];
+#pragma unroll
+        for (int k = 0; k < kMostTogether; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.f);
+          o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k < static_cast<int>(ctas) && first_tile(tiles, k) < first_tile(tiles, k + 1)) {
+            ml[k] = ld_cluster(together_ml + y, k);
+            o[k] = ld_cluster(reinterpret_cast<const float4*>(together_o) + x, k);
+          }
+        }
+        float M = ml[0].x, L = 0.f;
+#pragma unroll
+        for (int k = 1; k < kMostTogether; ++k) M = fmaxf(M, ml[k].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kMostTogether; ++k) {
+          const float w = ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.f : ml[k].y) : exp2f(ml[k].x - M);
+          L = fmaf(ml[k].y, w, L);
+          acc.x = fmaf(o[k].x, w, acc.x);
+          acc.y = fmaf(o[k].y, w, acc.y);
+          acc.z = fmaf(o[k].z, w, acc.z);
+          acc.w = fmaf(o[k].w, w, acc.w);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
+                                     __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+        *reinterpret_cast<uint2*>(p.out + (row_q + y) * kCkv + 4 * d4) = *reinterpret_cast<const uint2*>(h);
+        if (d4 == 0) p.lse[row_q + y] = L == 0.f ? -INFINITY : M + log2f(L);
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its piece
   }
 }
 
@@ -1295,6 +1387,8 @@ join_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
 // ------------------------------------------------------------------ host
 std::once_flag g_once[64];
 int g_status[64];
+constexpr int kTogetherSizes = 4;       // clusters of 8, 4, 2 and 1 CTAs
+int g_clusters[64][kTogetherSizes];     // of each size, how many run at once
 
 struct Layout {
   size_t part_ml, part_o, plan, bytes;
@@ -1332,20 +1426,84 @@ int check_outputs(const void* output, const float* lse, size_t rows_q, const Ran
   return DSA_OK;
 }
 
+cudaLaunchConfig_t together_config(bool sparse, unsigned int grid, int ctas, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(sparse ? Shape<16, true>::kThreads : Shape<16, false>::kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned int>(ctas);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
 int setup(const DeviceInfo& info) {
   if (static_cast<size_t>(kSmemBytes) > info.max_smem_optin || info.num_sms > kMaxCtas) return DSA_ERR_UNSUPPORTED_DEVICE;
   std::call_once(g_once[info.device], [&]() {
     auto large = [](const void* f) {
       return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
     };
-    g_status[info.device] = large(reinterpret_cast<const void*>(attend_kernel<16, false>)) &&
-                                    large(reinterpret_cast<const void*>(attend_kernel<32, false>)) &&
-                                    large(reinterpret_cast<const void*>(attend_kernel<16, true>)) &&
-                                    large(reinterpret_cast<const void*>(attend_kernel<32, true>))
-                                ? DSA_OK
-                                : DSA_ERR_CUDA;
+    const void* all[] = {reinterpret_cast<const void*>(attend_kernel<16, false, false>),
+                         reinterpret_cast<const void*>(attend_kernel<32, false, false>),
+                         reinterpret_cast<const void*>(attend_kernel<16, true, false>),
+                         reinterpret_cast<const void*>(attend_kernel<32, true, false>),
+                         reinterpret_cast<const void*>(attend_kernel<16, false, true>),
+                         reinterpret_cast<const void*>(attend_kernel<16, true, true>)};
+    g_status[info.device] = DSA_OK;
+    for (const void* f : all)
+      if (!large(f)) g_status[info.device] = DSA_ERR_CUDA;
+    for (int x = 0; x < kTogetherSizes && g_status[info.device] == DSA_OK; ++x) {
+      const int ctas = kMostTogether >> x;
+      cudaLaunchAttribute attr[2];
+      int dense = 0, sparse = 0;
+      cudaLaunchConfig_t cfg = together_config(false, ctas, ctas, attr);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&dense, attend_kernel<16, false, true>, &cfg) != cudaSuccess)
+        g_status[info.device] = DSA_ERR_CUDA;
+      cfg.blockDim = dim3(Shape<16, true>::kThreads);
+      if (cudaOccupancyMaxActiveClusters(&sparse, attend_kernel<16, true, true>, &cfg) != cudaSuccess)
+        g_status[info.device] = DSA_ERR_CUDA;
+      g_clusters[info.device][x] = dense < sparse ? dense : sparse;
+    }
   });
   return g_status[info.device];
+}
+
+// Upper bound of the groups of R rows of a call: with one row for each request
+// (all of sparse calls) what they are.
+int64_t most_groups(const Params& p, int r) {
+  return p.cu == nullptr ? static_cast<int64_t>(p.num_rows) * ((p.heads + r - 1) / r)
+                         : (static_cast<int64_t>(p.num_rows) * p.heads + static_cast<int64_t>(p.num_requests) * (r - 1)) / r;
+}
+
+// CTAs of the clusters that have a group of 16 rows each, or 0: slices.  Clusters,
+// as large as all groups' fit at once (15 of 8 CTAs, 33 of 4, 74 of 2, 148 of 1),
+// have no second launch, no records and no join (3.5 us and more on the device,
+// 3.5 on the host); slices even out what they have to do.  So clusters are taken
+// where a CTA has four tiles at most, and at most two more than a slice would (one
+// and a half where slots are gathered).  Their number is bounded by the width of
+// the table, which is what the host knows; lengths well below it lose little, as
+// a CTA's tiles end with its group's.  Graph replays in us, slices against clusters:
+//   requests of one row of 16 heads x tokens: 1 x 128 10.9 and 9.5, 1 x 1024 12.7 and
+//   11.3, 1 x 4096 (not taken) 13.4 and 14.5; 14 x 2048 15.2 and 13.5; 32 x 1024 15.8
+//   and 14.5; 40 x 1024 16.4 and 16.7; 128 x 512 20.1 and 15.1
+//   1 x 1024 of four rows 15.0 and 11.6, of 128 heads 15.5 and 12.1; 16 x 300 of 128
+//   heads 20.1 and 13.5; 4 x 4096 of 128 (not taken) 21.1 and 21.9
+//   rows of 2048 selected slots of 16 heads: 1 (not taken) 11.2 and 11.6, 5 12.2 and
+//   12.0, 14 13.8 and 12.7, 16 (not taken) 14.1 and 15.4, 32 18.9 and 17.5
+int together_for(const Params& p, const DeviceInfo& info) {
+  const int64_t groups = most_groups(p, 16);
+  const int64_t tiles = p.picked != nullptr ? (p.topk + kTok - 1) / kTok : (p.max_pages + 1) / 2;
+  int turn = 0;
+  while (turn < kTogetherSizes && groups > g_clusters[info.device][turn]) ++turn;
+  if (turn == kTogetherSizes) return 0;
+  const int ctas = kMostTogether >> turn;
+  const int64_t each = (tiles + ctas - 1) / ctas, slice = groups * (tiles + kLead<16>);
+  return each <= 4 && 2 * (each * info.num_sms - slice) <= (p.picked != nullptr ? 3 : 4) * info.num_sms ? ctas : 0;
 }
 
 // The attention and its join; `p` without what the workspace gives.
@@ -1360,6 +1518,7 @@ int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaSt
                         kPageBytes, kKpe, kPage);
     if (st != DSA_OK) return st;
   }
+  const int together = together_for(p, info);
   const Layout a = layout(info.num_sms);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.status = reinterpret_cast<unsigned int*>(ws);
@@ -1369,20 +1528,26 @@ int launch(Params& p, const DeviceInfo& info, bool wide, void* workspace, cudaSt
   p.part_o = reinterpret_cast<float*>(ws + a.part_o);
   p.plan = reinterpret_cast<int*>(ws + a.plan);
   const std::lock_guard<std::mutex> turn(turn_of(workspace));  // the attention and its join share the records
-  const dim3 grid(info.num_sms);
-  cudaError_t err;
-  if (sparse && wide)
-    err = launch_programmatic(attend_kernel<32, true>, grid, dim3(Shape<32, true>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
-  else if (sparse)
-    err = launch_programmatic(attend_kernel<16, true>, grid, dim3(Shape<16, true>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
-  else if (wide)
-    err = launch_programmatic(attend_kernel<32, false>, grid, dim3(Shape<32, false>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
-  else
-    err = launch_programmatic(attend_kernel<16, false>, grid, dim3(Shape<16, false>::kThreads), kSmemBytes, s, maps[0], maps[1], p);
+  if (together > 0) {
+    // All groups of 16, and the most tiles one can have.
+    const int64_t groups = most_groups(p, 16);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = together_config(sparse, static_cast<unsigned int>(groups * together), together, attr);
+    cfg.stream = s;
+    const cudaError_t e = sparse ? cudaLaunchKernelEx(&cfg, attend_kernel<16, true, true>, maps[0], maps[1], p)
+                                 : cudaLaunchKernelEx(&cfg, attend_kernel<16, false, true>, maps[0], maps[1], p);
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  }
+  auto go = [&](auto kernel, int threads) {
+    return launch_programmatic(kernel, dim3(info.num_sms), dim3(threads), kSmemBytes, s, maps[0], maps[1], p);
+  };
+  const cudaError_t err = sparse && wide ? go(attend_kernel<32, true, false>, Shape<32, true>::kThreads)
+                          : sparse       ? go(attend_kernel<16, true, false>, Shape<16, true>::kThreads)
+                          : wide         ? go(attend_kernel<32, false, false>, Shape<32, false>::kThreads)
+                                         : go(attend_kernel<16, false, false>, Shape<16, false>::kThreads);
   if (err != cudaSuccess) return DSA_ERR_CUDA;
   const int r = wide ? 32 : 16;
-  const int64_t groups = sparse ? static_cast<int64_t>(p.num_rows) * ((p.heads + r - 1) / r)
-                                : groups_bound(p.num_rows, p.heads, p.num_requests, r);
+  const int64_t groups = most_groups(p, r);
   const bool by_record = groups > 2 * info.num_sms;
   const unsigned int across = static_cast<unsigned int>(by_record ? 2 * info.num_sms : groups);
   const int rows = across <= 32 ? 1 : (across <= 96 ? 2 : kJoinRows);

@@ -38,11 +38,19 @@ def break_tokens(cache, slots):
     scales[p[::3], t[::3]] = 0
 
 
+@pytest.fixture(params=[0, 520], autouse=True, ids=["narrow", "wide"])
+def _table_width(request, monkeypatch):
+    """Every test with tables as wide as the lengths, where small calls run as clusters, and far wider, where all run as slices."""
+    monkeypatch.setattr(Dense, "width", request.param)
+
+
 class Dense:
+    width = 0
+
     def __init__(self, lens, rows, heads, seed=0, spread=0.3, extra=2, tail=0, q_scale=1.0, hidden="broken"):
         g = torch.Generator().manual_seed(seed)
         need = [max(1, (n + 63) // 64) for n in lens]
-        pool, width = sum(need) + extra, max(need) + 1
+        pool, width = sum(need) + extra, max(max(need) + 1, self.width)
         perm = torch.randperm(pool, generator=g)
         self.table, at = torch.full((len(lens), width), -1, dtype=torch.int32), 0
         for b, n in enumerate(need):
@@ -100,6 +108,15 @@ def run(c, scale=SCALE):
 ])
 def test_dense(cuda_device, lens, rows, heads):
     c = Dense(lens, rows, heads, seed=len(lens) + heads)
+    c.check(*run(c))
+
+
+@pytest.mark.parametrize("requests", [15, 16, 33, 34, 74, 75, 148, 149])
+def test_clusters_of_all_sizes(cuda_device, requests):
+    """Numbers of groups at which the clusters become smaller, and end; contexts of no token to nine tiles."""
+    g = torch.Generator().manual_seed(requests)
+    lens = torch.randint(0, 1100 if requests < 20 else 500, (requests,), generator=g).tolist()
+    c = Dense([0, *lens[1:]], None, 16, seed=requests)
     c.check(*run(c))
 
 
@@ -262,6 +279,17 @@ def test_sparse(cuda_device, T, heads, topk, pages, holes, empty):
     out, lse = torch.full((T, heads, 512), 7.0).bfloat16().cuda(), torch.full((T, heads), 7.0).cuda()
     quant.attend_sparse(*[t.cuda() for t in case], SCALE, out, lse)
     compare(out, lse, *oq.sparse_reference(*case, SCALE))
+
+
+@pytest.mark.parametrize("T,heads,topk,empty", [(1, 16, 1, ()), (3, 16, 300, (1,)), (14, 20, 129, (0, 13)), (30, 128, 256, ())])
+def test_sparse_with_empty_room(cuda_device, T, heads, topk, empty):
+    """Selections of few slots in rows of many give what rows without the room give, but for the order of their sums."""
+    case = sparse_case(T, heads, topk, 20, T + topk, 0.2, empty)
+    for room in (0, 4200):
+        wide = (*case[:3], torch.cat([case[3], torch.full((T, room), -1, dtype=torch.int32)], 1))
+        out, lse = torch.full((T, heads, 512), 7.0).bfloat16().cuda(), torch.full((T, heads), 7.0).cuda()
+        quant.attend_sparse(*[t.cuda() for t in wide], SCALE, out, lse)
+        compare(out, lse, *oq.sparse_reference(*case, SCALE))
 
 
 def test_sparse_reports_bad_indices(cuda_device):
