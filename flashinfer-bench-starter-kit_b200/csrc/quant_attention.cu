@@ -385,22 +385,28 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-__device__ __forceinline__ uint32_t in_cluster(const void* mine, int rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ float2 ld_cluster(const float2* mine, int rank) {
+// What CTA `rank` of the cluster has at this address of its shared memory, or zeros.
+__device__ __forceinline__ float2 ld_cluster_or_zeros(uint32_t at, int rank, bool real) {
   float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_cluster(mine, rank)) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 a;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
+      "@p ld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+      : "=&f"(v.x), "=&f"(v.y)
+      : "r"(at), "r"(rank), "r"(static_cast<uint32_t>(real))
+      : "memory");
   return v;
 }
-__device__ __forceinline__ float4 ld_cluster(const float4* mine, int rank) {
+__device__ __forceinline__ float4 ld_cluster4_or_zeros(uint32_t at, int rank, bool real) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(in_cluster(mine, rank))
-               : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 a;\n\t"
+      "setp.ne.u32 p, %6, 0;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
+      "mov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+      "@p ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=&f"(v.x), "=&f"(v.y), "=&f"(v.z), "=&f"(v.w)
+      : "r"(at), "r"(rank), "r"(static_cast<uint32_t>(real))
+      : "memory");
   return v;
 }
 
@@ -507,7 +513,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   const unsigned int ctas = kTogether ? cluster_size() : 1u;
   const int rank = kTogether ? static_cast<int>(cluster_rank()) : 0;
   const int cluster = static_cast<int>(blockIdx.x / ctas);
-  auto first_tile = [&](int tiles, int of) { return static_cast<int>(static_cast<unsigned int>(tiles) * of / ctas); };  // < 2^27
+  auto each_of = [&](int tiles) { return static_cast<int>((static_cast<unsigned int>(tiles) + ctas - 1u) / ctas); };
   const bool keeper = blockIdx.x == 0;  // writes the groups for join_kernel
   int2* groups_out = reinterpret_cast<int2*>(p.plan + kPlanGroups);
   int total = 0;
@@ -522,7 +528,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       const int b = cluster / r.groups;
       Request mine = r;
       mine.row0 = b;
-      *found = Start{b, 0, 0, mine, cluster - b * r.groups, kLead<kR> + first_tile(r.tiles, rank)};
+      *found = Start{b, 0, 0, mine, cluster - b * r.groups, kLead<kR> + min(rank * each_of(r.tiles), r.tiles)};
     } else if (tid == 0) {
       const int u0 = slice_start(total, blockIdx.x, p.by_ctas);
       const int b = u0 / (r.groups * r.span), in = u0 - b * r.groups * r.span;
@@ -586,7 +592,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         const Request r = b == b_lo ? mine : load_request<kR, false>(p, b, bad);
         const int un = r.groups * (kTogether ? 1 : r.span);
         if (kTogether && u0 >= before && u0 < before + un) {
-          *found = Start{b, 0, 0, r, u0 - before, kLead<kR> + first_tile(r.tiles, rank)};
+          *found = Start{b, 0, 0, r, u0 - before, kLead<kR> + min(rank * each_of(r.tiles), r.tiles)};
         } else if (u0 >= before && u0 < before + un) {
           const int group = (u0 - before) / r.span;
           *found = Start{b, before, gbefore, r, group, u0 - before - group * r.span};
@@ -602,7 +608,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   }
   int u0 = 0, u1 = 0;
   if constexpr (kTogether) {
-    if (cluster < total) u1 = first_tile(found->r.tiles, rank + 1) - first_tile(found->r.tiles, rank);
+    if (cluster < total) u1 = max(min(each_of(found->r.tiles), found->r.tiles + kLead<kR> - found->unit), 0);
   } else {
     u0 = slice_start(total, blockIdx.x, p.by_ctas);
     u1 = slice_start(total, blockIdx.x + 1, p.by_ctas);
@@ -1190,27 +1196,27 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
   if constexpr (kTogether) {
     // The pieces as join_kernel joins records, in the order of the ranks; a CTA has
     // its share of the rows' 16-byte pieces.
-    if (ctas > 1 && cluster < total && found->r.tiles > 1) {  // else written whole
+    const int tiles = cluster < total ? found->r.tiles : 0, share = each_of(tiles);
+    if (share < tiles) {  // else written whole
       const Start& st = *found;
-      const int rows = min(kR, st.r.rows - st.group * kR), tiles = st.r.tiles;
+      const int rows = min(kR, st.r.rows - st.group * kR);
       const int64_t row_q = static_cast<int64_t>(st.r.row0) * p.heads + st.group * kR;
-      const int all = rows * (kCkv / 4), each = (all + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+      const int all = rows * (kCkv / 4), each = each_of(all);
+      const uint32_t o_at = smem_u32(together_o), ml_at = smem_u32(together_ml);
       for (int x = rank * each + tid; x < min((rank + 1) * each, all); x += kThreads) {
         const int y = x / (kCkv / 4), d4 = x % (kCkv / 4);
         float2 ml[kMostTogether];
         float4 o[kMostTogether];
 #pragma unroll
-        for (int k = 0; k < kMostTogether; ++k) {
-          ml[k] = make_float2(-INFINITY, 0.f);
-          o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (k < static_cast<int>(ctas) && first_tile(tiles, k) < first_tile(tiles, k + 1)) {
-            ml[k] = ld_cluster(together_ml + y, k);
-            o[k] = ld_cluster(reinterpret_cast<const float4*>(together_o) + x, k);
-          }
-        }
-        float M = ml[0].x, L = 0.f;
+        for (int k = 0; k < kMostTogether; ++k) ml[k] = ld_cluster_or_zeros(ml_at + y * 8, k, k * share < tiles);
 #pragma unroll
-        for (int k = 1; k < kMostTogether; ++k) M = fmaxf(M, ml[k].x);
+        for (int k = 0; k < kMostTogether; ++k) o[k] = ld_cluster4_or_zeros(o_at + x * 16, k, k * share < tiles);
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMostTogether; ++k) {
+          if (k * share >= tiles) ml[k].x = -INFINITY;
+          M = fmaxf(M, ml[k].x);
+        }
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < kMostTogether; ++k) {
@@ -1484,17 +1490,18 @@ int64_t most_groups(const Params& p, int r) {
 // as large as all groups' fit at once (15 of 8 CTAs, 33 of 4, 74 of 2, 148 of 1),
 // have no second launch, no records and no join (3.5 us and more on the device,
 // 3.5 on the host); slices even out what they have to do.  So clusters are taken
-// where a CTA has four tiles at most, and at most two more than a slice would (one
-// and a half where slots are gathered).  Their number is bounded by the width of
+// where a CTA has four tiles at most, and at most two and a half more than a slice
+// would (two where slots are gathered).  Their number is bounded by the width of
 // the table, which is what the host knows; lengths well below it lose little, as
 // a CTA's tiles end with its group's.  Graph replays in us, slices against clusters:
-//   requests of one row of 16 heads x tokens: 1 x 128 10.9 and 9.5, 1 x 1024 12.7 and
-//   11.3, 1 x 4096 (not taken) 13.4 and 14.5; 14 x 2048 15.2 and 13.5; 32 x 1024 15.8
-//   and 14.5; 40 x 1024 16.4 and 16.7; 128 x 512 20.1 and 15.1
-//   1 x 1024 of four rows 15.0 and 11.6, of 128 heads 15.5 and 12.1; 16 x 300 of 128
-//   heads 20.1 and 13.5; 4 x 4096 of 128 (not taken) 21.1 and 21.9
-//   rows of 2048 selected slots of 16 heads: 1 (not taken) 11.2 and 11.6, 5 12.2 and
-//   12.0, 14 13.8 and 12.7, 16 (not taken) 14.1 and 15.4, 32 18.9 and 17.5
+//   requests of one row of 16 heads x tokens: 1 x 128 10.9 and 9.4, 1 x 1024 12.5 and
+//   10.5, 1 x 4096 (not taken) 13.4 and 13.7; 14 x 2048 15.0 and 12.7; 16 x 4096 (not
+//   taken) 18.1 and 20.5; 32 x 1024 16.5 and 13.6; 128 x 512 20.7 and 15.2
+//   1 x 1024 of four rows 15.1 and 10.6, of 128 heads 15.7 and 11.4; 16 x 300 of 128
+//   heads 20.5 and 13.6; 4 x 4096 of 128 (not taken) 21.2 and 21.0
+//   rows of 2048 selected slots of 16 heads: 1 11.2 and 10.8, 5 12.2 and 11.3, 14 13.8
+//   and 12.0, 16 (not taken) 14.2 and 14.8, 32 19.0 and 17.1
+// Sixteen CTAs (7 such clusters run at once) joined slower than they saved.
 int together_for(const Params& p, const DeviceInfo& info) {
   const int64_t groups = most_groups(p, 16);
   const int64_t tiles = p.picked != nullptr ? (p.topk + kTok - 1) / kTok : (p.max_pages + 1) / 2;
@@ -1503,7 +1510,7 @@ int together_for(const Params& p, const DeviceInfo& info) {
   if (turn == kTogetherSizes) return 0;
   const int ctas = kMostTogether >> turn;
   const int64_t each = (tiles + ctas - 1) / ctas, slice = groups * (tiles + kLead<16>);
-  return each <= 4 && 2 * (each * info.num_sms - slice) <= (p.picked != nullptr ? 3 : 4) * info.num_sms ? ctas : 0;
+  return each <= 4 && 2 * (each * info.num_sms - slice) <= (p.picked != nullptr ? 4 : 5) * info.num_sms ? ctas : 0;
 }
 
 // The attention and its join; `p` without what the workspace gives.
