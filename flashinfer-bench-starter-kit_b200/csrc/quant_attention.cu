@@ -36,8 +36,8 @@
 // 64 x 65536 tokens 406-412 us (2.70 GB, 6.6 TB/s: HBM-bound; 434-466 back to back
 // under the power cap); 16 x 4096-16384 tokens, 1-4 rows 37 us (96 MB: start, end
 // and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 62 us (35
-// GFLOP: the softmax warps' chain of 2400 clocks a tile, where the products take
-// 1400); 300 x 2048 selected slots of 16 heads 93 us (406 MB; a kernel that only
+// GFLOP: a tile's way through its stage takes 5200 clocks, load 800, S^T 1800, softmax
+// 1800, O^T 800, and two stages fit; the products alone take 1400 a tile); 300 x 2048 selected slots of 16 heads 93 us (406 MB; a kernel that only
 // reads these rows takes 87: half-kilobyte pieces at random).  About 8 us are a
 // call's start (plan, page ids, first tile, its maxima) and end, 3.5-9 its join.
 #include <cuda_bf16.h>
