@@ -37,9 +37,9 @@
 // under the power cap); 16 x 4096-16384 tokens, 1-4 rows 37 us (96 MB: start, end
 // and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 62 us (35
 // GFLOP: a tile's way through its stage takes 5200 clocks, load 800, S^T 1800, softmax
-// 1800, O^T 800, and two stages fit; the products alone take 1400 a tile); 300 x 2048 selected slots of 16 heads 93 us (406 MB; a kernel that only
-// reads these rows takes 87: half-kilobyte pieces at random).  About 8 us are a
-// call's start (plan, page ids, first tile, its maxima) and end, 3.5-9 its join.
+// 1800, O^T 800, and two stages fit; the products alone take 1400 a tile); 300 x 2048
+// selected slots of 16 heads 93 us (406 MB; a kernel that only reads these rows takes
+// 87: half-kilobyte pieces at random).  About 8 us are a call's start (plan, page ids, first tile, its maxima) and end, 3.5-9 its join.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -749,10 +749,11 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             ok = ok && mbar_wait(&kv_free[st * kParts + x], ((i >> 1) & 1) ^ 1, wctx);
             if (!ok) break;
             uint64_t* bar = &kv_full[st * kParts + x];
-            mbar_arrive_expect_tx(bar, x == kParts - 1 ? 2 * kBlockBytes + kTok * 4 : kBlockBytes);
+            mbar_arrive_expect_tx(bar, x == 0 ? 2 * kBlockBytes + kTok * 4 : kBlockBytes);
             tma_load_3d(dst + x * kBlockBytes, &codes_map, bar, 128 * x, 0, p0);
             tma_load_3d(dst + x * kBlockBytes + kBlockBytes / 2, &codes_map, bar, 128 * x, 0, p1);
-            if (x == kParts - 1) {
+            // The position part and the scales with the first block: what read those of tile i - 2 was done before its O^T.
+            if (x == 0) {
               tma_load_3d(dst + kParts * kBlockBytes, &kpe_map, bar, 0, 0, p0);
               tma_load_3d(dst + kParts * kBlockBytes + kBlockBytes / 2, &kpe_map, bar, 0, 0, p1);
               const uint8_t* s0 = p.cache + static_cast<int64_t>(p0 < p.num_pages ? p0 : 0) * kPageBytes + kScaleAt;
@@ -800,12 +801,14 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             for (int k = 0; k < 4; ++k)  // +32 bytes per K32 step
               umma_f8(d, a + x * (kBlockBytes >> 4) + 2 * k, bq + x * (Sh::kQBlock >> 4) + 2 * k, Sh::kIdescS,
                       x + k > 0 ? 1u : 0u);
+            if (x == 0) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_bf16(d + 2u * kR, a + kParts * (kBlockBytes >> 4) + 2 * k, bq + kParts * (Sh::kQBlock >> 4) + 2 * k,
+                          Sh::kIdescE, k > 0 ? 1u : 0u);
+            }
           }
           if (!ok) break;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16(d + 2u * kR, a + kParts * (kBlockBytes >> 4) + 2 * k, bq + kParts * (Sh::kQBlock >> 4) + 2 * k,
-                      Sh::kIdescE, k > 0 ? 1u : 0u);
           umma_commit(&s_full[sb]);
           if (t == s.t1 - 1) umma_commit(&q_empty[qb]);
         }
@@ -955,7 +958,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         const bool hidden = at_place < 0 || at_place >= places;  // seen by no row
         const bool tail = !kSparse && (t + 1) * kTok > sure;
         if (!kSparse && hidden && pos < length && (e & 63) == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
-        ok = ok && mbar_wait(&kv_full[st * kParts + kParts - 1], (i >> 1) & 1, wctx);
+        ok = ok && mbar_wait(&kv_full[st * kParts + (kSparse ? kParts - 1 : 0)], (i >> 1) & 1, wctx);
         const float scale = scale_s[st * kTok + tok];
         ok = ok && mbar_wait(&s_full[sb], (i / Sh::kSBufs) & 1, wctx);
         tc_fence_after();
