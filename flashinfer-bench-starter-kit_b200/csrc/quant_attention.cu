@@ -34,8 +34,8 @@
 //
 // Measured, attention with its join in replayed graphs: one row of 16 heads over
 // 64 x 65536 tokens 406-412 us (2.70 GB, 6.6 TB/s: HBM-bound; 434-466 back to back
-// under the power cap); 16 x 4096-16384 tokens, 1-4 rows 37 us (96 MB: start, end
-// and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 62 us (35
+// under the power cap); 16 x 4096-16384 tokens, 1-4 rows 36 us (96 MB: start, end
+// and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 61 us (35
 // GFLOP: a tile's way through its stage takes 5200 clocks, load 800, S^T 1800, softmax
 // 1800, O^T 800, and two stages fit; the products alone take 1400 a tile); 300 x 2048
 // selected slots of 16 heads 93 us (406 MB; a kernel that only reads these rows takes
