@@ -385,12 +385,13 @@ __device__ __forceinline__ void cp_async4_or_zeros(uint32_t dst, const void* src
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-// What CTA `rank` of the cluster has at this address of its shared memory, or zeros.
+// What CTA `rank` of the cluster has at this address of its shared memory, or zeros
+// (where it may be no rank of the cluster: its address is not formed then).
 __device__ __forceinline__ float2 ld_cluster_or_zeros(uint32_t at, int rank, bool real) {
   float2 v;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b32 a;\n\t"
-      "setp.ne.u32 p, %4, 0;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\tmov.u32 a, %2;\n\t@p mapa.shared::cluster.u32 a, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
       "@p ld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
       : "=&f"(v.x), "=&f"(v.y)
       : "r"(at), "r"(rank), "r"(static_cast<uint32_t>(real))
@@ -401,7 +402,7 @@ __device__ __forceinline__ float4 ld_cluster4_or_zeros(uint32_t at, int rank, bo
   float4 v;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b32 a;\n\t"
-      "setp.ne.u32 p, %6, 0;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
+      "setp.ne.u32 p, %6, 0;\n\tmov.u32 a, %4;\n\t@p mapa.shared::cluster.u32 a, %4, %5;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\t"
       "mov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
       "@p ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
       : "=&f"(v.x), "=&f"(v.y), "=&f"(v.z), "=&f"(v.w)
