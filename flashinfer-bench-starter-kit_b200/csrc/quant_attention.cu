@@ -12,17 +12,20 @@
 //   q_nope f = a + b / 16 with a, b e4m3 and f a power of two for each row (its
 //     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
 //     b the other 4: the parts are exact down to 2^-22 of the row's largest.
-//   w = p s (weight by scale) = a + b / 8 + c / 64 with e5m2 parts of w in half
-//     precision, each to nearest: 3 + 3 + 3 bits, within 2^-9 of it (and it within
-//     2^-11 of w) from 2^15 down to 2^-14, and within 2^-23 below: many light
-//     tokens beside a heavy one still count.  Weights in bf16, as a bf16 product
-//     would take them, are within 2^-8.
+//   w = p s (weight by scale) = a + b + (c + d) / 128 with e5m2 parts, each to
+//     nearest: 3 bits, then 4 more each (what is left has a sign and is less than
+//     the last step).  Within 2^-14 of w (6e-6 in the mean) from 2^15 down to 2^-9,
+//     and within 2^-23 below: many light tokens beside a heavy one still count.
+//     Three parts, 2^-11 (1.2e-4), would make a difference that outputs show: bf16
+//     has 2^-9, and one in fifteen was rounded to a neighbour (one in 300).
 // Per tile of 128 tokens and group of R rows (token, head)
 //   S^T[128, 2R] = C[128, 512] . [a b]^T    16 x (M128 N2R K32, e4m3)
 //   E^T[128, R]  = E[128, 64] . (q_pe f)^T   4 x (M128 NR K16, bf16)
-//   O^T[512, 3R] += C^T[512, 128] . [a b c]^T   4 x 4 x (M128 N3R K32, e4m3 x e5m2)
+//   O^T += C^T[512, 128] . [a c b d]^T       4 x 4 x (M128 N64 K32, e4m3 x e5m2)
 // so the parts lie along N, which costs the tensor core nothing up to N = 64: it
-// is fed at 128 bytes of A a clock.  A tile's 82 KB cross shared memory once in,
+// is fed at 128 bytes of A a clock.  Of 16 rows each part has its own 16 columns
+// of O^T; of 32, whose 128 would leave TMEM no room for S^T, a product of a and c
+// is followed by one of b and d into the same 64.  A tile's 82 KB cross shared memory once in,
 // and once and a half out, against three and a half times for bf16 copies of it
 // (225 KB, 1750 clocks, where its share of the HBM rate takes 3500).
 //
@@ -70,7 +73,9 @@ constexpr int kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;
 constexpr float kScaleGrowth = 4.0f;
 constexpr float kUnit = 32.0f;               // of weights: 2^8 x 4 x 32 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kLowUnit = 1.0f / 128.0f;    // of their last two parts: what the first two leave is below 2^-7 of a weight
 constexpr int kMostRows = 32;
+constexpr int kColsO = 64;                   // of O^T for 128 dims
 
 // R = 16 rows with two buffers of queries and of S^T, or 32 with one.  Softmax
 // warps come in two sets of four, which have half of the columns each and a token
@@ -101,11 +106,12 @@ struct Shape {
   static constexpr int kQBlock = 2 * kR * 128;           // 128 dims of both parts
   static constexpr int kQBytes = kParts * kQBlock + kR * 128;
   static constexpr uint32_t kColS = 0;                   // a: 0, b: R, e: 2R of each buffer
-  static constexpr uint32_t kColO = kSBufs * 3 * kR;     // 4 blocks of 128 dims x 3R columns
-  static_assert(kColO + kParts * 3 * kR <= kTmemCols, "TMEM");
+  static constexpr uint32_t kColO = kSBufs * 3 * kR;     // 4 blocks of 128 dims x 64 columns
+  static constexpr int kSums = kColsO / kR;              // of a row: of a, c, b, d, or of a + b, c + d
+  static_assert(kColO + kParts * kColsO <= kTmemCols && kSums * kCols == 32, "TMEM");
   static constexpr uint32_t kIdescS = idesc_make(0, 0, false, false, 128, 2 * kR);
   static constexpr uint32_t kIdescE = idesc_make(1, 1, false, false, 128, kR);
-  static constexpr uint32_t kIdescO = idesc_make(0, 1, true, true, 128, 3 * kR);  // e4m3 codes, e5m2 weights
+  static constexpr uint32_t kIdescO = idesc_make(0, 1, true, true, 128, kColsO);  // e4m3 codes, e5m2 weights
 };
 
 constexpr int kOffQ = 2 * kStageBytes;                 // 163840
@@ -336,6 +342,49 @@ __device__ __forceinline__ void tmem_ld_three(uint32_t a0, uint32_t b0, uint32_t
   }
 }
 
+// A row's sums of 8 or 16 columns: 4 blocks of 8, 16 apart, or 2 of 16, 32 apart.
+__device__ __forceinline__ void tmem_ld_sums(uint32_t at, float (&v)[4][8]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at), "r"(at + 16), "r"(at + 32), "r"(at + 48)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i / 8][i % 8] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_ld_sums(uint32_t at, float (&v)[2][16]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at), "r"(at + 32)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i / 16][i % 16] = __uint_as_float(r[i]);
+}
+
+// The row's O from its sums.
+__device__ __forceinline__ float whole_sum(const float (&v)[4][8], int k) {
+  return fmaf(v[1][k] + v[3][k], kLowUnit, v[0][k] + v[2][k]);
+}
+__device__ __forceinline__ float whole_sum(const float (&v)[2][16], int k) { return fmaf(v[1][k], kLowUnit, v[0][k]); }
+
 __device__ __forceinline__ void tmem_st(uint32_t at, const float (&v)[16]) { tmem_st16(at, v); }
 __device__ __forceinline__ void tmem_st(uint32_t at, const float (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
@@ -411,26 +460,32 @@ __device__ __forceinline__ float4 ld_cluster4_or_zeros(uint32_t at, int rank, bo
   return v;
 }
 
-// Eight weights (at most 2^15) into their three e5m2 parts a + b / 8 + c / 64, in
-// half precision: rounded to its 11 bits, then each part to nearest.  An e5m2
-// value is the upper byte of the same value in half precision.
-__device__ __forceinline__ void in_parts(const float* w, uint2& a, uint2& b, uint2& c) {
-  uint32_t part[3][4];
+// Eight weights (at most 2^15) into their four e5m2 parts a + b + (c + d) / 128, in
+// the order a, c, b, d.  In half precision: the weight's upper 11 bits, from which
+// a and b are taken without rounding, and what they leave with its lower bits, to
+// 11 bits more.  An e5m2 value is the upper byte of the same value in half
+// precision; half a step added below it rounds (a carry moves the exponent), in two
+// integer operations (128 heads 71.0 us, with conversions 72.1; with three parts by
+// conversions 62.1).  (NaN may become 0 here; its row's sum l is NaN.)
+__device__ __forceinline__ void in_parts(const float* w, uint2 (&out)[4]) {
+  uint32_t part[4][4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    __half2 h = __floats2half2_rn(w[2 * k], w[2 * k + 1]);
+    const float u0 = __uint_as_float(__float_as_uint(w[2 * k]) & 0xFFFFE000u);
+    const float u1 = __uint_as_float(__float_as_uint(w[2 * k + 1]) & 0xFFFFE000u);
+    __half2 h = __floats2half2_rn(u0, u1);
+    const __half2 lower = __floats2half2_rn(w[2 * k] - u0, w[2 * k + 1] - u1);
 #pragma unroll
-    for (int x = 0; x < 3; ++x) {
-      const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E5M2);
-      part[x][k] = two;
-      const uint32_t back = __byte_perm(two, 0u, 0x1404);
-      // What is left, exactly, times 8: at most 2^12 x 8.
-      if (x < 2) h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&back)), __floats2half2_rn(8.f, 8.f));
+    for (int x = 0; x < 4; ++x) {
+      if (x == 2) h = __hmul2(__hadd2(h, lower), __float2half2_rn(1.0f / kLowUnit));
+      const uint32_t two = (*reinterpret_cast<const uint32_t*>(&h) + 0x00800080u) & 0xFF00FF00u;
+      part[x < 2 ? 2 * x : 2 * x - 3][k] = two;
+      if (x < 3) h = __hsub2(h, *reinterpret_cast<const __half2*>(&two));  // exact
     }
   }
-  a = make_uint2(__byte_perm(part[0][0], part[0][1], 0x5410), __byte_perm(part[0][2], part[0][3], 0x5410));
-  b = make_uint2(__byte_perm(part[1][0], part[1][1], 0x5410), __byte_perm(part[1][2], part[1][3], 0x5410));
-  c = make_uint2(__byte_perm(part[2][0], part[2][1], 0x5410), __byte_perm(part[2][2], part[2][3], 0x5410));
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    out[x] = make_uint2(__byte_perm(part[x][0], part[x][1], 0x7531), __byte_perm(part[x][2], part[x][3], 0x7531));
 }
 
 // kTogether: each cluster of CTAs has one group, whose tiles they share alike and
@@ -838,9 +893,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 #pragma unroll
           for (int mb = 0; mb < kParts; ++mb) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // a K32 step is 32 token rows of 128 bytes
-              umma_f8(tmem_base + Sh::kColO + 3u * kR * mb, a + mb * (kBlockBytes >> 4) + kk * (4096 >> 4),
-                      p_desc + kk * (4096 >> 4), Sh::kIdescO, kk > 0 ? 1u : more);
+            for (int kk = 0; kk < 4; ++kk) {  // a K32 step is 32 token rows of 128 bytes
+              const uint32_t d = tmem_base + Sh::kColO + kColsO * mb;
+              const uint64_t ak = a + mb * (kBlockBytes >> 4) + kk * (4096 >> 4), pk = p_desc + kk * (4096 >> 4);
+              umma_f8(d, ak, pk, Sh::kIdescO, kk > 0 ? 1u : more);
+              if (kR == 32) umma_f8(d, ak, pk + (kColsO >> 4), Sh::kIdescO, 1u);  // the rows' other 64 bytes
+            }
             umma_commit(&kv_free[st * kParts + mb]);
           }
         }
@@ -1051,18 +1109,15 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
             tc_fence_after();
 #pragma unroll 1
             for (int mb = 0; mb < kParts; ++mb) {
-              const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
-              float o[C], o1[C], o2[C];
-              tmem_ld_three(at, at + kR, at + 2 * kR, o, o1, o2);
+              const uint32_t at = tmem_base + lane_base + Sh::kColO + kColsO * mb + C * set;
+              float o[Sh::kSums][C];
+              tmem_ld_sums(at, o);
 #pragma unroll
-              for (int k = 0; k < C; ++k) {
-                o[k] *= alpha[k];
-                o1[k] *= alpha[k];
-                o2[k] *= alpha[k];
+              for (int x = 0; x < Sh::kSums; ++x) {
+#pragma unroll
+                for (int k = 0; k < C; ++k) o[x][k] *= alpha[k];
+                tmem_st(at + kR * x, o[x]);
               }
-              tmem_st(at, o);
-              tmem_st(at + kR, o1);
-              tmem_st(at + 2 * kR, o2);
             }
             tmem_wait_st();
           }
@@ -1091,10 +1146,10 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           }
         }
         // Weights (of d = -inf, 0; NaN stays), and their products with the scale in
-        // three parts.  Scales that are no number have made the logits NaN, and with
+        // four parts.  Scales that are no number have made the logits NaN, and with
         // them l, where they are seen; here they count as 0.
         const float by = !hidden && scale < INFINITY ? scale * by_ref : 0.f;
-        uint2 pa[C / 8], pb[C / 8], pc[C / 8];
+        uint2 part[C / 8][4];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
           d[k] = ex2_approx(d[k]);
@@ -1102,22 +1157,21 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           d[k] *= by;
         }
 #pragma unroll
-        for (int k = 0; k < C / 8; ++k) in_parts(d + 8 * k, pa[k], pb[k], pc[k]);
+        for (int k = 0; k < C / 8; ++k) in_parts(d + 8 * k, part[k]);
         // P was last read by PV(i - 1).
         if (i > 0) ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
         {
           // One 128-byte row per token: column n of part x at byte x R + n, 16-byte pieces swizzled by token & 7.
           uint8_t* at = p_mem + tok * 128;
-          auto put = [&](int byte, const uint2(&v)[C / 8]) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int byte = kR * x + C * set;
             uint8_t* to = at + (((byte >> 4) ^ (tok & 7)) << 4) + (byte & 8);
             if constexpr (C == 16)
-              *reinterpret_cast<uint4*>(to) = make_uint4(v[0].x, v[0].y, v[C / 8 - 1].x, v[C / 8 - 1].y);
+              *reinterpret_cast<uint4*>(to) = make_uint4(part[0][x].x, part[0][x].y, part[1][x].x, part[1][x].y);
             else
-              *reinterpret_cast<uint2*>(to) = v[0];
-          };
-          put(C * set, pa);
-          put(kR + C * set, pb);
-          put(2 * kR + C * set, pc);
+              *reinterpret_cast<uint2*>(to) = part[0][x];
+          }
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -1157,11 +1211,10 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         const int dim = 128 * mb + 32 * sp + lane;
         float o[C];
         {
-          float b[C], r[C];
-          const uint32_t at = tmem_base + lane_base + Sh::kColO + 3u * kR * mb + C * set;
-          tmem_ld_three(at, at + kR, at + 2 * kR, o, b, r);
+          float sums[Sh::kSums][C];
+          tmem_ld_sums(tmem_base + lane_base + Sh::kColO + kColsO * mb + C * set, sums);
 #pragma unroll
-          for (int k = 0; k < C; ++k) o[k] = fmaf(fmaf(r[k], 0.125f, b[k]), 0.125f, o[k]) * factor_s[C * set + k];
+          for (int k = 0; k < C; ++k) o[k] = whole_sum(sums, k) * factor_s[C * set + k];
         }
         if (seg.whole) {
           // Neighbouring lanes swap halves, so that each stores two dims of one row.

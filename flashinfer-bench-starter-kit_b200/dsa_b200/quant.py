@@ -46,7 +46,7 @@ of ``sparse_indices`` [T, K] (-1: none; a slot given twice counts twice), as
 sees nothing yields output 0 and lse -inf.  Tokens that no row sees may hold
 anything; a visible one with NaN makes the output NaN.  ``output`` may be ``q_nope``
 itself; other outputs over an input are refused.  Queries are used as they are
-(their products with the codes are exact), softmax weights to 2^-9 of each.
+(their products with the codes are exact), softmax weights to 2^-14 of each.
 
 Calls that overlap need different streams; threads may call on one stream.  A
 captured graph uses the workspace of the stream that it was captured on: it must

@@ -100,7 +100,7 @@ def _softmax(q_nope, q_pe, c, e, scales, see, scale):
     move = off.amax(1)
     w = torch.exp2(x - lse[:, None])
     out = w @ c
-    err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -19) * w
+    err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -14 + 2.0 ** -17) * w
     codes = torch.where(scales[:, None] == 0, 0.0, c.abs() / scales[:, None])
     bound = err @ c.abs() + 2.0 ** -27 * largest * w.amax(1, keepdim=True) * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
     return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
@@ -114,12 +114,13 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
       magnitudes (2^-23, not 2^-24, for accumulators that truncate).
     * The lse moves by at most the largest of these, the exponential's and the sum's errors (2^-18 is far above both) and
       one rounding; a weight by ln 2 times its logit's and the lse's error.
-    * A weight is rounded to half precision (2^-11 of itself), then split into three parts of 3 bits each, every one to
-      nearest: within 2^-9 (1 + 2^-11), as each leaves at most 2^-3 of what it is given.  Where it is far below the largest,
-      it is within half the smallest step of the third part, 2^-17 / 64 (and of half precision, 2^-25): of weights times
-      scales over `ref` / 32, where ref is at most the largest scale of the context, and relative to a maximum that is at
-      most the true one.  Each token's code may so count 2^-27.6 times the largest scale times the largest weight too much
-      or too little.  The output is rounded to bf16, 2^-8 of itself.
+    * A weight is split into four parts of 3 bits each, the last two of what its upper 11 bits leave with its lower ones.
+      Each is half a step off what the one before leaves, which may pass a power of two by an eighth: within 2^-14, and
+      2^-18 for the lower bits' rounding, 2^-22 for its products.  Where it is far below the largest, it is within half the
+      smallest step of the last part, 2^-17 / 128, and 2^-24 of half precision's: of weights times scales over `ref` / 32,
+      where ref is at most the largest scale of the context, and relative to a maximum that is at most the true one.  Each
+      token's code may so count 2^-28 times the largest scale times the largest weight too much or too little.  The output
+      is rounded to bf16, 2^-8 of itself.
     """
     T, H = q_nope.shape[:2]
     out = torch.full((T, H, CKV), math.nan, dtype=torch.float64)
