@@ -11,11 +11,13 @@
 // parts that add up to what they were:
 //   q_nope f = a + b / 16 with a, b e4m3 and f a power of two for each row (its
 //     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
-//     b the other 4: the parts are exact down to 2^-22 of the row's largest.
-//   w = p s (weight by scale) = a + b + (c + d) / 128 with e5m2 parts, each to
-//     nearest: 3 bits, then 4 more each (what is left has a sign and is less than
-//     the last step).  Within 2^-14 of w (6e-6 in the mean) from 2^15 down to 2^-9,
-//     and within 2^-23 below: many light tokens beside a heavy one still count.
+//     b the other 4: exact from 2^-13 of the row's largest up, to 2^-21 of that
+//     below.
+//   w = p s (weight by scale, the row's largest so far 2^7 or more) = a + b +
+//     (c + d) / 128 with e5m2 parts, each to nearest: 3 bits, then 4 more each (what
+//     is left has a sign and is less than the last step).  Within 2^-14 of w (6e-6 in
+//     the mean) from 2^15 down to 2^-9, and within 2^-23 below: many light tokens
+//     beside a heavy one still count.
 //     Three parts, 2^-11 (1.2e-4), would make a difference that outputs show: bf16
 //     has 2^-9, and one in fifteen was rounded to a neighbour (one in 300).
 // Per tile of 128 tokens and group of R rows (token, head)
@@ -25,9 +27,10 @@
 // so the parts lie along N, which costs the tensor core nothing up to N = 64: it
 // is fed at 128 bytes of A a clock.  Of 16 rows each part has its own 16 columns
 // of O^T; of 32, whose 128 would leave TMEM no room for S^T, a product of a and c
-// is followed by one of b and d into the same 64.  A tile's 82 KB cross shared memory once in,
-// and once and a half out, against three and a half times for bf16 copies of it
-// (225 KB, 1750 clocks, where its share of the HBM rate takes 3500).
+// is followed by one of b and d into the same 64.  A tile's 82 KB cross shared
+// memory once in, and once and a half out (twice and a half of 32 rows), against
+// three and a half times for bf16 copies of it (225 KB, 1750 clocks, where its share
+// of the HBM rate takes 3500).
 //
 // Units of work are (request, group, tile), cut into equal contiguous slices, one
 // per CTA; slices' pieces that do not cover their group's whole context are
@@ -71,8 +74,10 @@ constexpr int kTmemCols = 512;
 // holds up the other: at a threshold of 8 log2 units 2 of 34 tiles need one (normal
 // logits of spread 2.5, scales spread by e^0.3), at 6 four, at 4 six.
 constexpr float kRescaleThreshold = 8.0f;
-constexpr float kScaleGrowth = 4.0f;
-constexpr float kUnit = 32.0f;               // of weights: 2^8 x 4 x 32 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kUnit = 128.0f;              // of weights: 2^8 x 128 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kUnitLog2 = 7.0f;
+constexpr float kScaleRange = 60.0f;         // log2 units from a segment's unit of scales
+constexpr float kLeastRef = 0x1p-100f;       // of that unit: kUnit over it has to be a number
 constexpr float kLowUnit = 1.0f / 128.0f;    // of their last two parts: what the first two leave is below 2^-7 of a weight
 constexpr int kMostRows = 32;
 constexpr int kColsO = 64;                   // of O^T for 128 dims
@@ -975,14 +980,20 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     if (!kTogether && tid == 0) group_of[0] = group_of[1] = -1;
     int i = 0, segs = 0;
     bool ok = true;
-    // Online softmax in base 2.  A column's running max m is the same in every
-    // thread that has it (-inf: it has seen nothing; +inf: no row of the group,
-    // all weights 0).  It moves only when some token of the tile exceeds it by
-    // more than kRescaleThreshold (always at a segment's first tile), which one
-    // OR-barrier per tile tells the set; only then is the tile's max reduced
-    // over the tokens and O rescaled.  Weights by scales are taken relative to
-    // `ref`, the largest scale of the first tile, which moves in the same way
-    // when a scale exceeds it more than kScaleGrowth times.
+    // Online softmax in base 2.  A weight by its scale is 2^(x - m) s, and what a
+    // column's reference m follows is that product, not the logit alone: m is the
+    // running maximum of x + log2(s / ref), ref the power of two of the largest scale
+    // in the segment's first tile.  So the column's largest product is kUnit or more,
+    // and no token takes from the others' precision but by its own weight (with maxima
+    // of x and s apart, a token of a scale 2^20 times the others' and no weight left
+    // them 3 bits).  The sums l of 2^(x - m), in 32 bits, need no such reference: scales
+    // within 2^60 of ref cannot drive them out of the range.  Smaller ones (zeros
+    // among them) count as 2^-60 in m, larger ones move ref.
+    // m (-inf: the column has seen nothing; +inf: no row of the group, all weights 0)
+    // is the same in every thread that has the column.  It moves only when some token
+    // of the tile exceeds it by more than kRescaleThreshold (always at a segment's
+    // first tile), which one OR-barrier per tile tells the set; only then is the
+    // tile's max reduced over the tokens and O rescaled.
     for (;;) {
       const int qb = segs % Sh::kQBufs;
       ok = ok && mbar_wait(&q_full[qb], (segs / Sh::kQBufs) & 1, wctx);
@@ -994,8 +1005,21 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       float l[C];
       bool unset = C * set < rows;  // some column has seen nothing yet
       float ref = 0.f, by_ref = 0.f;
-      // (The first tile's values from minus_s count for nothing: its maxima are taken anyway.)
-      if (e < C) my_max[e] = C * set + e < rows ? -INFINITY : INFINITY;
+      if (e < C) {
+        my_max[e] = C * set + e < rows ? -INFINITY : INFINITY;
+        my_minus[e] = C * set + e < rows ? 0.f : -INFINITY;
+      }
+      // The power of two at or below the tile's largest scale of those that count (the set waits for one another).
+      auto unit_of_tile = [&](float scale, bool counts) {
+        const uint32_t largest = __reduce_max_sync(0xffffffffu, counts ? __float_as_uint(fabsf(scale)) : 0u);
+        if (lane == 0) most_s[4 * set + sp] = __uint_as_float(largest);
+        named_barrier_sync(1 + set, 128);
+        const float4 m4 = *reinterpret_cast<const float4*>(most_s + 4 * set);
+        const float largest4 = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+        return fmaxf(__uint_as_float(__float_as_uint(largest4) & 0x7F800000u), kLeastRef);
+      };
+      // log2(s / ref) of a scale in units (s kUnit / ref).
+      auto log_of = [](float by) { return fmaxf(lg2_approx(fabsf(by)) - kUnitLog2, -kScaleRange); };
       const float* my_c = c_s + qb * kMostRows + C * set;
 #pragma unroll
       for (int k = 0; k < C; ++k) l[k] = 0.f;
@@ -1019,6 +1043,13 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
         if (!kSparse && hidden && pos < length && (e & 63) == 0) atomicOr(p.status, DSA_DEV_BAD_PAGE);
         ok = ok && mbar_wait(&kv_full[st * kParts + (kSparse ? kParts - 1 : 0)], (i >> 1) & 1, wctx);
         const float scale = scale_s[st * kTok + tok];
+        // A scale that is no number has made the token's logits NaN, and with them l, where it is seen; it counts as 0 here.
+        bool counts = !hidden && fabsf(scale) < INFINITY;
+        if (t == t0) {  // (while S^T is computed)
+          ref = unit_of_tile(scale, counts);
+          by_ref = kUnit / ref;
+        }
+        float by = counts ? scale * by_ref : 0.f, log_by = log_of(by);
         ok = ok && mbar_wait(&s_full[sb], (i / Sh::kSBufs) & 1, wctx);
         tc_fence_after();
         float x[C];  // logits
@@ -1057,27 +1088,48 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 #pragma unroll
         for (int k = 2; k < C; k += 2) most = fmaxf(most, fmaxf(d[k], d[k + 1]));
         if (named_barrier_or(1 + set, 128,
-                             unset || most > kRescaleThreshold || (!hidden && scale > kScaleGrowth * ref))) {
+                             unset || most + log_by > kRescaleThreshold || log_by > kScaleRange)) {
+          // A row of zeros has no weight, whatever its scale; those that are written here have 1, which may be
+          // far above the scales of small latents.
+          if (__any_sync(0xffffffffu, counts && scale == 1.f)) {
+#pragma unroll
+            for (int y = 0; y < kParts; ++y)
+              if (!kSparse || y == kParts - 1) ok = ok && mbar_wait(&kv_full[st * kParts + y], (i >> 1) & 1, wctx);
+            if (counts && scale == 1.f) {
+              const uint8_t* codes = smem + st * kStageBytes + tok * 128;
+              uint32_t any = 0u;
+#pragma unroll 1
+              for (int q = 0; q < 32; ++q) {
+                const uint4 w = *reinterpret_cast<const uint4*>(codes + (q >> 3) * kBlockBytes + (q & 7) * 16);
+                any |= (w.x | w.y) | (w.z | w.w);
+              }
+              if ((any & 0x7F7F7F7Fu) == 0u) {
+                counts = false;
+                by = 0.f;
+                log_by = -kScaleRange;
+              }
+            }
+          }
           int col;
-          {
+          auto tile_maxima = [&]() {
             float v[C];
 #pragma unroll
-            for (int k = 0; k < C; ++k) v[k] = x[k];
+            for (int k = 0; k < C; ++k) v[k] = x[k] + log_by;
             // (fmaxf passes over NaN, which moves no maximum.)
             const float mt = over_tokens(v, lane, col, [](float a, float b) { return fmaxf(a, b); });
             red_set[C * sp + col] = mt == mt ? mt : -INFINITY;
-          }
-          const uint32_t sk = __float_as_uint(scale);
-          const uint32_t largest = __reduce_max_sync(0xffffffffu, !hidden && sk < 0x7F800000u ? sk : 0u);
-          if (lane == 0) most_s[4 * set + sp] = __uint_as_float(largest);
-          named_barrier_sync(1 + set, 128);
-          const float4 m4 = *reinterpret_cast<const float4*>(most_s + 4 * set);
-          const float largest4 = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+          };
+          tile_maxima();
           float shrink = 1.f;
-          if (largest4 > kScaleGrowth * ref) {
-            shrink = ref == 0.f ? 1.f : ref / largest4;  // scales of 0 so far: O is 0
-            ref = largest4;
-            by_ref = largest4 < 1e-35f ? 0.f : kUnit / largest4;
+          if (named_barrier_or(1 + set, 128, log_by > kScaleRange)) {
+            const float now = unit_of_tile(scale, counts);
+            shrink = ref / now;
+            ref = now;
+            by_ref = kUnit / now;
+            by = counts ? scale * by_ref : 0.f;
+            log_by = log_of(by);
+            tile_maxima();
+            named_barrier_sync(1 + set, 128);
           }
           if (sp == 0) {
             const float mt = fmaxf(fmaxf(red_set[col], red_set[C + col]), fmaxf(red_set[2 * C + col], red_set[3 * C + col]));
@@ -1146,9 +1198,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           }
         }
         // Weights (of d = -inf, 0; NaN stays), and their products with the scale in
-        // four parts.  Scales that are no number have made the logits NaN, and with
-        // them l, where they are seen; here they count as 0.
-        const float by = !hidden && scale < INFINITY ? scale * by_ref : 0.f;
+        // four parts.
         uint2 part[C / 8][4];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
@@ -1194,14 +1244,12 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
       if (e < C) {
         const int col = C * set + e;
         const float sum = (red_set[e] + red_set[C + e]) + (red_set[2 * C + e] + red_set[3 * C + e]);
-        const float unit = by_ref == 0.f ? 0.f : ref * (1.f / kUnit);
-        if (seg.whole) {
-          factor_s[col] = sum == 0.f ? 0.f : unit / sum;
-          if (col < rows) p.lse[row_q + col] = sum == 0.f ? -INFINITY : max_s[col] + log2f(sum);
-        } else {
-          factor_s[col] = unit;
+        // A piece is normalised too: its sum of scaled codes alone could leave the range.
+        factor_s[col] = sum == 0.f ? 0.f : ref * (1.f / kUnit) / sum;
+        if (!seg.whole)
           (kTogether ? together_ml : p.part_ml + rec * kMostRows)[col] = make_float2(max_s[col], sum);
-        }
+        else if (col < rows)
+          p.lse[row_q + col] = sum == 0.f ? -INFINITY : max_s[col] + log2f(sum);
       }
       ok = ok && mbar_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, wctx);
       named_barrier_sync(1 + set, 128);
@@ -1274,19 +1322,22 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
           if (k * share >= tiles) ml[k].x = -INFINITY;
           M = fmaxf(M, ml[k].x);
         }
+#pragma unroll
+        for (int k = 0; k < kMostTogether; ++k) {
+          ml[k].y = ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.f : ml[k].y) : ml[k].y * exp2f(ml[k].x - M);
+          L += ml[k].y;
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < kMostTogether; ++k) {
-          const float w = ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.f : ml[k].y) : exp2f(ml[k].x - M);
-          L = fmaf(ml[k].y, w, L);
+          const float w = ml[k].y * inv;
           acc.x = fmaf(o[k].x, w, acc.x);
           acc.y = fmaf(o[k].y, w, acc.y);
           acc.z = fmaf(o[k].z, w, acc.z);
           acc.w = fmaf(o[k].w, w, acc.w);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
-                                     __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+        const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x, acc.y), __floats2bfloat162_rn(acc.z, acc.w)};
         *reinterpret_cast<uint2*>(p.out + (row_q + y) * kCkv + 4 * d4) = *reinterpret_cast<const uint2*>(h);
         if (d4 == 0) p.lse[row_q + y] = L == 0.f ? -INFINITY : M + log2f(L);
       }
@@ -1296,7 +1347,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
 }
 
 // Joins the records of a group that several slices share: per row
-//   M = max m_i, L = sum l_i 2^(m_i - M), lse = M + log2 L, out = sum O_i 2^(m_i - M) / L,
+//   M = max m_i, w_i = l_i 2^(m_i - M), L = sum w_i, lse = M + log2 L, out = sum O_i w_i / L,
 // in an order that the slices alone give.  Block x has the group x, or where
 // groups outnumber records the group of record x if x is its first one; block y
 // its rows y * rows_per_block ...  Each kSplit-th of the block takes every
@@ -1390,8 +1441,8 @@ join_kernel(const Params p, int ctas, int rows_per_block, bool by_record) {
     for (int k = lane; k < count; k += 32) {
       const float2 q = k == lane ? first : __ldcg(ml + static_cast<int64_t>(recs[k]) * kMostRows);
       // NaN sums have a place even where the max of what is left of a piece is -inf.
-      const float w = q.x == -INFINITY ? (q.y == q.y ? 0.f : q.y) : exp2f(q.x - M);
-      L = fmaf(q.y, w, L);
+      const float w = q.x == -INFINITY ? (q.y == q.y ? 0.f : q.y) : q.y * exp2f(q.x - M);
+      L += w;
       weight[y][k] = w;
     }
 #pragma unroll

@@ -45,8 +45,10 @@ of ``sparse_indices`` [T, K] (-1: none; a slot given twice counts twice), as
 ``dsa_b200.attention.run`` does.  Both take 1 to 128 heads; ``lse`` is the base-2 log-sum-exp of the scaled logits; a row that
 sees nothing yields output 0 and lse -inf.  Tokens that no row sees may hold
 anything; a visible one with NaN makes the output NaN.  ``output`` may be ``q_nope``
-itself; other outputs over an input are refused.  Queries are used as they are
-(their products with the codes are exact), softmax weights to 2^-14 of each.
+itself; other outputs over an input are refused.  Values of a query are exact from
+2^-13 of its row's largest up, smaller ones to 2^-21 of that; softmax weights times
+scales to 2^-14 of each and 2^-30 of the row's largest.  Where scales of one request
+differ by 2^60 and more, tokens of the small ones may count as zeros.
 
 Calls that overlap need different streams; threads may call on one stream.  A
 captured graph uses the workspace of the stream that it was captured on: it must

@@ -88,7 +88,6 @@ def _softmax(q_nope, q_pe, c, e, scales, see, scale):
     """(output, lse and their bounds) of one row's heads over tokens c, e [n, ...] of these scales, of which `see` [n] are
     visible."""
     H = q_nope.shape[0]
-    largest = scales[torch.isfinite(scales)].max() if torch.isfinite(scales).any() else 0.0
     c, e, scales = c[see], e[see], scales[see]
     if len(c) == 0:
         z = torch.zeros(H, CKV, dtype=torch.float64)
@@ -102,7 +101,8 @@ def _softmax(q_nope, q_pe, c, e, scales, see, scale):
     out = w @ c
     err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -14 + 2.0 ** -17) * w
     codes = torch.where(scales[:, None] == 0, 0.0, c.abs() / scales[:, None])
-    bound = err @ c.abs() + 2.0 ** -27 * largest * w.amax(1, keepdim=True) * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
+    largest = torch.where(codes.any(1) | (scales != 1), w * scales, 0.0).amax(1, keepdim=True)
+    bound = err @ c.abs() + 2.0 ** -30 * largest * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
     return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
 
 
@@ -117,10 +117,9 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
     * A weight is split into four parts of 3 bits each, the last two of what its upper 11 bits leave with its lower ones.
       Each is half a step off what the one before leaves, which may pass a power of two by an eighth: within 2^-14, and
       2^-18 for the lower bits' rounding, 2^-22 for its products.  Where it is far below the largest, it is within half the
-      smallest step of the last part, 2^-17 / 128, and 2^-24 of half precision's: of weights times scales over `ref` / 32,
-      where ref is at most the largest scale of the context, and relative to a maximum that is at most the true one.  Each
-      token's code may so count 2^-28 times the largest scale times the largest weight too much or too little.  The output
-      is rounded to bf16, 2^-8 of itself.
+      smallest step of the last part, 2^-17 / 128, and 2^-24 of half precision's: in units of which the largest weight times
+      its scale is 2^7 or more (rows of zeros that have the scale 1 apart).  Each token's code may so count 2^-30 times that
+      product too much or too little.  The output is rounded to bf16, 2^-8 of itself.
     """
     T, H = q_nope.shape[:2]
     out = torch.full((T, H, CKV), math.nan, dtype=torch.float64)

@@ -57,9 +57,9 @@ def pairs(logits, seed=0):
     return cache, both, x.double() * SCALE * oq.LOG2E
 
 
-def wanted(scales, x):
-    """(outputs, bounds) [512] of any row with these logits."""
-    lse = torch.logsumexp(x / oq.LOG2E, 0) * oq.LOG2E
+def wanted(scales, x, others=()):
+    """(outputs, bounds) [512] of any row with these logits, and with `others` that have no part in the outputs."""
+    lse = torch.logsumexp(torch.cat([x, *others]) / oq.LOG2E, 0) * oq.LOG2E
     w = torch.exp2(x - lse) * scales.double() * 448
     out = (w[0::2] - w[1::2]).repeat_interleave(4)
     return out, WEIGHT * (w[0::2] + w[1::2]).repeat_interleave(4) + (2.0 ** -8 + 2.0 ** -16) * out.abs()
@@ -109,6 +109,95 @@ def test_selected_pairs_that_cancel(cuda_device, rows, heads):
                         cache.to(cuda_device), picked.to(cuda_device), SCALE, out, lse)
     want, bound = wanted(scales, x)
     assert ((out.cpu().double() - want).abs() <= bound).all()
+
+
+KINDS = {  # (their scale, factor of the pairs' scales, their base-2 logit, their codes)
+    "heavy": (2.0 ** 24, 1.0, -100.0, "random"), "heavier": (2.0 ** 45, 1.0, -140.0, "random"),
+    "zeros": (1.0, 2.0 ** -24, 0.0, "zeros"), "light": (2.0 ** -100, 1.0, 0.0, "random"),
+}
+
+
+def among_others(kind, first, seed=3):
+    """The pairs behind or before a tile of tokens that have next to no part in the outputs: scales far above the pairs' and no
+    weight, rows of zeros with the scale that they are written with, scales far below."""
+    scale, by, logit, what = KINDS[kind]
+    cache, scales, x = pairs(True)
+    more = torch.zeros(2, quant.PAGE_BYTES, dtype=torch.uint8)
+    codes, kpe, s = oq.pieces(more)
+    if what == "random":
+        g = torch.Generator().manual_seed(seed)
+        codes[:] = (torch.randn(codes.shape, generator=g) * 140).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    s[:] = scale
+    kpe[:, :, 0] = round(logit / (SCALE * oq.LOG2E))
+    oq.pieces(cache)[2].mul_(by)
+    other = kpe[:, :, 0].double().flatten() * SCALE * oq.LOG2E
+    out, bound = wanted(scales * by, x, (other,))
+    # what the others do add
+    lse = torch.logsumexp(torch.cat([x, other]) / oq.LOG2E, 0) * oq.LOG2E
+    bound = bound + scale * 448 * 2.0 ** float(other.max() - lse) * 128 * (what == "random")
+    cache = torch.cat([cache, more])
+    return cache, torch.tensor([4, 5, 0, 1, 2, 3] if first else [0, 1, 2, 3, 4, 5], dtype=torch.int32)[None], out, bound
+
+
+def unit_queries(rows, heads, device):
+    q_pe = torch.zeros(rows, heads, 64, dtype=torch.bfloat16, device=device)
+    q_pe[:, :, 0] = 1
+    return (torch.zeros(rows, heads, 512, dtype=torch.bfloat16, device=device), q_pe,
+            torch.zeros(rows, heads, 512, dtype=torch.bfloat16, device=device), torch.zeros(rows, heads, device=device))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("heads,pages", [(16, 6), (16, 900), (24, 900), (128, 6)])
+def test_tokens_that_do_not_count_take_nothing(cuda_device, kind, first, heads, pages):
+    cache, table, want, bound = among_others(kind, first)
+    q_nope, q_pe, out, lse = unit_queries(1, heads, cuda_device)
+    wide = torch.zeros(1, pages, dtype=torch.int32)
+    wide[:, :6] = table
+    quant.attend(q_nope, q_pe, cache.to(cuda_device), torch.tensor([N + 128], device=cuda_device), wide.to(cuda_device), None, SCALE,
+                 out, lse)
+    assert ((out[0].cpu().double() - want).abs() <= bound).all()
+    picked = (table[0].long()[:, None] * 64 + torch.arange(64)).flatten()[None].repeat(1 if heads == 16 else 100, 1)
+    q_nope, q_pe, out, lse = unit_queries(len(picked), heads, cuda_device)
+    quant.attend_sparse(q_nope, q_pe, cache.to(cuda_device), picked.to(cuda_device), SCALE, out, lse)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [5, 900])
+def test_later_drafts_take_nothing(cuda_device, pages):
+    """Drafts of large scales that a chain's first row does not see."""
+    cache, scales, x = pairs(True)
+    more = torch.zeros(1, quant.PAGE_BYTES, dtype=torch.uint8)
+    codes, _, s = oq.pieces(more)
+    codes[:], s[:] = 0x7E, 2.0 ** 40
+    table = torch.zeros(1, pages, dtype=torch.int32)
+    table[0, :5] = torch.arange(5)
+    q_nope, q_pe, out, lse = unit_queries(3, 16, cuda_device)
+    quant.attend(q_nope, q_pe, torch.cat([cache, more]).to(cuda_device), torch.tensor([N + 2], device=cuda_device),
+                 table.to(cuda_device), torch.tensor([0, 3], device=cuda_device), SCALE, out, lse)
+    want, bound = wanted(scales, x)
+    assert ((out[0].cpu().double() - want).abs() <= bound).all()
+    assert (out[1:] > 2.0 ** 40).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [-125, -118, -60, 60, 115])
+@pytest.mark.parametrize("pages", [5, 900])
+def test_scales_of_all_sizes(cuda_device, exponent, pages):
+    """One scale in all rows, one code in all places: that value, to bf16 and what a quotient near 2^-133 has (15 bits)."""
+    cache = torch.zeros(5, quant.PAGE_BYTES, dtype=torch.uint8)
+    codes, _, s = oq.pieces(cache)
+    codes[:], s[:] = 0x7E, 2.0 ** exponent
+    table = torch.zeros(1, pages, dtype=torch.int32)
+    table[0, :5] = torch.arange(5)
+    q_nope, q_pe, out, lse = unit_queries(1, 16, cuda_device)
+    quant.attend(q_nope, q_pe, cache.to(cuda_device), torch.tensor([300], device=cuda_device), table.to(cuda_device), None, SCALE,
+                 out, lse)
+    want = 448 * 2.0 ** exponent
+    assert ((out.cpu().double() - want).abs() <= (2.0 ** -8 + 2.0 ** -13) * want).all()
+    assert ((lse.cpu().double() - math.log2(300)).abs() <= 2.0 ** -17).all()
 
 
 @pytest.mark.gpu
