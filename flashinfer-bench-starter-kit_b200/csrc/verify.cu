@@ -45,6 +45,7 @@ constexpr int kMaxCluster = 8;
 constexpr int kMaxRows = 4096;   // of a request
 constexpr int kStep = 128;       // values a warp reads at once: four a lane
 constexpr int kDepth = 4;        // steps whose loads are in flight together
+constexpr double kWide = 0x1p896;  // see difference()
 
 struct Params {
   const float* target;
@@ -105,12 +106,21 @@ __device__ __forceinline__ double left_of(float p, float q, double c) {
 
 // The same before the maximum, for whole rows, where conversions to 64 bits would
 // bound it (one takes 8 clocks of its unit): q is widened by three integer
-// instructions instead.  Exact for normal numbers; what is below 2^-126, 0 among
-// it, comes out between 2^-127 and 2^-126 and takes that much too much from p.
-__device__ __forceinline__ double difference(float p, float q, double c) {
+// instructions instead, without its sign (of 0) and without another exponent: that
+// double, a subnormal one if q is 0 or subnormal, is q 2^-896 exactly, and `c_wide`
+// is c 2^896.  An infinity comes out as 2^128, more than any p; NaN is looked for in
+// another way (segment_sum).
+__device__ __forceinline__ double difference(float p, float q, double c_wide) {
   const uint32_t b = __float_as_uint(q);
-  const double wide = __hiloint2double(static_cast<int>((b >> 3) + 0x38000000u), static_cast<int>(b << 29));
-  return fma(-c, wide, static_cast<double>(p));
+  const double wide = __hiloint2double(static_cast<int>((b >> 3) & 0x0FFFFFFFu), static_cast<int>(b << 29));
+  return fma(-c_wide, wide, static_cast<double>(p));
+}
+
+// The largest of three, NaN if any is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 
 // Weights of the four values from v on, doubled where q counts (max(w, 0) is half
@@ -118,10 +128,11 @@ __device__ __forceinline__ double difference(float p, float q, double c) {
 // lie in the warp's segment.
 __device__ __forceinline__ void weights(const Left& s, float4 p, float4 q, int v, bool struck, double (&w)[4]) {
   if (s.q != nullptr && s.c != 0.0) {
-    w[0] = difference(p.x, q.x, s.c);
-    w[1] = difference(p.y, q.y, s.c);
-    w[2] = difference(p.z, q.z, s.c);
-    w[3] = difference(p.w, q.w, s.c);
+    const double c = s.c * kWide;
+    w[0] = difference(p.x, q.x, c);
+    w[1] = difference(p.y, q.y, c);
+    w[2] = difference(p.z, q.z, c);
+    w[3] = difference(p.w, q.w, c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] += fabs(w[e]);
     return;
@@ -141,11 +152,13 @@ __device__ __forceinline__ void weights(const Left& s, float4 p, float4 q, int v
   }
 }
 
-// Sum of these over the warp's segment [from, to), in every lane.
+// Sum of these over the warp's segment [from, to), in every lane; NaN where p holds
+// one, or q where it counts.
 template <bool kWide>
 __device__ double segment_sum(const Left& s, int from, int to, int vocab, bool struck) {
   const int lane = threadIdx.x & 31;
   double sum = 0.0;
+  float most = 0.f;  // of q
   for (int v0 = from; v0 < to; v0 += kStep * kDepth) {
     float4 p[kDepth], q[kDepth];
 #pragma unroll
@@ -164,9 +177,11 @@ __device__ double segment_sum(const Left& s, int from, int to, int vocab, bool s
         double w[4];
         weights(s, p[d], q[d], v, struck, w);
         sum += (w[0] + w[1]) + (w[2] + w[3]);
+        most = max_nan(max_nan(most, q[d].x, q[d].y), q[d].z, q[d].w);
       }
     }
   }
+  if (most != most) sum = most;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;

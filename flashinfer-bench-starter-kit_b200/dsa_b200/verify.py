@@ -28,8 +28,10 @@ that is full ends the walk.
   buffer); random numbers are float32 in [0, 1).  Distributions are taken as
   summing to 1.  Comparisons and sums are made in 64 bits.
 * Where nothing is left of p' (draws that had no probability), the next token is
-  drawn from the target's distribution; if that has none either, or holds NaN, it
-  is -1.  So it is for a request without rows.
+  drawn from the target's distribution; if that has none either, it is -1.  So it
+  is for a request without rows, and where what is drawn from holds NaN: in the
+  target's row, or after a rejection in the draft's.  Probabilities are 0 (of
+  either sign) or more.
 * A token outside of the vocabulary is never accepted and sets a status bit
   (``device_status``), as do ``cu_drafts`` that do not fit (the request is then
   taken as empty) and requests of over 4096 rows (the others are left out).

@@ -480,7 +480,8 @@ DSA_API int dsa_latent_sparse_attention_run(const void* q_nope, const void* q_pe
  *   rejected:      c += R, R = sum max(p - c q, 0)
  * The walk goes on at an accepted row.  Where it ends, the next token is the first
  * whose running sum of max(p - c q, 0) exceeds sample_u of the whole (of p, if the
- * whole is 0; -1 if that is 0 or NaN too).  All in 64 bits.
+ * whole is 0; -1 if that is 0 too, or if either holds NaN: q's counts once something
+ * was rejected).  Probabilities are 0, of either sign, or more.  All in 64 bits.
  *
  *   target_probs   num_rows rows of vocab fp32, target_stride values apart: the
  *                  target's distribution after each row

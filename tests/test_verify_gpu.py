@@ -159,3 +159,50 @@ def test_in_a_graph_with_new_numbers(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert [t.tolist() for t in got] == list(ov.verify_reference(*case[:5], u, s, 8))
+
+
+@pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("vocab,most,branch", [(9, 12, 4), (140, 10, 3), (5003, 8, 3)])
+def test_zeros_of_either_sign(cuda_device, vocab, most, branch, certain):
+    """-0.0 is 0 in both distributions, with rejections before siblings and before the draw."""
+    for seed in range(8):
+        target, draft, tokens, parents, cu, _, s = ov.random_case(5, most, vocab, branch, certain, seed, dyadic=True)
+        negative = lambda t: None if t is None else torch.where(t == 0, -0.0, t)  # noqa: E731
+        u = torch.full((len(tokens),), 1 - 2.0 ** -6) - (torch.arange(len(tokens)) % 3) / 4
+        for case in ((negative(target), negative(draft)), (target, negative(draft))):
+            check((*case, tokens, parents, cu, u, s), cuda_device, most, exact=vocab < 1000)
+
+
+@pytest.mark.parametrize("vocab", [4, 300, 3001])
+def test_subnormal_probabilities_count(cuda_device, vocab):
+    """What is left after a rejection is one token of 2^-130, where the draft has 0, and beside it 2^-140 of one of 2^-139."""
+    p, q = torch.zeros(2, vocab), torch.zeros(2, vocab)
+    p[:, 0], p[:, 1], p[:, 2] = 0.5, 0.5, 2.0 ** -130
+    q[:, 0], q[:, 1], q[:, 3] = 0.5, 0.5, 2.0 ** -149
+    for u, token in ((0.0, 2), (0.9, 2)):
+        got = outs(1, 1, cuda_device)
+        verify.run(*on((p, q, torch.tensor([0, 3]), torch.tensor([-1, 0]), torch.tensor([0, 2]), torch.zeros(2), torch.tensor([u])),
+                       cuda_device), *got)
+        assert [g.tolist() for g in got] == [[[-1]], [0], [token]]
+    p[:, 2], p[:, vocab - 2], q[:, vocab - 2] = 2.0 ** -140, 2.0 ** -139, 2.0 ** -140
+    if vocab > 4:  # two tokens of 2^-140 each are left
+        for u, token in ((0.49, 2), (0.51, vocab - 2)):
+            got = outs(1, 1, cuda_device)
+            verify.run(*on((p, q, torch.tensor([0, 3]), torch.tensor([-1, 0]), torch.tensor([0, 2]), torch.zeros(2), torch.tensor([u])),
+                           cuda_device), *got)
+            assert [g.tolist() for g in got] == [[[-1]], [0], [token]]
+
+
+@pytest.mark.parametrize("vocab", [5, 700, 20001])
+def test_nan_in_the_draft_is_not_drawn_from(cuda_device, vocab):
+    """A rejection takes q away from p: with NaN in it nothing can be drawn, and no sibling accepted.  Where no child is
+    rejected q is not read."""
+    p = torch.softmax(torch.randn(3, vocab, generator=torch.Generator().manual_seed(vocab)), 1)
+    q = p.clone()
+    q[0, vocab // 2] = float("nan")
+    for u, want in (([0.0, 1.0, 0.5], [[[-1, -1]], [0], [-1]]), ([0.0, 0.0, 0.0], [[[1, -1]], [1], None])):
+        got = outs(1, 2, cuda_device)
+        verify.run(*on((p, q, torch.tensor([0, 0, 1]), torch.tensor([-1, 0, 0]), torch.tensor([0, 3]), torch.tensor(u),
+                        torch.tensor([0.5])), cuda_device), *got)
+        assert [g.tolist() for g in got[:2]] == want[:2]
+        assert got[2].tolist() == want[2] if want[2] else got[2].item() >= 0
