@@ -217,7 +217,7 @@ write_kernel(const WriteParams p) {
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
             const float q = __fmul_rn(t[4 * k + z], rcp);
-            v[z] = __fmaf_rn(__fmaf_rn(-q, D, t[4 * k + z]), rcp, q);
+            v[z] = __fmaf_rn(__fmaf_rn(q, D, -t[4 * k + z]), -rcp, q);  // (signs that keep -0)
           }
           const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
           const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);

@@ -83,6 +83,16 @@ def test_write_ties_zeros_and_what_is_not_finite(cuda_device):
     assert ((scales[0, :8].double() - scale).abs() <= 2.0 ** -23 * scale).all()
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_write_keeps_the_sign_of_zeros(cuda_device, norm):
+    kv = kv_rows(40, 3)
+    kv[:, ::3], kv[:, 1::5] = -0.0, 0.0
+    w = torch.randn(512, generator=torch.Generator().manual_seed(4)).bfloat16() if norm else None
+    cache = torch.zeros(1, quant.PAGE_BYTES, dtype=torch.uint8, device=cuda_device)
+    quant.write(kv.to(cuda_device), torch.arange(40, device=cuda_device), cache, None if w is None else w.to(cuda_device))
+    assert torch.equal(oq.pieces(cache.cpu())[0][0, :40], oq.write_rows(kv, w)[0])
+
+
 def test_write_reports_what_does_not_fit(cuda_device):
     args, want, slots = written(cuda_device, 20, 2, 3)
     for k, bad in ((1, 128), (5, -1), (5, 300)):
