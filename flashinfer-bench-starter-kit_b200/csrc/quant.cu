@@ -14,7 +14,8 @@
 // do not depend on a sum: t is the exact product of two bf16, and the quotient
 // of two integers of 16 bits by 448 is a border of e4m3 or at least 2^-21 of
 // itself away from one.  A correctly rounded quotient (2^-24) therefore rounds
-// to the code that exact arithmetic gives.
+// to the code that exact arithmetic gives.  Rows whose squares or products leave
+// fp32's range are scaled by powers of two first (write_far_row).
 //
 // One scale a token, not one for each 128 values: e4m3 keeps its three bits down
 // to 2^-15 of the row's largest value, and the attention over this cache can
@@ -39,6 +40,8 @@ static_assert(kScaleAt + kPage * 4 == kPageBytes, "page layout");
 constexpr int kWarps = 8;
 constexpr float kMostCode = 448.0f;
 constexpr float kLeastScale = 1.1754943508222875e-38f;  // 2^-126
+constexpr float kMostScale = 3.4028234663852886e38f;
+constexpr uint32_t kSmall = (127u - 100u) << 23;        // the bits of 2^-100
 
 __device__ __forceinline__ float2 bf16x2(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -71,15 +74,209 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return y;
 }
 
+// M / 2^9 of 7/8 M, M = max |c w|, exactly: a first quotient, its remainder by one
+// FMA, and the sum of both rounded.
+__device__ __forceinline__ float most_over_512(float top7) {
+  const float first = top7 * (1.f / kMostCode);
+  return fmaf(fmaf(-first, kMostCode, top7), 1.f / kMostCode, first);
+}
+
+// 2^n in 64 bits, -1022 <= n <= 1023.
+__device__ __forceinline__ double power_of_two(int n) { return __hiloint2double((n + 1023) << 20, 0); }
+
+// Codes e4m3(t / D) of a lane's 16 values, D = 7/8 M / 448 of a row.
+__device__ __forceinline__ void codes_of(float (&t)[16], float D, uint32_t (&code)[4]) {
+  if (D < 1e-18f || D > 1e18f) {  // by a power of two, so that no reciprocal or quotient leaves the range
+    const float by = D < 1.f ? 1.8446744073709552e19f : 5.421010862427522e-20f;  // 2^64, 2^-64
+    D *= by;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t[k] *= by;
+  }
+  // t / D = 448 c w / M in the same way as D: within 2^-44 of itself before it is
+  // rounded, so exact where it is a border of e4m3 (what underflows is far below
+  // half of the smallest code).
+  float rcp;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(D));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float v[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const float q = __fmul_rn(t[4 * k + z], rcp);
+      v[z] = __fmaf_rn(__fmaf_rn(q, D, -t[4 * k + z]), -rcp, q);  // (signs that keep -0)
+    }
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+    code[k] = lo | (hi << 16);
+  }
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* codes, const uint32_t (&code)[4], float* to_scale, float scale) {
+  const int lane = threadIdx.x & 31;
+  *reinterpret_cast<uint2*>(codes + 8 * lane) = make_uint2(code[0], code[1]);
+  *reinterpret_cast<uint2*>(codes + 256 + 8 * lane) = make_uint2(code[2], code[3]);
+  if (lane == 0) *to_scale = scale;
+}
+
+// The latent of a row whose squares or products leave the range of fp32, or its
+// normal numbers, of a row of zeros and of one that is not finite: again, with c and
+// the weights scaled by powers of two to magnitudes of 1 (the codes are the same),
+// and the scale in 64 bits.  For a whole warp.
+__device__ __forceinline__ void write_far_row(const uint8_t* row, const __nv_bfloat16* norm, float eps, uint8_t* codes, float* to_scale) {
+  const int lane = threadIdx.x & 31;
+  uint4 c_raw[2], w_raw[2];
+  c_raw[0] = *reinterpret_cast<const uint4*>(row + 16 * lane);
+  c_raw[1] = *reinterpret_cast<const uint4*>(row + 512 + 16 * lane);
+  w_raw[0] = w_raw[1] = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);  // ones
+  if (norm != nullptr) {
+    w_raw[0] = *reinterpret_cast<const uint4*>(norm + 8 * lane);
+    w_raw[1] = *reinterpret_cast<const uint4*>(norm + 256 + 8 * lane);
+  }
+  const uint32_t* x = reinterpret_cast<const uint32_t*>(c_raw);
+  const uint32_t* y = reinterpret_cast<const uint32_t*>(w_raw);
+  uint32_t c_top = 0u, w_top = 0u;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    c_top = max(c_top, max((x[k] << 16) & 0x7FFFFFFFu, x[k] & 0x7FFF0000u));
+    w_top = max(w_top, max((y[k] << 16) & 0x7FFFFFFFu, y[k] & 0x7FFF0000u));
+  }
+  c_top = __reduce_max_sync(0xffffffffu, c_top);
+  w_top = __reduce_max_sync(0xffffffffu, w_top);
+  // Exponents of the largest values (of subnormal ones the least), and what brings them to 1.
+  const int c_exp = min(max(static_cast<int>(c_top >> 23), 1), 253) - 127;
+  const int w_exp = min(max(static_cast<int>(w_top >> 23), 1), 253) - 127;
+  const float by_c = __uint_as_float(static_cast<uint32_t>(127 - c_exp) << 23);
+  const float by_w = __uint_as_float(static_cast<uint32_t>(127 - w_exp) << 23) * (kMostCode / 512.f);
+  float t[16];
+  float sum = 0.f, most = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 c = bf16x2(x[k]), w = bf16x2(y[k]);
+    const float a = c.x * by_c, b = c.y * by_c;
+    sum = fmaf(a, a, sum);
+    sum = fmaf(b, b, sum);
+    t[2 * k] = a * (w.x * by_w);
+    t[2 * k + 1] = b * (w.y * by_w);
+    most = fmaxf(most, fmaxf(fabsf(t[2 * k]), fabsf(t[2 * k + 1])));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float D = most_over_512(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))));
+  double scale = static_cast<double>(D * (512.f / kMostCode)) * power_of_two(c_exp) * power_of_two(w_exp);
+  if (norm != nullptr) {
+    // 1 / sqrt of v = m 4^n with 1 <= m < 4.
+    const double v = static_cast<double>(sum) * (1.0 / kCkv) * power_of_two(2 * c_exp) + static_cast<double>(eps);
+    const int n = ((__double2hiint(v) >> 20) - 1023) >> 1;
+    scale = v > 0.0 ? scale * power_of_two(-n) * static_cast<double>(rsqrtf(static_cast<float>(v * power_of_two(-n) * power_of_two(-n))))
+                    : 0.0;
+  }
+  float to_store = static_cast<float>(scale);
+  uint32_t code[4];
+  if (c_top >= 0x7F800000u || w_top >= 0x7F800000u || to_store > kMostScale) {  // the whole row is NaN
+    to_store = 1.f;
+    code[0] = code[1] = code[2] = code[3] = 0x7F7F7F7Fu;
+  } else if (!(to_store >= kLeastScale)) {  // zeros, or too small for a scale
+    to_store = 1.f;
+    code[0] = code[1] = code[2] = code[3] = 0u;
+  } else {
+    codes_of(t, D, code);
+  }
+  store_codes(codes, code, to_scale, to_store);
+}
+
+// A lane's weights times 7/8 (ones without a norm).
+__device__ __forceinline__ void load_weights(const __nv_bfloat16* norm, float (&w78)[16]) {
+  const int lane = threadIdx.x & 31;
+  uint4 raw[2] = {make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u),
+                  make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)};  // ones
+  if (norm != nullptr) {
+    raw[0] = *reinterpret_cast<const uint4*>(norm + 8 * lane);
+    raw[1] = *reinterpret_cast<const uint4*>(norm + 256 + 8 * lane);
+  }
+  const uint32_t* x = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 w = bf16x2(x[k]);
+    w78[2 * k] = w.x * (kMostCode / 512.f);
+    w78[2 * k + 1] = w.y * (kMostCode / 512.f);
+  }
+}
+
+// Of a row in the ordinary way: a lane's t = 7/8 c w, exact; the largest |t| as
+// bits, whose order is that of non-negative floats with NaN on top; the sum of c^2
+// (with a norm).  The last two are the same in every lane.
+__device__ __forceinline__ void row_sums(const uint4 (&c_raw)[2], const float (&w78)[16], bool norm, float (&t)[16], uint32_t& top,
+                                         float& sum) {
+  const uint32_t* x = reinterpret_cast<const uint32_t*>(c_raw);
+  float most = 0.f;
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 c = bf16x2(x[k]);
+    sum = fmaf(c.x, c.x, sum);
+    sum = fmaf(c.y, c.y, sum);
+    t[2 * k] = c.x * w78[2 * k];
+    t[2 * k + 1] = c.y * w78[2 * k + 1];
+    most = max3_nan(most, fabsf(t[2 * k]), fabsf(t[2 * k + 1]));
+  }
+  top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+  if (norm) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+}
+
+// For a whole warp: whether a row's latent is zeros, of either sign.
+__device__ __forceinline__ bool is_zero(const uint4 (&c_raw)[2]) {
+  const uint32_t any = (c_raw[0].x | c_raw[0].y) | (c_raw[0].z | c_raw[0].w) | (c_raw[1].x | c_raw[1].y) | (c_raw[1].z | c_raw[1].w);
+  return !__any_sync(0xffffffffu, (any & 0x7FFF7FFFu) != 0u);
+}
+
+// Whether the ordinary way serves: t and squares in the range of normal fp32 numbers (a mean square is its own
+// measure), and so the scale; rows of zeros are told apart before.
+// (Comparisons of bits: negative numbers and NaN are above infinity.)
+__device__ __forceinline__ bool is_far(uint32_t top, float mean, float scale) {
+  constexpr uint32_t kRange = 0x7F800000u - kSmall, kScaleRange = 0x7F800000u - 0x00800000u;
+  return top - kSmall >= kRange || __float_as_uint(scale) - 0x00800000u >= kScaleRange || __float_as_uint(mean) - kSmall >= kRange;
+}
+
+// A warp that met rows out of range goes over its tokens again, for these alone.  Behind the others and not inlined:
+// as a branch for each row, their registers cost every row (94 us for 74).
+__device__ __noinline__ void far_rows(const uint8_t* kv, int64_t kv_row, const int64_t* slots, int num_tokens,
+                                      const __nv_bfloat16* norm, float eps, const int64_t* positions, int64_t max_positions,
+                                      uint8_t* cache, int64_t num_slots) {
+  const int lane = threadIdx.x & 31;
+  float w78[16];
+  load_weights(norm, w78);
+  const uint32_t stride = gridDim.x * kWarps;
+  for (uint32_t token = blockIdx.x * kWarps + (threadIdx.x >> 5); token < static_cast<uint32_t>(num_tokens); token += stride) {
+    const int64_t slot = slots[token];
+    if (slot < 0 || slot >= num_slots) continue;
+    if (positions != nullptr && (positions[token] < 0 || positions[token] >= max_positions)) continue;
+    const uint8_t* row = kv + static_cast<int64_t>(token) * kv_row;
+    const uint4 c[2] = {*reinterpret_cast<const uint4*>(row + 16 * lane), *reinterpret_cast<const uint4*>(row + 512 + 16 * lane)};
+    float t[16], sum;
+    uint32_t top;
+    row_sums(c, w78, norm != nullptr, t, top, sum);
+    const float mean = norm != nullptr ? fmaf(sum, 1.f / kCkv, eps) : 1.f;
+    const float scale = most_over_512(__uint_as_float(top)) * (512.f / kMostCode) * rsqrtf(mean);
+    if ((top == 0u && is_zero(c)) || !is_far(top, mean, scale)) continue;
+    const int64_t page = slot / kPage;
+    const int in_page = static_cast<int>(slot - page * kPage);
+    uint8_t* base = cache + page * kPageBytes;
+    write_far_row(row, norm, eps, base + in_page * kCkv, reinterpret_cast<float*>(base + kScaleAt + 4 * in_page));
+  }
+}
+
 // Warps walk the tokens; of a token a lane has the values 8 l .. 8 l + 7 and 256
 // + 8 l .. of the latent (16-byte loads, 8-byte stores, each of a warp's in one
 // piece) and the pair 2 l, 2 l + 1 of the position part.  A warp loads its next
-// token before it works on the one it has: 24 warps an SM of 79 registers have
+// token before it works on the one it has: 24 warps an SM of 80 registers have
 // 33 KB on their way.  About 300 instructions a token, three quarters of the issue
 // slots; DRAM at 57 % of its peak.  Packed FMAs save 40 of them and 0.3 us; a load
 // two tokens ahead needs 122 registers, 16 warps: 85 us.  200003 tokens with norm
-// and rotation: 74 us, 5.4 TB/s (60 us at the copy's rate); without the load
-// ahead 86, two tokens a warp 88, four in 159 registers (8 warps an SM) 185; two
+// and rotation: 76 us, 5.2 TB/s (60 us at the copy's rate; 74 without the look for
+// rows out of range); without the load ahead 86, two tokens a warp 88, four in 159 registers (8 warps an SM) 185; two
 // blocks an SM 88, four (spilling) 98.
 constexpr int kBlocksPerSm = 3;
 
@@ -96,34 +293,23 @@ write_kernel(const WriteParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
+  __shared__ bool met_far[kWarps];
+  met_far[threadIdx.x >> 5] = false;
   float w78[16];
-  {
-    uint4 raw[2] = {make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u),
-                    make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)};  // ones
-    if (p.norm != nullptr) {
-      raw[0] = *reinterpret_cast<const uint4*>(p.norm + 8 * lane);
-      raw[1] = *reinterpret_cast<const uint4*>(p.norm + 256 + 8 * lane);
-    }
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(raw);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float2 w = bf16x2(x[k]);
-      w78[2 * k] = w.x * (kMostCode / 512.f);
-      w78[2 * k + 1] = w.y * (kMostCode / 512.f);
-    }
-  }
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps;
-  int64_t t_next = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  load_weights(p.norm, w78);
+  // Unsigned 32 bits hold a token and 32 strides beyond.
+  const uint32_t stride = gridDim.x * kWarps;
+  uint32_t t_next = blockIdx.x * kWarps + (threadIdx.x >> 5);
   // Lane x has slot and position of the warp's x-th token from here on, so that
   // no load waits for another but once in 32 tokens.
   int64_t lane_slot = -1, lane_pos = 0;
   int turn = 0;
   auto load = [&]() {
     if (turn == 0) {
-      const int64_t at = t_next + lane * stride;
+      const uint32_t at = t_next + lane * stride;
       lane_slot = -1;
       lane_pos = 0;
-      if (at < p.num_tokens) {
+      if (at < static_cast<uint32_t>(p.num_tokens)) {
         lane_slot = p.slots[at];
         if (p.positions != nullptr) lane_pos = p.positions[at];
         const bool outside = p.positions != nullptr && (lane_pos < 0 || lane_pos >= p.max_positions);
@@ -140,7 +326,7 @@ write_kernel(const WriteParams p) {
     n.cs = n.sn = make_float2(0.f, 0.f);
     n.slot = __shfl_sync(0xffffffffu, lane_slot, turn);
     if (n.slot >= 0) {
-      const uint8_t* row = p.kv + t_next * p.kv_row;
+      const uint8_t* row = p.kv + static_cast<int64_t>(t_next) * p.kv_row;
       n.c[0] = *reinterpret_cast<const uint4*>(row + 16 * lane);
       n.c[1] = *reinterpret_cast<const uint4*>(row + 512 + 16 * lane);
       n.pe = *reinterpret_cast<const uint32_t*>(row + 2 * kCkv + 4 * lane);
@@ -161,76 +347,34 @@ write_kernel(const WriteParams p) {
     t_next += stride;
     return n;
   };
-  if (t_next >= p.num_tokens) return;
+  if (t_next >= static_cast<uint32_t>(p.num_tokens)) return;
   TokenPart next = load();
   for (;;) {
     const TokenPart now = next;
-    const bool more = t_next < p.num_tokens;
+    const bool more = t_next < static_cast<uint32_t>(p.num_tokens);
     if (more) next = load();
     if (now.slot >= 0) {  // the whole warp
-      const uint32_t* x = reinterpret_cast<const uint32_t*>(now.c);
-      float t[16];  // 7/8 c w, exact
-      float sum = 0.f, most = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float2 c = bf16x2(x[k]);
-        sum = fmaf(c.x, c.x, sum);
-        sum = fmaf(c.y, c.y, sum);
-        t[2 * k] = c.x * w78[2 * k];
-        t[2 * k + 1] = c.y * w78[2 * k + 1];
-        most = max3_nan(most, fabsf(t[2 * k]), fabsf(t[2 * k + 1]));
-      }
-      // The order of non-negative floats is that of their bits, NaN on top.
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-      if (p.norm != nullptr) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      }
-      const float r = p.norm != nullptr ? rsqrtf(fmaf(sum, 1.f / kCkv, p.eps)) : 1.f;
-      // M / 2^9 with M = max |c w|, and the row's scale.  That quotient is exact:
-      // a first one, its remainder by one FMA, and the sum of both rounded.
-      const float top7 = __uint_as_float(top), first = top7 * (1.f / kMostCode);
-      float D = fmaf(fmaf(-first, kMostCode, top7), 1.f / kMostCode, first);
-      float scale = D * (512.f / kMostCode) * r;
-      uint32_t code[4];
-      if (top >= 0x7F800000u) {  // an infinity or NaN: the whole row is NaN
-        scale = 1.f;
-        code[0] = code[1] = code[2] = code[3] = 0x7F7F7F7Fu;
-      } else if (!(scale >= kLeastScale)) {  // zeros, or too small for a scale
-        scale = 1.f;
-        code[0] = code[1] = code[2] = code[3] = 0u;
-      } else {
-        if (D < 1e-18f || D > 1e18f) {  // by a power of two, so that no reciprocal or quotient leaves the range
-          const float by = D < 1.f ? 1.8446744073709552e19f : 5.421010862427522e-20f;  // 2^64, 2^-64
-          D *= by;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) t[k] *= by;
-        }
-        // t / D = 448 c w / M in the same way: within 2^-44 of itself before it is
-        // rounded, so exact where it is a border of e4m3 (what underflows is far
-        // below half of the smallest code).
-        float rcp;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(D));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float v[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float q = __fmul_rn(t[4 * k + z], rcp);
-            v[z] = __fmaf_rn(__fmaf_rn(q, D, -t[4 * k + z]), -rcp, q);  // (signs that keep -0)
-          }
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
-          code[k] = lo | (hi << 16);
-        }
-      }
+      float t[16], sum;
+      uint32_t top;
+      row_sums(now.c, w78, p.norm != nullptr, t, top, sum);
       const int64_t page = now.slot / kPage;
       const int row = static_cast<int>(now.slot - page * kPage);
       uint8_t* base = p.cache + page * kPageBytes;
       uint8_t* codes = base + row * kCkv;
-      *reinterpret_cast<uint2*>(codes + 8 * lane) = make_uint2(code[0], code[1]);
-      *reinterpret_cast<uint2*>(codes + 256 + 8 * lane) = make_uint2(code[2], code[3]);
-      if (lane == 0) *reinterpret_cast<float*>(base + kScaleAt + 4 * row) = scale;
+      float* to_scale = reinterpret_cast<float*>(base + kScaleAt + 4 * row);
+      const float mean = p.norm != nullptr ? fmaf(sum, 1.f / kCkv, p.eps) : 1.f;
+      const float D = most_over_512(__uint_as_float(top));
+      const float scale = D * (512.f / kMostCode) * rsqrtf(mean);
+      if (top == 0u && is_zero(now.c)) {
+        const uint32_t code[4] = {0u, 0u, 0u, 0u};
+        store_codes(codes, code, to_scale, 1.f);
+      } else if (is_far(top, mean, scale)) {
+        met_far[threadIdx.x >> 5] = true;  // behind all others
+      } else {
+        uint32_t code[4];
+        codes_of(t, D, code);
+        store_codes(codes, code, to_scale, scale);
+      }
       uint32_t rotated = now.pe;
       if (p.positions != nullptr) {
         const float2 v = bf16x2(now.pe);
@@ -248,6 +392,9 @@ write_kernel(const WriteParams p) {
     }
     if (!more) break;
   }
+  __syncwarp();
+  if (!met_far[threadIdx.x >> 5]) return;
+  far_rows(p.kv, p.kv_row, p.slots, p.num_tokens, p.norm, p.eps, p.positions, p.max_positions, p.cache, p.num_slots);
 }
 
 // ------------------------------------------------------------------ read

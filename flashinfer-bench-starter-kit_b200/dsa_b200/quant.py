@@ -27,8 +27,9 @@ the last 64 are rotated by their position's 32 angles (``cos_sin``: [positions,
 stored as given, without ``cos_sin`` the position part.  Negative slots are
 padding and skipped; a slot beyond the cache or a position beyond the table
 sets a status bit, and the token is not written.  A slot given twice in a call
-holds either of its tokens, or parts of both.  A latent with an infinity or NaN
-is stored as NaN throughout; one whose scale would be below 2^-126 as zeros.
+holds either of its tokens, or parts of both.  A latent with an infinity or NaN,
+or whose scale would be above float32's largest number, is stored as NaN
+throughout; one whose scale would be below 2^-126 as zeros (both with scale 1).
 
 ``read`` makes row ``cu_rows[r] + i`` of ``ckv`` [T, 512] and ``kpe`` [T, 64]
 (bf16, rows may be strided, such as the two parts of one [T, 576] buffer) the

@@ -385,9 +385,10 @@ DSA_API int dsa_cache_evict_run(const float* acc, int64_t acc_stride, const int3
  *                  in for a slot >= num_pages * 64 or a position outside of the
  *                  table; such a token is not written
  *
- * A row with an infinity or NaN in its latent is stored as NaN throughout, one
- * whose scale would be below 2^-126 as zeros.  A cache that shares memory with an
- * input: DSA_ERR_OVERLAP. */
+ * A row with an infinity or NaN in its latent, or whose scale would be above the
+ * largest fp32 number, is stored as NaN throughout, one whose scale would be below
+ * 2^-126 as zeros; both have the scale 1.  A cache that shares memory with an input:
+ * DSA_ERR_OVERLAP. */
 DSA_API int dsa_latent_cache_write(const void* kv, int64_t kv_row_bytes, const int64_t* slot_mapping,
                                    int32_t num_tokens, const void* norm_weight, float eps,
                                    const int64_t* positions, const float* cos_sin, int64_t max_positions,

@@ -55,7 +55,7 @@ def write_rows(kv, norm=None, eps=1e-6, positions=None, cos_sin=None, interleave
     top = t.abs().amax(1)
     scale = top * r / 448
     small = ~(scale >= 2.0 ** -126)
-    broken = ~torch.isfinite(t).all(1)
+    broken = ~torch.isfinite(t).all(1) | (scale > torch.finfo(torch.float32).max)
     code = e4m3(448 * t / torch.where(small | broken, 1.0, top)[:, None].clamp(min=1e-300))
     code[small] = 0
     code[broken] = 0x7F

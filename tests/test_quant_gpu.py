@@ -37,7 +37,7 @@ def written(device, n, pages, seed, norm=True, rope=True, interleaved=False, str
     return args, oq.write_rows(kv, w, 1e-6, pos, table, interleaved), slots
 
 
-def check(cache, want, slots):
+def check(cache, want, slots, least=0.0):
     code, scale, e = want
     cache = cache.cpu()
     codes, kpe, scales = oq.pieces(cache)
@@ -48,7 +48,7 @@ def check(cache, want, slots):
     # A product and an FMA in fp32, 2^-24 of |b sin| and of the result, |b| at most sqrt 2 of the row's largest rotated
     # value (a rotation keeps a pair's length); then half a step of bf16.
     off = (kpe[p, t].double() - e[real]).abs()
-    assert (off <= 2.0 ** -8 * e[real].abs() + 2.0 ** -22 * e[real].abs().amax(1, keepdim=True)).all()
+    assert (off <= 2.0 ** -8 * e[real].abs() + 2.0 ** -22 * e[real].abs().amax(1, keepdim=True) + least).all()
     untouched = torch.ones(codes.shape[:2], dtype=torch.bool)
     untouched[p, t] = False
     assert (codes[untouched] == 0x5A).all() and (kpe.view(torch.uint8)[untouched] == 0x5A).all()
@@ -91,6 +91,53 @@ def test_write_keeps_the_sign_of_zeros(cuda_device, norm):
     cache = torch.zeros(1, quant.PAGE_BYTES, dtype=torch.uint8, device=cuda_device)
     quant.write(kv.to(cuda_device), torch.arange(40, device=cuda_device), cache, None if w is None else w.to(cuda_device))
     assert torch.equal(oq.pieces(cache.cpu())[0][0, :40], oq.write_rows(kv, w)[0])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-30, 1e30])
+@pytest.mark.parametrize("spread", [0.0, 6.0])
+def test_write_of_rows_of_all_sizes_with_a_norm(cuda_device, eps, spread):
+    """Latents and weights whose squares and products leave fp32's range on either side, where the scale is an ordinary number;
+    rows whose scale is beyond it."""
+    g = torch.Generator().manual_seed(int(spread) + 1)
+    sizes = [2.0 ** e for e in (-132, -126, -110, -75, -63, -50, -20, 0, 20, 40, 59, 60, 63, 64, 80, 100, 120, 124)]
+    kv = torch.randn(len(sizes) + 5, 576, generator=g) * torch.exp(spread * torch.randn(len(sizes) + 5, 576, generator=g).clamp(-3, 3) / 3)
+    kv[:len(sizes)] *= torch.tensor(sizes)[:, None]
+    kv = kv.clamp(-3e38, 3e38)
+    kv[len(sizes)] = 0
+    kv[len(sizes) + 1, :512] = 0
+    kv[len(sizes) + 1, 7] = 3e38  # one value alone
+    kv[len(sizes) + 2, :512] = 1e-38
+    kv[len(sizes) + 3, 9], kv[len(sizes) + 4, 9] = math.inf, math.nan
+    kv = kv.bfloat16()
+    for size in (1.0, 1e-36, 1e-20, 1e20, 1e36):
+        w = ((1 + 0.3 * torch.randn(512, generator=g)) * size).bfloat16()
+        cache = torch.zeros(1, quant.PAGE_BYTES, dtype=torch.uint8, device=cuda_device)
+        quant.write(kv.to(cuda_device), torch.arange(len(kv), device=cuda_device), cache, w.to(cuda_device), eps)
+        codes, _, scales = oq.pieces(cache.cpu())
+        want, scale, _ = oq.write_rows(kv, w, float(torch.tensor(eps, dtype=torch.float32)))
+        n = len(kv)
+        # where the scale is within its own error of the border, either is right
+        border = ((scale / 2.0 ** -126 - 1).abs() < 2 * SCALE_RTOL) & (codes[0, :n] == 0).all(1)
+        assert torch.equal(codes[0, :n][~border], want[~border])
+        assert ((scales[0, :n].double() - scale).abs() <= SCALE_RTOL * scale)[~border].all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_write_of_rows_out_of_range_among_others(cuda_device, interleaved):
+    """Many rows a warp, some of them beyond fp32's squares or below its products, zeros, padding, slots and positions outside."""
+    args, _, slots = written(cuda_device, 20001, 320, 11, True, True, interleaved, True)
+    kv, pos = args[0].cpu(), args[5].cpu()
+    kv[::97] *= 1e25
+    kv[5::101] *= 1e-37
+    kv[7::89, :512] = 0
+    pos[11::1000], slots[13::1000] = 300, 320 * 64
+    args[0].copy_(kv)
+    args[5].copy_(pos)
+    args[1].copy_(slots)
+    with pytest.raises(DsaError, match="outside"):
+        quant.write(*args)
+    kept = torch.where((pos < 300) & (slots < 320 * 64), slots, -1)
+    want = oq.write_rows(kv, args[3].cpu(), float(torch.tensor(1e-6)), pos.clamp(max=299), args[6].cpu(), interleaved)
+    # The position parts of the smallest rows are subnormal numbers of bf16: steps of 2^-133, whatever the value; and fp32's of 2^-149.
+    check(args[2], want, kept, 2.0 ** -134 + 2.0 ** -148)
 
 
 def test_write_reports_what_does_not_fit(cuda_device):
