@@ -13,7 +13,7 @@
 //     largest value to 128 .. 256).  a takes the upper 4 of the 8 bits of a bf16,
 //     b the other 4: exact from 2^-13 of the row's largest up, to 2^-21 of that
 //     below.
-//   w = p s (weight by scale, the row's largest so far 2^7 or more) = a + b +
+//   w = p s (weight by scale, the row's largest so far 2^5 or more) = a + b +
 //     (c + d) / 128 with e5m2 parts, each to nearest: 3 bits, then 4 more each (what
 //     is left has a sign and is less than the last step).  Within 2^-14 of w (6e-6 in
 //     the mean) from 2^15 down to 2^-9, and within 2^-23 below: many light tokens
@@ -72,10 +72,12 @@ constexpr int kStageBytes = (kParts + 1) * kBlockBytes;  // 81920
 constexpr int kTmemCols = 512;
 // A rescale of O costs its tile some 2300 clocks, and of two sets whichever needs one
 // holds up the other: at a threshold of 8 log2 units 2 of 34 tiles need one (normal
-// logits of spread 2.5, scales spread by e^0.3), at 6 four, at 4 six.
-constexpr float kRescaleThreshold = 8.0f;
-constexpr float kUnit = 128.0f;              // of weights: 2^8 x 128 = 2^15 is the largest, e5m2 goes to 57344
-constexpr float kUnitLog2 = 7.0f;
+// logits of spread 2.5, scales spread by e^0.3), at 6 four, at 4 six.  Graph replays
+// at 8, 9 and 10: 128 heads 66.9, 65.7 and 65.0 us, 16 x 4096-16384 tokens 38.6, 38.3
+// and 38.3; each halves the unit that is left for light weights.
+constexpr float kRescaleThreshold = 10.0f;
+constexpr float kUnit = 32.0f;               // of weights: 2^10 x 32 = 2^15 is the largest, e5m2 goes to 57344
+constexpr float kUnitLog2 = 5.0f;
 constexpr float kScaleRange = 60.0f;         // log2 units from a segment's unit of scales
 constexpr float kLeastRef = 0x1p-100f;       // of that unit: kUnit over it has to be a number
 constexpr float kLowUnit = 1.0f / 128.0f;    // of their last two parts: what the first two leave is below 2^-7 of a weight
@@ -483,7 +485,8 @@ __device__ __forceinline__ void in_parts(const float* w, uint2 (&out)[4]) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (x == 2) h = __hmul2(__hadd2(h, lower), __float2half2_rn(1.0f / kLowUnit));
-      const uint32_t two = (*reinterpret_cast<const uint32_t*>(&h) + 0x00800080u) & 0xFF00FF00u;
+      uint32_t two = *reinterpret_cast<const uint32_t*>(&h) + 0x00800080u;
+      if (x < 3) two &= 0xFF00FF00u;
       part[x < 2 ? 2 * x : 2 * x - 3][k] = two;
       if (x < 3) h = __hsub2(h, *reinterpret_cast<const __half2*>(&two));  // exact
     }
@@ -985,7 +988,7 @@ attend_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_consta
     // running maximum of x + log2(s / ref), ref the power of two of the largest scale
     // in the segment's first tile.  So the column's largest product is kUnit or more,
     // and no token takes from the others' precision but by its own weight (with maxima
-    // of x and s apart, a token of a scale 2^20 times the others' and no weight left
+    // of x and s apart, a token of a scale 2^24 times the others' and no weight left
     // them 3 bits).  The sums l of 2^(x - m), in 32 bits, need no such reference: scales
     // within 2^60 of ref cannot drive them out of the range.  Smaller ones (zeros
     // among them) count as 2^-60 in m, larger ones move ref.

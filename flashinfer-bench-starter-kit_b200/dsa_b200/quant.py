@@ -48,7 +48,7 @@ sees nothing yields output 0 and lse -inf.  Tokens that no row sees may hold
 anything; a visible one with NaN makes the output NaN.  ``output`` may be ``q_nope``
 itself; other outputs over an input are refused.  Values of a query are exact from
 2^-13 of its row's largest up, smaller ones to 2^-21 of that; softmax weights times
-scales to 2^-14 of each and 2^-30 of the row's largest.  Where scales of one request
+scales to 2^-14 of each and 2^-28 of the row's largest.  Where scales of one request
 differ by 2^60 and more, tokens of the small ones may count as zeros.
 
 Calls that overlap need different streams; threads may call on one stream.  A

@@ -443,7 +443,7 @@ DSA_API size_t dsa_latent_attention_workspace_bytes(void);
  * (num_rows * num_heads / 16 + num_requests) * (max_pages / 2 + 4) <= 2^30.  Tokens
  * that no row sees may hold anything; a visible one with NaN makes the output NaN.
  * Values of q_nope are exact from 2^-13 of their row's largest up, smaller ones to
- * 2^-21 of that; weights times scales to 2^-14 of each and 2^-30 of the row's largest.
+ * 2^-21 of that; weights times scales to 2^-14 of each and 2^-28 of the row's largest.
  * Where scales of one request differ by 2^60 and more, tokens of the small ones may
  * count as zeros.
  * Outputs that share memory with anything else: DSA_ERR_OVERLAP.  Data-dependent

@@ -102,7 +102,7 @@ def _softmax(q_nope, q_pe, c, e, scales, see, scale):
     err = (2 * math.log(2) * (off + move[:, None]) + 2.0 ** -14 + 2.0 ** -17) * w
     codes = torch.where(scales[:, None] == 0, 0.0, c.abs() / scales[:, None])
     largest = torch.where(codes.any(1) | (scales != 1), w * scales, 0.0).amax(1, keepdim=True)
-    bound = err @ c.abs() + 2.0 ** -30 * largest * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
+    bound = err @ c.abs() + 2.0 ** -28 * largest * codes.sum(0) + 2.0 ** -8 * out.abs() + 2.0 ** -20 * c.abs().amax()
     return out, lse, bound, move + 2.0 ** -18 + 2.0 ** -23 * lse.abs()
 
 
@@ -118,7 +118,7 @@ def attend_reference(q_nope, q_pe, cache, seq_lens, table, cu, scale):
       Each is half a step off what the one before leaves, which may pass a power of two by an eighth: within 2^-14, and
       2^-18 for the lower bits' rounding, 2^-22 for its products.  Where it is far below the largest, it is within half the
       smallest step of the last part, 2^-17 / 128, and 2^-24 of half precision's: in units of which the largest weight times
-      its scale is 2^7 or more (rows of zeros that have the scale 1 apart).  Each token's code may so count 2^-30 times that
+      its scale is 2^5 or more (rows of zeros that have the scale 1 apart).  Each token's code may so count 2^-28 times that
       product too much or too little.  The output is rounded to bf16, 2^-8 of itself.
     """
     T, H = q_nope.shape[:2]
