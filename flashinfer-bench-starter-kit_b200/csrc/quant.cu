@@ -92,9 +92,10 @@ __device__ __forceinline__ void codes_of(float (&t)[16], float D, uint32_t (&cod
 #pragma unroll
     for (int k = 0; k < 16; ++k) t[k] *= by;
   }
-  // t / D = 448 c w / M in the same way as D: within 2^-44 of itself before it is
-  // rounded, so exact where it is a border of e4m3 (what underflows is far below
-  // half of the smallest code).
+  // t / D = 448 c w / M in the same way as D (a quotient corrected by its remainder:
+  // P. Markstein, as in cache_write.cu): within 2^-44 of itself before it is rounded,
+  // so exact where it is a border of e4m3 (what underflows is far below half of the
+  // smallest code).
   float rcp;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(D));
 #pragma unroll
@@ -273,7 +274,7 @@ __device__ __noinline__ void far_rows(const uint8_t* kv, int64_t kv_row, const i
 // piece) and the pair 2 l, 2 l + 1 of the position part.  A warp loads its next
 // token before it works on the one it has: 24 warps an SM of 80 registers have
 // 33 KB on their way.  About 300 instructions a token, three quarters of the issue
-// slots; DRAM at 57 % of its peak.  Packed FMAs save 40 of them and 0.3 us; a load
+// slots; DRAM at 56 % of its peak.  Packed FMAs save 40 of them and 0.3 us; a load
 // two tokens ahead needs 122 registers, 16 warps: 85 us.  200003 tokens with norm
 // and rotation: 76 us, 5.2 TB/s (60 us at the copy's rate; 74 without the look for
 // rows out of range); without the load ahead 86, two tokens a warp 88, four in 159 registers (8 warps an SM) 185; two

@@ -39,13 +39,17 @@
 // join their pieces through shared memory (together_for).
 //
 // Measured, attention with its join in replayed graphs: one row of 16 heads over
-// 64 x 65536 tokens 406-412 us (2.70 GB, 6.6 TB/s: HBM-bound; 434-466 back to back
-// under the power cap); 16 x 4096-16384 tokens, 1-4 rows 36 us (96 MB: start, end
-// and join, see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 61 us (35
-// GFLOP: a tile's way through its stage takes 5200 clocks, load 800, S^T 1800, softmax
-// 1800, O^T 800, and two stages fit; the products alone take 1400 a tile); 300 x 2048
-// selected slots of 16 heads 93 us (406 MB; a kernel that only reads these rows takes
-// 87: half-kilobyte pieces at random).  About 8 us are a call's start (plan, page ids, first tile, its maxima) and end, 3.5-9 its join.
+// 64 x 65536 tokens 416 us (2.70 GB, 6.5 TB/s: HBM-bound; 443-480 back to back under
+// the power cap); 16 x 4096-16384 tokens, 1-4 rows 38 us (96 MB: start, end and join,
+// see below); 1-2 rows of 128 heads over 5 x 8000-30001 tokens 65 us (35 GFLOP: a
+// tile's way through its stage takes 5600 clocks, load 800, S^T 1800, softmax 1800,
+// O^T 1200, and two stages fit; the products alone take 1660 a tile); 300 x 2048
+// selected slots of 16 heads 95 us (406 MB; a kernel that only reads these rows takes
+// 87: half-kilobyte pieces at random, and 14 us of it the scales, a sector each).
+// About 8 us are a call's start (plan, page ids, first tile, its maxima) and end,
+// 3.5-9 its join.  With weights in three parts, and the product of 32 rows in one, the
+// four took 406, 36, 62 and 93 us.  (Comparisons beside choices below that do not
+// choose between 16 rows and 32, or clusters and slices, are of that time.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -472,8 +476,8 @@ __device__ __forceinline__ float4 ld_cluster4_or_zeros(uint32_t at, int rank, bo
 // a and b are taken without rounding, and what they leave with its lower bits, to
 // 11 bits more.  An e5m2 value is the upper byte of the same value in half
 // precision; half a step added below it rounds (a carry moves the exponent), in two
-// integer operations (128 heads 71.0 us, with conversions 72.1; with three parts by
-// conversions 62.1).  (NaN may become 0 here; its row's sum l is NaN.)
+// integer operations (by conversions 128 heads took 1 us more).  (NaN may become 0
+// here; its row's sum l is NaN.)
 __device__ __forceinline__ void in_parts(const float* w, uint2 (&out)[4]) {
   uint32_t part[4][4];
 #pragma unroll
@@ -1605,13 +1609,13 @@ int64_t most_groups(const Params& p, int r) {
 // would (two where slots are gathered).  Their number is bounded by the width of
 // the table, which is what the host knows; lengths well below it lose little, as
 // a CTA's tiles end with its group's.  Graph replays in us, slices against clusters:
-//   requests of one row of 16 heads x tokens: 1 x 128 10.9 and 9.4, 1 x 1024 12.5 and
-//   10.5, 1 x 4096 (not taken) 13.4 and 13.7; 14 x 2048 15.0 and 12.7; 16 x 4096 (not
-//   taken) 18.1 and 20.5; 32 x 1024 16.5 and 13.6; 128 x 512 20.7 and 15.2
-//   1 x 1024 of four rows 15.1 and 10.6, of 128 heads 15.7 and 11.4; 16 x 300 of 128
-//   heads 20.5 and 13.6; 4 x 4096 of 128 (not taken) 21.2 and 21.0
-//   rows of 2048 selected slots of 16 heads: 1 11.2 and 10.8, 5 12.2 and 11.3, 14 13.8
-//   and 12.0, 16 (not taken) 14.2 and 14.8, 32 19.0 and 17.1
+//   requests of one row of 16 heads x tokens: 1 x 128 9.3 and 8.1, 1 x 1024 11.1 and
+//   9.3, 1 x 4096 (not taken) 12.2 and 13.1; 14 x 2048 14.5 and 11.7; 16 x 4096 (not
+//   taken) 17.8 and 19.9; 32 x 1024 15.3 and 12.7; 128 x 512 20.1 and 14.2
+//   1 x 1024 of four rows 14.3 and 9.5, of 128 heads 14.8 and 10.1; 16 x 300 of 128
+//   heads 21.3 and 13.2; 4 x 4096 of 128 (not taken) 21.0 and 20.3
+//   rows of 2048 selected slots of 16 heads: 1 11.1 and 10.8, 5 12.1 and 10.9, 14 13.8
+//   and 11.6, 16 (not taken) 13.7 and 14.8, 32 18.9 and 16.6
 // Sixteen CTAs (7 such clusters run at once) joined slower than they saved.
 int together_for(const Params& p, const DeviceInfo& info) {
   const int64_t groups = most_groups(p, 16);
@@ -1736,8 +1740,9 @@ extern "C" int dsa_latent_attention_run(const void* q_nope, const void* q_pe, co
   p.out = static_cast<__nv_bfloat16*>(output);
   p.lse = lse;
   // Groups of 16 rows or 32: 32 where requests have more than 16 rows on average, since a group reads the whole context.
-  // Graph replays in us, 16 rows against 32: 64 x 1000-3000 tokens of two rows of 16 heads 38.9 and 37.1, of 64 x 300-900
-  // of four 34.0 and 31.2, of one row of 128 heads and 64 x 500-1500 tokens 64.2 and 57.0.
+  // Graph replays in us, 16 rows against 32: 64 x 1000-3000 tokens of two rows of 16 heads 37.2 and 34.1, of 64 x 300-900
+  // of four 32.6 and 28.4, of 64 x 1000-3000 of one row of 24 heads 36.7 and 35.0, of one row of 128 heads and 64 x
+  // 500-1500 tokens 63.3 and 54.0.
   const bool wide = static_cast<int64_t>(num_rows) * num_heads > 16 * static_cast<int64_t>(num_requests);
   return qattn::launch(p, info, wide, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1785,9 +1790,9 @@ extern "C" int dsa_latent_sparse_attention_run(const void* q_nope, const void* q
   p.lse = lse;
   // Groups of 16 heads or 32: 32 where a row has more than 16 and groups of 16 make more than 8 tiles an SM.  A group
   // gathers its row's slots anew; where there are few, the shorter start and end of 16 win.  Graph replays in us, 16
-  // against 32, 2048 slots, rows x heads (tiles an SM at 16): 4 x 32 (0.9) 11.9 and 14.0, 16 x 64 (6.9) 24.7 and 24.9,
-  // 8 x 128 (6.9) 24.4 and 24.8, 64 x 24 (14) 45.0 and 41.0, 64 x 32 (14) 44.8 and 43.3, 64 x 64 (28) 75.0 and 62.3,
-  // 64 x 128 (55) 129.6 and 106.3.
+  // against 32, 2048 slots, rows x heads (tiles an SM at 16): 16 x 64 (6.9) 25.2 and 25.4, 8 x 128 (6.9) 24.8 and 24.9,
+  // 64 x 24 (14) 45.1 and 42.0, 64 x 32 (14) 45.6 and 43.8, 64 x 64 (28) 76.5 and 63.4, 64 x 128 (55) 133.3 and 109.2,
+  // 256 x 32 (55) 146.7 and 115.1.
   const int64_t tiles = groups * ((topk + qattn::kTok - 1) / qattn::kTok);
   const bool wide = num_heads > 16 && tiles > 8 * static_cast<int64_t>(info.num_sms);
   return qattn::launch(p, info, wide, workspace, reinterpret_cast<cudaStream_t>(stream));
